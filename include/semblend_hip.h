@@ -35,6 +35,7 @@ extern "C" {
 #define SB_DTYPE_F32 0
 #define SB_DTYPE_F16 1
 #define SB_DTYPE_BF16 2
+#define SB_DTYPE_MXFP4 3 /* caches of sb_append_kv_paged, sb_gather_kv_paged, sb_paged_attention */
 
 /* Flags of the multi-layer scatters (sb_*_paged_layers, sb_composite_scatter_paged_layers).
  * SB_SCATTER_REPEATED_DONOR_ROWS: a donor row may be the source of several pairs (one
@@ -578,6 +579,85 @@ int sb_partial_attention_paged_varlen(void* out, const void* q, const void* kv_c
                                       const int64_t* kv_strides, int32_t dtype, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * A serving batch over a paged cache: new tokens appended, attention of single tokens and prompt
+ * chunks (optionally under a sliding window), 4-bit pages. No reference counterparts: the
+ * reference leaves decoding to its host engines.
+ *
+ * Shared by the three entries:
+ *   - Rows (tokens) of num_requests requests lie back to back: request r's are row_starts[r] ..
+ *     row_starts[r + 1] - 1 (device int32, num_requests + 1 entries, ascending). row_starts NULL:
+ *     row i is request i's only one, or, with num_requests 1, all rows are that one's. Rows from row_starts[num_requests] on, and rows with a
+ *     negative position, are padding: nothing is read, appended or written for them.
+ *   - block_tables: row r (table_stride entries apart) names request r's pages; entries that are
+ *     no page of the pool ([0, num_blocks_total)) take no token, and their keys are not seen.
+ *   - cache_dtype is the cache's type: the tensors' dtype, with kv_strides[5] = (block, kv, head,
+ *     pos, dim) in elements and kv_scales NULL; or SB_DTYPE_MXFP4: kv_cache holds head_dim / 2
+ *     bytes a row (value 2i in the low half of byte i: sign, two exponent bits, one mantissa
+ *     bit), kv_scales head_dim / 32 bytes a row (e + 127: a block of 32 values is 2^e times the
+ *     4-bit ones; 255: every value of the block is NaN), both with strides in bytes. head_dim is
+ *     then a multiple of 32.
+ * ---------------------------------------------------------------------------------------- */
+
+/* Writes K and V of num_tokens tokens (key, value [num_tokens, num_kv_heads, head_dim], strides
+ * token, head, dim in elements) to the slots of their positions. With inv_freq (device fp32
+ * [head_dim / 2], 1 / base^(2i/head_dim) <= 1), K is rotated in interleaved pairs by rotations[t] (or, NULL,
+ * positions[t]) * inv_freq[i], the product and its sine and cosine in 64 bits; and query
+ * (NULL: none; [num_tokens, num_q_heads, head_dim]) likewise into query_out. One rounding to the
+ * cache's type. 4-bit blocks: 2^e is the smallest power with max |x| <= 7 * 2^e (e >= -127),
+ * x / 2^e rounds to the nearest 4-bit value, ties to even; a block with an infinity or a NaN is
+ * stored as NaN. Two tokens of one slot race. head_dim even, at most 512. */
+int sb_append_kv_paged(void* kv_cache, void* kv_scales, const void* key, const void* value,
+                       const void* query, void* query_out, const int32_t* block_tables,
+                       int64_t table_stride, const int32_t* positions, const int32_t* rotations,
+                       const int32_t* row_starts, const float* inv_freq, int64_t num_tokens,
+                       int64_t num_requests, int64_t num_kv_heads, int64_t num_q_heads,
+                       int64_t head_dim, int64_t block_size, int64_t num_blocks_total,
+                       int64_t num_blocks_per_seq, const int64_t* k_strides,
+                       const int64_t* v_strides, const int64_t* q_strides,
+                       const int64_t* qo_strides, const int64_t* kv_strides,
+                       const int64_t* scale_strides, int32_t dtype, int32_t cache_dtype,
+                       void* stream);
+
+/* out[kv, h, i, :] = the cache's row of position positions[i] (NULL: i) of one request, in dtype
+ * (a 4-bit value is exact in bf16 and fp32, rounded once to fp16); zeros where the position has
+ * no page. out [2, num_kv_heads, num_rows, head_dim] by o_strides[4] in elements: the donor
+ * buffers of sb_scatter_donor_kv_paged. */
+int sb_gather_kv_paged(void* out, const void* kv_cache, const void* kv_scales,
+                       const int32_t* block_table, const int32_t* positions, int64_t num_rows,
+                       int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                       int64_t num_blocks_total, int64_t num_blocks_per_seq,
+                       const int64_t* o_strides, const int64_t* kv_strides,
+                       const int64_t* scale_strides, int32_t dtype, int32_t cache_dtype,
+                       void* stream);
+
+/* out[r, h] = sum_j softmax_j(scale * q[r, h] . k_j) v_j, h's KV head h / (num_q_heads /
+ * num_kv_heads), over the keys j <= p_r = positions[r] with (window > 0) j > p_r - window or
+ * j < sinks, inside the table and in a page of the pool; zeros for a row that sees none. Pages
+ * between the sinks and the window are not read. fp32 scores, weights' sums and outputs; weights
+ * rounded to dtype for their product with V (16-bit dtypes).
+ * max_rows: no request has more rows (0: unknown). It chooses kernels (with max_rows * group <= 32
+ * only the single-token one is launched); any value gives the same rows.
+ * q, out [num_rows, num_q_heads, head_dim] by strides (row, head, dim). head_dim at most 512;
+ * 64 and 128 with 16-byte aligned rows (fp32 queries: over fp32 pages) run on the matrix cores.
+ * workspace: 16-byte aligned, sb_paged_attention_workspace_size(...) bytes (has_starts: row_starts
+ * is given), fp32 partials of key ranges that are split; may be NULL where that is 0. */
+int64_t sb_paged_attention_workspace_size(int64_t num_rows, int64_t num_requests, int32_t has_starts,
+                                          int64_t max_rows, int64_t num_q_heads,
+                                          int64_t num_kv_heads, int64_t head_dim,
+                                          int64_t block_size, int64_t num_blocks_per_seq,
+                                          int64_t window, int64_t sinks, int32_t dtype);
+int sb_paged_attention(void* out, const void* q, const void* kv_cache, const void* kv_scales,
+                       const int32_t* block_tables, int64_t table_stride,
+                       const int32_t* positions, const int32_t* row_starts, void* workspace,
+                       int64_t workspace_bytes, int64_t num_rows, int64_t num_requests,
+                       int64_t max_rows, int64_t num_q_heads, int64_t num_kv_heads,
+                       int64_t head_dim, int64_t block_size, int64_t num_blocks_total,
+                       int64_t num_blocks_per_seq, int64_t window, int64_t sinks, float scale,
+                       const int64_t* q_strides, const int64_t* o_strides,
+                       const int64_t* kv_strides, const int64_t* scale_strides, int32_t dtype,
+                       int32_t cache_dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Flat device copy (measurement reference; no reference counterpart)
  * ---------------------------------------------------------------------------------------- */
 
@@ -596,7 +676,8 @@ int sb_device_copy(void* dst, const void* src, int64_t num_bytes, void* stream);
  * kernel's own start and end, so no extra work enters the stream); enable == 0 stops logging
  * (the log stays readable). At most 65536 launches are logged. Kernel names:
  * "move_rows", "rope_rows", "rope_index", "fill_i32", "attn_mfma", "attn_valu", "attn_merge",
- * "mask_compact", "zero_rows", "copy". */
+ * "mask_compact", "zero_rows", "copy", "append_kv", "gather_kv", "paged_decode", "paged_f32",
+ * "paged_rows", "paged_valu", "paged_merge". */
 int sb_kernel_timing_enable(int32_t enable);
 
 /* Sum of the logged durations (ms) and number of logged launches of one kernel. Waits for the

@@ -31,6 +31,8 @@ SB_GROUPED_PAIR_ALIGN = 256
 # Constant RoPE deltas must lie strictly within +-2^31 (the C ABI's check; the kernels'
 # sin/cos reduce angles below 2^32 exactly).
 MAX_ROPE_DELTA = 1 << 31
+# Cache type of 4-bit pages (append, gather and attention of semblend_amd.paged_cache).
+SB_DTYPE_MXFP4 = 3
 SB_DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 _vp = ctypes.c_void_p
@@ -110,6 +112,14 @@ SIGNATURES: dict[str, list] = {
                                       _f32, _i64p, _i64p, _i64p, _i64p, _i32, _vp],
     "sb_prefill_output_projection": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
                                      _i64, _i64, _i32, _vp],
+    "sb_append_kv_paged": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64,
+                           _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p, _i64p,
+                           _i64p, _i64p, _i32, _i32, _vp],
+    "sb_gather_kv_paged": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64p,
+                           _i64p, _i64p, _i32, _i32, _vp],
+    "sb_paged_attention": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                           _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i64p, _i64p,
+                           _i64p, _i64p, _i32, _i32, _vp],
     "sb_device_copy": [_vp, _vp, _i64, _vp],
     "sb_kernel_timing_enable": [_i32],
     "sb_kernel_timing_read": [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double), _i64p],
@@ -127,6 +137,8 @@ SIZE_QUERIES: dict[str, list] = {
     "sb_partial_attention_paged_planned_workspace_size": [_i64, _i64, _i64, _i64, _i32, _i32],
     "sb_masked_qkv_projection_workspace_size": [_i64],
     "sb_qkv_projection_paged_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i32],
+    "sb_paged_attention_workspace_size": [_i64, _i64, _i32, _i64, _i64, _i64, _i64, _i64, _i64,
+                                          _i64, _i64, _i32],
 }
 
 # Python index lists to host arrays (csrc/sb_host.cpp): None until first wanted, False where it

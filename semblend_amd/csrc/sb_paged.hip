@@ -1,0 +1,1583 @@
+// Attention over a paged cache for the rows of a serving batch, for gfx950: single tokens, prompt
+// chunks and mixtures of them, over 16-bit, fp32 or MXFP4 pages, with an optional sliding window
+// and first tokens that stay visible (sinks):
+//     out[r, h] = sum_j softmax_j(scale * q[r, h] . k_j) v_j
+// over the keys j <= p_r with j > p_r - window or j < sinks, j inside the request's block table and
+// in a page whose table entry is a page of the pool. A row that sees no key gets zeros; a row with
+// a negative position is left as it was.
+//
+// Query rows of one KV head are flattened as (row, q-head-in-group), so the heads of a group share
+// every K / V row that is read. A row tile's keys are a list of key tiles: the sink tiles, then the
+// tiles from the window's lower edge to the last position; what lies between is never read.
+//
+// Three kernels (plus one for other head sizes, alignments and scales):
+//   * paged_decode_kernel: 16 flattened rows, 16-bit arithmetic. What bounds it is reading the
+//     cache once; every wave walks its own key tiles with a softmax state of its own, so waves
+//     never wait for each other, and the states meet in LDS at the end.
+//   * paged_f32_kernel: the same for fp32 pages on the fp32 matrix cores.
+//   * paged_rows_kernel: 256 flattened rows (8 waves x 32), 16-bit arithmetic; K / V tiles of 64
+//     keys are staged in LDS for all of them. Matrix-core bound.
+// Long key lists are split over workgroups; paged_merge_kernel joins the fp32 partials.
+//
+// Masked places may hold anything. A masked score is replaced, so K never leaks; a weight of zero
+// times an infinite or NaN V would leak through the sum, so tiles that some row sees only in part
+// take V apart: finite values are multiplied as they are, and where a value is not finite the
+// weights that meet it are added up on their own (product with an indicator), which turns the
+// rows that do see it, and only those, into what the sum gives them.
+#include "sb_mma.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace sb {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kNoWindow = 0x7fffffff;
+constexpr int kDecodeRows = 16;
+constexpr int kDecodeWaves = 4;
+constexpr int kRowsTile = 256;
+constexpr int kRowsWaves = 8;
+
+struct PagedArgs {
+  const char* q;
+  char* o;
+  int64_t q_row, q_head, o_row, o_head;   // byte strides
+  const char* k;                          // K plane (4 bit: codes)
+  const char* v;
+  int64_t c_head, c_pos;                  // byte strides
+  const char* ks;                         // scale bytes of K and V (4 bit)
+  const char* vs;
+  int64_t s_head, s_pos;
+  uint32_t c_block, s_block;
+  const int32_t* tables;
+  int64_t table_stride;
+  const int32_t* positions;
+  const int32_t* row_starts;              // nullptr: row i is request i's, or the only one's
+  int num_rows, num_requests, num_kv_heads, group, head_dim;
+  int block_size, bs_log2, num_blocks_total;
+  int kv_len;                             // keys that a block table can name
+  int window, sinks;
+  float scale, scale_log2, scale_log2_lo; // scale_log2_lo: what scale * log2(e) rounds off
+  int flat_min, flat_max;                 // flattened rows of the requests this launch takes
+  int num_tiles;                          // row tiles of the launch (bound)
+  int nsplit, min_tiles;                  // key splits of a row tile; fewest key tiles of one
+  float* part_o;                          // [tile][kv head][split][row][D]
+  float* part_ml;                         // [tile][kv head][split][row][2]
+};
+
+__device__ __forceinline__ int wave_sum_i(int v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// Row tile `idx` of a launch: its request and which tile of TR flattened rows of it.
+struct TileRef {
+  int request;  // -1: behind the last tile
+  int row0, rows, tile;
+};
+template <int TR>
+__device__ __forceinline__ TileRef find_tile(const PagedArgs& a, int idx) {
+  TileRef t = {-1, 0, 0, 0};
+  if (!a.row_starts) {
+    if (a.num_requests == 1) {
+      if (static_cast<int64_t>(idx) * TR < static_cast<int64_t>(a.num_rows) * a.group)
+        t = {0, 0, a.num_rows, idx};
+      return t;
+    }
+    const int per = (a.group + TR - 1) / TR;
+    const int r = idx / per;
+    if (r < a.num_rows) t = {r, r, 1, idx - r * per};
+    return t;
+  }
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int c = 0; c < a.num_requests; c += 64) {
+    const int r = c + lane;
+    int s = 0, n = 0, tiles = 0;
+    if (r < a.num_requests) {
+      s = min(max(a.row_starts[r], 0), a.num_rows);
+      n = max(min(a.row_starts[r + 1], a.num_rows) - s, 0);
+      const int64_t flat = static_cast<int64_t>(n) * a.group;
+      if (flat > a.flat_min && flat <= a.flat_max) tiles = static_cast<int>((flat + TR - 1) / TR);
+    }
+    int incl = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(incl, d, 64);
+      if (lane >= d) incl += y;
+    }
+    const uint64_t past = __ballot(idx < base + incl);
+    if (past) {
+      const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
+      t.request = c + l;
+      t.row0 = __builtin_amdgcn_readfirstlane(__shfl(s, l, 64));
+      t.rows = __builtin_amdgcn_readfirstlane(__shfl(n, l, 64));
+      t.tile = idx - base -
+               __builtin_amdgcn_readfirstlane(__shfl(incl, l, 64) - __shfl(tiles, l, 64));
+      return t;
+    }
+    base += __builtin_amdgcn_readfirstlane(__shfl(incl, 63, 64));
+  }
+  return t;
+}
+
+// The key tiles (of KT keys) that rows at positions [pmin, pmax] see: n_sink tiles from 0 on,
+// then those from lo on; `total` of both.
+struct KeyTiles {
+  int n_sink, lo, total;
+};
+template <int KT>
+__device__ __forceinline__ KeyTiles key_tiles(const PagedArgs& a, int pmin, int pmax) {
+  const int hi_key = min(pmax, a.kv_len - 1);
+  const int lo_key = max(0, pmin - a.window + 1);  // (a.window >= 1: no overflow)
+  const int sink_keys = min(a.sinks, hi_key + 1);
+  KeyTiles t;
+  t.n_sink = (sink_keys + KT - 1) / KT;
+  t.lo = lo_key / KT;
+  int n_win = 0;
+  if (lo_key <= hi_key) {
+    n_win = hi_key / KT - t.lo + 1;
+    t.n_sink = min(t.n_sink, t.lo);
+  }
+  t.total = t.n_sink + n_win;
+  return t;
+}
+template <int KT>
+__device__ __forceinline__ int tile_key(const KeyTiles& t, int i) {
+  return (i < t.n_sink ? i : t.lo + i - t.n_sink) * KT;
+}
+__device__ __forceinline__ int split_count(const PagedArgs& a, int total) {
+  return max(1, min(a.nsplit, total / a.min_tiles));
+}
+
+// Page of a key: its number in the pool, or -1 (outside the table, or no page of the pool).
+__device__ __forceinline__ int page_of(const PagedArgs& a, const int32_t* table, int key) {
+  if (key >= a.kv_len) return -1;
+  const int lb = a.bs_log2 >= 0 ? key >> a.bs_log2 : key / a.block_size;
+  const int pb = table[lb];
+  return pb >= 0 && pb < a.num_blocks_total ? pb : -1;
+}
+// Byte offset of a key's row from its plane and head (page given; no page: page 0, masked later).
+__device__ __forceinline__ int64_t row_offset(const PagedArgs& a, int key, int pb, uint32_t s_block,
+                                              int64_t s_pos) {
+  const int slot = a.bs_log2 >= 0 ? key & (a.block_size - 1) : key % a.block_size;
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(max(pb, 0))) * s_block) +
+         slot * s_pos;
+}
+__device__ __forceinline__ bool sees(const PagedArgs& a, int p, int key) {
+  return key <= p && (key > p - a.window || key < a.sinks);
+}
+
+template <int DT> struct Half;  // 16-bit arithmetic beyond Mma<DT>
+template <> struct Half<SB_DTYPE_BF16> {
+  static constexpr uint32_t kExp = 0x7f80u, kOne = 0x3f80u;
+  static constexpr int kShift = 0;  // powers of two taken off 4-bit values
+  __device__ __forceinline__ static f32x4 mma16(bf16x8_t a, bf16x8_t b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  template <int SEL>
+  __device__ __forceinline__ static uint32_t fp4(uint32_t w, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL));
+  }
+};
+// fp16: 4-bit values are taken times 2^-2 and the scores and outputs times 2^2, so that a block
+// whose largest value rounds to 65536 (its fp16 source was at most 65504) stays finite. Values are
+// exact from 2^-22 to 2^17; below that the last bits of a block are lost, at most 2^-23 of a value.
+template <> struct Half<SB_DTYPE_F16> {
+  static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u;
+  static constexpr int kShift = 2;
+  __device__ __forceinline__ static f32x4 mma16(f16x8_t a, f16x8_t b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  template <int SEL>
+  __device__ __forceinline__ static uint32_t fp4(uint32_t w, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, SEL));
+  }
+};
+
+// The fp32 scale of a scale byte, for the conversions (which read the exponent field: 0 is 2^-127,
+// 255 makes every value NaN).
+template <int SHIFT>
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+  if constexpr (SHIFT > 0) byte = byte == 255 ? 255 : static_cast<uint32_t>(max(static_cast<int>(byte) - SHIFT, 0));
+  return __uint_as_float(byte << 23);
+}
+
+// 8 values (one word of codes) as packed 16-bit numbers.
+template <int DT>
+__device__ __forceinline__ u32x4_t fp4x8(uint32_t w, float scale) {
+  using H = Half<DT>;
+  const u32x4_t r = {H::template fp4<0>(w, scale), H::template fp4<1>(w, scale),
+                     H::template fp4<2>(w, scale), H::template fp4<3>(w, scale)};
+  return r;
+}
+
+// Whether one of the packed 16-bit values is infinite or NaN.
+template <int DT>
+__device__ __forceinline__ bool not_finite(u32x4_t v) {
+  constexpr uint32_t lo = Half<DT>::kExp, hi = lo << 16;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (v[i] & lo) == lo || (v[i] & hi) == hi;
+  return bad;
+}
+// The packed values where v is finite (0 elsewhere), and 1 where it is of one kind that is not.
+enum NotFinite { kNaN = 0, kPosInf = 1, kNegInf = 2 };
+template <int DT>
+__device__ __forceinline__ uint32_t finite_part(uint32_t w) {
+  constexpr uint32_t lo = Half<DT>::kExp, hi = lo << 16;
+  return w & (((w & lo) == lo ? 0u : 0xffffu) | ((w & hi) == hi ? 0u : 0xffff0000u));
+}
+template <int DT>
+__device__ __forceinline__ uint32_t indicator(uint32_t w, int kind) {
+  constexpr uint32_t e = Half<DT>::kExp, one = Half<DT>::kOne;
+  const uint32_t a = w & 0xffffu, b = w >> 16;
+  const uint32_t inf = kind == kPosInf ? e : e | 0x8000u;
+  const bool la = kind == kNaN ? (a & 0x7fffu) > e : a == inf;
+  const bool lb = kind == kNaN ? (b & 0x7fffu) > e : b == inf;
+  return (la ? one : 0u) | (lb ? one << 16 : 0u);
+}
+// acc += V^T P^T for a fragment v of a tile that some row sees only in part: a weight of zero
+// times an infinity or a NaN adds nothing.
+template <int DT, typename Acc, typename Vec8, typename Mma>
+__device__ __forceinline__ void mma_masked(u32x4_t v, Vec8 w, Acc& acc, Mma mma) {
+  if (!__any(not_finite<DT>(v))) {
+    acc = mma(__builtin_bit_cast(Vec8, v), w, acc);
+    return;
+  }
+  const u32x4_t fin = {finite_part<DT>(v[0]), finite_part<DT>(v[1]), finite_part<DT>(v[2]),
+                       finite_part<DT>(v[3])};
+  acc = mma(__builtin_bit_cast(Vec8, fin), w, acc);
+#pragma unroll 1
+  for (int kind = kNaN; kind <= kNegInf; ++kind) {
+    const u32x4_t ind = {indicator<DT>(v[0], kind), indicator<DT>(v[1], kind),
+                         indicator<DT>(v[2], kind), indicator<DT>(v[3], kind)};
+    const Acc n = mma(__builtin_bit_cast(Vec8, ind), w, Acc{});
+    const float x = kind == kNaN ? __builtin_nanf("") : kind == kPosInf ? INFINITY : -INFINITY;
+#pragma unroll
+    for (int e = 0; e < static_cast<int>(sizeof(Acc) / 4); ++e) acc[e] += n[e] > 0.f ? x : 0.f;
+  }
+}
+
+// The softmax state's reference of a row that has seen keys, but none with a score above -inf:
+// the sum of its weights is zero and its output NaN, as the formula's 0 / 0.
+constexpr float kSeenNothing = -3.0e38f;
+
+// ---------------------------------------------------------------------------------------
+// 16 flattened rows: one token's heads, or a few tokens'
+// ---------------------------------------------------------------------------------------
+
+// Joins the states of the workgroup's waves, which each hold (m, l, O) of the same 16 rows in
+// `area` ([wave][16][D + 4] fp32, then [wave][16][2] in ml), and writes the output rows or this
+// split's partials.
+template <int DT, int D, int WAVES>
+__device__ __forceinline__ void join_waves(const PagedArgs& a, const float* area, const float* ml,
+                                           const TileRef& t, int kvh, int tile_idx, int split,
+                                           int nsplit, float out_scale) {
+  constexpr int VPR = D / 4;  // float4 per row
+  for (int i = threadIdx.x; i < kDecodeRows * VPR; i += WAVES * 64) {
+    const int row = i / VPR, d = (i % VPR) * 4;
+    const int flat = t.tile * kDecodeRows + row;
+    if (flat >= t.rows * a.group) continue;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, ml[(w * kDecodeRows + row) * 2]);
+    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    if (m > -INFINITY) {
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const float mw = ml[(w * kDecodeRows + row) * 2];
+        if (mw == -INFINITY) continue;
+        const float f = __builtin_amdgcn_exp2f(mw - m);
+        l += f * ml[(w * kDecodeRows + row) * 2 + 1];
+        const float4 x = *reinterpret_cast<const float4*>(
+            area + (static_cast<size_t>(w) * kDecodeRows + row) * (D + 4) + d);
+        o[0] += f * x.x, o[1] += f * x.y, o[2] += f * x.z, o[3] += f * x.w;
+      }
+    }
+    const int pi = flat / a.group;
+    if (nsplit > 1) {
+      const int64_t slot =
+          ((static_cast<int64_t>(tile_idx) * a.num_kv_heads + kvh) * a.nsplit + split) *
+              kDecodeRows + row;
+      *reinterpret_cast<float4*>(a.part_o + slot * D + d) = make_float4(o[0], o[1], o[2], o[3]);
+      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(m, l);
+      continue;
+    }
+    if (a.positions[t.row0 + pi] < 0) continue;
+    const float inv = m == -INFINITY ? 0.f : out_scale / l;
+    char* op = a.o + (t.row0 + pi) * a.o_row + (kvh * a.group + flat - pi * a.group) * a.o_head;
+    if constexpr (DT == SB_DTYPE_F32) {
+      *reinterpret_cast<float4*>(op + d * 4) =
+          make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    } else {
+      const uint32_t w0 = Mma<DT>::cvt1(o[0] * inv) | Mma<DT>::cvt1(o[1] * inv) << 16;
+      const uint32_t w1 = Mma<DT>::cvt1(o[2] * inv) | Mma<DT>::cvt1(o[3] * inv) << 16;
+      *reinterpret_cast<uint2*>(op + d * 2) = make_uint2(w0, w1);
+    }
+  }
+}
+
+// The item of workgroup b (KV head fastest, then row tile, then split).
+struct DecodeItem {
+  int kvh, tile_idx, split;
+};
+__device__ __forceinline__ DecodeItem decode_item(const PagedArgs& a, int b) {
+  const int rest = b / a.num_kv_heads;
+  const int split = rest / a.num_tiles;
+  return {b - rest * a.num_kv_heads, rest - split * a.num_tiles, split};
+}
+
+template <int DT, int D, bool Q4>
+__global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_decode_kernel(const PagedArgs a) {
+  using M = Mma<DT>;
+  using H = Half<DT>;
+  using vec8 = typename M::vec8;
+  constexpr int KT = 32;             // keys of a wave's step: two MFMA key blocks
+  constexpr int NKS = D / 32;        // QK^T k-steps
+  constexpr int NDT = D / 16;        // output d-tiles
+  constexpr int CH = D / 8;          // 16-byte chunks of a V row in LDS
+  // V rows in LDS, 16-byte chunks XOR-swizzled by row: eight consecutive rows' 32-byte pieces of
+  // one column range fall on different banks. The same memory takes the waves' O at the end.
+  constexpr int kArea = kDecodeRows * (D + 4) * 4;
+  static_assert(kArea >= KT * D * 2, "O area covers the V stage");
+  __shared__ __align__(16) char lds[kDecodeWaves][kArea];
+  __shared__ float ml[kDecodeWaves][kDecodeRows][2];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lq = lane & 15, lg = lane >> 4;
+  const DecodeItem it = decode_item(a, blockIdx.x);
+  const TileRef t = find_tile<kDecodeRows>(a, it.tile_idx);
+  if (t.request < 0) return;
+  const int flat = t.tile * kDecodeRows + lq;
+  const bool valid = flat < t.rows * a.group;
+  const int pi = valid ? flat / a.group : 0;
+  const int p = valid ? a.positions[t.row0 + pi] : -1;
+  int pmin = p >= 0 ? p : 0x7fffffff, pmax = p;
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) {
+    pmin = min(pmin, __shfl_xor(pmin, o, 64));
+    pmax = max(pmax, __shfl_xor(pmax, o, 64));
+  }
+  pmin = __builtin_amdgcn_readfirstlane(pmin);
+  pmax = __builtin_amdgcn_readfirstlane(pmax);
+  if (pmax < 0) return;
+  const KeyTiles kt = key_tiles<KT>(a, pmin, pmax);
+  const int nsplit = split_count(a, kt.total);
+  if (it.split >= nsplit) return;
+  const int i1 = static_cast<int>(static_cast<int64_t>(kt.total) * (it.split + 1) / nsplit);
+  int i = static_cast<int>(static_cast<int64_t>(kt.total) * it.split / nsplit) + wave;
+
+  const int32_t* table = a.tables + t.request * a.table_stride;
+  const char* kbase = a.k + it.kvh * a.c_head;
+  const char* vbase = a.v + it.kvh * a.c_head;
+  const char* ksb = a.ks + it.kvh * a.s_head;
+  const char* vsb = a.vs + it.kvh * a.s_head;
+
+  // Query fragments (B operand). k-slot (step s, lane group lg, j) is dim 32 s + 8 lg + j over
+  // 16-bit pages, and dim lg D/4 + 8 s + j over 4-bit ones, where a lane reads D/4 values at once.
+  vec8 qf[NKS];
+  {
+    const char* qp = a.q + (t.row0 + pi) * a.q_row +
+                     (it.kvh * a.group + flat - pi * a.group) * a.q_head;
+#pragma unroll
+    for (int s = 0; s < NKS; ++s) {
+      vec8 v = {};
+      const int dim = Q4 ? lg * (D / 4) + 8 * s : 32 * s + 8 * lg;
+      if (p >= 0) v = *reinterpret_cast<const vec8*>(qp + dim * 2);
+      qf[s] = v;
+    }
+  }
+
+  // Registers of one step: the raw rows lq and lq + 16 of K and V, this lane's share of each.
+  constexpr int RAW = Q4 ? 1 : NKS;
+  using raw_t = std::conditional_t<Q4 && D == 64, u32x2_t, u32x4_t>;
+  struct Stage {
+    raw_t k[2][RAW], v[2][RAW];
+    uint32_t sk[2], sv[2];
+    int page[2];
+  };
+  auto lookup = [&](int idx, int* page) {
+    const int k0 = tile_key<KT>(kt, idx);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) page[h] = idx < i1 ? page_of(a, table, k0 + 16 * h + lq) : -1;
+  };
+  auto fetch = [&](int idx, Stage& st) {
+    const int k0 = tile_key<KT>(kt, idx);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = k0 + 16 * h + lq;
+      const int64_t off = row_offset(a, key, st.page[h], a.c_block, a.c_pos);
+#pragma unroll
+      for (int s = 0; s < RAW; ++s) {
+        const int64_t at = off + (Q4 ? lg * (D / 8) : 64 * s + 16 * lg);
+        st.k[h][s] = *reinterpret_cast<const raw_t*>(kbase + at);
+        st.v[h][s] = *reinterpret_cast<const raw_t*>(vbase + at);
+      }
+      if constexpr (Q4) {
+        const int64_t so = row_offset(a, key, st.page[h], a.s_block, a.s_pos) + lg * (D / 32) / 4;
+        st.sk[h] = static_cast<uint8_t>(ksb[so]);
+        st.sv[h] = static_cast<uint8_t>(vsb[so]);
+      }
+    }
+  };
+
+  float m_ref = -INFINITY, negm = 0.f, l_run = 0.f;
+  bool seen = false;
+  f32x4 o[NDT];
+#pragma unroll
+  for (int d = 0; d < NDT; ++d) o[d] = f32x4{};
+  const float c_log2 = Q4 ? a.scale_log2 * (1 << H::kShift) : a.scale_log2;
+  char* vst = lds[wave];
+  auto vchunk = [&](int row, int c) -> int {  // byte offset of chunk c of a row
+    const int x = CH >= 16 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
+    return row * (D * 2) + 16 * (c ^ x);
+  };
+
+  auto step = [&](int idx, const Stage& st) {
+    const int k0 = tile_key<KT>(kt, idx);
+    // V rows to LDS
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = 16 * h + lq;
+      if constexpr (Q4) {
+        const float sc = scale_of<H::kShift>(st.sv[h]);
+#pragma unroll
+        for (int s = 0; s < NKS; ++s)
+          *reinterpret_cast<u32x4_t*>(vst + vchunk(row, lg * NKS + s)) =
+              fp4x8<DT>(st.v[h][0][s], sc);
+      } else {
+#pragma unroll
+        for (int s = 0; s < NKS; ++s)
+          *reinterpret_cast<u32x4_t*>(vst + vchunk(row, 4 * s + lg)) = st.v[h][s];
+      }
+    }
+    // S^T = K Q^T: lane (lq, lg) gets row lq's scores of keys 16 h + 4 lg + 0..3
+    f32x4 sc[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      sc[h] = f32x4{};
+      const float ksc = Q4 ? scale_of<H::kShift>(st.sk[h]) : 0.f;
+#pragma unroll
+      for (int s = 0; s < NKS; ++s) {
+        u32x4_t w;
+        if constexpr (Q4) w = fp4x8<DT>(st.k[h][0][s], ksc);
+        else w = st.k[h][s];
+        sc[h] = H::mma16(__builtin_bit_cast(vec8, w), qf[s], sc[h]);
+      }
+    }
+    const uint32_t live = static_cast<uint32_t>(__ballot(st.page[0] >= 0) & 0xffffu) |
+                          static_cast<uint32_t>(__ballot(st.page[1] >= 0) & 0xffffu) << 16;
+    const bool whole = live == 0xffffffffu && k0 + KT - 1 <= pmin &&
+                       (k0 > pmax - a.window || k0 + KT - 1 < a.sinks);
+    if (whole) {
+      seen = true;
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 16 * h + 4 * lg + e;
+          const bool on = (live >> r & 1u) && sees(a, p, k0 + r);
+          seen |= on;
+          if (!on) sc[h][e] = -INFINITY;
+        }
+    }
+    float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                      fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+    // The reference moves only when a weight would pass 2^8: the row's largest score so far
+    // otherwise lies within 2^8 of it, which costs no accuracy in fp32 sums.
+    if (__any(__builtin_fmaf(c_log2, top, negm) > (m_ref == -INFINITY ? -INFINITY : 8.f))) {
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float x = c_log2 * top;
+      if (x > m_ref) {
+        const float f = m_ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref - x);
+        l_run *= f;
+#pragma unroll
+        for (int d = 0; d < NDT; ++d) o[d] *= f;
+        m_ref = x;
+        negm = -x;
+      }
+    }
+    float pf[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      pf[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(c_log2, sc[0][e], negm));
+      pf[4 + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(c_log2, sc[1][e], negm));
+    }
+    const vec8 pb = M::cvt8(pf);  // rounded weights, which the sum takes as well
+    l_run = M::sum8(pb, l_run);
+    // O^T += V^T P^T. Weight slot (lg, j) is key 4 lg + j, or 16 + 4 lg + j - 4: two transposing
+    // reads give lane (lq, lg) its column of those keys.
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int d = 0; d < NDT; ++d) {
+      u32x2_t w[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = 16 * h + 4 * lg + (lq >> 2), col = 16 * d + 4 * (lq & 3);
+        const char* src = vst + vchunk(row, col >> 3) + (col & 7) * 2;
+        w[h] = __builtin_bit_cast(u32x2_t,
+                                  __builtin_amdgcn_ds_read_tr16_b64_v4i16((SB_LDS s16x4_t*)src));
+      }
+      const u32x4_t v = {w[0].x, w[0].y, w[1].x, w[1].y};
+      if (whole) o[d] = H::mma16(__builtin_bit_cast(vec8, v), pb, o[d]);
+      else mma_masked<DT>(v, pb, o[d], H::mma16);
+    }
+    asm volatile("" ::: "memory");
+  };
+
+  // One step ahead in registers, the pages two ahead.
+  Stage st[2];
+  if (i < i1) {
+    lookup(i, st[0].page);
+    fetch(i, st[0]);
+    lookup(i + kDecodeWaves, st[1].page);
+  }
+  while (i < i1) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (i < i1) {
+        const int next = i + kDecodeWaves;
+        int page[2];
+        if (next < i1) {
+          fetch(next, st[u ^ 1]);
+          lookup(next + kDecodeWaves, page);
+        }
+        step(i, st[u]);
+        if (next < i1) {
+          st[u].page[0] = page[0];
+          st[u].page[1] = page[1];
+        }
+        i = next;
+      }
+    }
+  }
+
+  l_run += __shfl_xor(l_run, 16, 64);
+  l_run += __shfl_xor(l_run, 32, 64);
+  const int any_seen = static_cast<int>(seen) | __shfl_xor(static_cast<int>(seen), 16, 64);
+  const bool row_seen = (any_seen | __shfl_xor(any_seen, 32, 64)) != 0;
+  if (lg == 0) {
+    ml[wave][lq][0] = m_ref == -INFINITY && row_seen ? kSeenNothing : m_ref;
+    ml[wave][lq][1] = l_run;
+  }
+  float* area = reinterpret_cast<float*>(vst);
+#pragma unroll
+  for (int d = 0; d < NDT; ++d)
+    *reinterpret_cast<f32x4*>(area + lq * (D + 4) + 16 * d + 4 * lg) = o[d];
+  __syncthreads();
+  join_waves<DT, D, kDecodeWaves>(a, reinterpret_cast<const float*>(&lds[0][0]), &ml[0][0][0], t,
+                                  it.kvh, it.tile_idx, it.split, nsplit,
+                                  Q4 ? static_cast<float>(1 << H::kShift) : 1.f);
+}
+
+// fp32 pages: v_mfma_f32_16x16x4_f32, 16 keys a step. Lane (lq, lg) holds of K row lq the dims
+// 16 c + 4 lg + 0..3 of every c (one 16-byte load each; k-step (c, e) multiplies dim
+// 16 c + 4 lg + e), and of V rows 4 lg + s the dims 64 u + 4 lq + 0..3: element e of them is the A
+// operand of output tile (u, e), whose row m is dim 64 u + 4 m + e, so V needs no transposition.
+// Weight s of a lane is key 4 lg + s, as the scores leave it.
+template <int D>
+__global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const PagedArgs a) {
+  constexpr int KT = 16;
+  constexpr int NC = D / 16, NU = D / 64;
+  __shared__ __align__(16) float area[kDecodeWaves][kDecodeRows][D + 4];
+  __shared__ float ml[kDecodeWaves][kDecodeRows][2];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lq = lane & 15, lg = lane >> 4;
+  const DecodeItem it = decode_item(a, blockIdx.x);
+  const TileRef t = find_tile<kDecodeRows>(a, it.tile_idx);
+  if (t.request < 0) return;
+  const int flat = t.tile * kDecodeRows + lq;
+  const bool valid = flat < t.rows * a.group;
+  const int pi = valid ? flat / a.group : 0;
+  const int p = valid ? a.positions[t.row0 + pi] : -1;
+  int pmin = p >= 0 ? p : 0x7fffffff, pmax = p;
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) {
+    pmin = min(pmin, __shfl_xor(pmin, o, 64));
+    pmax = max(pmax, __shfl_xor(pmax, o, 64));
+  }
+  pmin = __builtin_amdgcn_readfirstlane(pmin);
+  pmax = __builtin_amdgcn_readfirstlane(pmax);
+  if (pmax < 0) return;
+  const KeyTiles kt = key_tiles<KT>(a, pmin, pmax);
+  const int nsplit = split_count(a, kt.total);
+  if (it.split >= nsplit) return;
+  const int i1 = static_cast<int>(static_cast<int64_t>(kt.total) * (it.split + 1) / nsplit);
+  int i = static_cast<int>(static_cast<int64_t>(kt.total) * it.split / nsplit) + wave;
+
+  const int32_t* table = a.tables + t.request * a.table_stride;
+  const char* kbase = a.k + it.kvh * a.c_head + 16 * lg;
+  const char* vbase = a.v + it.kvh * a.c_head + 16 * lq;
+  f32x4 qf[NC];
+  {
+    const char* qp = a.q + (t.row0 + pi) * a.q_row +
+                     (it.kvh * a.group + flat - pi * a.group) * a.q_head + 16 * lg;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      f32x4 v = {};
+      if (p >= 0) v = *reinterpret_cast<const f32x4*>(qp + 64 * c);
+      qf[c] = v;
+    }
+  }
+  struct Stage {
+    f32x4 k[NC];
+    int64_t off;
+    int page;
+  };
+  auto lookup = [&](int idx) -> int {
+    return idx < i1 ? page_of(a, table, tile_key<KT>(kt, idx) + lq) : -1;
+  };
+  auto fetch = [&](int idx, Stage& st) {
+    const int k0 = tile_key<KT>(kt, idx);
+    st.off = row_offset(a, k0 + lq, st.page, a.c_block, a.c_pos);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) st.k[c] = *reinterpret_cast<const f32x4*>(kbase + st.off + 64 * c);
+  };
+  float m_ref = -INFINITY, negm = 0.f, l_run = 0.f;
+  bool seen = false;
+  f32x4 o[NU][4];
+#pragma unroll
+  for (int u = 0; u < NU; ++u)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[u][e] = f32x4{};
+  const float c_hi = a.scale_log2, c_lo = a.scale_log2_lo;
+
+  auto step = [&](int idx, int next, const Stage& st, Stage& ahead) {
+    const int k0 = tile_key<KT>(kt, idx);
+    f32x4 v[4][NU];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {  // the offset of key 4 lg + x is lane 4 lg + x's
+      const int64_t vo = __shfl(st.off, 4 * lg + x, 64);
+#pragma unroll
+      for (int u = 0; u < NU; ++u) v[x][u] = *reinterpret_cast<const f32x4*>(vbase + vo + 256 * u);
+    }
+    if (next < i1) fetch(next, ahead);
+    f32x4 sc[2] = {f32x4{}, f32x4{}};  // two chains
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        sc[c & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(st.k[c][e], qf[c][e], sc[c & 1], 0, 0, 0);
+    f32x4 s = sc[0] + sc[1];
+    const uint32_t live = static_cast<uint32_t>(__ballot(st.page >= 0) & 0xffffu);
+    const bool whole = live == 0xffffu && k0 + KT - 1 <= pmin &&
+                       (k0 > pmax - a.window || k0 + KT - 1 < a.sinks);
+    if (whole) {
+      seen = true;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * lg + e;
+        const bool on = (live >> r & 1u) && sees(a, p, k0 + r);
+        seen |= on;
+        if (!on) s[e] = -INFINITY;
+      }
+    }
+    float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+    if (__any(__builtin_fmaf(c_hi, top, negm) > (m_ref == -INFINITY ? -INFINITY : 8.f))) {
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float x = c_hi * top;
+      if (x > m_ref) {
+        const float f = m_ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref - x);
+        l_run *= f;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[u][e] *= f;
+        m_ref = x;
+        negm = -x;
+      }
+    }
+    float w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // (scale * log2(e) in two parts: rounded alone it would be off by 2^-25 of the score)
+      w[e] = s[e] == -INFINITY
+                 ? 0.f
+                 : __builtin_amdgcn_exp2f(__builtin_fmaf(c_hi, s[e], __builtin_fmaf(c_lo, s[e], negm)));
+      l_run += w[e];
+    }
+    bool bad = false;
+    if (!whole) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bad |= !(fabsf(v[x][u][e]) < INFINITY);
+    }
+    if (__any(bad)) {  // as mma_masked does
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f32x4& acc = o[u][e];
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                fabsf(v[x][u][e]) < INFINITY ? v[x][u][e] : 0.f, w[x], acc, 0, 0, 0);
+#pragma unroll 1
+          for (int kind = kNaN; kind <= kNegInf; ++kind) {
+            const float inf = kind == kPosInf ? INFINITY : -INFINITY;
+            f32x4 n = {};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float y = v[x][u][e];
+              n = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                  (kind == kNaN ? y != y : y == inf) ? 1.f : 0.f, w[x], n, 0, 0, 0);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              acc[x] += n[x] > 0.f ? (kind == kNaN ? __builtin_nanf("") : inf) : 0.f;
+          }
+        }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[u][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[x][u][e], w[x], o[u][e], 0, 0, 0);
+    }
+  };
+
+  // K one step ahead in registers, the pages two; V is requested before the scores are formed.
+  Stage st[2];
+  if (i < i1) {
+    st[0].page = lookup(i);
+    fetch(i, st[0]);
+    st[1].page = lookup(i + kDecodeWaves);
+  }
+  while (i < i1) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (i < i1) {
+        const int next = i + kDecodeWaves;
+        const int page = lookup(next + kDecodeWaves);
+        step(i, next, st[u], st[u ^ 1]);
+        st[u].page = page;
+        i = next;
+      }
+    }
+  }
+  l_run += __shfl_xor(l_run, 16, 64);
+  l_run += __shfl_xor(l_run, 32, 64);
+  const int any_seen = static_cast<int>(seen) | __shfl_xor(static_cast<int>(seen), 16, 64);
+  const bool row_seen = (any_seen | __shfl_xor(any_seen, 32, 64)) != 0;
+  if (lg == 0) {
+    ml[wave][lq][0] = m_ref == -INFINITY && row_seen ? kSeenNothing : m_ref;
+    ml[wave][lq][1] = l_run;
+  }
+#pragma unroll
+  for (int u = 0; u < NU; ++u)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const f32x4 w = {o[u][0][x], o[u][1][x], o[u][2][x], o[u][3][x]};
+      *reinterpret_cast<f32x4*>(&area[wave][lq][64 * u + 16 * lg + 4 * x]) = w;
+    }
+  __syncthreads();
+  join_waves<SB_DTYPE_F32, D, kDecodeWaves>(a, &area[0][0][0], &ml[0][0][0], t, it.kvh,
+                                            it.tile_idx, it.split, nsplit, 1.f);
+}
+
+// ---------------------------------------------------------------------------------------
+// 256 flattened rows: prompt chunks
+// ---------------------------------------------------------------------------------------
+
+// One workgroup of 8 waves, 32 rows each; K and V tiles of 64 keys in two LDS stages, filled while
+// the stage before is multiplied: 16-bit rows by direct-to-LDS loads, 4-bit ones through registers
+// (fetched a tile ahead, converted and written behind the products of the tile before). S^T = K Q^T
+// and O^T += V^T P^T with v_mfma_f32_32x32x16 (a lane owns one row), V through transposing reads.
+template <int DT, int D, bool Q4>
+__global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const PagedArgs a) {
+  using M = Mma<DT>;
+  using H = Half<DT>;
+  using vec8 = typename M::vec8;
+  constexpr int KT = 64;
+  constexpr int THREADS = kRowsWaves * 64;
+  constexpr int NKS = D / 16, NDT = D / 32, CH = D / 8;
+  constexpr int NLD = KT * CH / THREADS;      // 16-byte loads per thread and plane
+  __shared__ __align__(16) uint16_t Ks[2][KT * D];
+  __shared__ __align__(16) uint16_t Vs[2][KT * D];
+  __shared__ int red[2][kRowsWaves];
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, lq = lane & 31, lg = lane >> 5;
+  const DecodeItem it = decode_item(a, blockIdx.x);
+  const TileRef t = find_tile<kRowsTile>(a, it.tile_idx);
+  if (t.request < 0) return;
+  const int flat = t.tile * kRowsTile + wave * 32 + lq;
+  const bool valid = flat < static_cast<int64_t>(t.rows) * a.group;
+  const int pi = valid ? flat / a.group : 0;
+  const int head = it.kvh * a.group + (valid ? flat - pi * a.group : 0);
+  const int p = valid ? a.positions[t.row0 + pi] : -1;
+  const int pmin = __builtin_amdgcn_readfirstlane(wave_min_i(p >= 0 ? p : 0x7fffffff));
+  const int pmax = __builtin_amdgcn_readfirstlane(wave_max_i(p));
+  if (lane == 0) {
+    red[0][wave] = pmin;
+    red[1][wave] = pmax;
+  }
+  __syncthreads();
+  int tmin = red[0][0], tmax = red[1][0];
+#pragma unroll
+  for (int w = 1; w < kRowsWaves; ++w) {
+    tmin = min(tmin, red[0][w]);
+    tmax = max(tmax, red[1][w]);
+  }
+  tmin = __builtin_amdgcn_readfirstlane(tmin);
+  tmax = __builtin_amdgcn_readfirstlane(tmax);
+  if (tmax < 0) return;  // uniform
+  const KeyTiles kt = key_tiles<KT>(a, tmin, tmax);
+  const int nsplit = split_count(a, kt.total);
+  if (it.split >= nsplit) return;  // uniform
+  const int i0 = static_cast<int>(static_cast<int64_t>(kt.total) * it.split / nsplit);
+  const int i1 = static_cast<int>(static_cast<int64_t>(kt.total) * (it.split + 1) / nsplit);
+
+  const int32_t* table = a.tables + t.request * a.table_stride;
+  const char* kbase = a.k + it.kvh * a.c_head;
+  const char* vbase = a.v + it.kvh * a.c_head;
+  const char* ksb = a.ks + it.kvh * a.s_head;
+  const char* vsb = a.vs + it.kvh * a.s_head;
+
+  vec8 qf[NKS];
+  {
+    const char* qp = a.q + (t.row0 + pi) * a.q_row + head * a.q_head;
+#pragma unroll
+    for (int s = 0; s < NKS; ++s) {
+      vec8 v = {};
+      if (p >= 0) v = *reinterpret_cast<const vec8*>(qp + (16 * s + 8 * lg) * 2);
+      qf[s] = v;
+    }
+  }
+
+  // 16-bit pages: load q of a plane fills LDS slots q * THREADS + tid: row q * (THREADS / CH) +
+  // tid / CH at chunk tid % CH, which holds the row's chunk that the swizzle puts there.
+  // 4-bit pages: thread tid converts D / 8 values of row tid / 8.
+  constexpr int PAGES = Q4 ? 1 : NLD;
+  constexpr int RPL = Q4 ? 0 : THREADS / CH;
+  const int my_row = Q4 ? tid / 8 : tid / CH;
+  struct Pages {
+    int at[PAGES];
+    int lane_key;  // page of key `lane` of the tile
+  };
+  auto lookup = [&](int idx) -> Pages {
+    Pages pg;
+    const int k0 = tile_key<KT>(kt, idx);
+#pragma unroll
+    for (int q = 0; q < PAGES; ++q) pg.at[q] = page_of(a, table, k0 + q * RPL + my_row);
+    pg.lane_key = page_of(a, table, k0 + lane);
+    return pg;
+  };
+  const uint32_t kpiece = 16 * kswz<CH>(tid / CH, tid % CH);
+  const uint32_t vpiece = 16 * vswz<CH>(tid / CH, tid % CH);
+  using code_t = std::conditional_t<D == 128, u32x2_t, uint32_t>;
+  struct Codes {
+    code_t k, v;
+    uint32_t sk, sv;
+  };
+  auto dma = [&](int idx, const Pages& pg, int stage) {
+    const int k0 = tile_key<KT>(kt, idx);
+#pragma unroll
+    for (int q = 0; q < PAGES; ++q) {
+      const int64_t off = row_offset(a, k0 + q * RPL + my_row, pg.at[q], a.c_block, a.c_pos);
+      const uint32_t dst = (q * THREADS + wave * 64) * 16;
+      dma_row_chunk(kbase + off + kpiece, lds_addr(Ks[stage]) + dst);
+      dma_row_chunk(vbase + off + vpiece, lds_addr(Vs[stage]) + dst);
+    }
+  };
+  auto fetch = [&](int idx, const Pages& pg, Codes& c) {
+    const int key = tile_key<KT>(kt, idx) + my_row;
+    const int64_t off = row_offset(a, key, pg.at[0], a.c_block, a.c_pos) + (tid & 7) * (D / 16);
+    const int64_t so = row_offset(a, key, pg.at[0], a.s_block, a.s_pos) + (tid & 7) * (D / 8) / 32;
+    c.k = *reinterpret_cast<const code_t*>(kbase + off);
+    c.v = *reinterpret_cast<const code_t*>(vbase + off);
+    c.sk = static_cast<uint8_t>(ksb[so]);
+    c.sv = static_cast<uint8_t>(vsb[so]);
+  };
+  auto unpack = [&](const Codes& c, int stage) {
+    const float sk = scale_of<H::kShift>(c.sk), sv = scale_of<H::kShift>(c.sv);
+    char* kd = reinterpret_cast<char*>(Ks[stage]) + my_row * (D * 2);
+    char* vd = reinterpret_cast<char*>(Vs[stage]) + my_row * (D * 2);
+    constexpr int NW = D / 64;  // words of 8 codes per thread and plane
+    uint32_t kw[NW], vw[NW];
+    __builtin_memcpy(kw, &c.k, 4 * NW);
+    __builtin_memcpy(vw, &c.v, 4 * NW);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const int ch = (tid & 7) * NW + w;
+      *reinterpret_cast<u32x4_t*>(kd + 16 * kswz<CH>(my_row, ch)) = fp4x8<DT>(kw[w], sk);
+      *reinterpret_cast<u32x4_t*>(vd + 16 * vswz<CH>(my_row, ch)) = fp4x8<DT>(vw[w], sv);
+    }
+  };
+
+  // K fragment (half j, step k): row 32 j + lq, chunk 2 k + lg. V^T fragment (d-tile d, step s,
+  // half j): keys 32 j + 16 s + {4 lg + 0..3, 8 + 4 lg + 0..3}, the order of the weights.
+  int kl[NKS], vl[NDT];
+#pragma unroll
+  for (int k = 0; k < NKS; ++k) kl[k] = lq * D * 2 + 16 * kswz<CH>(lq, 2 * k + lg);
+  const int grp = lane >> 4, gi = lane & 15;
+#pragma unroll
+  for (int d = 0; d < NDT; ++d) {
+    const int col = 32 * d + 16 * (grp & 1) + 4 * (gi & 3);
+    const int row = 4 * lg + (gi >> 2);
+    vl[d] = 2 * (row * D + 8 * vswz<CH>(row, col >> 3) + (col & 7));
+  }
+  auto kfrag = [&](int stage, int j, int k) -> vec8 {
+    return *reinterpret_cast<const vec8*>(reinterpret_cast<const char*>(Ks[stage]) +
+                                          j * (32 * D * 2) + kl[k]);
+  };
+  auto vfrag = [&](int stage, int d, int s, int j) -> u32x4_t {
+    u32x2_t h[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const char* src = reinterpret_cast<const char*>(Vs[stage]) +
+                        (32 * j + 16 * s + 8 * e) * (D * 2) + vl[d];
+      h[e] = __builtin_bit_cast(u32x2_t,
+                                __builtin_amdgcn_ds_read_tr16_b64_v4i16((SB_LDS s16x4_t*)src));
+    }
+    const u32x4_t w = {h[0].x, h[0].y, h[1].x, h[1].y};
+    return w;
+  };
+
+  const float c_log2 = Q4 ? a.scale_log2 * (1 << H::kShift) : a.scale_log2;
+  float m_ref = 0.f, negm = 0.f, l_run = 0.f;
+  bool seeded = p < 0, seen = false;
+  f32x16_t o[NDT];
+#pragma unroll
+  for (int d = 0; d < NDT; ++d) o[d] = f32x16_t{};
+
+  auto compute = [&](int idx, const Pages& pg, int stage) {
+    const int k0 = tile_key<KT>(kt, idx);
+    const uint64_t live = __ballot(pg.lane_key >= 0);
+    if (k0 > pmax || (k0 + KT - 1 <= pmin - a.window && k0 >= a.sinks)) return;  // no row sees it
+    const bool whole = live == ~0ull && k0 + KT - 1 <= pmin &&
+                       (k0 > pmax - a.window || k0 + KT - 1 < a.sinks);
+    f32x16_t sc[2];
+#pragma unroll
+    for (int k = 0; k < NKS; ++k)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        sc[j] = M::mma(kfrag(stage, j, k), qf[k], k == 0 ? f32x16_t{} : sc[j]);
+    if (whole) {
+      seen = true;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t lv = static_cast<uint32_t>(live >> (32 * j)) >> (4 * lg);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int r = 8 * (e >> 2) + (e & 3);
+          const bool on = (lv >> r & 1u) && sees(a, p, k0 + 32 * j + 4 * lg + r);
+          seen |= on;
+          if (!on) sc[j][e] = -INFINITY;
+        }
+      }
+    }
+    vec8 pb[2][2];
+    float tsum;
+    auto weights = [&]() {
+      float t = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            f[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(c_log2, sc[j][8 * s + e], negm));
+          pb[j][s] = M::cvt8(f);
+          t = M::sum8(pb[j][s], t);
+        }
+      tsum = t;
+    };
+    weights();
+    // The reference moves only where the sum of the (rounded) weights shows that it must, or at
+    // the row's first tile: no row maximum is formed otherwise.
+    const float pair = tsum + xor32(tsum);
+    const bool bad = !seeded || !(pair <= M::kPMax);
+    if (__any(bad)) {
+      float v = sc[0][0];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v = fmaxf(v, sc[j][e]);
+      const float mx = __builtin_fmaf(c_log2, fmaxf(v, xor32(v)), negm);
+      if (bad && mx != -INFINITY) {
+        const float f = seeded ? __builtin_amdgcn_exp2f(-mx) : 0.f;
+        l_run *= f;
+#pragma unroll
+        for (int d = 0; d < NDT; ++d) o[d] *= f;
+        m_ref += mx;
+        negm = -m_ref;
+        seeded = true;
+        weights();
+      }
+    }
+    l_run += tsum;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int d = 0; d < NDT; ++d) {
+          const u32x4_t v = vfrag(stage, d, s, j);
+          if (whole) o[d] = M::mma(__builtin_bit_cast(vec8, v), pb[j][s], o[d]);
+          else mma_masked<DT>(v, pb[j][s], o[d], M::mma);
+        }
+  };
+
+  Pages cur = lookup(i0), nxt = lookup(i0 + 1);
+  Codes codes;
+  if constexpr (Q4) {
+    fetch(i0, cur, codes);
+    unpack(codes, 0);
+  } else {
+    dma(i0, cur, 0);
+    wait_vmem();
+  }
+  __syncthreads();
+  for (int idx = i0; idx < i1; ++idx) {
+    const int stage = (idx - i0) & 1;
+    const bool more = idx + 1 < i1;
+    if (more) {
+      if constexpr (Q4) fetch(idx + 1, nxt, codes);
+      else dma(idx + 1, nxt, stage ^ 1);
+    }
+    const Pages after = lookup(idx + 2);
+    compute(idx, cur, stage);
+    if constexpr (Q4) {
+      if (more) unpack(codes, stage ^ 1);
+    } else {
+      wait_vmem();
+    }
+    __syncthreads();
+    cur = nxt;
+    nxt = after;
+  }
+
+  const float l_tot = l_run + xor32(l_run);
+  const int other_seen = __shfl_xor(static_cast<int>(seen), 32, 64);  // (by every lane)
+  const bool row_seen = seen || other_seen != 0;
+  if (p < 0) return;
+  if (nsplit > 1) {
+    const int64_t slot =
+        ((static_cast<int64_t>(it.tile_idx) * a.num_kv_heads + it.kvh) * a.nsplit + it.split) *
+            kRowsTile + wave * 32 + lq;
+    float* po = a.part_o + slot * D;
+#pragma unroll
+    for (int d = 0; d < NDT; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<float4*>(po + 32 * d + 8 * e + 4 * lg) =
+            make_float4(o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]);
+    if (lg == 0)
+      *reinterpret_cast<float2*>(a.part_ml + slot * 2) =
+          make_float2(seeded ? m_ref : row_seen ? kSeenNothing : -INFINITY, l_tot);
+    return;
+  }
+  const float out_scale = Q4 ? static_cast<float>(1 << H::kShift) : 1.f;
+  const float inv = !row_seen ? 0.f : out_scale / l_tot;
+  char* op = a.o + (t.row0 + pi) * a.o_row + head * a.o_head;
+#pragma unroll
+  for (int d = 0; d < NDT; ++d)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = o[d][8 * h + e] * inv;
+      const u32x4_t w = __builtin_bit_cast(u32x4_t, M::cvt8(f));
+      const int d0 = 32 * d + 16 * h + 4 * lg;
+      *reinterpret_cast<uint2*>(op + d0 * 2) = make_uint2(w.x, w.y);
+      *reinterpret_cast<uint2*>(op + (d0 + 8) * 2) = make_uint2(w.z, w.w);
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Joins the partials of row tiles whose keys were split: blockIdx.x = (tile, KV head), blockIdx.y
+// = which 16 rows of the tile.
+// ---------------------------------------------------------------------------------------
+constexpr int kMergeThreads = 256;
+template <int DT, int D, int TR, int KT>
+__global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedArgs a,
+                                                                   float out_scale) {
+  __shared__ int red[2][kMergeThreads / 64];
+  const int tile_idx = blockIdx.x / a.num_kv_heads;
+  const int kvh = blockIdx.x - tile_idx * a.num_kv_heads;
+  const TileRef t = find_tile<TR>(a, tile_idx);
+  if (t.request < 0) return;
+  const int nflat = static_cast<int>(
+      min(static_cast<int64_t>(t.rows) * a.group - static_cast<int64_t>(t.tile) * TR,
+          static_cast<int64_t>(TR)));
+  const int row_base = blockIdx.y * 16;
+  if (row_base >= nflat) return;
+  // the tile's key range, as the attention kernel saw it
+  int pmin = 0x7fffffff, pmax = -1;
+  static_assert(TR <= kMergeThreads, "one row per thread");
+  if (static_cast<int>(threadIdx.x) < nflat) {
+    const int p = a.positions[t.row0 + (t.tile * TR + static_cast<int>(threadIdx.x)) / a.group];
+    if (p >= 0) pmin = p;
+    pmax = p;
+  }
+  pmin = wave_min_i(pmin);
+  pmax = wave_max_i(pmax);
+  if ((threadIdx.x & 63) == 0) {
+    red[0][threadIdx.x >> 6] = pmin;
+    red[1][threadIdx.x >> 6] = pmax;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMergeThreads / 64; ++w) {
+    pmin = min(pmin, red[0][w]);
+    pmax = max(pmax, red[1][w]);
+  }
+  if (pmax < 0) return;
+  const int nsplit = split_count(a, key_tiles<KT>(a, pmin, pmax).total);
+  if (nsplit <= 1) return;
+  constexpr int VPR = D / 4;
+  for (int i = threadIdx.x; i < 16 * VPR; i += kMergeThreads) {
+    const int row = row_base + i / VPR, d = (i % VPR) * 4;
+    if (row >= nflat) continue;
+    const int flat = t.tile * TR + row;
+    const int pi = flat / a.group;
+    if (a.positions[t.row0 + pi] < 0) continue;
+    const int64_t slot0 =
+        ((static_cast<int64_t>(tile_idx) * a.num_kv_heads + kvh) * a.nsplit) * TR + row;
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int B = 8;  // splits in flight
+    for (int s0 = 0; s0 < nsplit; s0 += B) {
+      float2 ml[B];
+      float4 x[B];
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        const int64_t slot = slot0 + static_cast<int64_t>(min(s0 + b, nsplit - 1)) * TR;
+        ml[b] = *reinterpret_cast<const float2*>(a.part_ml + slot * 2);
+        x[b] = *reinterpret_cast<const float4*>(a.part_o + slot * D + d);
+      }
+      float mb = m;
+#pragma unroll
+      for (int b = 0; b < B; ++b) mb = fmaxf(mb, ml[b].x);
+      if (mb == -INFINITY) continue;
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mb);
+      l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        if (s0 + b >= nsplit || ml[b].x == -INFINITY) continue;
+        const float w = __builtin_amdgcn_exp2f(ml[b].x - mb);
+        l += w * ml[b].y;
+        o.x += w * x[b].x, o.y += w * x[b].y, o.z += w * x[b].z, o.w += w * x[b].w;
+      }
+      m = mb;
+    }
+    const float inv = m == -INFINITY ? 0.f : out_scale / l;
+    char* op = a.o + (t.row0 + pi) * a.o_row + (kvh * a.group + flat - pi * a.group) * a.o_head;
+    if constexpr (DT == SB_DTYPE_F32) {
+      *reinterpret_cast<float4*>(op + d * 4) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    } else {
+      const uint32_t w0 = Mma<DT>::cvt1(o.x * inv) | Mma<DT>::cvt1(o.y * inv) << 16;
+      const uint32_t w1 = Mma<DT>::cvt1(o.z * inv) | Mma<DT>::cvt1(o.w * inv) << 16;
+      *reinterpret_cast<uint2*>(op + d * 2) = make_uint2(w0, w1);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Any other head size (even, at most 512), alignment or scale: one wave per (row, query head).
+// ---------------------------------------------------------------------------------------
+constexpr int kValuMaxDim = 512;
+template <int DT>
+__device__ __forceinline__ float load16(const char* p, int i) {
+  if constexpr (DT == SB_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];
+  else if constexpr (DT == SB_DTYPE_F16) return f16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
+  else return bf16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]);
+}
+template <int DT, bool Q4>
+__device__ __forceinline__ float load_kv(const char* row, const char* scales, int i) {
+  if constexpr (Q4) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const uint32_t w = static_cast<uint8_t>(row[i >> 1]);
+    const float sc = scale_of<0>(static_cast<uint8_t>(scales[i >> 5]));
+    const f32x2 r = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, sc, 0);
+    return (i & 1) ? r.y : r.x;
+  } else {
+    return load16<DT>(row, i);
+  }
+}
+
+template <int DT, bool Q4>
+__global__ __launch_bounds__(64) void paged_valu_kernel(const PagedArgs a) {
+  constexpr int KT = 64;
+  constexpr int PER = kValuMaxDim / 64;
+  __shared__ float qs[kValuMaxDim];
+  __shared__ float ws[KT];
+  __shared__ int ps[KT];
+  const int lane = threadIdx.x;
+  const int hq = a.num_kv_heads * a.group;
+  const int row = blockIdx.x / hq, h = blockIdx.x - row * hq, kvh = h / a.group;
+  const int p = a.positions[row];
+  if (p < 0) return;
+  int request = a.num_requests == 1 ? 0 : row;
+  if (a.row_starts) {
+    if (row >= a.row_starts[a.num_requests]) return;
+    int lo = 0, hi = a.num_requests;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.row_starts[mid] <= row) lo = mid;
+      else hi = mid;
+    }
+    request = lo;
+    if (row < a.row_starts[lo]) return;
+  }
+  const int D = a.head_dim;
+  const char* qp = a.q + row * a.q_row + h * a.q_head;
+  for (int d = lane; d < D; d += 64) qs[d] = load16<DT>(qp, d);
+  __syncthreads();
+  const KeyTiles kt = key_tiles<KT>(a, p, p);
+  const int32_t* table = a.tables + request * a.table_stride;
+  const char* kbase = a.k + kvh * a.c_head;
+  const char* vbase = a.v + kvh * a.c_head;
+  const char* ksb = a.ks + kvh * a.s_head;
+  const char* vsb = a.vs + kvh * a.s_head;
+  float m = -INFINITY, l = 0.f, o[PER];
+  bool seen = false;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) o[i] = 0.f;
+  for (int idx = 0; idx < kt.total; ++idx) {
+    const int k0 = tile_key<KT>(kt, idx), key = k0 + lane;
+    const int pb = page_of(a, table, key);
+    const bool on = pb >= 0 && sees(a, p, key);
+    float s = -INFINITY;
+    if (on) {
+      const char* kr = kbase + row_offset(a, key, pb, a.c_block, a.c_pos);
+      const char* sr = Q4 ? ksb + row_offset(a, key, pb, a.s_block, a.s_pos) : nullptr;
+      float acc = 0.f;
+      for (int d = 0; d < D; ++d) acc = __builtin_fmaf(qs[d], load_kv<DT, Q4>(kr, sr, d), acc);
+      s = acc * a.scale;
+    }
+    seen |= __any(on) != 0;
+    const float mt = fmaxf(m, wave_max(s));
+    const float f = mt == -INFINITY || m == -INFINITY ? 0.f : expf(m - mt);
+    const float w = !on || (mt == -INFINITY) ? 0.f : expf(s - mt);
+    l = l * f + wave_sum(w);
+    m = mt;
+    __syncthreads();
+    ws[lane] = w;
+    ps[lane] = on ? pb : -1;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int d = lane + 64 * i;
+      if (d >= D) break;
+      float acc = o[i] * f;
+      for (int k = 0; k < KT; ++k) {
+        if (ps[k] < 0) continue;
+        const char* vr = vbase + row_offset(a, k0 + k, ps[k], a.c_block, a.c_pos);
+        const char* sr = Q4 ? vsb + row_offset(a, k0 + k, ps[k], a.s_block, a.s_pos) : nullptr;
+        acc = __builtin_fmaf(ws[k], load_kv<DT, Q4>(vr, sr, d), acc);
+      }
+      o[i] = acc;
+    }
+  }
+  char* op = a.o + row * a.o_row + h * a.o_head;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int d = lane + 64 * i;
+    if (d >= D) break;
+    const float r = seen ? o[i] / l : 0.f;
+    if constexpr (DT == SB_DTYPE_F32) reinterpret_cast<float*>(op)[d] = r;
+    else if constexpr (DT == SB_DTYPE_F16) reinterpret_cast<uint16_t*>(op)[d] = f32_to_f16(r);
+    else reinterpret_cast<uint16_t*>(op)[d] = f32_to_bf16(r);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Launch plan: which kernels a call takes, their tiles and splits, and the workspace.
+// ---------------------------------------------------------------------------------------
+struct PartPlan {  // one attention launch
+  bool on;
+  int64_t tiles;
+  int nsplit;
+  int64_t o_floats, ml_floats;
+};
+struct PagedPlan {
+  bool matrix;          // the matrix-core kernels (else the VALU kernel)
+  PartPlan few, rows;   // requests of few flattened rows, and the others
+  int few_max;          // flattened rows up to which a request takes the `few` kernel
+  int64_t bytes;
+};
+
+constexpr int kFewRows = 32;       // 16-bit arithmetic: two row tiles of 16
+constexpr int kFewMinTiles = 8;    // fewest 32-key tiles of a split (two per wave)
+constexpr int kF32MinTiles = 8;    // ... 16-key tiles, fp32
+constexpr int kRowsMinTiles = 4;   // ... 64-key tiles of the rows kernel
+
+int split_for(int64_t items, int64_t slots, int64_t tiles, int min_tiles) {
+  if (items >= slots) return 1;
+  const int64_t want = (slots + items - 1) / items;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, tiles / min_tiles, 128})));
+}
+
+PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_t max_rows,
+                     int64_t num_kv_heads, int64_t group, int64_t head_dim, int64_t kv_len,
+                     int64_t window, int64_t sinks, int32_t dtype, bool matrix) {
+  PagedPlan pl = {};
+  pl.matrix = matrix && (head_dim == 64 || head_dim == 128);
+  if (!pl.matrix) return pl;
+  const bool f32 = dtype == SB_DTYPE_F32;
+  const bool ragged = starts || num_requests == 1;  // else one row per request
+  // keys that a row may see, tables taken as full
+  const int64_t keys = std::min(kv_len, std::min<int64_t>(window, kv_len) + sinks + 64);
+  const int64_t per_few = (group + kDecodeRows - 1) / kDecodeRows;
+  const int64_t flat = num_rows * group;
+  pl.few_max = 0x7fffffff;
+  const bool rows_kernel = !f32 && ragged && max_rows * group > kFewRows;
+  if (rows_kernel) pl.few_max = kFewRows;
+  const int64_t tiles_bound = (flat + kDecodeRows - 1) / kDecodeRows + num_requests;
+  pl.few.on = !rows_kernel || num_requests > 1;
+  if (pl.few.on) {
+    // with both kernels a `few` request has two tiles at most
+    pl.few.tiles = !ragged ? num_rows * per_few
+                           : rows_kernel ? std::min<int64_t>(tiles_bound, 2 * num_requests)
+                                         : std::min<int64_t>(tiles_bound, flat);
+    const int kt = f32 ? 16 : 32;
+    pl.few.nsplit = split_for(pl.few.tiles * num_kv_heads, 1024, (keys + kt - 1) / kt,
+                              f32 ? kF32MinTiles : kFewMinTiles);
+    const int64_t slots = pl.few.nsplit > 1
+                              ? pl.few.tiles * num_kv_heads * pl.few.nsplit * kDecodeRows : 0;
+    pl.few.o_floats = slots * head_dim;
+    pl.few.ml_floats = slots * 2;
+  }
+  pl.rows.on = rows_kernel;
+  if (rows_kernel) {
+    if (num_requests == 1) pl.few_max = 0;
+    pl.rows.tiles = std::min<int64_t>(flat / kRowsTile + num_requests,
+                                      (flat + kFewRows - 1) / kFewRows);
+    pl.rows.nsplit = split_for(((flat + kRowsTile - 1) / kRowsTile) * num_kv_heads, 256,
+                               (keys + 63) / 64, kRowsMinTiles);
+    const int64_t slots = pl.rows.nsplit > 1
+                              ? pl.rows.tiles * num_kv_heads * pl.rows.nsplit * kRowsTile : 0;
+    pl.rows.o_floats = slots * head_dim;
+    pl.rows.ml_floats = slots * 2;
+  }
+  pl.bytes = 4 * (pl.few.o_floats + pl.few.ml_floats + pl.rows.o_floats + pl.rows.ml_floats);
+  return pl;
+}
+
+}  // namespace
+}  // namespace sb
+
+extern "C" int64_t sb_paged_attention_workspace_size(int64_t num_rows, int64_t num_requests,
+                                                     int32_t has_starts, int64_t max_rows,
+                                                     int64_t num_q_heads, int64_t num_kv_heads,
+                                                     int64_t head_dim, int64_t block_size,
+                                                     int64_t num_blocks_per_seq, int64_t window,
+                                                     int64_t sinks, int32_t dtype) {
+  using namespace sb;
+  if (num_rows <= 0 || num_requests <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
+      num_q_heads % num_kv_heads || block_size <= 0 || num_blocks_per_seq <= 0 || window < 0 ||
+      sinks < 0)
+    return 0;
+  const int64_t kv_len = std::min<int64_t>(block_size * num_blocks_per_seq, 0x7fff0000);
+  return plan_paged(num_rows, num_requests, has_starts != 0,
+                    max_rows > 0 && max_rows < num_rows ? max_rows : num_rows, num_kv_heads,
+                    num_q_heads / num_kv_heads, head_dim, kv_len,
+                    window > 0 ? window : kNoWindow, sinks, dtype, true)
+      .bytes;
+}
+
+extern "C" int sb_paged_attention(
+    void* out, const void* q, const void* kv_cache, const void* kv_scales,
+    const int32_t* block_tables, int64_t table_stride, const int32_t* positions,
+    const int32_t* row_starts, void* workspace, int64_t workspace_bytes, int64_t num_rows,
+    int64_t num_requests, int64_t max_rows, int64_t num_q_heads, int64_t num_kv_heads,
+    int64_t head_dim, int64_t block_size, int64_t num_blocks_total, int64_t num_blocks_per_seq,
+    int64_t window, int64_t sinks, float scale, const int64_t* q_strides,
+    const int64_t* o_strides, const int64_t* kv_strides, const int64_t* scale_strides,
+    int32_t dtype, int32_t cache_dtype, void* stream) {
+  using namespace sb;
+  const char* fn = "sb_paged_attention";
+  clear_error();
+  if (num_rows == 0) return SB_OK;
+  const int64_t es = elem_size(dtype);
+  if (!es) return fail(fn, "invalid dtype");
+  const bool q4 = cache_dtype == SB_DTYPE_MXFP4;
+  if (!q4 && cache_dtype != dtype) return fail(fn, "the cache's dtype is neither the query's nor MXFP4");
+  if (!out || !q || !kv_cache || !block_tables || !positions || !q_strides || !o_strides ||
+      !kv_strides || (q4 && (!kv_scales || !scale_strides)))
+    return fail(fn, "null pointer");
+  if (num_rows < 0 || num_requests <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      block_size <= 0 || num_blocks_total <= 0 || num_blocks_per_seq <= 0)
+    return fail(fn, "sizes must be positive");
+  if (num_q_heads % num_kv_heads) return fail(fn, "num_q_heads must be a multiple of num_kv_heads");
+  if (head_dim <= 0 || head_dim > kValuMaxDim || (q4 && head_dim % 32))
+    return fail(fn, "head_dim must be at most 512, and a multiple of 32 over 4-bit pages");
+  if (window < 0 || sinks < 0) return fail(fn, "window and sinks must not be negative");
+  if (!row_starts && num_requests > 1 && num_rows > num_requests)
+    return fail(fn, "without row_starts there is one row per request");
+  const int64_t group = num_q_heads / num_kv_heads;
+  if (num_rows * num_q_heads > 0x7fffffff - 0x10000 || num_requests > 0x3fffffff ||
+      num_blocks_total > 0x7fffffff || block_size > 0x7fffffff ||
+      num_blocks_per_seq > 0x7fffffff)
+    return fail(fn, "size past 32 bits");
+  if (q_strides[2] != 1 || o_strides[2] != 1 || kv_strides[4] != 1 ||
+      (q4 && scale_strides[4] != 1))
+    return fail(fn, "the last dimension must be contiguous");
+  const int64_t cs = q4 ? 1 : es;
+  if (kv_strides[0] < 0 || kv_strides[0] * cs > 0xffffffffll ||
+      (q4 && (scale_strides[0] < 0 || scale_strides[0] > 0xffffffffll)))
+    return fail(fn, "a page must be smaller than 4 GiB");
+
+  PagedArgs a = {};
+  a.q = static_cast<const char*>(q);
+  a.o = static_cast<char*>(out);
+  a.q_row = q_strides[0] * es, a.q_head = q_strides[1] * es;
+  a.o_row = o_strides[0] * es, a.o_head = o_strides[1] * es;
+  a.k = static_cast<const char*>(kv_cache);
+  a.v = a.k + kv_strides[1] * cs;
+  a.c_block = static_cast<uint32_t>(kv_strides[0] * cs);
+  a.c_head = kv_strides[2] * cs, a.c_pos = kv_strides[3] * cs;
+  if (q4) {
+    a.ks = static_cast<const char*>(kv_scales);
+    a.vs = a.ks + scale_strides[1];
+    a.s_block = static_cast<uint32_t>(scale_strides[0]);
+    a.s_head = scale_strides[2], a.s_pos = scale_strides[3];
+  }
+  a.tables = block_tables;
+  a.table_stride = table_stride;
+  a.positions = positions;
+  a.row_starts = row_starts;
+  a.num_rows = static_cast<int>(num_rows);
+  a.num_requests = static_cast<int>(num_requests);
+  a.num_kv_heads = static_cast<int>(num_kv_heads);
+  a.group = static_cast<int>(group);
+  a.head_dim = static_cast<int>(head_dim);
+  a.block_size = static_cast<int>(block_size);
+  a.bs_log2 = -1;
+  if ((block_size & (block_size - 1)) == 0) {
+    a.bs_log2 = 0;
+    while ((1ll << a.bs_log2) < block_size) ++a.bs_log2;
+  }
+  a.num_blocks_total = static_cast<int>(num_blocks_total);
+  a.kv_len = static_cast<int>(std::min<int64_t>(block_size * num_blocks_per_seq, 0x7fff0000));
+  a.window = window > 0 ? static_cast<int>(std::min<int64_t>(window, kNoWindow)) : kNoWindow;
+  a.sinks = static_cast<int>(std::min<int64_t>(sinks, a.kv_len));
+  a.scale = scale;
+  const double sl = static_cast<double>(scale) * 1.4426950408889634;
+  a.scale_log2 = static_cast<float>(sl);
+  a.scale_log2_lo = static_cast<float>(sl - static_cast<double>(a.scale_log2));
+
+  const auto addr = [](const void* p) { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)); };
+  const int64_t c0 = addr(kv_cache), cell = q4 ? head_dim / 8 : 16;
+  bool aligned = vec_bytes({addr(q), a.q_row, a.q_head}) == 16 &&
+                 vec_bytes({addr(out), a.o_row, a.o_head}) >= (es == 4 ? 16 : 8);
+  for (int64_t x : {c0, static_cast<int64_t>(a.c_block), kv_strides[1] * cs, a.c_head, a.c_pos})
+    aligned = aligned && x % cell == 0;
+  // (scales that 2^8 times a score's rounding could turn, and those of no sign, are the VALU's)
+  const bool matrix = aligned && !(dtype == SB_DTYPE_F32 && q4) && a.scale_log2 > 1e-37f &&
+                      a.scale_log2 < 1e30f;
+  const PagedPlan pl = plan_paged(num_rows, num_requests, row_starts != nullptr,
+                                  max_rows > 0 && max_rows < num_rows ? max_rows : num_rows,
+                                  num_kv_heads, group, head_dim, a.kv_len, a.window, a.sinks,
+                                  dtype, matrix);
+  if (pl.bytes > workspace_bytes || (pl.bytes && !workspace))
+    return fail(fn, "workspace too small");
+  if (workspace && addr(workspace) % 16) return fail(fn, "workspace must be 16-byte aligned");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+
+  if (!pl.matrix) {
+    const int64_t g = num_rows * num_q_heads;
+#define SB_VALU(DT)                                                                             \
+  if (dtype == DT) {                                                                            \
+    if (q4)                                                                                     \
+      SB_LAUNCH("paged_valu", (paged_valu_kernel<DT, true>), dim3(static_cast<unsigned>(g)),    \
+                dim3(64), st, a);                                                               \
+    else                                                                                        \
+      SB_LAUNCH("paged_valu", (paged_valu_kernel<DT, false>), dim3(static_cast<unsigned>(g)),   \
+                dim3(64), st, a);                                                               \
+  }
+    SB_VALU(SB_DTYPE_F32)
+    SB_VALU(SB_DTYPE_F16)
+    SB_VALU(SB_DTYPE_BF16)
+#undef SB_VALU
+    return check_launch(fn);
+  }
+
+  float* ws = static_cast<float*>(workspace);
+  const float out_scale = q4 && dtype == SB_DTYPE_F16 ? 4.f : 1.f;
+  const auto part = [&](const PartPlan& p, int min_tiles) {
+    PagedArgs b = a;
+    b.num_tiles = static_cast<int>(p.tiles);
+    b.nsplit = p.nsplit;
+    b.min_tiles = min_tiles;
+    b.part_o = ws;
+    b.part_ml = ws + p.o_floats;
+    ws += p.o_floats + p.ml_floats;
+    return b;
+  };
+#define SB_D(X)                     \
+  if (head_dim == 64) { X(64) }     \
+  else { X(128) }
+#define SB_MERGE(DT, D, TR, KT, B, P)                                                           \
+  if ((P).nsplit > 1) {                                                                         \
+    const dim3 mg(static_cast<unsigned>((P).tiles * num_kv_heads), TR / 16);                    \
+    SB_LAUNCH("paged_merge", (paged_merge_kernel<DT, D, TR, KT>), mg, dim3(kMergeThreads), st,  \
+              B, out_scale);                                                                    \
+  }
+  const int64_t most = 0x7fffffff;
+  if (pl.few.tiles * num_kv_heads * std::max(pl.few.nsplit, 1) > most ||
+      pl.rows.tiles * num_kv_heads * std::max(pl.rows.nsplit, 1) > most)
+    return fail(fn, "grid too large");
+  if (pl.rows.on) {
+    PagedArgs b = part(pl.rows, kRowsMinTiles);
+    b.flat_min = pl.few_max;
+    b.flat_max = 0x7fffffff;
+    const dim3 grid(static_cast<unsigned>(pl.rows.tiles * num_kv_heads * pl.rows.nsplit));
+#define SB_ROWS(DT, D)                                                                          \
+  {                                                                                             \
+    if (q4)                                                                                     \
+      SB_LAUNCH("paged_rows", (paged_rows_kernel<DT, D, true>), grid, dim3(kRowsWaves * 64), st, b); \
+    else                                                                                        \
+      SB_LAUNCH("paged_rows", (paged_rows_kernel<DT, D, false>), grid, dim3(kRowsWaves * 64), st, b); \
+    SB_MERGE(DT, D, kRowsTile, 64, b, pl.rows)                                                  \
+  }
+#define SB_ROWS_BF16(D) SB_ROWS(SB_DTYPE_BF16, D)
+#define SB_ROWS_F16(D) SB_ROWS(SB_DTYPE_F16, D)
+    if (dtype == SB_DTYPE_BF16) { SB_D(SB_ROWS_BF16) }
+    else { SB_D(SB_ROWS_F16) }
+  }
+  if (pl.few.on) {
+    PagedArgs b = part(pl.few, dtype == SB_DTYPE_F32 ? kF32MinTiles : kFewMinTiles);
+    b.flat_min = 0;
+    b.flat_max = pl.few_max;
+    const dim3 grid(static_cast<unsigned>(pl.few.tiles * num_kv_heads * pl.few.nsplit));
+    const dim3 block(kDecodeWaves * 64);
+#define SB_FEW(DT, D)                                                                           \
+  {                                                                                             \
+    if (q4) SB_LAUNCH("paged_decode", (paged_decode_kernel<DT, D, true>), grid, block, st, b);  \
+    else SB_LAUNCH("paged_decode", (paged_decode_kernel<DT, D, false>), grid, block, st, b);    \
+    SB_MERGE(DT, D, kDecodeRows, 32, b, pl.few)                                                 \
+  }
+#define SB_FEW_BF16(D) SB_FEW(SB_DTYPE_BF16, D)
+#define SB_FEW_F16(D) SB_FEW(SB_DTYPE_F16, D)
+#define SB_FEW_F32(D)                                                                           \
+  {                                                                                             \
+    SB_LAUNCH("paged_f32", (paged_f32_kernel<D>), grid, block, st, b);                          \
+    SB_MERGE(SB_DTYPE_F32, D, kDecodeRows, 16, b, pl.few)                                       \
+  }
+    if (dtype == SB_DTYPE_BF16) { SB_D(SB_FEW_BF16) }
+    else if (dtype == SB_DTYPE_F16) { SB_D(SB_FEW_F16) }
+    else { SB_D(SB_FEW_F32) }
+  }
+  return check_launch(fn);
+}

@@ -1,0 +1,344 @@
+"""A serving batch's operators over the paged K/V caches of this path: new tokens appended, their
+attention (single tokens, prompt chunks, sliding window with first tokens that stay visible), and
+4-bit pages.
+
+The reference reuses donor K/V for a prefill and leaves the decode steps behind it to its host
+engine (synapse_kv_connector/model_runner_hook.py:519-585 walks one request's layers); these are
+extensions with no reference counterpart, on the same caches, block tables and positions as
+``triton_kernels`` and ``rope_correction``:
+
+* :func:`append_kv_paged` — K and V of new tokens into their slots, K (and Q) rotated on the way;
+* :func:`paged_attention` — attention of a batch's rows over their pages;
+* :class:`QuantizedKVCache` — pages of MXFP4 (blocks of 32 4-bit values that share a power of
+  two), a cache of either function at 0.27 of the bytes of a 16-bit one;
+* :func:`gather_kv_paged` — a request's rows read back as a donor buffer
+  (``scatter_donor_kv_paged`` and ``rope_correct_scatter_paged`` take it; ``append_kv_paged`` with
+  ``rotations`` appends it to 4-bit pages).
+
+Batches: ``row_starts`` [num_requests + 1] (int32, on the device) says where each request's rows
+begin; without it row i is request i's only one, as in a decode step, or, with one request, all
+rows are that one's. Rows behind the last request and rows with a negative position are padding and
+left as they are. All metadata is read on the
+device, so a step can be captured into a HIP graph once and replayed with new positions.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+
+import torch
+
+from . import _lib
+from .rope_correction import inv_freq_table
+
+__all__ = ["QuantizedKVCache", "append_kv_paged", "gather_kv_paged", "paged_attention"]
+
+
+@functools.lru_cache(maxsize=1024)
+def _stride_array(strides: tuple[int, ...]):
+    """Host array of strides for the library, which only reads it (the same few layouts come back
+    in every call: building the array takes about a microsecond)."""
+    return (ctypes.c_int64 * len(strides))(*strides)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*sizes: int) -> int:
+    return _lib.size_query("sb_paged_attention_workspace_size", *sizes)
+
+
+class QuantizedKVCache:
+    """Paged K/V in MXFP4: ``codes`` [num_blocks, 2, num_kv_heads, block_size, head_dim / 2] uint8
+    (value 2i in the low half of byte i: sign, two exponent bits, one mantissa bit) and ``scales``
+    [num_blocks, 2, num_kv_heads, block_size, head_dim / 32] uint8 (e + 127: the 32 values are 2^e
+    times the 4-bit ones; 255: NaN). Any strides with unit last ones."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("codes and scales must be uint8")
+        if codes.dim() != 5 or codes.shape[1] != 2 or codes.shape[4] % 16:
+            raise ValueError("codes must be [num_blocks, 2, num_kv_heads, block_size, head_dim / 2] "
+                             "with a head_dim that is a multiple of 32")
+        if scales.shape != (*codes.shape[:4], codes.shape[4] // 16):
+            raise ValueError("scales must be [num_blocks, 2, num_kv_heads, block_size, "
+                             "head_dim / 32]")
+        if codes.stride(4) != 1 or scales.stride(4) != 1:
+            raise ValueError("codes and scales need unit last strides")
+        if codes.device != scales.device:
+            raise RuntimeError("codes and scales on different devices")
+        self.codes, self.scales = codes, scales
+        nb, _, heads, bs, half = codes.shape
+        self.shape = (nb, 2, heads, bs, 2 * half)
+        self.device = codes.device
+
+    @classmethod
+    def allocate(cls, num_blocks: int, num_kv_heads: int, block_size: int, head_dim: int,
+                 device) -> "QuantizedKVCache":
+        """An empty cache (every value 0)."""
+        if head_dim % 32:
+            raise ValueError("head_dim must be a multiple of 32")
+        shape = (num_blocks, 2, num_kv_heads, block_size)
+        return cls(torch.zeros((*shape, head_dim // 2), dtype=torch.uint8, device=device),
+                   torch.zeros((*shape, head_dim // 32), dtype=torch.uint8, device=device))
+
+
+def _cache_args(kv_cache, dtype: torch.dtype):
+    """(device, shape, base, scale base, strides, scale strides, dtype code) of either cache."""
+    if isinstance(kv_cache, QuantizedKVCache):
+        dev = _lib.require_device(kv_cache.codes, kv_cache.scales)
+        return (dev, kv_cache.shape, kv_cache.codes.data_ptr(), kv_cache.scales.data_ptr(),
+                _stride_array(kv_cache.codes.stride()),
+                _stride_array(kv_cache.scales.stride()), _lib.SB_DTYPE_MXFP4)
+    dev = _lib.require_device(kv_cache)
+    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2:
+        raise ValueError("kv_cache must be [num_blocks, 2, num_kv_heads, block_size, head_dim]")
+    if kv_cache.dtype != dtype:
+        raise TypeError("the rows and kv_cache must share a dtype (or kv_cache be a "
+                        "QuantizedKVCache)")
+    if kv_cache.stride(4) != 1:
+        raise ValueError("kv_cache needs a unit last stride")
+    return (dev, tuple(kv_cache.shape), kv_cache.data_ptr(), None, _stride_array(kv_cache.stride()), None,
+            _lib.dtype_code(kv_cache))
+
+
+def _batch_args(dev, num_rows: int, block_tables, positions, row_starts):
+    """(tables, positions, row_starts, number of requests) checked and on the device. A 1-D table
+    is one request's, and all rows are that request's."""
+    bt = block_tables
+    if not isinstance(bt, torch.Tensor):
+        bt = torch.as_tensor(bt, dtype=torch.int32)
+    if bt.dim() == 1:
+        if row_starts is not None:
+            raise ValueError("row_starts goes with block_tables [num_requests, max_blocks]")
+        bt = _lib.as_index(bt, dev).unsqueeze(0)
+    elif bt.dim() != 2:
+        raise ValueError("block_tables must be [num_requests, max_blocks], or [max_blocks] for "
+                         "one request")
+    elif bt.device != dev or bt.dtype != torch.int32 or (bt.shape[1] > 1 and bt.stride(1) != 1):
+        shape = bt.shape
+        bt = _lib.as_index(bt.reshape(-1), dev).view(shape)
+    pos = _lib.as_index(positions, dev)
+    if pos.shape[0] != num_rows:
+        raise ValueError("positions must have one entry per row")
+    requests = bt.shape[0]
+    if row_starts is not None:
+        row_starts = _lib.as_index(row_starts, dev)
+        if row_starts.shape[0] != requests + 1:
+            raise ValueError("row_starts must have num_requests + 1 entries")
+    elif num_rows > requests != 1:
+        raise ValueError("without row_starts there is one row per request: "
+                         f"{num_rows} rows, {requests} block tables")
+    if bt.shape[1] == 0 or requests == 0:
+        raise ValueError("block_tables is empty")
+    return bt, pos, row_starts, requests
+
+
+def _rows3(t: torch.Tensor, name: str, num_rows: int | None, head_dim: int) -> torch.Tensor:
+    if t.dim() != 3 or t.shape[2] != head_dim or (num_rows is not None and t.shape[0] != num_rows):
+        raise ValueError(f"{name} must be [rows, heads, head_dim], one row per token, with the "
+                         "cache's head_dim")
+    return t if t.stride(2) == 1 else t.contiguous()
+
+
+def append_kv_paged(
+    kv_cache,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    block_tables: torch.Tensor,
+    positions: torch.Tensor,
+    row_starts: torch.Tensor | None = None,
+    rope_base: float | None = None,
+    rotations: torch.Tensor | None = None,
+    query: torch.Tensor | None = None,
+    query_out: torch.Tensor | None = None,
+) -> torch.Tensor | None:
+    """K and V of new tokens into the cache slots of their positions, in one launch.
+
+    kv_cache: [num_blocks, 2, num_kv_heads, block_size, head_dim] of the keys' dtype, or a
+    :class:`QuantizedKVCache`; key / value: [T, num_kv_heads, head_dim] (bf16, fp16 or fp32, any
+    strides); block_tables: [num_requests, max_blocks], or [max_blocks] for one request;
+    positions: [T], each token's position in its request; row_starts: see the module.
+    With ``rope_base`` (at least 1), K is rotated by its position with the interleaved RoPE of
+    this path before its one rounding, and so is ``query`` [T, num_q_heads, head_dim], which goes
+    to ``query_out`` (a new tensor by default; returned). The angle is position * inv_freq with
+    the path's fp32 frequencies, the product and its sine and cosine in 64 bits.
+    ``rotations``: [T], the positions to rotate by instead (a donor's K, rotated already at d and
+    appended at t: t - d).
+    Tokens whose position has no page are not appended (their query is rotated still); padding
+    rows are left out altogether. Two tokens with one slot race: slots must be distinct.
+    Extension with no reference counterpart (``partial_prefill`` writes its new K/V into
+    contiguous caches, semblend_core/triton_kernels.py:904-909).
+    """
+    dev, shape, base, sbase, st, sst, code = _cache_args(kv_cache, key.dtype)
+    _lib.require_device(key, value, query, query_out, *_tensors(kv_cache))
+    _, _, heads, bs, d = shape
+    if value.dtype != key.dtype or (query is not None and query.dtype != key.dtype):
+        raise TypeError("key, value and query must share a dtype")
+    num = key.shape[0]
+    k, v = _rows3(key, "key", num, d), _rows3(value, "value", num, d)
+    if k.shape[1] != heads or v.shape[1] != heads:
+        raise ValueError("key and value must have the cache's heads")
+    if rope_base is None and (rotations is not None or query is not None):
+        raise ValueError("rotations and query go with rope_base")
+    if rope_base is not None and not rope_base >= 1.0:
+        raise ValueError("rope_base must be at least 1")
+    if d % 2:
+        raise ValueError("head_dim must be even")
+    q = None
+    if query is not None:
+        q = _rows3(query, "query", num, d)
+        if query_out is None:
+            query_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        elif query_out.shape != q.shape or query_out.dtype != q.dtype or query_out.stride(2) != 1:
+            raise ValueError("query_out must be like query, with a unit last stride")
+    elif query_out is not None:
+        raise ValueError("query_out goes with query")
+    if num == 0:
+        return query_out
+    bt, pos, starts, requests = _batch_args(dev, num, block_tables, positions, row_starts)
+    rot = None
+    if rotations is not None:
+        rot = _lib.as_index(rotations, dev)
+        if rot.shape[0] != num:
+            raise ValueError("rotations must have one entry per token")
+    inv = inv_freq_table(rope_base, d, dev) if rope_base is not None else None
+    with _lib.on_device(dev):
+        _lib.call(
+            "sb_append_kv_paged",
+            base, sbase, k.data_ptr(), v.data_ptr(), _lib.ptr(q),
+            None if q is None else query_out.data_ptr(), bt.data_ptr(), bt.stride(0),
+            pos.data_ptr(), _lib.ptr(rot), _lib.ptr(starts), _lib.ptr(inv), num, requests, heads,
+            0 if q is None else q.shape[1], d, bs, shape[0], bt.shape[1], _stride_array(k.stride()),
+            _stride_array(v.stride()), None if q is None else _stride_array(q.stride()),
+            None if q is None else _stride_array(query_out.stride()), st, sst, _lib.dtype_code(k), code,
+            _lib.stream_handle(dev),
+        )
+    return query_out
+
+
+def _tensors(kv_cache):
+    return ((kv_cache.codes, kv_cache.scales) if isinstance(kv_cache, QuantizedKVCache)
+            else (kv_cache,))
+
+
+def gather_kv_paged(
+    kv_cache,
+    block_table: torch.Tensor,
+    positions: torch.Tensor | None = None,
+    num_rows: int | None = None,
+    dtype: torch.dtype | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """A request's cache rows as a contiguous donor buffer [2, num_kv_heads, N, head_dim].
+
+    Row i is position ``positions[i]``, or position i of the first ``num_rows`` (default: all the
+    table names). dtype: the cache's own; for a :class:`QuantizedKVCache` bf16 (the default) and
+    fp32, which hold its values exactly, or fp16, rounded once. Positions without a page give
+    zeros. Extension with no reference counterpart (the reference's connectors copy donor rows
+    out of the cache with torch indexing, synapse_kv_connector/model_runner_hook.py:215-276).
+    """
+    quant = isinstance(kv_cache, QuantizedKVCache)
+    if dtype is None:
+        dtype = torch.bfloat16 if quant else kv_cache.dtype
+    dev, shape, base, sbase, st, sst, code = _cache_args(kv_cache, dtype)
+    _, _, heads, bs, d = shape
+    bt = _lib.as_index(block_table, dev)
+    pos = None
+    if positions is not None:
+        pos = _lib.as_index(positions, dev)
+        if num_rows is not None and num_rows != pos.shape[0]:
+            raise ValueError("num_rows and positions differ")
+        num_rows = pos.shape[0]
+    elif num_rows is None:
+        num_rows = bt.shape[0] * bs
+    if num_rows < 0:
+        raise ValueError("num_rows must not be negative")
+    if out is None:
+        out = torch.empty((2, heads, num_rows, d), dtype=dtype, device=dev)
+    elif (out.shape != (2, heads, num_rows, d) or out.dtype != dtype or out.device != dev
+          or out.stride(3) != 1):
+        raise ValueError("out must be [2, num_kv_heads, rows, head_dim] of dtype on the cache's "
+                         "device, with a unit last stride")
+    dt = _lib.dtype_code(out)
+    if num_rows == 0:
+        return out
+    if bt.shape[0] == 0:
+        return out.zero_()
+    with _lib.on_device(dev):
+        _lib.call("sb_gather_kv_paged", out.data_ptr(), base, sbase, bt.data_ptr(),
+                  _lib.ptr(pos), num_rows, heads, d, bs, shape[0], bt.shape[0],
+                  _stride_array(out.stride()), st, sst, dt, code, _lib.stream_handle(dev))
+    return out
+
+
+def paged_attention(
+    query: torch.Tensor,
+    kv_cache,
+    block_tables: torch.Tensor,
+    positions: torch.Tensor,
+    row_starts: torch.Tensor | None = None,
+    max_rows: int | None = None,
+    window: int | None = None,
+    sinks: int = 0,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """GQA attention of a batch's rows over their paged caches.
+
+    query: [R, num_q_heads, head_dim] (bf16, fp16 or fp32), row r the token at ``positions[r]`` of
+    its request; kv_cache: [num_blocks, 2, num_kv_heads, block_size, head_dim] of the query's
+    dtype (any strides), or a :class:`QuantizedKVCache`; block_tables: [num_requests,
+    max_blocks], or [max_blocks] for one request; row_starts: see the module. Query head h reads
+    KV head ``h // (num_q_heads // num_kv_heads)``; ``scale`` is 1 / sqrt(head_dim) by default.
+    Row r sees the keys j <= positions[r]; with ``window``, only those with
+    ``j > positions[r] - window`` or ``j < sinks``. Keys behind the block table, or in a page that
+    is none of the pool's (-1 for instance), are not seen; pages between the sinks and the window
+    are not read, and their entries may hold anything. What lies in keys that a row does not see
+    (NaN included) does not reach it. A row that sees no key gets zeros.
+    ``max_rows``: no request has more rows than this; it only helps to choose kernels (a decode
+    step of several rows a request runs as one launch fewer). Scores, sums and outputs are fp32,
+    rounded once; 16-bit calls round the weights to their dtype for the product with V.
+    Returns [R, num_q_heads, head_dim] (``out`` if given; padding rows of it are left as they
+    are). Extension with no reference counterpart: the reference's attention is MHA over
+    contiguous K/V (semblend_core/triton_kernels.py:655-734), without window.
+    """
+    if query.dim() != 3:
+        raise ValueError("query must be [rows, num_q_heads, head_dim]")
+    dev, shape, base, sbase, st, sst, code = _cache_args(kv_cache, query.dtype)
+    _lib.require_device(query, out, *_tensors(kv_cache))
+    num, hq, d = query.shape
+    nb, _, heads, bs, hd = shape
+    if hd != d:
+        raise ValueError("query and kv_cache head_dim differ")
+    if hq % heads:
+        raise ValueError("num_q_heads must be a multiple of num_kv_heads")
+    if window is not None and window < 1:
+        raise ValueError("window must be at least 1 (None: no window)")
+    if sinks < 0:
+        raise ValueError("sinks must not be negative")
+    q = query if query.stride(2) == 1 else query.contiguous()
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    if out is None:
+        out = torch.empty((num, hq, d), dtype=query.dtype, device=dev)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.stride(2) != 1:
+        raise ValueError("out must be like query, with a unit last stride")
+    dt = _lib.dtype_code(q)
+    if num == 0:
+        return out
+    bt, pos, starts, requests = _batch_args(dev, num, block_tables, positions, row_starts)
+    most = num if max_rows is None else max(1, int(max_rows))
+    win = 0 if window is None else min(int(window), 0x7fffffff)
+    ws_bytes = _workspace_bytes(num, requests, int(starts is not None), most, hq, heads, d, bs,
+                                bt.shape[1], win, int(sinks), dt)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    with _lib.on_device(dev):
+        _lib.call(
+            "sb_paged_attention",
+            out.data_ptr(), q.data_ptr(), base, sbase, bt.data_ptr(), bt.stride(0),
+            pos.data_ptr(), _lib.ptr(starts), _lib.ptr(ws), ws_bytes, num, requests, most, hq,
+            heads, d, bs, nb, bt.shape[1], win, int(sinks), float(scale), _stride_array(q.stride()),
+            _stride_array(out.stride()), st, sst, dt, code, _lib.stream_handle(dev),
+        )
+    return out
