@@ -39,6 +39,7 @@ constexpr int kDecodeRows = 16;
 constexpr int kDecodeWaves = 4;
 constexpr int kRowsTile = 256;
 constexpr int kRowsWaves = 8;
+constexpr int kAhead = 2;  // fragments read ahead of their MFMA (ring of 4)
 
 struct PagedArgs {
   const char* q;
@@ -56,7 +57,9 @@ struct PagedArgs {
   const int32_t* positions;
   const int32_t* row_starts;              // nullptr: row i is request i's, or the only one's
   int num_rows, num_requests, num_kv_heads, group, head_dim;
-  int block_size, bs_log2, num_blocks_total;
+  int block_size, num_blocks_total;
+  uint32_t bs_magic;                      // key / block_size = (key * bs_magic) >> bs_shift
+  int bs_shift;
   int kv_len;                             // keys that a block table can name
   int window, sinks;
   float scale, scale_log2, scale_log2_lo; // scale_log2_lo: what scale * log2(e) rounds off
@@ -153,17 +156,23 @@ __device__ __forceinline__ int split_count(const PagedArgs& a, int total) {
   return max(1, min(a.nsplit, total / a.min_tiles));
 }
 
+// Quotient of a key (31 bits) by the block size d: with l = ceil(log2 d) and m = ceil(2^(31+l) / d),
+// m d - 2^(31+l) < d <= 2^l, so key * m >> (31 + l) is exact for keys below 2^31 (T. Granlund and
+// P. Montgomery, "Division by invariant integers using multiplication", 1994).
+__device__ __forceinline__ int block_of(const PagedArgs& a, int key) {
+  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(key)) * a.bs_magic) >>
+                          a.bs_shift);
+}
 // Page of a key: its number in the pool, or -1 (outside the table, or no page of the pool).
 __device__ __forceinline__ int page_of(const PagedArgs& a, const int32_t* table, int key) {
   if (key >= a.kv_len) return -1;
-  const int lb = a.bs_log2 >= 0 ? key >> a.bs_log2 : key / a.block_size;
-  const int pb = table[lb];
+  const int pb = table[block_of(a, key)];
   return pb >= 0 && pb < a.num_blocks_total ? pb : -1;
 }
 // Byte offset of a key's row from its plane and head (page given; no page: page 0, masked later).
 __device__ __forceinline__ int64_t row_offset(const PagedArgs& a, int key, int pb, uint32_t s_block,
                                               int64_t s_pos) {
-  const int slot = a.bs_log2 >= 0 ? key & (a.block_size - 1) : key % a.block_size;
+  const int slot = key - block_of(a, key) * a.block_size;
   return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(max(pb, 0))) * s_block) +
          slot * s_pos;
 }
@@ -171,10 +180,20 @@ __device__ __forceinline__ bool sees(const PagedArgs& a, int p, int key) {
   return key <= p && (key > p - a.window || key < a.sinks);
 }
 
+// Bit r: a row at position p sees key k0 + r (0 <= r < 32), window, sinks and causality.
+__device__ __forceinline__ uint32_t bits_to(int m) {  // bits 0 .. m (none below 0)
+  return m < 0 ? 0u : m >= 31 ? ~0u : (2u << m) - 1u;
+}
+__device__ __forceinline__ uint32_t seen_bits(const PagedArgs& a, int p, int k0) {
+  const int d = max(p - k0, -1);  // (below 0 no key is seen; p >= -1, so nothing overflows)
+  return bits_to(d) & (~bits_to(d - a.window) | bits_to(a.sinks - k0 - 1));
+}
+
 template <int DT> struct Half;  // 16-bit arithmetic beyond Mma<DT>
 template <> struct Half<SB_DTYPE_BF16> {
   static constexpr uint32_t kExp = 0x7f80u, kOne = 0x3f80u;
   static constexpr int kShift = 0;  // powers of two taken off 4-bit values
+  __device__ __forceinline__ static float to_f32(uint32_t x) { return bf16_to_f32(x); }
   __device__ __forceinline__ static f32x4 mma16(bf16x8_t a, bf16x8_t b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -189,6 +208,7 @@ template <> struct Half<SB_DTYPE_BF16> {
 template <> struct Half<SB_DTYPE_F16> {
   static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u;
   static constexpr int kShift = 2;
+  __device__ __forceinline__ static float to_f32(uint32_t x) { return f16_to_f32(x); }
   __device__ __forceinline__ static f32x4 mma16(f16x8_t a, f16x8_t b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -215,15 +235,21 @@ __device__ __forceinline__ u32x4_t fp4x8(uint32_t w, float scale) {
   return r;
 }
 
-// Whether one of the packed 16-bit values is infinite or NaN.
+// Bits 15 and 31 of the result are set where a packed 16-bit value is infinite or NaN: adding one
+// to an exponent field of all ones carries into the sign bit's place, and never past it.
 template <int DT>
-__device__ __forceinline__ bool not_finite(u32x4_t v) {
-  constexpr uint32_t lo = Half<DT>::kExp, hi = lo << 16;
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= (v[i] & lo) == lo || (v[i] & hi) == hi;
-  return bad;
+__device__ __forceinline__ uint32_t not_finite_bits(uint32_t w) {
+  constexpr uint32_t e = Half<DT>::kExp | Half<DT>::kExp << 16;
+  constexpr uint32_t one = (0x8000u - Half<DT>::kExp) | (0x8000u - Half<DT>::kExp) << 16;
+  return (w & e) + one;
 }
+template <int DT>
+__device__ __forceinline__ uint32_t not_finite_bits(u32x4_t v) {
+  return not_finite_bits<DT>(v[0]) | not_finite_bits<DT>(v[1]) | not_finite_bits<DT>(v[2]) |
+         not_finite_bits<DT>(v[3]);
+}
+constexpr uint32_t kNotFinite = 0x80008000u;
+
 // The packed values where v is finite (0 elsewhere), and 1 where it is of one kind that is not.
 enum NotFinite { kNaN = 0, kPosInf = 1, kNegInf = 2 };
 template <int DT>
@@ -240,14 +266,10 @@ __device__ __forceinline__ uint32_t indicator(uint32_t w, int kind) {
   const bool lb = kind == kNaN ? (b & 0x7fffu) > e : b == inf;
   return (la ? one : 0u) | (lb ? one << 16 : 0u);
 }
-// acc += V^T P^T for a fragment v of a tile that some row sees only in part: a weight of zero
-// times an infinity or a NaN adds nothing.
+// acc += V^T P^T for a fragment v of a tile that some row sees only in part and that holds values
+// that are not finite: a weight of zero times one of those adds nothing.
 template <int DT, typename Acc, typename Vec8, typename Mma>
 __device__ __forceinline__ void mma_masked(u32x4_t v, Vec8 w, Acc& acc, Mma mma) {
-  if (!__any(not_finite<DT>(v))) {
-    acc = mma(__builtin_bit_cast(Vec8, v), w, acc);
-    return;
-  }
   const u32x4_t fin = {finite_part<DT>(v[0]), finite_part<DT>(v[1]), finite_part<DT>(v[2]),
                        finite_part<DT>(v[3])};
   acc = mma(__builtin_bit_cast(Vec8, fin), w, acc);
@@ -474,18 +496,27 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_decode_kernel(cons
                           static_cast<uint32_t>(__ballot(st.page[1] >= 0) & 0xffffu) << 16;
     const bool whole = live == 0xffffffffu && k0 + KT - 1 <= pmin &&
                        (k0 > pmax - a.window || k0 + KT - 1 < a.sinks);
+    bool odd = false;  // V holds values that are not finite, and some row sees the tile in part
     if (whole) {
       seen = true;
     } else {
+      const uint32_t on = (seen_bits(a, p, k0) & live) >> (4 * lg);
+      seen |= (on & 0x000f000fu) != 0;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 16 * h + 4 * lg + e;
-          const bool on = (live >> r & 1u) && sees(a, p, k0 + r);
-          seen |= on;
-          if (!on) sc[h][e] = -INFINITY;
-        }
+        for (int e = 0; e < 4; ++e)
+          if (!(on >> (16 * h + e) & 1u)) sc[h][e] = -INFINITY;
+      if constexpr (Q4) {
+        odd = __any(st.sv[0] == 255 || st.sv[1] == 255);
+      } else {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int s = 0; s < NKS; ++s) bits |= not_finite_bits<DT>(st.v[h][s]);
+        odd = __any((bits & kNotFinite) != 0);
+      }
     }
     float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                       fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
@@ -526,7 +557,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_decode_kernel(cons
                                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((SB_LDS s16x4_t*)src));
       }
       const u32x4_t v = {w[0].x, w[0].y, w[1].x, w[1].y};
-      if (whole) o[d] = H::mma16(__builtin_bit_cast(vec8, v), pb, o[d]);
+      if (!odd) o[d] = H::mma16(__builtin_bit_cast(vec8, v), pb, o[d]);
       else mma_masked<DT>(v, pb, o[d], H::mma16);
     }
     asm volatile("" ::: "memory");
@@ -673,13 +704,11 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
     if (whole) {
       seen = true;
     } else {
+      const uint32_t on = (seen_bits(a, p, k0) & live) >> (4 * lg);
+      seen |= (on & 15u) != 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 4 * lg + e;
-        const bool on = (live >> r & 1u) && sees(a, p, k0 + r);
-        seen |= on;
-        if (!on) s[e] = -INFINITY;
-      }
+      for (int e = 0; e < 4; ++e)
+        if (!(on >> e & 1u)) s[e] = -INFINITY;
     }
     float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
     if (__any(__builtin_fmaf(c_hi, top, negm) > (m_ref == -INFINITY ? -INFINITY : 8.f))) {
@@ -810,6 +839,7 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
   __shared__ __align__(16) uint16_t Ks[2][KT * D];
   __shared__ __align__(16) uint16_t Vs[2][KT * D];
   __shared__ int red[2][kRowsWaves];
+  __shared__ int odd_tiles[2];  // first and last tile that look_over took values out of
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -828,6 +858,7 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
     red[0][wave] = pmin;
     red[1][wave] = pmax;
   }
+  if (tid < 2) odd_tiles[tid] = tid ? -1 : 0x7fffffff;
   __syncthreads();
   int tmin = red[0][0], tmax = red[1][0];
 #pragma unroll
@@ -861,68 +892,107 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
     }
   }
 
+  // Byte offsets of the keys' rows, in a ring of tiles (K and V rows share one; 4-bit pages have a
+  // second for the scale bytes), and which keys have a page. One wave fills a tile's: it reads the
+  // block table one iteration and writes the offsets the next. 4-bit codes are fetched an iteration
+  // before they are written to LDS, so their offsets are needed one earlier.
+  constexpr int RING = Q4 ? 4 : 3;
+  __shared__ int64_t ofs[RING][KT];
+  __shared__ int64_t sofs[Q4 ? RING : 1][Q4 ? KT : 1];
+  __shared__ uint64_t paged[RING];
+  auto slot_at = [](int slot, int x) { return slot + x >= RING ? slot + x - RING : slot + x; };
+  const int n = i1 - i0;  // key tiles of this workgroup
+  auto key_of = [&](int i) { return tile_key<KT>(kt, i0 + i); };
+  auto fill = [&](int slot, int i, int key_in_tile, int page) {
+    const int key = key_of(i) + key_in_tile;
+    ofs[slot][key_in_tile] = row_offset(a, key, page, a.c_block, a.c_pos);
+    if constexpr (Q4) sofs[slot][key_in_tile] = row_offset(a, key, page, a.s_block, a.s_pos);
+    const uint64_t has = __ballot(page >= 0);
+    if (lane == 0) paged[slot] = has;
+  };
+  if (wave < RING) fill(wave, wave, lane, wave < n ? page_of(a, table, key_of(wave) + lane) : -1);
+  int ahead = -1;  // page of key `lane` of the tile that this wave fills next
+  if (n > RING && wave == (RING & 3)) ahead = page_of(a, table, key_of(RING) + lane);
+
   // 16-bit pages: load q of a plane fills LDS slots q * THREADS + tid: row q * (THREADS / CH) +
   // tid / CH at chunk tid % CH, which holds the row's chunk that the swizzle puts there.
-  // 4-bit pages: thread tid converts D / 8 values of row tid / 8.
-  constexpr int PAGES = Q4 ? 1 : NLD;
-  constexpr int RPL = Q4 ? 0 : THREADS / CH;
-  const int my_row = Q4 ? tid / 8 : tid / CH;
-  struct Pages {
-    int at[PAGES];
-    int lane_key;  // page of key `lane` of the tile
-  };
-  auto lookup = [&](int idx) -> Pages {
-    Pages pg;
-    const int k0 = tile_key<KT>(kt, idx);
+  const char* ksrc = kbase + 16 * kswz<CH>(tid / CH, tid % CH);
+  const char* vsrc = vbase + 16 * vswz<CH>(tid / CH, tid % CH);
+  auto read_ofs = [&](int slot, int64_t* ro) {
 #pragma unroll
-    for (int q = 0; q < PAGES; ++q) pg.at[q] = page_of(a, table, k0 + q * RPL + my_row);
-    pg.lane_key = page_of(a, table, k0 + lane);
-    return pg;
+    for (int q = 0; q < NLD; ++q) ro[q] = ofs[slot][q * (THREADS / CH) + tid / CH];
   };
-  const uint32_t kpiece = 16 * kswz<CH>(tid / CH, tid % CH);
-  const uint32_t vpiece = 16 * vswz<CH>(tid / CH, tid % CH);
-  using code_t = std::conditional_t<D == 128, u32x2_t, uint32_t>;
+  auto dma_dst = [&](uint16_t* dst, int q) -> uint32_t {
+    return lds_addr(dst) + (q * THREADS + wave * 64) * 16;
+  };
+  // 4-bit pages: thread tid converts D / 8 values of row tid / 8, read one tile ahead. (tid through
+  // an empty asm: its addresses are formed anew in each iteration rather than held in registers
+  // that the score block needs.)
+  int tid4 = tid;
+  constexpr int NW = D / 64;  // words of 8 codes
+  using code_t = std::conditional_t<NW == 2, u32x2_t, uint32_t>;
   struct Codes {
-    code_t k, v;
-    uint32_t sk, sv;
+    code_t w;
+    uint32_t scale;
   };
-  auto dma = [&](int idx, const Pages& pg, int stage) {
-    const int k0 = tile_key<KT>(kt, idx);
+  auto fetch = [&](const char* codes, const char* scales, int slot) -> Codes {
+    Codes c;
+    const int row = tid4 >> 3, part = tid4 & 7;
+    c.w = *reinterpret_cast<const code_t*>(codes + ofs[slot][row] + part * (4 * NW));
+    c.scale = static_cast<uint8_t>(scales[sofs[slot][row] + part * NW / 4]);
+    return c;
+  };
+  auto unpack = [&](const Codes& c, uint16_t* dst, auto is_v) {
+    const float sc = scale_of<H::kShift>(c.scale);
+    uint32_t w[NW];
+    __builtin_memcpy(w, &c.w, 4 * NW);
+    const int row = tid4 >> 3, part = tid4 & 7;
 #pragma unroll
-    for (int q = 0; q < PAGES; ++q) {
-      const int64_t off = row_offset(a, k0 + q * RPL + my_row, pg.at[q], a.c_block, a.c_pos);
-      const uint32_t dst = (q * THREADS + wave * 64) * 16;
-      dma_row_chunk(kbase + off + kpiece, lds_addr(Ks[stage]) + dst);
-      dma_row_chunk(vbase + off + vpiece, lds_addr(Vs[stage]) + dst);
+    for (int x = 0; x < NW; ++x) {
+      const int ch = part * NW + x;
+      const int at = decltype(is_v)::value ? vswz<CH>(row, ch) : kswz<CH>(row, ch);
+      *reinterpret_cast<u32x4_t*>(reinterpret_cast<char*>(dst) + row * (D * 2) + 16 * at) =
+          fp4x8<DT>(w[x], sc);
     }
   };
-  auto fetch = [&](int idx, const Pages& pg, Codes& c) {
-    const int key = tile_key<KT>(kt, idx) + my_row;
-    const int64_t off = row_offset(a, key, pg.at[0], a.c_block, a.c_pos) + (tid & 7) * (D / 16);
-    const int64_t so = row_offset(a, key, pg.at[0], a.s_block, a.s_pos) + (tid & 7) * (D / 8) / 32;
-    c.k = *reinterpret_cast<const code_t*>(kbase + off);
-    c.v = *reinterpret_cast<const code_t*>(vbase + off);
-    c.sk = static_cast<uint8_t>(ksb[so]);
-    c.sv = static_cast<uint8_t>(vsb[so]);
+  using IsV = std::true_type;
+  using IsK = std::false_type;
+
+  // Looks this thread's part of V of tile i over, if the tile is one that some row of the
+  // workgroup sees only in part (before the barrier that publishes the tile): values that are not
+  // finite are taken out of it, and the tile is noted for `put_back`.
+  auto in_part = [&](int k0, uint64_t has) -> bool {
+    return !(has == ~0ull && k0 + KT - 1 <= tmin &&
+             (k0 > tmax - a.window || k0 + KT - 1 < a.sinks));
   };
-  auto unpack = [&](const Codes& c, int stage) {
-    const float sk = scale_of<H::kShift>(c.sk), sv = scale_of<H::kShift>(c.sv);
-    char* kd = reinterpret_cast<char*>(Ks[stage]) + my_row * (D * 2);
-    char* vd = reinterpret_cast<char*>(Vs[stage]) + my_row * (D * 2);
-    constexpr int NW = D / 64;  // words of 8 codes per thread and plane
-    uint32_t kw[NW], vw[NW];
-    __builtin_memcpy(kw, &c.k, 4 * NW);
-    __builtin_memcpy(vw, &c.v, 4 * NW);
+  auto look_over = [&](int i, int slot, int stage, uint32_t scale) {
+    if (!in_part(key_of(i), paged[slot])) return;
+    bool odd = false;
+    if constexpr (Q4) {
+      odd = scale == 255;
+      if (odd) unpack(Codes{}, Vs[stage], IsV{});  // zeros
+    } else {
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const int ch = (tid & 7) * NW + w;
-      *reinterpret_cast<u32x4_t*>(kd + 16 * kswz<CH>(my_row, ch)) = fp4x8<DT>(kw[w], sk);
-      *reinterpret_cast<u32x4_t*>(vd + 16 * vswz<CH>(my_row, ch)) = fp4x8<DT>(vw[w], sv);
+      for (int q = 0; q < NLD; ++q) {
+        u32x4_t* at = reinterpret_cast<u32x4_t*>(reinterpret_cast<char*>(Vs[stage]) +
+                                                 (q * THREADS + tid) * 16);
+        const u32x4_t v = *at;
+        if ((not_finite_bits<DT>(v) & kNotFinite) == 0) continue;
+        odd = true;
+        const u32x4_t fin = {finite_part<DT>(v[0]), finite_part<DT>(v[1]), finite_part<DT>(v[2]),
+                             finite_part<DT>(v[3])};
+        *at = fin;
+      }
+    }
+    if (odd) {
+      atomicMin(&odd_tiles[0], i);
+      atomicMax(&odd_tiles[1], i);
     }
   };
 
   // K fragment (half j, step k): row 32 j + lq, chunk 2 k + lg. V^T fragment (d-tile d, step s,
-  // half j): keys 32 j + 16 s + {4 lg + 0..3, 8 + 4 lg + 0..3}, the order of the weights.
+  // half j): keys 32 j + 16 s + {4 lg + 0..3, 8 + 4 lg + 0..3}, the order of the weights. Both
+  // swizzles depend on the row modulo 16 at most: a lane's part of each address, and a constant.
   int kl[NKS], vl[NDT];
 #pragma unroll
   for (int k = 0; k < NKS; ++k) kl[k] = lq * D * 2 + 16 * kswz<CH>(lq, 2 * k + lg);
@@ -933,15 +1003,17 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
     const int row = 4 * lg + (gi >> 2);
     vl[d] = 2 * (row * D + 8 * vswz<CH>(row, col >> 3) + (col & 7));
   }
-  auto kfrag = [&](int stage, int j, int k) -> vec8 {
-    return *reinterpret_cast<const vec8*>(reinterpret_cast<const char*>(Ks[stage]) +
-                                          j * (32 * D * 2) + kl[k]);
+  auto kfrag = [&](int stage, int m) -> vec8 {  // m = 2 k + j
+    return *reinterpret_cast<const vec8*>(reinterpret_cast<const char*>(&Ks[0][0]) +
+                                          stage * (KT * D * 2) + (m & 1) * (32 * D * 2) +
+                                          kl[m >> 1]);
   };
-  auto vfrag = [&](int stage, int d, int s, int j) -> u32x4_t {
+  auto vfrag = [&](int stage, int m) -> u32x4_t {  // m = (2 j + s) NDT + d
+    const int d = m % NDT, s = (m / NDT) & 1, j = m / (2 * NDT);
     u32x2_t h[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const char* src = reinterpret_cast<const char*>(Vs[stage]) +
+      const char* src = reinterpret_cast<const char*>(&Vs[0][0]) + stage * (KT * D * 2) +
                         (32 * j + 16 * s + 8 * e) * (D * 2) + vl[d];
       h[e] = __builtin_bit_cast(u32x2_t,
                                 __builtin_amdgcn_ds_read_tr16_b64_v4i16((SB_LDS s16x4_t*)src));
@@ -956,62 +1028,167 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
   f32x16_t o[NDT];
 #pragma unroll
   for (int d = 0; d < NDT; ++d) o[d] = f32x16_t{};
+  using Scores = f32x16_t[2];
+  constexpr int NQ = 2 * NKS, NV = 4 * NDT;
 
-  auto compute = [&](int idx, const Pages& pg, int stage) {
-    const int k0 = tile_key<KT>(kt, idx);
-    const uint64_t live = __ballot(pg.lane_key >= 0);
-    if (k0 > pmax || (k0 + KT - 1 <= pmin - a.window && k0 >= a.sinks)) return;  // no row sees it
-    const bool whole = live == ~0ull && k0 + KT - 1 <= pmin &&
-                       (k0 > pmax - a.window || k0 + KT - 1 < a.sinks);
-    f32x16_t sc[2];
-#pragma unroll
-    for (int k = 0; k < NKS; ++k)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        sc[j] = M::mma(kfrag(stage, j, k), qf[k], k == 0 ? f32x16_t{} : sc[j]);
-    if (whole) {
+  // Whether every row of this wave sees all of tile i (then its scores are taken as they are).
+  auto whole = [&](int i, int slot) -> bool {
+    const int k0 = key_of(i);
+    return paged[slot] == ~0ull && k0 + KT - 1 <= pmin &&
+           (k0 > pmax - a.window || k0 + KT - 1 < a.sinks);
+  };
+  auto mask = [&](int i, int slot, Scores& sc) {
+    if (__builtin_amdgcn_readfirstlane(whole(i, slot))) {
       seen = true;
+      return;
+    }
+    const int k0 = key_of(i);
+    const uint64_t has = paged[slot];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t on =
+          (seen_bits(a, p, k0 + 32 * j) & static_cast<uint32_t>(has >> (32 * j))) >> (4 * lg);
+      seen |= (on & 0x0f0f0f0fu) != 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (!(on >> (8 * (e >> 2) + (e & 3)) & 1u)) sc[j][e] = -INFINITY;
+    }
+  };
+  vec8 pb[2][2];
+  float tsum = 0.f;
+  auto weights = [&](const Scores& sc) {
+    float t = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          f[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(c_log2, sc[j][8 * s + e], negm));
+        pb[j][s] = M::cvt8(f);
+        t = M::sum8(pb[j][s], t);
+      }
+    tsum = t;
+  };
+
+  // Iteration i: S(i + 1) = K Q^T on the matrix cores while the weights of tile i are formed from
+  // S(i), then O += V(i)^T P(i). K runs two tiles ahead of its use and V one, each in two LDS
+  // stages; one barrier per tile. The first block is laid out by hand, as attn_mfma_kernel's is:
+  // step m reads the K fragment of step m + kAhead, issues one MFMA, then fma, exp2 and packing of
+  // three successive weight pairs, so that no instruction waits for another of its own step; tile
+  // loads of 16-bit pages ride on the first steps.
+  Codes ck = {}, cv = {};  // of K(i + 2) and V(i + 1) at the top of iteration i
+  auto iteration = [&](int i, int slot, auto has_next, auto parity, auto swap, Scores& s_cur,
+                       Scores& s_nxt, auto full) {
+    constexpr bool NEXT = decltype(has_next)::value;
+    constexpr bool FULL = decltype(full)::value;  // both loads are due
+    constexpr int PAR = decltype(parity)::value;
+    const int par = PAR >= 0 ? PAR : (i & 1);
+    if (PAR >= 0) {
+      // (carried through an empty asm, so that the stage constants fold into the LDS offsets)
+#pragma unroll
+      for (int k = 0; k < NKS; ++k) asm volatile("" : "+v"(kl[k]));
+#pragma unroll
+      for (int d = 0; d < NDT; ++d) asm volatile("" : "+v"(vl[d]));
+    }
+    const int slot1 = slot_at(slot, 1), slot2 = slot_at(slot, 2);
+    int64_t ro_k[NLD], ro_v[NLD];
+    const bool k_due = FULL || i + 2 < n, v_due = FULL || i + 1 < n;
+    if constexpr (Q4) {
+      asm volatile("" : "+v"(tid4));
+      if (k_due) unpack(ck, Ks[par], IsK{});
+      if (v_due) {
+        unpack(cv, Vs[par ^ 1], IsV{});
+        look_over(i + 1, slot1, par ^ 1, cv.scale);
+      }
     } else {
+      if (k_due) read_ofs(slot2, ro_k);
+      if (v_due) read_ofs(slot1, ro_v);
+      if (!FULL) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t lv = static_cast<uint32_t>(live >> (32 * j)) >> (4 * lg);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int r = 8 * (e >> 2) + (e & 3);
-          const bool on = (lv >> r & 1u) && sees(a, p, k0 + 32 * j + 4 * lg + r);
-          seen |= on;
-          if (!on) sc[j][e] = -INFINITY;
+        for (int q = 0; q < NLD; ++q) {
+          if (k_due) dma_row_chunk(ksrc + ro_k[q], dma_dst(Ks[par], q));
+          if (v_due) dma_row_chunk(vsrc + ro_v[q], dma_dst(Vs[par ^ 1], q));
         }
       }
     }
-    vec8 pb[2][2];
-    float tsum;
-    auto weights = [&]() {
-      float t = 0.f;
+    if (i + RING < n && wave == ((i + RING) & 3)) fill(slot, i + RING, lane, ahead);
+    if (i + RING + 1 < n && wave == ((i + RING + 1) & 3))
+      ahead = page_of(a, table, key_of(i + RING + 1) + lane);
+
+    if (NEXT) {
+      constexpr int NPAIR = 16, PPS = NPAIR / NQ;  // weight pairs, and of them per step
+      static_assert(NPAIR % NQ == 0, "pairs split evenly over the steps");
+      vec8 ring[4];
+#pragma unroll
+      for (int m = 0; m < kAhead; ++m) ring[m] = kfrag(par ^ 1, m);
+      uint32_t pw[2][2][4];
+      float acc[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+      auto s_at = [&](int q, int e) -> float { return s_cur[q / 8][2 * (q % 8) + e]; };
+      auto pack = [&](int q, float e0, float e1) {
+        const auto pr = M::cvt2(e0, e1);
+        pw[q / 8][(q / 4) % 2][q % 4] = __builtin_bit_cast(uint32_t, pr);
+        acc[q / 8][(q / 4) % 2] = M::sum2(pr, acc[q / 8][(q / 4) % 2]);
+      };
+      float f0[NPAIR], f1[NPAIR], e0[NPAIR], e1[NPAIR];
+#pragma unroll
+      for (int q = 0; q < PPS; ++q) {
+        f0[q] = __builtin_fmaf(c_log2, s_at(q, 0), negm);
+        f1[q] = __builtin_fmaf(c_log2, s_at(q, 1), negm);
+      }
+      auto load_dst = [&](int m) -> uint32_t {
+        return m < NLD ? dma_dst(Ks[par], m) : dma_dst(Vs[par ^ 1], m - NLD);
+      };
+      if (!Q4 && FULL) dma_set_m0(load_dst(0));
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int m = 0; m < NQ; ++m) {
+        if (m + kAhead < NQ) ring[(m + kAhead) & 3] = kfrag(par ^ 1, m + kAhead);
+        s_nxt[m & 1] = M::mma(ring[m & 3], qf[m >> 1], m < 2 ? f32x16_t{} : s_nxt[m & 1]);
+        if (!Q4 && FULL) {
+          static_assert(2 * NLD <= NQ, "one load per step");
+          if (m < NLD) dma_at_m0(ksrc + ro_k[m]);
+          else if (m < 2 * NLD) dma_at_m0(vsrc + ro_v[m - NLD]);
+          if (m + 1 < 2 * NLD) dma_set_m0(load_dst(m + 1));
+        }
+#pragma unroll
+        for (int x = 0; x < PPS; ++x) {
+          const int q = m * PPS + x;
+          if (q + PPS < NPAIR) {
+            f0[q + PPS] = __builtin_fmaf(c_log2, s_at(q + PPS, 0), negm);
+            f1[q + PPS] = __builtin_fmaf(c_log2, s_at(q + PPS, 1), negm);
+          }
+          e0[q] = __builtin_amdgcn_exp2f(f0[q]);
+          e1[q] = __builtin_amdgcn_exp2f(f1[q]);
+          if (q >= PPS) pack(q - PPS, e0[q - PPS], e1[q - PPS]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int q = NPAIR - PPS; q < NPAIR; ++q) pack(q, e0[q], e1[q]);
+      tsum = (acc[0][0] + acc[0][1]) + (acc[1][0] + acc[1][1]);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          float f[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            f[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(c_log2, sc[j][8 * s + e], negm));
-          pb[j][s] = M::cvt8(f);
-          t = M::sum8(pb[j][s], t);
+          const u32x4_t w = {pw[j][s][0], pw[j][s][1], pw[j][s][2], pw[j][s][3]};
+          pb[j][s] = __builtin_bit_cast(vec8, w);
         }
-      tsum = t;
-    };
-    weights();
+    } else {
+      weights(s_cur);
+    }
     // The reference moves only where the sum of the (rounded) weights shows that it must, or at
     // the row's first tile: no row maximum is formed otherwise.
     const float pair = tsum + xor32(tsum);
     const bool bad = !seeded || !(pair <= M::kPMax);
+    if (NEXT) mask(i + 1, slot1, s_nxt);
     if (__any(bad)) {
-      float v = sc[0][0];
+      float v = s_cur[0][0];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v = fmaxf(v, sc[j][e]);
+        for (int e = 0; e < 16; ++e) v = fmaxf(v, s_cur[j][e]);
       const float mx = __builtin_fmaf(c_log2, fmaxf(v, xor32(v)), negm);
       if (bad && mx != -INFINITY) {
         const float f = seeded ? __builtin_amdgcn_exp2f(-mx) : 0.f;
@@ -1021,49 +1198,128 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
         m_ref += mx;
         negm = -m_ref;
         seeded = true;
-        weights();
+        weights(s_cur);
       }
     }
     l_run += tsum;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int d = 0; d < NDT; ++d) {
-          const u32x4_t v = vfrag(stage, d, s, j);
-          if (whole) o[d] = M::mma(__builtin_bit_cast(vec8, v), pb[j][s], o[d]);
-          else mma_masked<DT>(v, pb[j][s], o[d], M::mma);
-        }
-  };
-
-  Pages cur = lookup(i0), nxt = lookup(i0 + 1);
-  Codes codes;
-  if constexpr (Q4) {
-    fetch(i0, cur, codes);
-    unpack(codes, 0);
-  } else {
-    dma(i0, cur, 0);
-    wait_vmem();
-  }
-  __syncthreads();
-  for (int idx = i0; idx < i1; ++idx) {
-    const int stage = (idx - i0) & 1;
-    const bool more = idx + 1 < i1;
-    if (more) {
-      if constexpr (Q4) fetch(idx + 1, nxt, codes);
-      else dma(idx + 1, nxt, stage ^ 1);
+    if constexpr (Q4) {  // (behind the QK block, where registers are scarcest)
+      asm volatile("" : "+v"(tid4));
+      if (i + 3 < n) ck = fetch(kbase, ksb, slot_at(slot, 3));
+      if (i + 2 < n) cv = fetch(vbase, vsb, slot2);
     }
-    const Pages after = lookup(idx + 2);
-    compute(idx, cur, stage);
-    if constexpr (Q4) {
-      if (more) unpack(codes, stage ^ 1);
-    } else {
+    __builtin_amdgcn_s_setprio(1);
+    {
+      u32x4_t ring[4];
+#pragma unroll
+      for (int m = 0; m < kAhead; ++m) ring[m] = vfrag(par, m);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int m = 0; m < NV; ++m) {
+        if (m + kAhead < NV) ring[(m + kAhead) & 3] = vfrag(par, m + kAhead);
+        o[m % NDT] = M::mma(__builtin_bit_cast(vec8, ring[m & 3]),
+                            pb[m / (2 * NDT)][(m / NDT) & 1], o[m % NDT]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __builtin_amdgcn_s_setprio(0);
+    if (NEXT && !decltype(swap)::value) {
+      s_cur[0] = s_nxt[0];
+      s_cur[1] = s_nxt[1];
+    }
+    if constexpr (!Q4) {
       wait_vmem();
+      if (v_due) look_over(i + 1, slot1, par ^ 1, 0);
     }
     __syncthreads();
-    cur = nxt;
-    nxt = after;
+  };
+
+  __syncthreads();  // the first offsets
+  Scores s_a, s_b;
+  {
+    uint32_t scale = 0;
+    if constexpr (Q4) {
+      const Codes k_first = fetch(kbase, ksb, 0), v_first = fetch(vbase, vsb, 0);
+      Codes k_second = {};
+      if (n > 1) k_second = fetch(kbase, ksb, 1);
+      unpack(k_first, Ks[0], IsK{});
+      unpack(v_first, Vs[0], IsV{});
+      if (n > 1) unpack(k_second, Ks[1], IsK{});
+      scale = v_first.scale;
+      if (n > 2) ck = fetch(kbase, ksb, 2);
+      if (n > 1) cv = fetch(vbase, vsb, 1);
+    } else {
+      int64_t ro[2][NLD];
+      read_ofs(0, ro[0]);
+      read_ofs(1, ro[1]);
+#pragma unroll
+      for (int q = 0; q < NLD; ++q) {
+        dma_row_chunk(ksrc + ro[0][q], dma_dst(Ks[0], q));
+        dma_row_chunk(vsrc + ro[0][q], dma_dst(Vs[0], q));
+        if (n > 1) dma_row_chunk(ksrc + ro[1][q], dma_dst(Ks[1], q));
+      }
+      wait_vmem();
+    }
+    look_over(0, 0, 0, scale);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < NQ; ++m)
+    s_a[m & 1] = M::mma(kfrag(0, m), qf[m >> 1], m < 2 ? f32x16_t{} : s_a[m & 1]);
+  mask(0, 0, s_a);
+  __syncthreads();  // K stage 0 is refilled from here on
+
+  using P0 = std::integral_constant<int, 0>;
+  using P1 = std::integral_constant<int, 1>;
+  using PR = std::integral_constant<int, -1>;
+  using Yes = std::true_type;
+  using No = std::false_type;
+  auto next_slot = [&](int sl) { return slot_at(sl, 1); };
+  int i = 0, slot = 0;
+  for (; i + 3 < n; i += 2) {  // two tiles a trip: constant stages, score buffers in turn
+    iteration(i, slot, Yes{}, P0{}, Yes{}, s_a, s_b, Yes{});
+    slot = next_slot(slot);
+    iteration(i + 1, slot, Yes{}, P1{}, Yes{}, s_b, s_a, Yes{});
+    slot = next_slot(slot);
+  }
+  for (; i + 1 < n; ++i) {
+    iteration(i, slot, Yes{}, PR{}, No{}, s_a, s_b, No{});
+    slot = next_slot(slot);
+  }
+  iteration(i, slot, No{}, PR{}, No{}, s_a, s_b, No{});
+
+  // What look_over took out, added where it is seen: an infinity or a NaN of a seen key decides the
+  // sum, whatever (positive) weight it has.
+  for (int x = odd_tiles[0]; x <= odd_tiles[1]; ++x) {
+    const int k0 = key_of(x);
+    const uint64_t has = __ballot(page_of(a, table, k0 + lane) >= 0);
+    if (!in_part(k0, has)) continue;
+    for (int r = 0; r < KT; ++r) {
+      const int key = k0 + r;
+      const bool on = (has >> r & 1u) && sees(a, p, key);
+      if (!__any(on)) continue;
+      const int page = page_of(a, table, key);
+      const char* row = vbase + row_offset(a, key, page, a.c_block, a.c_pos);
+      if constexpr (Q4) {
+        const char* sr = vsb + row_offset(a, key, page, a.s_block, a.s_pos);
+#pragma unroll
+        for (int d = 0; d < NDT; ++d)
+          if (on && static_cast<uint8_t>(sr[d]) == 255) o[d] += __builtin_nanf("");
+      } else {
+#pragma unroll
+        for (int d = 0; d < NDT; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint2 w = *reinterpret_cast<const uint2*>(row + 2 * (32 * d + 8 * e + 4 * lg));
+            if (!on || ((not_finite_bits<DT>(w.x) | not_finite_bits<DT>(w.y)) & kNotFinite) == 0)
+              continue;
+            w.x &= ~finite_part<DT>(w.x), w.y &= ~finite_part<DT>(w.y);
+            o[d][4 * e] += H::to_f32(w.x & 0xffffu);
+            o[d][4 * e + 1] += H::to_f32(w.x >> 16);
+            o[d][4 * e + 2] += H::to_f32(w.y & 0xffffu);
+            o[d][4 * e + 3] += H::to_f32(w.y >> 16);
+          }
+      }
+    }
   }
 
   const float l_tot = l_run + xor32(l_run);
@@ -1322,10 +1578,19 @@ constexpr int kFewMinTiles = 8;    // fewest 32-key tiles of a split (two per wa
 constexpr int kF32MinTiles = 8;    // ... 16-key tiles, fp32
 constexpr int kRowsMinTiles = 4;   // ... 64-key tiles of the rows kernel
 
-int split_for(int64_t items, int64_t slots, int64_t tiles, int min_tiles) {
-  if (items >= slots) return 1;
-  const int64_t want = (slots + items - 1) / items;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, tiles / min_tiles, 128})));
+// Splits of each of `items` row tiles over `tiles` key tiles: those that a launch of `slots`
+// workgroups at a time takes the fewest rounds x (key tiles + a workgroup's fixed cost, in key
+// tiles) for, the partials' writes and their merge counted as `parts` key tiles of a round each.
+int split_for(int64_t items, int64_t slots, int64_t tiles, int min_tiles, int fixed, int parts) {
+  int64_t best = 1, cost = 0;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(tiles / min_tiles, 128));
+  for (int64_t n = 1; n <= most && items * (n - 1) < 2 * slots; ++n) {
+    const int64_t rounds = (items * n + slots - 1) / slots;
+    const int64_t c = rounds * ((tiles + n - 1) / n + fixed + (n > 1 ? parts : 0)) +
+                      (n > 1 ? 2 + items * n * parts / slots : 0);
+    if (n == 1 || c < cost) best = n, cost = c;
+  }
+  return static_cast<int>(best);
 }
 
 PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_t max_rows,
@@ -1352,7 +1617,7 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
                                          : std::min<int64_t>(tiles_bound, flat);
     const int kt = f32 ? 16 : 32;
     pl.few.nsplit = split_for(pl.few.tiles * num_kv_heads, 1024, (keys + kt - 1) / kt,
-                              f32 ? kF32MinTiles : kFewMinTiles);
+                              f32 ? kF32MinTiles : kFewMinTiles, 16, 2);
     const int64_t slots = pl.few.nsplit > 1
                               ? pl.few.tiles * num_kv_heads * pl.few.nsplit * kDecodeRows : 0;
     pl.few.o_floats = slots * head_dim;
@@ -1364,7 +1629,7 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
     pl.rows.tiles = std::min<int64_t>(flat / kRowsTile + num_requests,
                                       (flat + kFewRows - 1) / kFewRows);
     pl.rows.nsplit = split_for(((flat + kRowsTile - 1) / kRowsTile) * num_kv_heads, 256,
-                               (keys + 63) / 64, kRowsMinTiles);
+                               (keys + 63) / 64, kRowsMinTiles, 5, 3);
     const int64_t slots = pl.rows.nsplit > 1
                               ? pl.rows.tiles * num_kv_heads * pl.rows.nsplit * kRowsTile : 0;
     pl.rows.o_floats = slots * head_dim;
@@ -1463,11 +1728,10 @@ extern "C" int sb_paged_attention(
   a.group = static_cast<int>(group);
   a.head_dim = static_cast<int>(head_dim);
   a.block_size = static_cast<int>(block_size);
-  a.bs_log2 = -1;
-  if ((block_size & (block_size - 1)) == 0) {
-    a.bs_log2 = 0;
-    while ((1ll << a.bs_log2) < block_size) ++a.bs_log2;
-  }
+  int log2_up = 0;
+  while ((1ll << log2_up) < block_size) ++log2_up;
+  a.bs_shift = 31 + log2_up;
+  a.bs_magic = static_cast<uint32_t>(((1ull << a.bs_shift) + block_size - 1) / block_size);
   a.num_blocks_total = static_cast<int>(num_blocks_total);
   a.kv_len = static_cast<int>(std::min<int64_t>(block_size * num_blocks_per_seq, 0x7fff0000));
   a.window = window > 0 ? static_cast<int>(std::min<int64_t>(window, kNoWindow)) : kNoWindow;
