@@ -118,6 +118,11 @@ __device__ __forceinline__ float round_to_odd(double x) {
   return __uint_as_float(u);
 }
 
+// A thread takes vector tid % vpr of rows tid / vpr + k rpi (K, V, then query heads, token after
+// token), kRowsInFlight of them at a time. (Requesting the first ones before the positions, table
+// entries and sines are known was slower for prompts: 28.5 against 24.3 us for 4602 tokens of
+// 32 / 8 heads x 128; the workgroups' phases then overlap less.)
+constexpr int kRowsInFlight = 4;
 template <int DT, int VEC, bool Q4>
 __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendArgs a) {
   constexpr bool kWide64 = Q4 || DT == SB_DTYPE_F32;  // rotate in 64 bits
@@ -131,6 +136,30 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
   const int half = a.head_dim >> 1;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens_per_wg;
   const int ntok = static_cast<int>(min(static_cast<int64_t>(a.tokens_per_wg), a.num_tokens - t0));
+
+  const int vpr = a.head_dim / VEC;             // vectors per row (at most kAppendThreads)
+  const int rpi = kAppendThreads / vpr;         // rows per step of the workgroup
+  const int rsub = tid / vpr, vec = tid - rsub * vpr;
+  const int hk = a.num_kv_heads;
+  const int nrows = 2 * hk + a.num_q_heads;     // rows of a token
+  const int j0 = blockIdx.y * a.rows_per_y;     // (with several, a workgroup has one token)
+  const int j1 = min(j0 + a.rows_per_y, ntok * nrows);
+  RowVec<DT, VEC> x[kRowsInFlight];
+  auto fetch = [&](int jb) {
+#pragma unroll
+    for (int u = 0; u < kRowsInFlight; ++u) {
+      const int r = min(jb + u * rpi, j1 - 1);
+      const int tok = static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(nrows));
+      const int j = r - tok * nrows;
+      const int64_t t = t0 + tok;
+      const char* src = j < hk       ? a.k + t * a.k_tok + j * a.k_head
+                        : j < 2 * hk ? a.v + t * a.v_tok + (j - hk) * a.v_head
+                                     : a.q + t * a.q_tok + (j - 2 * hk) * a.q_head;
+      x[u].load(src + static_cast<int64_t>(vec) * VEC * ES);
+    }
+  };
+  const bool works = rsub < rpi && j0 + rsub < j1;
+
   if (tid < ntok) {
     const int64_t t = t0 + tid;
     const int p = a.positions[t];
@@ -156,8 +185,9 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
     tok_live[tid] = live;
   }
   if (a.inv_freq) {
+    // (from the last wave down: the first one looks the pages up)
     const int n = ntok * half;
-    for (int i = tid; i < n; i += kAppendThreads) {
+    for (int i = kAppendThreads - 1 - tid; i < n; i += kAppendThreads) {
       const int tok = i / half, f = i - tok * half;
       const int p = (a.rotations ? a.rotations : a.positions)[t0 + tok];
       double s, c;
@@ -167,103 +197,85 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
     }
   }
   __syncthreads();
+  if (!works) return;
 
-  const int vpr = a.head_dim / VEC;             // vectors per row (at most kAppendThreads)
-  const int rpi = kAppendThreads / vpr;         // rows per step of the workgroup
-  const int rsub = tid / vpr, vec = tid - rsub * vpr;
-  if (rsub >= rpi) return;
-  const int hk = a.num_kv_heads;
-  const int nrows = 2 * hk + a.num_q_heads;     // K, V, then the query heads
-  const int j0 = blockIdx.y * a.rows_per_y;
-  const int j1 = min(j0 + a.rows_per_y, nrows);
-  constexpr int U = 4;                          // rows in flight
-  for (int tok = 0; tok < ntok; ++tok) {
-    if (!tok_live[tok]) continue;
-    const int64_t t = t0 + tok;
-    const int64_t oc = tok_c[tok];
-    const CS* trig = cs + 2 * (tok * half + vec * (VEC / 2));
-    for (int jb = j0 + rsub; jb < j1; jb += U * rpi) {
-      RowVec<DT, VEC> x[U];
+  for (int jb = j0 + rsub; jb < j1; jb += kRowsInFlight * rpi) {
+    fetch(jb);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int j = jb + u * rpi;
-        if (j >= j1 || (j < 2 * hk && oc < 0)) continue;
-        const char* src = j < hk       ? a.k + t * a.k_tok + j * a.k_head
-                          : j < 2 * hk ? a.v + t * a.v_tok + (j - hk) * a.v_head
-                                       : a.q + t * a.q_tok + (j - 2 * hk) * a.q_head;
-        x[u].load(src + static_cast<int64_t>(vec) * VEC * ES);
-      }
+    for (int u = 0; u < kRowsInFlight; ++u) {
+      const int r = jb + u * rpi;
+      if (r >= j1) break;
+      const int tok = static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(nrows));
+      const int j = r - tok * nrows;
+      const int64_t t = t0 + tok, oc = tok_c[tok];
+      if (!tok_live[tok] || (j < 2 * hk && oc < 0)) continue;
+      const CS* trig = cs + 2 * (tok * half + vec * (VEC / 2));
+      const bool turn = a.inv_freq && (j < hk || j >= 2 * hk);
+      float f[VEC];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int j = jb + u * rpi;
-        if (j >= j1 || (j < 2 * hk && oc < 0)) continue;
-        const bool turn = a.inv_freq && (j < hk || j >= 2 * hk);
-        float f[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; i += 2) {
-          const CS e = Elem<DT>::get(x[u].e[i]), o = Elem<DT>::get(x[u].e[i + 1]);
-          if (turn) {
-            const CS c = trig[i], s = trig[i + 1];
-            const CS r0 = e * c - o * s, r1 = e * s + o * c;
-            if constexpr (Q4) {
-              // (a query is not quantised: its one rounding is from the 64-bit value)
-              f[i] = j < hk ? round_to_odd(r0) : static_cast<float>(r0);
-              f[i + 1] = j < hk ? round_to_odd(r1) : static_cast<float>(r1);
-            } else {
-              f[i] = static_cast<float>(r0);
-              f[i + 1] = static_cast<float>(r1);
-            }
+      for (int i = 0; i < VEC; i += 2) {
+        const CS e = Elem<DT>::get(x[u].e[i]), o = Elem<DT>::get(x[u].e[i + 1]);
+        if (turn) {
+          const CS c = trig[i], s = trig[i + 1];
+          const CS r0 = e * c - o * s, r1 = e * s + o * c;
+          if constexpr (Q4) {
+            // (a query is not quantised: its one rounding is from the 64-bit value)
+            f[i] = j < hk ? round_to_odd(r0) : static_cast<float>(r0);
+            f[i + 1] = j < hk ? round_to_odd(r1) : static_cast<float>(r1);
           } else {
-            f[i] = static_cast<float>(e);
-            f[i + 1] = static_cast<float>(o);
+            f[i] = static_cast<float>(r0);
+            f[i + 1] = static_cast<float>(r1);
           }
-        }
-        if (Q4 && j < 2 * hk) {
-          const int kv = j >= hk, h = j - kv * hk;
-          uint32_t top = 0;
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-#pragma unroll
-          for (int o = 16 / VEC; o >= 1; o >>= 1)  // the 32 / VEC lanes of the block
-            top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, 64)));
-          // top in [4, 8) * 2^(E - 2 - 127); one power more above 7 (mantissa above 1.75). A
-          // block that holds an infinity or a NaN is marked as one: scale byte 255.
-          const bool bad = top >= 0x7f800000u;
-          const int e = static_cast<int>(top >> 23) - 2 + ((top & 0x7fffffu) > 0x600000u);
-          const int sb = bad ? 255 : max(e, 0);
-          const float scale = __uint_as_float(sb > 0 && !bad ? static_cast<uint32_t>(sb) << 23
-                                                             : 0x00400000u);
-          uint32_t w = 0;
-          if (!bad) {
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[0], f[1], scale, 0);
-            if constexpr (VEC >= 4)
-              w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[2], f[3], scale, 1);
-            if constexpr (VEC >= 8) {
-              w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[4], f[5], scale, 2);
-              w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[6], f[7], scale, 3);
-            }
-          }
-          char* dst = a.cache + oc + kv * a.c_kv + h * a.c_head + vec * (VEC / 2);
-          if constexpr (VEC == 8) *reinterpret_cast<uint32_t*>(dst) = w;
-          else if constexpr (VEC == 4) *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(w);
-          else *reinterpret_cast<uint8_t*>(dst) = static_cast<uint8_t>(w);
-          if ((vec & (32 / VEC - 1)) == 0)
-            a.scales[tok_s[tok] + kv * a.s_kv + h * a.s_head + vec * VEC / 32] =
-                static_cast<char>(sb);
         } else {
-          if (turn) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) x[u].e[i] = Elem<DT>::put(f[i]);
-          }
-          char* dst;
-          if (j < 2 * hk) {
-            const int kv = j >= hk;
-            dst = a.cache + oc + kv * a.c_kv + (j - kv * hk) * a.c_head;
-          } else {
-            dst = a.q_out + t * a.qo_tok + (j - 2 * hk) * a.qo_head;
-          }
-          x[u].store(dst + static_cast<int64_t>(vec) * VEC * ES);
+          f[i] = static_cast<float>(e);
+          f[i + 1] = static_cast<float>(o);
         }
+      }
+      if (Q4 && j < 2 * hk) {
+        const int kv = j >= hk, h = j - kv * hk;
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 16 / VEC; o >= 1; o >>= 1)  // the 32 / VEC lanes of the block
+          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, 64)));
+        // top in [4, 8) * 2^(E - 2 - 127); one power more above 7 (mantissa above 1.75). A
+        // block that holds an infinity or a NaN is marked as one: scale byte 255.
+        const bool bad = top >= 0x7f800000u;
+        const int e = static_cast<int>(top >> 23) - 2 + ((top & 0x7fffffu) > 0x600000u);
+        const int sb = bad ? 255 : max(e, 0);
+        const float scale = __uint_as_float(sb > 0 && !bad ? static_cast<uint32_t>(sb) << 23
+                                                           : 0x00400000u);
+        uint32_t w = 0;
+        if (!bad) {
+          w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[0], f[1], scale, 0);
+          if constexpr (VEC >= 4)
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[2], f[3], scale, 1);
+          if constexpr (VEC >= 8) {
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[4], f[5], scale, 2);
+            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[6], f[7], scale, 3);
+          }
+        }
+        char* dst = a.cache + oc + kv * a.c_kv + h * a.c_head + vec * (VEC / 2);
+        if constexpr (VEC == 8) *reinterpret_cast<uint32_t*>(dst) = w;
+        else if constexpr (VEC == 4) *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(w);
+        else *reinterpret_cast<uint8_t*>(dst) = static_cast<uint8_t>(w);
+        if ((vec & (32 / VEC - 1)) == 0)
+          a.scales[tok_s[tok] + kv * a.s_kv + h * a.s_head + vec * VEC / 32] =
+              static_cast<char>(sb);
+      } else {
+        if (turn) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) x[u].e[i] = Elem<DT>::put(f[i]);
+        }
+        char* dst;
+        if (j < 2 * hk) {
+          const int kv = j >= hk;
+          dst = a.cache + oc + kv * a.c_kv + (j - kv * hk) * a.c_head;
+        } else {
+          dst = a.q_out + t * a.qo_tok + (j - 2 * hk) * a.qo_head;
+        }
+        x[u].store(dst + static_cast<int64_t>(vec) * VEC * ES);
       }
     }
   }
@@ -459,20 +471,22 @@ extern "C" int sb_append_kv_paged(
     if (x % cell) vb = 2;
   const bool wide = vb == 16;
   const int vec = wide ? static_cast<int>(16 / es) : 2;
-  // Tokens per workgroup: one while that leaves workgroups for every CU, else as many as the
-  // table of sines and cosines takes (up to four), so that its latency is paid once for them.
-  const int fit = std::max<int>(1, kTableEntries / (a.head_dim / 2));
-  a.tokens_per_wg = num_tokens >= 2048 ? std::min(4, fit) : 1;
-  const int64_t gx = (num_tokens + a.tokens_per_wg - 1) / a.tokens_per_wg;
+  // Tokens per workgroup: as many as fill its threads' first rows in flight (and the table of sines
+  // and cosines takes). Few tokens: one, and its rows spread over workgroups until there are 512
+  // (each repeats the sines and cosines).
   const int nrows = 2 * a.num_kv_heads + a.num_q_heads;
   const int rpi = kAppendThreads / (a.head_dim / vec);
-  // Few tokens: their rows spread over more workgroups (each repeats the sines and cosines).
-  const int64_t want = std::max<int64_t>(1, 512 / gx);
-  const int steps = (nrows + rpi - 1) / rpi;
-  const int ny = static_cast<int>(std::min<int64_t>(want, steps));
+  const int fit = std::min(kTokensMax, std::max(1, kTableEntries / (a.head_dim / 2)));
+  const int full = std::max(1, std::min(fit, kRowsInFlight * rpi / nrows));
+  a.tokens_per_wg = num_tokens >= 512 * static_cast<int64_t>(full) ? full : 1;
+  const int64_t gx = (num_tokens + a.tokens_per_wg - 1) / a.tokens_per_wg;
+  const int all = a.tokens_per_wg * nrows;
+  const int steps = (all + rpi - 1) / rpi;
+  const int ny = a.tokens_per_wg > 1
+                     ? 1 : static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, 512 / gx), steps));
   a.rows_per_y = (steps + ny - 1) / ny * rpi;
   const dim3 grid(static_cast<unsigned>(gx),
-                  static_cast<unsigned>((nrows + a.rows_per_y - 1) / a.rows_per_y));
+                  static_cast<unsigned>((all + a.rows_per_y - 1) / a.rows_per_y));
   const hipStream_t st = static_cast<hipStream_t>(stream);
 #define SB_APPEND(DT, VEC)                                                                      \
   if (dtype == DT && vec == VEC) {                                                              \
@@ -548,9 +562,9 @@ extern "C" int sb_gather_kv_paged(void* out, const void* kv_cache, const void* k
   const int64_t gx = (num_rows * (head_dim / vec) + kGatherThreads - 1) / kGatherThreads;
   if (gx > 0x7fffffff) return fail(fn, "grid too large");
   const int planes = 2 * a.num_kv_heads;
+  // Up to eight rows a thread behind one lookup, fewer until there are 2048 workgroups.
   const int64_t want = std::max<int64_t>(1, 2048 / gx);
-  const int ny = static_cast<int>(std::min<int64_t>(want, planes));
-  a.planes_per_y = (planes + ny - 1) / ny;
+  a.planes_per_y = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, planes / want)));
   const dim3 grid(static_cast<unsigned>(gx),
                   static_cast<unsigned>((planes + a.planes_per_y - 1) / a.planes_per_y));
   const hipStream_t st = static_cast<hipStream_t>(stream);

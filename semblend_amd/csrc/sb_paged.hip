@@ -37,6 +37,12 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kNoWindow = 0x7fffffff;
 constexpr int kDecodeRows = 16;
 constexpr int kDecodeWaves = 4;
+constexpr int kFewSlots = 512;     // workgroups of the decode kernels at a time (two per CU)
+constexpr int kFewTarget = 1536;   // balanced items of a launch
+constexpr int kFewMinTiles = 8;    // fewest key tiles of an item (two per wave)
+constexpr int kShortItem = 24;     // key tiles of an item up to which one round is cut
+constexpr int64_t kLongTiles = 256;
+constexpr int kDecodeAhead4 = 1;  // steps of 4-bit rows in flight per wave
 constexpr int kRowsTile = 256;
 constexpr int kRowsWaves = 8;
 constexpr int kAhead = 2;  // fragments read ahead of their MFMA (ring of 4)
@@ -66,6 +72,8 @@ struct PagedArgs {
   int flat_min, flat_max;                 // flattened rows of the requests this launch takes
   int num_tiles;                          // row tiles of the launch (bound)
   int nsplit, min_tiles;                  // key splits of a row tile; fewest key tiles of one
+  int target;                             // > 0: items of about 1 / target of all key tiles (one
+                                          // row per request), instead of nsplit per row tile
   float* part_o;                          // [tile][kv head][split][row][D]
   float* part_ml;                         // [tile][kv head][split][row][2]
 };
@@ -250,38 +258,27 @@ __device__ __forceinline__ uint32_t not_finite_bits(u32x4_t v) {
 }
 constexpr uint32_t kNotFinite = 0x80008000u;
 
-// The packed values where v is finite (0 elsewhere), and 1 where it is of one kind that is not.
-enum NotFinite { kNaN = 0, kPosInf = 1, kNegInf = 2 };
+// The packed values where they are finite, 0 elsewhere.
 template <int DT>
 __device__ __forceinline__ uint32_t finite_part(uint32_t w) {
   constexpr uint32_t lo = Half<DT>::kExp, hi = lo << 16;
   return w & (((w & lo) == lo ? 0u : 0xffffu) | ((w & hi) == hi ? 0u : 0xffff0000u));
 }
 template <int DT>
-__device__ __forceinline__ uint32_t indicator(uint32_t w, int kind) {
-  constexpr uint32_t e = Half<DT>::kExp, one = Half<DT>::kOne;
-  const uint32_t a = w & 0xffffu, b = w >> 16;
-  const uint32_t inf = kind == kPosInf ? e : e | 0x8000u;
-  const bool la = kind == kNaN ? (a & 0x7fffu) > e : a == inf;
-  const bool lb = kind == kNaN ? (b & 0x7fffu) > e : b == inf;
-  return (la ? one : 0u) | (lb ? one << 16 : 0u);
+__device__ __forceinline__ u32x4_t finite_part(u32x4_t v) {
+  const u32x4_t r = {finite_part<DT>(v[0]), finite_part<DT>(v[1]), finite_part<DT>(v[2]),
+                     finite_part<DT>(v[3])};
+  return r;
 }
-// acc += V^T P^T for a fragment v of a tile that some row sees only in part and that holds values
-// that are not finite: a weight of zero times one of those adds nothing.
-template <int DT, typename Acc, typename Vec8, typename Mma>
-__device__ __forceinline__ void mma_masked(u32x4_t v, Vec8 w, Acc& acc, Mma mma) {
-  const u32x4_t fin = {finite_part<DT>(v[0]), finite_part<DT>(v[1]), finite_part<DT>(v[2]),
-                       finite_part<DT>(v[3])};
-  acc = mma(__builtin_bit_cast(Vec8, fin), w, acc);
-#pragma unroll 1
-  for (int kind = kNaN; kind <= kNegInf; ++kind) {
-    const u32x4_t ind = {indicator<DT>(v[0], kind), indicator<DT>(v[1], kind),
-                         indicator<DT>(v[2], kind), indicator<DT>(v[3], kind)};
-    const Acc n = mma(__builtin_bit_cast(Vec8, ind), w, Acc{});
-    const float x = kind == kNaN ? __builtin_nanf("") : kind == kPosInf ? INFINITY : -INFINITY;
-#pragma unroll
-    for (int e = 0; e < static_cast<int>(sizeof(Acc) / 4); ++e) acc[e] += n[e] > 0.f ? x : 0.f;
-  }
+// acc[0..3] += the four packed values that are not finite.
+template <int DT, typename Acc>
+__device__ __forceinline__ void add_not_finite(uint2 w, Acc& acc, int e) {
+  if (((not_finite_bits<DT>(w.x) | not_finite_bits<DT>(w.y)) & kNotFinite) == 0) return;
+  w.x &= ~finite_part<DT>(w.x), w.y &= ~finite_part<DT>(w.y);
+  acc[e] += Half<DT>::to_f32(w.x & 0xffffu);
+  acc[e + 1] += Half<DT>::to_f32(w.x >> 16);
+  acc[e + 2] += Half<DT>::to_f32(w.y & 0xffffu);
+  acc[e + 3] += Half<DT>::to_f32(w.y >> 16);
 }
 
 // The softmax state's reference of a row that has seen keys, but none with a score above -inf:
@@ -292,14 +289,104 @@ constexpr float kSeenNothing = -3.0e38f;
 // 16 flattened rows: one token's heads, or a few tokens'
 // ---------------------------------------------------------------------------------------
 
+// Work item of a workgroup: one KV head, a row tile, and which of its nsplit key splits; its partials
+// are at rows slot * (rows of a tile) of the workspace.
+struct Item {
+  int kvh, nsplit, split;
+  int64_t slot;
+  TileRef t;
+};
+
+// Items of even splits: every row tile has its keys split nsplit ways (fewer if they are few); KV
+// head fastest, then row tile, then split. (nsplit is filled in once the tile's positions are read.)
+template <int TR>
+__device__ __forceinline__ Item even_item(const PagedArgs& a, int b) {
+  const int rest = b / a.num_kv_heads, split = rest / a.num_tiles;
+  const int tile_idx = rest - split * a.num_tiles, kvh = b - rest * a.num_kv_heads;
+  return {kvh, 1, split,
+          (static_cast<int64_t>(tile_idx) * a.num_kv_heads + kvh) * a.nsplit + split,
+          find_tile<TR>(a, tile_idx)};
+}
+
+// Items of one row per request, whose lengths may differ widely: all requests' key tiles together
+// are cut into items of about 1 / target of them, so a long request has many and a short one has
+// one. `c` counts the items of a KV head; with `merge`, it counts the row tiles, and the item
+// returned is the row tile's first. Every wave goes through all positions (a load and two lane
+// scans for 64 requests).
+template <int KT>
+__device__ __forceinline__ Item balanced_item(const PagedArgs& a, int c, int kvh, bool merge) {
+  const int lane = threadIdx.x & 63;
+  const int per = (a.group + kDecodeRows - 1) / kDecodeRows;  // row tiles of a request
+  auto tiles_of = [&](int r) -> int {
+    const int p = r < a.num_rows ? a.positions[r] : -1;
+    return p < 0 ? -1 : key_tiles<KT>(a, p, p).total;
+  };
+  const int first = tiles_of(lane);
+  int64_t all = max(first, 0);
+  for (int r = 64; r < a.num_rows; r += 64) all += max(tiles_of(r + lane), 0);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) all += __shfl_xor(all, o, 64);
+  // Key tiles of an item: one round of kFewSlots items while those are short, because there a
+  // workgroup's fixed cost weighs; else `target` items, of which late ones make up for early ones.
+  all *= per * a.num_kv_heads;
+  int64_t size64 = (all + kFewSlots - 1) / kFewSlots;
+  if (size64 > kShortItem)
+    size64 = max((all + a.target - 1) / a.target, static_cast<int64_t>(kShortItem));
+  const int size = static_cast<int>(max(size64, static_cast<int64_t>(a.min_tiles)));
+  Item it = {kvh, 0, 0, 0, {-1, 0, 0, 0}};
+  int base = 0, row_base = 0;  // items, row tiles before this block of requests
+  for (int r0 = 0; r0 < a.num_rows; r0 += 64) {
+    const int tiles = r0 == 0 ? first : tiles_of(r0 + lane);
+    const int n = tiles < 0 ? 0 : max((tiles + size - 1) / size, 1);  // items of a row tile
+    int incl = n * per;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(incl, d, 64);
+      if (lane >= d) incl += y;
+    }
+    const int before = incl - n * per;
+    const uint64_t past =
+        __ballot(merge ? c < row_base + (lane + 1) * per : c < base + incl);
+    if (past) {
+      const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
+      const int r = r0 + l;
+      if (r >= a.num_rows) return it;
+      const int nl = __builtin_amdgcn_readfirstlane(__shfl(n, l, 64));
+      const int start = base + __builtin_amdgcn_readfirstlane(__shfl(before, l, 64));
+      const int in = merge ? (c - row_base - l * per) * nl : c - start;
+      if (nl == 0) return it;  // (a padding row of the merge)
+      it.nsplit = nl;
+      it.t = {r, r, 1, in / nl};
+      it.split = in - it.t.tile * nl;
+      it.slot = static_cast<int64_t>(start + in) * a.num_kv_heads + kvh;
+      return it;
+    }
+    base += __builtin_amdgcn_readfirstlane(__shfl(incl, 63, 64));
+    row_base += 64 * per;
+  }
+  return it;
+}
+// Distance of two splits' slots of one row tile.
+__device__ __forceinline__ int slot_step(const PagedArgs& a) {
+  return a.target > 0 ? a.num_kv_heads : 1;
+}
+template <int KT>
+__device__ __forceinline__ Item decode_item(const PagedArgs& a, int b) {
+  if (a.target > 0) {
+    const int c = b / a.num_kv_heads;
+    return balanced_item<KT>(a, c, b - c * a.num_kv_heads, false);
+  }
+  return even_item<kDecodeRows>(a, b);
+}
+
 // Joins the states of the workgroup's waves, which each hold (m, l, O) of the same 16 rows in
-// `area` ([wave][16][D + 4] fp32, then [wave][16][2] in ml), and writes the output rows or this
+// `area` ([wave][16][D + 4] fp32, and [wave][16][2] in ml), and writes the output rows or this
 // split's partials.
 template <int DT, int D, int WAVES>
 __device__ __forceinline__ void join_waves(const PagedArgs& a, const float* area, const float* ml,
-                                           const TileRef& t, int kvh, int tile_idx, int split,
-                                           int nsplit, float out_scale) {
+                                           const Item& it, int nsplit, float out_scale) {
   constexpr int VPR = D / 4;  // float4 per row
+  const TileRef& t = it.t;
   for (int i = threadIdx.x; i < kDecodeRows * VPR; i += WAVES * 64) {
     const int row = i / VPR, d = (i % VPR) * 4;
     const int flat = t.tile * kDecodeRows + row;
@@ -322,16 +409,14 @@ __device__ __forceinline__ void join_waves(const PagedArgs& a, const float* area
     }
     const int pi = flat / a.group;
     if (nsplit > 1) {
-      const int64_t slot =
-          ((static_cast<int64_t>(tile_idx) * a.num_kv_heads + kvh) * a.nsplit + split) *
-              kDecodeRows + row;
+      const int64_t slot = it.slot * kDecodeRows + row;
       *reinterpret_cast<float4*>(a.part_o + slot * D + d) = make_float4(o[0], o[1], o[2], o[3]);
       if (d == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(m, l);
       continue;
     }
     if (a.positions[t.row0 + pi] < 0) continue;
     const float inv = m == -INFINITY ? 0.f : out_scale / l;
-    char* op = a.o + (t.row0 + pi) * a.o_row + (kvh * a.group + flat - pi * a.group) * a.o_head;
+    char* op = a.o + (t.row0 + pi) * a.o_row + (it.kvh * a.group + flat - pi * a.group) * a.o_head;
     if constexpr (DT == SB_DTYPE_F32) {
       *reinterpret_cast<float4*>(op + d * 4) =
           make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
@@ -343,18 +428,12 @@ __device__ __forceinline__ void join_waves(const PagedArgs& a, const float* area
   }
 }
 
-// The item of workgroup b (KV head fastest, then row tile, then split).
-struct DecodeItem {
-  int kvh, tile_idx, split;
-};
-__device__ __forceinline__ DecodeItem decode_item(const PagedArgs& a, int b) {
-  const int rest = b / a.num_kv_heads;
-  const int split = rest / a.num_tiles;
-  return {b - rest * a.num_kv_heads, rest - split * a.num_tiles, split};
-}
-
-template <int DT, int D, bool Q4>
-__global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_decode_kernel(const PagedArgs a) {
+// UNIFORM: pages of whole groups of 16 keys (block_size a multiple of 16). A group of 16 keys then
+// lies in one page, so its offset is a scalar: the offsets of 32 steps are looked up at once, two
+// per step in the lanes, and read from there (the scale bytes' are a sixteenth of the codes', as a
+// row's bytes are). Other block sizes and strides look every lane's keys up.
+template <int DT, int D, bool Q4, bool UNIFORM>
+__global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_kernel(const PagedArgs a) {
   using M = Mma<DT>;
   using H = Half<DT>;
   using vec8 = typename M::vec8;
@@ -362,8 +441,9 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_decode_kernel(cons
   constexpr int NKS = D / 32;        // QK^T k-steps
   constexpr int NDT = D / 16;        // output d-tiles
   constexpr int CH = D / 8;          // 16-byte chunks of a V row in LDS
-  // V rows in LDS, 16-byte chunks XOR-swizzled by row: eight consecutive rows' 32-byte pieces of
-  // one column range fall on different banks. The same memory takes the waves' O at the end.
+  // V rows in LDS, 16-byte chunks XOR-swizzled by row (vchunk): sixteen rows' chunks of one column
+  // fall on different banks (the writes), and so do four rows' two chunks of one 16-column tile
+  // (the transposing reads). The same memory takes the waves' O at the end.
   constexpr int kArea = kDecodeRows * (D + 4) * 4;
   static_assert(kArea >= KT * D * 2, "O area covers the V stage");
   __shared__ __align__(16) char lds[kDecodeWaves][kArea];
@@ -372,9 +452,10 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_decode_kernel(cons
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lq = lane & 15, lg = lane >> 4;
-  const DecodeItem it = decode_item(a, blockIdx.x);
-  const TileRef t = find_tile<kDecodeRows>(a, it.tile_idx);
+  const Item it = decode_item<KT>(a, blockIdx.x);
+  const TileRef& t = it.t;
   if (t.request < 0) return;
+  const int kvh = it.kvh;
   const int flat = t.tile * kDecodeRows + lq;
   const bool valid = flat < t.rows * a.group;
   const int pi = valid ? flat / a.group : 0;
@@ -389,23 +470,26 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_decode_kernel(cons
   pmax = __builtin_amdgcn_readfirstlane(pmax);
   if (pmax < 0) return;
   const KeyTiles kt = key_tiles<KT>(a, pmin, pmax);
-  const int nsplit = split_count(a, kt.total);
+  const int nsplit = a.target > 0 ? it.nsplit : split_count(a, kt.total);
   if (it.split >= nsplit) return;
-  const int i1 = static_cast<int>(static_cast<int64_t>(kt.total) * (it.split + 1) / nsplit);
-  int i = static_cast<int>(static_cast<int64_t>(kt.total) * it.split / nsplit) + wave;
+  // this wave's share of the split's tiles
+  const int64_t share = static_cast<int64_t>(it.split) * kDecodeWaves + wave;
+  const int64_t shares = static_cast<int64_t>(nsplit) * kDecodeWaves;
+  const int i0 = static_cast<int>(kt.total * share / shares);
+  const int i1 = static_cast<int>(kt.total * (share + 1) / shares);
 
   const int32_t* table = a.tables + t.request * a.table_stride;
-  const char* kbase = a.k + it.kvh * a.c_head;
-  const char* vbase = a.v + it.kvh * a.c_head;
-  const char* ksb = a.ks + it.kvh * a.s_head;
-  const char* vsb = a.vs + it.kvh * a.s_head;
+  const char* kbase = a.k + kvh * a.c_head;
+  const char* vbase = a.v + kvh * a.c_head;
+  const char* ksb = a.ks + kvh * a.s_head;
+  const char* vsb = a.vs + kvh * a.s_head;
 
   // Query fragments (B operand). k-slot (step s, lane group lg, j) is dim 32 s + 8 lg + j over
   // 16-bit pages, and dim lg D/4 + 8 s + j over 4-bit ones, where a lane reads D/4 values at once.
   vec8 qf[NKS];
   {
     const char* qp = a.q + (t.row0 + pi) * a.q_row +
-                     (it.kvh * a.group + flat - pi * a.group) * a.q_head;
+                     (kvh * a.group + flat - pi * a.group) * a.q_head;
 #pragma unroll
     for (int s = 0; s < NKS; ++s) {
       vec8 v = {};
@@ -421,29 +505,77 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_decode_kernel(cons
   struct Stage {
     raw_t k[2][RAW], v[2][RAW];
     uint32_t sk[2], sv[2];
-    int page[2];
+    uint32_t live;  // which of the step's keys have a page
   };
-  auto lookup = [&](int idx, int* page) {
-    const int k0 = tile_key<KT>(kt, idx);
+  const uint32_t lane_row = static_cast<uint32_t>(lq * a.c_pos) + (Q4 ? lg * (D / 8) : 16 * lg);
+  const uint32_t lane_scale = static_cast<uint32_t>(lq * a.s_pos) + lg * (D / 32) / 4;
+  int64_t group_off = 0;                   // UNIFORM: of group lane & 1 of step lane / 2
+  uint64_t group_live = 0;
+  int page[2] = {-1, -1};                  // else: of keys lq and lq + 16 of the next step
+  auto lookup = [&](int idx) {
+    if constexpr (UNIFORM) {
+      if (((idx - i0) & 31) != 0 || idx >= i1) return;
+      const int step = min(idx + (lane >> 1), i1 - 1);
+      const int key = tile_key<KT>(kt, step) + 16 * (lane & 1);
+      const int pb = page_of(a, table, key);
+      group_off = row_offset(a, key, pb, a.c_block, a.c_pos);
+      group_live = __ballot(pb >= 0);
+    } else {
+      const int k0 = tile_key<KT>(kt, min(idx, i1 - 1));
 #pragma unroll
-    for (int h = 0; h < 2; ++h) page[h] = idx < i1 ? page_of(a, table, k0 + 16 * h + lq) : -1;
+      for (int h = 0; h < 2; ++h) page[h] = page_of(a, table, k0 + 16 * h + lq);
+    }
   };
-  auto fetch = [&](int idx, Stage& st) {
-    const int k0 = tile_key<KT>(kt, idx);
+  auto lane64 = [](int64_t v, int l) -> int64_t {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), l);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), l);
+    return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+  };
+  auto fetch = [&](int idx, Stage& st) {  // (behind lookup(idx))
+    if constexpr (UNIFORM) {
+      const int at = 2 * ((idx - i0) & 31);
+      const uint32_t two = static_cast<uint32_t>(group_live >> at) & 3u;
+      st.live = (two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int key = k0 + 16 * h + lq;
-      const int64_t off = row_offset(a, key, st.page[h], a.c_block, a.c_pos);
+      for (int h = 0; h < 2; ++h) {
+        // (the group's address stays in scalar registers, the lane's part is one of 32 bits)
+        const int64_t off = lane64(group_off, at + h);
+        const SB_GLOBAL char* kg = (const SB_GLOBAL char*)(kbase + off);
+        const SB_GLOBAL char* vg = (const SB_GLOBAL char*)(vbase + off);
+        asm volatile("" : "+s"(kg), "+s"(vg));
 #pragma unroll
-      for (int s = 0; s < RAW; ++s) {
-        const int64_t at = off + (Q4 ? lg * (D / 8) : 64 * s + 16 * lg);
-        st.k[h][s] = *reinterpret_cast<const raw_t*>(kbase + at);
-        st.v[h][s] = *reinterpret_cast<const raw_t*>(vbase + at);
+        for (int s = 0; s < RAW; ++s) {
+          st.k[h][s] = *(const SB_GLOBAL raw_t*)(kg + lane_row + 64 * s);
+          st.v[h][s] = *(const SB_GLOBAL raw_t*)(vg + lane_row + 64 * s);
+        }
+        if constexpr (Q4) {
+          const SB_GLOBAL char* ksg = (const SB_GLOBAL char*)(ksb + (off >> 4));
+          const SB_GLOBAL char* vsg = (const SB_GLOBAL char*)(vsb + (off >> 4));
+          asm volatile("" : "+s"(ksg), "+s"(vsg));
+          st.sk[h] = static_cast<uint8_t>(ksg[lane_scale]);
+          st.sv[h] = static_cast<uint8_t>(vsg[lane_scale]);
+        }
       }
-      if constexpr (Q4) {
-        const int64_t so = row_offset(a, key, st.page[h], a.s_block, a.s_pos) + lg * (D / 32) / 4;
-        st.sk[h] = static_cast<uint8_t>(ksb[so]);
-        st.sv[h] = static_cast<uint8_t>(vsb[so]);
+    } else {
+      const int k0 = tile_key<KT>(kt, idx);
+      st.live = static_cast<uint32_t>(__ballot(page[0] >= 0) & 0xffffu) |
+                static_cast<uint32_t>(__ballot(page[1] >= 0) & 0xffffu) << 16;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = k0 + 16 * h + lq;
+        const int64_t off = row_offset(a, key, page[h], a.c_block, a.c_pos);
+#pragma unroll
+        for (int s = 0; s < RAW; ++s) {
+          const int64_t at = off + (Q4 ? lg * (D / 8) : 64 * s + 16 * lg);
+          st.k[h][s] = *reinterpret_cast<const raw_t*>(kbase + at);
+          st.v[h][s] = *reinterpret_cast<const raw_t*>(vbase + at);
+        }
+        if constexpr (Q4) {
+          const int64_t so =
+              row_offset(a, key, page[h], a.s_block, a.s_pos) + lg * (D / 32) / 4;
+          st.sk[h] = static_cast<uint8_t>(ksb[so]);
+          st.sv[h] = static_cast<uint8_t>(vsb[so]);
+        }
       }
     }
   };
@@ -456,12 +588,43 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_decode_kernel(cons
   const float c_log2 = Q4 ? a.scale_log2 * (1 << H::kShift) : a.scale_log2;
   char* vst = lds[wave];
   auto vchunk = [&](int row, int c) -> int {  // byte offset of chunk c of a row
-    const int x = CH >= 16 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
+    const int y = CH >= 16 ? row & 15 : (row >> 1) & 7;
+    const int x = CH >= 16 ? (y & 7) << 1 | y >> 3 : (y & 3) << 1 | y >> 2;
     return row * (D * 2) + 16 * (c ^ x);
   };
 
-  auto step = [&](int idx, const Stage& st) {
+  int odd_first = 0x7fffffff, odd_last = -1;  // tiles that V values were taken out of
+  auto step = [&](int idx, Stage& st) {
     const int k0 = tile_key<KT>(kt, idx);
+    const uint32_t live = st.live;
+    const bool whole = live == 0xffffffffu && k0 + KT - 1 <= pmin &&
+                       (k0 > pmax - a.window || k0 + KT - 1 < a.sinks);
+    if (!whole) {  // values that are not finite are taken out of V, and added where they are seen
+      bool odd;
+      if constexpr (Q4) {
+        odd = st.sv[0] == 255 || st.sv[1] == 255;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (st.sv[h] == 255) st.v[h][0] = raw_t{}, st.sv[h] = 0;
+      } else {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int s = 0; s < NKS; ++s) bits |= not_finite_bits<DT>(st.v[h][s]);
+        odd = (bits & kNotFinite) != 0;
+        if (odd) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int s = 0; s < NKS; ++s) st.v[h][s] = finite_part<DT>(st.v[h][s]);
+        }
+      }
+      if (__any(odd)) {
+        odd_first = min(odd_first, idx);
+        odd_last = idx;
+      }
+    }
     // V rows to LDS
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -492,11 +655,6 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_decode_kernel(cons
         sc[h] = H::mma16(__builtin_bit_cast(vec8, w), qf[s], sc[h]);
       }
     }
-    const uint32_t live = static_cast<uint32_t>(__ballot(st.page[0] >= 0) & 0xffffu) |
-                          static_cast<uint32_t>(__ballot(st.page[1] >= 0) & 0xffffu) << 16;
-    const bool whole = live == 0xffffffffu && k0 + KT - 1 <= pmin &&
-                       (k0 > pmax - a.window || k0 + KT - 1 < a.sinks);
-    bool odd = false;  // V holds values that are not finite, and some row sees the tile in part
     if (whole) {
       seen = true;
     } else {
@@ -507,16 +665,6 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_decode_kernel(cons
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (!(on >> (16 * h + e) & 1u)) sc[h][e] = -INFINITY;
-      if constexpr (Q4) {
-        odd = __any(st.sv[0] == 255 || st.sv[1] == 255);
-      } else {
-        uint32_t bits = 0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int s = 0; s < NKS; ++s) bits |= not_finite_bits<DT>(st.v[h][s]);
-        odd = __any((bits & kNotFinite) != 0);
-      }
     }
     float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                       fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
@@ -557,35 +705,60 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_decode_kernel(cons
                                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((SB_LDS s16x4_t*)src));
       }
       const u32x4_t v = {w[0].x, w[0].y, w[1].x, w[1].y};
-      if (!odd) o[d] = H::mma16(__builtin_bit_cast(vec8, v), pb, o[d]);
-      else mma_masked<DT>(v, pb, o[d], H::mma16);
+      o[d] = H::mma16(__builtin_bit_cast(vec8, v), pb, o[d]);
     }
     asm volatile("" ::: "memory");
   };
 
-  // One step ahead in registers, the pages two ahead.
-  Stage st[2];
-  if (i < i1) {
-    lookup(i, st[0].page);
-    fetch(i, st[0]);
-    lookup(i + kDecodeWaves, st[1].page);
-  }
-  while (i < i1) {
+  // Steps ahead in registers: 4-bit rows are an eighth of a step's registers and latency shows,
+  // 16-bit ones fill them with one.
+  constexpr int PD = UNIFORM && Q4 ? kDecodeAhead4 : 1;
+  // Every trip issues its loads, past the end those of the last step again: behind a branch the
+  // compiler would have to wait for all of them, the ones just issued as well.
+  Stage st[PD + 1];
+  if (i0 < i1) {
+    lookup(i0);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (i < i1) {
-        const int next = i + kDecodeWaves;
-        int page[2];
-        if (next < i1) {
-          fetch(next, st[u ^ 1]);
-          lookup(next + kDecodeWaves, page);
+    for (int x = 0; x < PD; ++x) {
+      fetch(min(i0 + x, i1 - 1), st[x]);
+      if (!UNIFORM) lookup(i0 + x + 1);
+    }
+    int i = i0;
+    for (; i + PD < i1; i += PD + 1) {
+#pragma unroll
+      for (int u = 0; u <= PD; ++u) {
+        if (UNIFORM) lookup(i + u + PD);
+        fetch(min(i + u + PD, i1 - 1), st[(u + PD) % (PD + 1)]);
+        if (!UNIFORM) lookup(i + u + PD + 1);
+        step(i + u, st[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < PD; ++u)
+      if (i + u < i1) step(i + u, st[u]);
+  }
+
+  // What was taken out, added where it is seen: an infinity or a NaN of a seen key decides the sum,
+  // whatever (positive) weight it has.
+  for (int x = odd_first; x <= odd_last; ++x) {
+    const int k0 = tile_key<KT>(kt, x);
+    const uint64_t has = __ballot(page_of(a, table, k0 + (lane & 31)) >= 0);
+    if (has == ~0ull && k0 + KT - 1 <= pmin && (k0 > pmax - a.window || k0 + KT - 1 < a.sinks))
+      continue;  // (seen whole: nothing was taken out)
+    for (int r = 0; r < KT; ++r) {
+      const int key = k0 + r, pb = page_of(a, table, key);
+      const bool on = pb >= 0 && sees(a, p, key);
+      if (!__any(on)) continue;
+      const char* row = vbase + row_offset(a, key, pb, a.c_block, a.c_pos);
+      const char* sr = Q4 ? vsb + row_offset(a, key, pb, a.s_block, a.s_pos) : nullptr;
+#pragma unroll
+      for (int d = 0; d < NDT; ++d) {
+        if constexpr (Q4) {
+          if (on && static_cast<uint8_t>(sr[d / 2]) == 255) o[d] += __builtin_nanf("");
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2*>(row + 2 * (16 * d + 4 * lg));
+          if (on) add_not_finite<DT>(w, o[d], 0);
         }
-        step(i, st[u]);
-        if (next < i1) {
-          st[u].page[0] = page[0];
-          st[u].page[1] = page[1];
-        }
-        i = next;
       }
     }
   }
@@ -603,8 +776,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_decode_kernel(cons
   for (int d = 0; d < NDT; ++d)
     *reinterpret_cast<f32x4*>(area + lq * (D + 4) + 16 * d + 4 * lg) = o[d];
   __syncthreads();
-  join_waves<DT, D, kDecodeWaves>(a, reinterpret_cast<const float*>(&lds[0][0]), &ml[0][0][0], t,
-                                  it.kvh, it.tile_idx, it.split, nsplit,
+  join_waves<DT, D, kDecodeWaves>(a, reinterpret_cast<const float*>(&lds[0][0]), &ml[0][0][0], it, nsplit,
                                   Q4 ? static_cast<float>(1 << H::kShift) : 1.f);
 }
 
@@ -622,9 +794,10 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lq = lane & 15, lg = lane >> 4;
-  const DecodeItem it = decode_item(a, blockIdx.x);
-  const TileRef t = find_tile<kDecodeRows>(a, it.tile_idx);
+  const Item it = decode_item<KT>(a, blockIdx.x);
+  const TileRef& t = it.t;
   if (t.request < 0) return;
+  const int kvh = it.kvh;
   const int flat = t.tile * kDecodeRows + lq;
   const bool valid = flat < t.rows * a.group;
   const int pi = valid ? flat / a.group : 0;
@@ -639,18 +812,20 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
   pmax = __builtin_amdgcn_readfirstlane(pmax);
   if (pmax < 0) return;
   const KeyTiles kt = key_tiles<KT>(a, pmin, pmax);
-  const int nsplit = split_count(a, kt.total);
+  const int nsplit = a.target > 0 ? it.nsplit : split_count(a, kt.total);
   if (it.split >= nsplit) return;
-  const int i1 = static_cast<int>(static_cast<int64_t>(kt.total) * (it.split + 1) / nsplit);
-  int i = static_cast<int>(static_cast<int64_t>(kt.total) * it.split / nsplit) + wave;
+  const int64_t share = static_cast<int64_t>(it.split) * kDecodeWaves + wave;
+  const int64_t shares = static_cast<int64_t>(nsplit) * kDecodeWaves;
+  const int i0 = static_cast<int>(kt.total * share / shares);
+  const int i1 = static_cast<int>(kt.total * (share + 1) / shares);
 
   const int32_t* table = a.tables + t.request * a.table_stride;
-  const char* kbase = a.k + it.kvh * a.c_head + 16 * lg;
-  const char* vbase = a.v + it.kvh * a.c_head + 16 * lq;
+  const char* kbase = a.k + kvh * a.c_head + 16 * lg;
+  const char* vbase = a.v + kvh * a.c_head + 16 * lq;
   f32x4 qf[NC];
   {
     const char* qp = a.q + (t.row0 + pi) * a.q_row +
-                     (it.kvh * a.group + flat - pi * a.group) * a.q_head + 16 * lg;
+                     (kvh * a.group + flat - pi * a.group) * a.q_head + 16 * lg;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       f32x4 v = {};
@@ -664,7 +839,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
     int page;
   };
   auto lookup = [&](int idx) -> int {
-    return idx < i1 ? page_of(a, table, tile_key<KT>(kt, idx) + lq) : -1;
+    return page_of(a, table, tile_key<KT>(kt, min(idx, i1 - 1)) + lq);
   };
   auto fetch = [&](int idx, Stage& st) {
     const int k0 = tile_key<KT>(kt, idx);
@@ -681,7 +856,8 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
     for (int e = 0; e < 4; ++e) o[u][e] = f32x4{};
   const float c_hi = a.scale_log2, c_lo = a.scale_log2_lo;
 
-  auto step = [&](int idx, int next, const Stage& st, Stage& ahead) {
+  int odd_first = 0x7fffffff, odd_last = -1;
+  auto step = [&](int idx, const Stage& st, Stage& ahead) {
     const int k0 = tile_key<KT>(kt, idx);
     f32x4 v[4][NU];
 #pragma unroll
@@ -690,7 +866,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
 #pragma unroll
       for (int u = 0; u < NU; ++u) v[x][u] = *reinterpret_cast<const f32x4*>(vbase + vo + 256 * u);
     }
-    if (next < i1) fetch(next, ahead);
+    fetch(min(idx + 1, i1 - 1), ahead);
     f32x4 sc[2] = {f32x4{}, f32x4{}};  // two chains
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -704,6 +880,18 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
     if (whole) {
       seen = true;
     } else {
+      bool odd = false;  // as in paged_decode_kernel
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(fabsf(v[x][u][e]) < INFINITY)) odd = true, v[x][u][e] = 0.f;
+      if (__any(odd)) {
+        odd_first = min(odd_first, idx);
+        odd_last = idx;
+      }
       const uint32_t on = (seen_bits(a, p, k0) & live) >> (4 * lg);
       seen |= (on & 15u) != 0;
 #pragma unroll
@@ -735,68 +923,53 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
                  : __builtin_amdgcn_exp2f(__builtin_fmaf(c_hi, s[e], __builtin_fmaf(c_lo, s[e], negm)));
       l_run += w[e];
     }
-    bool bad = false;
-    if (!whole) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) bad |= !(fabsf(v[x][u][e]) < INFINITY);
-    }
-    if (__any(bad)) {  // as mma_masked does
+    for (int x = 0; x < 4; ++x)
 #pragma unroll
       for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          f32x4& acc = o[u][e];
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                fabsf(v[x][u][e]) < INFINITY ? v[x][u][e] : 0.f, w[x], acc, 0, 0, 0);
-#pragma unroll 1
-          for (int kind = kNaN; kind <= kNegInf; ++kind) {
-            const float inf = kind == kPosInf ? INFINITY : -INFINITY;
-            f32x4 n = {};
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float y = v[x][u][e];
-              n = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                  (kind == kNaN ? y != y : y == inf) ? 1.f : 0.f, w[x], n, 0, 0, 0);
-            }
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              acc[x] += n[x] > 0.f ? (kind == kNaN ? __builtin_nanf("") : inf) : 0.f;
-          }
-        }
-    } else {
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            o[u][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[x][u][e], w[x], o[u][e], 0, 0, 0);
-    }
+        for (int e = 0; e < 4; ++e)
+          o[u][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[x][u][e], w[x], o[u][e], 0, 0, 0);
   };
 
   // K one step ahead in registers, the pages two; V is requested before the scores are formed.
+  // (Loads past the end are those of the last step again, as in paged_decode_kernel.)
   Stage st[2];
-  if (i < i1) {
-    st[0].page = lookup(i);
-    fetch(i, st[0]);
-    st[1].page = lookup(i + kDecodeWaves);
-  }
-  while (i < i1) {
+  if (i0 < i1) {
+    st[0].page = lookup(i0);
+    fetch(i0, st[0]);
+    st[1].page = lookup(i0 + 1);
+    int i = i0;
+    for (; i + 1 < i1; i += 2) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (i < i1) {
-        const int next = i + kDecodeWaves;
-        const int page = lookup(next + kDecodeWaves);
-        step(i, next, st[u], st[u ^ 1]);
+      for (int u = 0; u < 2; ++u) {
+        const int page = lookup(i + u + 2);
+        step(i + u, st[u], st[u ^ 1]);
         st[u].page = page;
-        i = next;
       }
+    }
+    if (i < i1) step(i, st[0], st[1]);
+  }
+  for (int x = odd_first; x <= odd_last; ++x) {
+    const int k0 = tile_key<KT>(kt, x);
+    const uint64_t has = __ballot(page_of(a, table, k0 + lq) >= 0);
+    if (has == ~0ull && k0 + KT - 1 <= pmin && (k0 > pmax - a.window || k0 + KT - 1 < a.sinks))
+      continue;
+    for (int r = 0; r < KT; ++r) {
+      const int key = k0 + r, pb = page_of(a, table, key);
+      const bool on = pb >= 0 && sees(a, p, key);
+      if (!__any(on)) continue;
+      const char* row =
+          a.v + kvh * a.c_head + row_offset(a, key, pb, a.c_block, a.c_pos);
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const f32x4 w = *reinterpret_cast<const f32x4*>(row + 4 * (64 * u + 16 * lg + 4 * y));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (on && !(fabsf(w[e]) < INFINITY)) o[u][e][y] += w[e];
+        }
     }
   }
   l_run += __shfl_xor(l_run, 16, 64);
@@ -815,8 +988,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
       *reinterpret_cast<f32x4*>(&area[wave][lq][64 * u + 16 * lg + 4 * x]) = w;
     }
   __syncthreads();
-  join_waves<SB_DTYPE_F32, D, kDecodeWaves>(a, &area[0][0][0], &ml[0][0][0], t, it.kvh,
-                                            it.tile_idx, it.split, nsplit, 1.f);
+  join_waves<SB_DTYPE_F32, D, kDecodeWaves>(a, &area[0][0][0], &ml[0][0][0], it, nsplit, 1.f);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -844,8 +1016,8 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, lq = lane & 31, lg = lane >> 5;
-  const DecodeItem it = decode_item(a, blockIdx.x);
-  const TileRef t = find_tile<kRowsTile>(a, it.tile_idx);
+  const Item it = even_item<kRowsTile>(a, blockIdx.x);
+  const TileRef& t = it.t;
   if (t.request < 0) return;
   const int flat = t.tile * kRowsTile + wave * 32 + lq;
   const bool valid = flat < static_cast<int64_t>(t.rows) * a.group;
@@ -979,9 +1151,7 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
         const u32x4_t v = *at;
         if ((not_finite_bits<DT>(v) & kNotFinite) == 0) continue;
         odd = true;
-        const u32x4_t fin = {finite_part<DT>(v[0]), finite_part<DT>(v[1]), finite_part<DT>(v[2]),
-                             finite_part<DT>(v[3])};
-        *at = fin;
+        *at = finite_part<DT>(v);
       }
     }
     if (odd) {
@@ -1309,14 +1479,9 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
         for (int d = 0; d < NDT; ++d)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            uint2 w = *reinterpret_cast<const uint2*>(row + 2 * (32 * d + 8 * e + 4 * lg));
-            if (!on || ((not_finite_bits<DT>(w.x) | not_finite_bits<DT>(w.y)) & kNotFinite) == 0)
-              continue;
-            w.x &= ~finite_part<DT>(w.x), w.y &= ~finite_part<DT>(w.y);
-            o[d][4 * e] += H::to_f32(w.x & 0xffffu);
-            o[d][4 * e + 1] += H::to_f32(w.x >> 16);
-            o[d][4 * e + 2] += H::to_f32(w.y & 0xffffu);
-            o[d][4 * e + 3] += H::to_f32(w.y >> 16);
+            const uint2 w =
+                *reinterpret_cast<const uint2*>(row + 2 * (32 * d + 8 * e + 4 * lg));
+            if (on) add_not_finite<DT>(w, o[d], 4 * e);
           }
       }
     }
@@ -1327,9 +1492,7 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
   const bool row_seen = seen || other_seen != 0;
   if (p < 0) return;
   if (nsplit > 1) {
-    const int64_t slot =
-        ((static_cast<int64_t>(it.tile_idx) * a.num_kv_heads + it.kvh) * a.nsplit + it.split) *
-            kRowsTile + wave * 32 + lq;
+    const int64_t slot = it.slot * kRowsTile + wave * 32 + lq;
     float* po = a.part_o + slot * D;
 #pragma unroll
     for (int d = 0; d < NDT; ++d)
@@ -1361,21 +1524,35 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
 
 // ---------------------------------------------------------------------------------------
 // Joins the partials of row tiles whose keys were split: blockIdx.x = (tile, KV head), blockIdx.y
-// = which 16 rows of the tile.
+// = which RPW rows of the tile. D / 4 lanes take a row, and the groups of them that RPW rows leave
+// share the row's splits: a decode row of 60 splits is then one batch of loads each for 8 groups
+// instead of eight batches in turn (28 / 4 heads x 128, one row of 16000: 8.5 -> 5.4 us).
 // ---------------------------------------------------------------------------------------
 constexpr int kMergeThreads = 256;
-template <int DT, int D, int TR, int KT>
+template <int DT, int D, int TR, int KT, int RPW>
 __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedArgs a,
                                                                    float out_scale) {
+  constexpr int VPR = D / 4;                           // lanes of a row
+  constexpr int G = kMergeThreads / (RPW * VPR);       // groups that share a row
+  static_assert(G >= 1 && G * RPW * VPR == kMergeThreads, "every thread has a row");
   __shared__ int red[2][kMergeThreads / 64];
+  __shared__ __align__(16) float4 part[G > 1 ? kMergeThreads : 1];
+  __shared__ float2 part_ml[G > 1 ? RPW * G : 1];
   const int tile_idx = blockIdx.x / a.num_kv_heads;
   const int kvh = blockIdx.x - tile_idx * a.num_kv_heads;
-  const TileRef t = find_tile<TR>(a, tile_idx);
+  Item it;
+  if (TR == kDecodeRows && a.target > 0) {
+    it = balanced_item<KT>(a, tile_idx, kvh, true);
+  } else {
+    it = {kvh, 0, 0, (static_cast<int64_t>(tile_idx) * a.num_kv_heads + kvh) * a.nsplit,
+          find_tile<TR>(a, tile_idx)};
+  }
+  const TileRef& t = it.t;
   if (t.request < 0) return;
   const int nflat = static_cast<int>(
       min(static_cast<int64_t>(t.rows) * a.group - static_cast<int64_t>(t.tile) * TR,
           static_cast<int64_t>(TR)));
-  const int row_base = blockIdx.y * 16;
+  const int row_base = blockIdx.y * RPW;
   if (row_base >= nflat) return;
   // the tile's key range, as the attention kernel saw it
   int pmin = 0x7fffffff, pmax = -1;
@@ -1398,53 +1575,73 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedA
     pmax = max(pmax, red[1][w]);
   }
   if (pmax < 0) return;
-  const int nsplit = split_count(a, key_tiles<KT>(a, pmin, pmax).total);
+  const int nsplit =
+      it.nsplit > 0 ? it.nsplit : split_count(a, key_tiles<KT>(a, pmin, pmax).total);
   if (nsplit <= 1) return;
-  constexpr int VPR = D / 4;
-  for (int i = threadIdx.x; i < 16 * VPR; i += kMergeThreads) {
-    const int row = row_base + i / VPR, d = (i % VPR) * 4;
-    if (row >= nflat) continue;
-    const int flat = t.tile * TR + row;
-    const int pi = flat / a.group;
-    if (a.positions[t.row0 + pi] < 0) continue;
-    const int64_t slot0 =
-        ((static_cast<int64_t>(tile_idx) * a.num_kv_heads + kvh) * a.nsplit) * TR + row;
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int B = 8;  // splits in flight
-    for (int s0 = 0; s0 < nsplit; s0 += B) {
-      float2 ml[B];
-      float4 x[B];
+  const int lane = threadIdx.x % VPR, row_in = threadIdx.x / VPR % RPW;
+  const int grp = threadIdx.x / (VPR * RPW);
+  const int row = min(row_base + row_in, nflat - 1), d = lane * 4;
+  const int flat = t.tile * TR + row, pi = flat / a.group;
+  const int64_t slot0 = it.slot * TR + row;
+  const int64_t step = static_cast<int64_t>(slot_step(a)) * TR;
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int B = TR == kDecodeRows ? 8 : 4;  // splits in flight
+  for (int s0 = grp; s0 < nsplit; s0 += B * G) {
+    float2 ml[B];
+    float4 x[B];
 #pragma unroll
-      for (int b = 0; b < B; ++b) {
-        const int64_t slot = slot0 + static_cast<int64_t>(min(s0 + b, nsplit - 1)) * TR;
-        ml[b] = *reinterpret_cast<const float2*>(a.part_ml + slot * 2);
-        x[b] = *reinterpret_cast<const float4*>(a.part_o + slot * D + d);
-      }
-      float mb = m;
-#pragma unroll
-      for (int b = 0; b < B; ++b) mb = fmaxf(mb, ml[b].x);
-      if (mb == -INFINITY) continue;
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mb);
-      l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
-#pragma unroll
-      for (int b = 0; b < B; ++b) {
-        if (s0 + b >= nsplit || ml[b].x == -INFINITY) continue;
-        const float w = __builtin_amdgcn_exp2f(ml[b].x - mb);
-        l += w * ml[b].y;
-        o.x += w * x[b].x, o.y += w * x[b].y, o.z += w * x[b].z, o.w += w * x[b].w;
-      }
-      m = mb;
+    for (int b = 0; b < B; ++b) {
+      const int64_t slot = slot0 + min(s0 + b * G, nsplit - 1) * step;
+      ml[b] = *reinterpret_cast<const float2*>(a.part_ml + slot * 2);
+      x[b] = *reinterpret_cast<const float4*>(a.part_o + slot * D + d);
     }
-    const float inv = m == -INFINITY ? 0.f : out_scale / l;
-    char* op = a.o + (t.row0 + pi) * a.o_row + (kvh * a.group + flat - pi * a.group) * a.o_head;
-    if constexpr (DT == SB_DTYPE_F32) {
-      *reinterpret_cast<float4*>(op + d * 4) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    } else {
-      const uint32_t w0 = Mma<DT>::cvt1(o.x * inv) | Mma<DT>::cvt1(o.y * inv) << 16;
-      const uint32_t w1 = Mma<DT>::cvt1(o.z * inv) | Mma<DT>::cvt1(o.w * inv) << 16;
-      *reinterpret_cast<uint2*>(op + d * 2) = make_uint2(w0, w1);
+    float mb = m;
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+      if (s0 + b * G < nsplit) mb = fmaxf(mb, ml[b].x);
+    if (mb == -INFINITY) continue;
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mb);
+    l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      if (s0 + b * G >= nsplit || ml[b].x == -INFINITY) continue;
+      const float w = __builtin_amdgcn_exp2f(ml[b].x - mb);
+      l += w * ml[b].y;
+      o.x += w * x[b].x, o.y += w * x[b].y, o.z += w * x[b].z, o.w += w * x[b].w;
     }
+    m = mb;
+  }
+  if constexpr (G > 1) {
+    part[threadIdx.x] = o;
+    if (lane == 0) part_ml[row_in * G + grp] = make_float2(m, l);
+    __syncthreads();
+    if (grp > 0) return;
+    float mb = m;
+#pragma unroll
+    for (int g = 1; g < G; ++g) mb = fmaxf(mb, part_ml[row_in * G + g].x);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mb);
+    l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll
+    for (int g = 1; g < G; ++g) {
+      const float2 ml = part_ml[row_in * G + g];
+      if (ml.x == -INFINITY) continue;
+      const float w = __builtin_amdgcn_exp2f(ml.x - mb);
+      const float4 x = part[g * VPR * RPW + threadIdx.x];
+      l += w * ml.y;
+      o.x += w * x.x, o.y += w * x.y, o.z += w * x.z, o.w += w * x.w;
+    }
+    m = mb;
+  }
+  if (row_base + row_in >= nflat || a.positions[t.row0 + pi] < 0) return;
+  const float inv = m == -INFINITY ? 0.f : out_scale / l;
+  char* op = a.o + (t.row0 + pi) * a.o_row + (kvh * a.group + flat - pi * a.group) * a.o_head;
+  if constexpr (DT == SB_DTYPE_F32) {
+    *reinterpret_cast<float4*>(op + d * 4) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  } else {
+    const uint32_t w0 = Mma<DT>::cvt1(o.x * inv) | Mma<DT>::cvt1(o.y * inv) << 16;
+    const uint32_t w1 = Mma<DT>::cvt1(o.z * inv) | Mma<DT>::cvt1(o.w * inv) << 16;
+    *reinterpret_cast<uint2*>(op + d * 2) = make_uint2(w0, w1);
   }
 }
 
@@ -1562,8 +1759,8 @@ __global__ __launch_bounds__(64) void paged_valu_kernel(const PagedArgs a) {
 // ---------------------------------------------------------------------------------------
 struct PartPlan {  // one attention launch
   bool on;
-  int64_t tiles;
-  int nsplit;
+  int64_t tiles, grid;
+  int nsplit, min_tiles, target;
   int64_t o_floats, ml_floats;
 };
 struct PagedPlan {
@@ -1574,20 +1771,20 @@ struct PagedPlan {
 };
 
 constexpr int kFewRows = 32;       // 16-bit arithmetic: two row tiles of 16
-constexpr int kFewMinTiles = 8;    // fewest 32-key tiles of a split (two per wave)
-constexpr int kF32MinTiles = 8;    // ... 16-key tiles, fp32
-constexpr int kRowsMinTiles = 4;   // ... 64-key tiles of the rows kernel
+constexpr int kRowsMinTiles = 4;   // fewest 64-key tiles of a split of the rows kernel
 
-// Splits of each of `items` row tiles over `tiles` key tiles: those that a launch of `slots`
-// workgroups at a time takes the fewest rounds x (key tiles + a workgroup's fixed cost, in key
-// tiles) for, the partials' writes and their merge counted as `parts` key tiles of a round each.
-int split_for(int64_t items, int64_t slots, int64_t tiles, int min_tiles, int fixed, int parts) {
+// Splits of each of `items` row tiles over `tiles` key tiles, `waves` of a workgroup taking a share
+// of them each: those that a launch of `slots` workgroups at a time takes the fewest rounds x (key
+// tiles of a wave + a workgroup's fixed cost, in key tiles) for. With more than one, the merge
+// launch counts `merge` and the partials `parts` key tiles a round.
+int split_for(int64_t items, int64_t slots, int64_t tiles, int waves, int min_tiles, int fixed,
+              int merge, int parts) {
   int64_t best = 1, cost = 0;
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(tiles / min_tiles, 128));
   for (int64_t n = 1; n <= most && items * (n - 1) < 2 * slots; ++n) {
     const int64_t rounds = (items * n + slots - 1) / slots;
-    const int64_t c = rounds * ((tiles + n - 1) / n + fixed + (n > 1 ? parts : 0)) +
-                      (n > 1 ? 2 + items * n * parts / slots : 0);
+    const int64_t c = rounds * ((tiles + n * waves - 1) / (n * waves) + fixed) +
+                      (n > 1 ? merge + rounds * parts + items * n * parts / slots : 0);
     if (n == 1 || c < cost) best = n, cost = c;
   }
   return static_cast<int>(best);
@@ -1607,7 +1804,7 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
   const int64_t flat = num_rows * group;
   pl.few_max = 0x7fffffff;
   const bool rows_kernel = !f32 && ragged && max_rows * group > kFewRows;
-  if (rows_kernel) pl.few_max = kFewRows;
+  if (rows_kernel) pl.few_max = num_requests == 1 ? 0 : kFewRows;
   const int64_t tiles_bound = (flat + kDecodeRows - 1) / kDecodeRows + num_requests;
   pl.few.on = !rows_kernel || num_requests > 1;
   if (pl.few.on) {
@@ -1615,23 +1812,39 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
     pl.few.tiles = !ragged ? num_rows * per_few
                            : rows_kernel ? std::min<int64_t>(tiles_bound, 2 * num_requests)
                                          : std::min<int64_t>(tiles_bound, flat);
+    const int64_t key_tiles = (keys + (f32 ? 15 : 31)) / (f32 ? 16 : 32);
+    const int64_t items = pl.few.tiles * num_kv_heads;
+    pl.few.min_tiles = kFewMinTiles;
+    pl.few.nsplit = split_for(items, kFewSlots, key_tiles, kDecodeWaves, kFewMinTiles, 8, 10, 1);
+    if (!ragged || num_rows == 1) {
+      // Balanced items, unless there are enough of them as they are and none is long.
+      const bool split = pl.few.nsplit > 1 || key_tiles > kLongTiles;
+      pl.few.target = split ? kFewTarget : 0;
+      pl.few.nsplit = 1;
+    }
     const int kt = f32 ? 16 : 32;
-    pl.few.nsplit = split_for(pl.few.tiles * num_kv_heads, 1024, (keys + kt - 1) / kt,
-                              f32 ? kF32MinTiles : kFewMinTiles, 16, 2);
-    const int64_t slots = pl.few.nsplit > 1
-                              ? pl.few.tiles * num_kv_heads * pl.few.nsplit * kDecodeRows : 0;
+    const int64_t most_tiles =  // of any row
+        std::min<int64_t>((kv_len + kt - 1) / kt,
+                          (std::min(window, kv_len) + kt - 2) / kt + 1 + (sinks + kt - 1) / kt);
+    // (a row of t tiles has at most t / size + 1 items, of `size` tiles, and all tiles are at most
+    // target * size)
+    pl.few.grid = pl.few.target > 0
+                      ? items + std::min<int64_t>(kFewTarget, items * (most_tiles / kFewMinTiles))
+                      : items * pl.few.nsplit;
+    const int64_t slots =
+        pl.few.target > 0 || pl.few.nsplit > 1 ? pl.few.grid * kDecodeRows : 0;
     pl.few.o_floats = slots * head_dim;
     pl.few.ml_floats = slots * 2;
   }
   pl.rows.on = rows_kernel;
   if (rows_kernel) {
-    if (num_requests == 1) pl.few_max = 0;
     pl.rows.tiles = std::min<int64_t>(flat / kRowsTile + num_requests,
                                       (flat + kFewRows - 1) / kFewRows);
+    pl.rows.min_tiles = kRowsMinTiles;
     pl.rows.nsplit = split_for(((flat + kRowsTile - 1) / kRowsTile) * num_kv_heads, 256,
-                               (keys + 63) / 64, kRowsMinTiles, 5, 3);
-    const int64_t slots = pl.rows.nsplit > 1
-                              ? pl.rows.tiles * num_kv_heads * pl.rows.nsplit * kRowsTile : 0;
+                               (keys + 63) / 64, 1, kRowsMinTiles, 5, 2, 3);
+    pl.rows.grid = pl.rows.tiles * num_kv_heads * pl.rows.nsplit;
+    const int64_t slots = pl.rows.nsplit > 1 ? pl.rows.grid * kRowsTile : 0;
     pl.rows.o_floats = slots * head_dim;
     pl.rows.ml_floats = slots * 2;
   }
@@ -1779,11 +1992,12 @@ extern "C" int sb_paged_attention(
 
   float* ws = static_cast<float*>(workspace);
   const float out_scale = q4 && dtype == SB_DTYPE_F16 ? 4.f : 1.f;
-  const auto part = [&](const PartPlan& p, int min_tiles) {
+  const auto part = [&](const PartPlan& p) {
     PagedArgs b = a;
     b.num_tiles = static_cast<int>(p.tiles);
     b.nsplit = p.nsplit;
-    b.min_tiles = min_tiles;
+    b.min_tiles = p.min_tiles;
+    b.target = p.target;
     b.part_o = ws;
     b.part_ml = ws + p.o_floats;
     ws += p.o_floats + p.ml_floats;
@@ -1793,20 +2007,21 @@ extern "C" int sb_paged_attention(
   if (head_dim == 64) { X(64) }     \
   else { X(128) }
 #define SB_MERGE(DT, D, TR, KT, B, P)                                                           \
-  if ((P).nsplit > 1) {                                                                         \
-    const dim3 mg(static_cast<unsigned>((P).tiles * num_kv_heads), TR / 16);                    \
-    SB_LAUNCH("paged_merge", (paged_merge_kernel<DT, D, TR, KT>), mg, dim3(kMergeThreads), st,  \
-              B, out_scale);                                                                    \
+  if ((P).nsplit > 1 || (P).target > 0) {                                                                         \
+    constexpr int rpw = TR == kDecodeRows ? 1 : 1024 / D;                                       \
+    const int live = (P).target > 0 ? std::min<int>(TR, static_cast<int>(group)) : TR;          \
+    const dim3 mg(static_cast<unsigned>((P).tiles * num_kv_heads), (live + rpw - 1) / rpw);     \
+    SB_LAUNCH("paged_merge", (paged_merge_kernel<DT, D, TR, KT, rpw>), mg, dim3(kMergeThreads), \
+              st, B, out_scale);                                                                \
   }
   const int64_t most = 0x7fffffff;
-  if (pl.few.tiles * num_kv_heads * std::max(pl.few.nsplit, 1) > most ||
-      pl.rows.tiles * num_kv_heads * std::max(pl.rows.nsplit, 1) > most)
+  if (pl.few.grid > most || pl.rows.grid > most)
     return fail(fn, "grid too large");
   if (pl.rows.on) {
-    PagedArgs b = part(pl.rows, kRowsMinTiles);
+    PagedArgs b = part(pl.rows);
     b.flat_min = pl.few_max;
     b.flat_max = 0x7fffffff;
-    const dim3 grid(static_cast<unsigned>(pl.rows.tiles * num_kv_heads * pl.rows.nsplit));
+    const dim3 grid(static_cast<unsigned>(pl.rows.grid));
 #define SB_ROWS(DT, D)                                                                          \
   {                                                                                             \
     if (q4)                                                                                     \
@@ -1821,15 +2036,24 @@ extern "C" int sb_paged_attention(
     else { SB_D(SB_ROWS_F16) }
   }
   if (pl.few.on) {
-    PagedArgs b = part(pl.few, dtype == SB_DTYPE_F32 ? kF32MinTiles : kFewMinTiles);
+    PagedArgs b = part(pl.few);
     b.flat_min = 0;
     b.flat_max = pl.few_max;
-    const dim3 grid(static_cast<unsigned>(pl.few.tiles * num_kv_heads * pl.few.nsplit));
+    const dim3 grid(static_cast<unsigned>(pl.few.grid));
     const dim3 block(kDecodeWaves * 64);
+    // (a lane's offset inside a group of 16 keys is 32 bits there)
+    const bool uniform = block_size % 16 == 0 && a.c_pos >= 0 && a.c_pos < (1 << 27) &&
+                         (!q4 || (a.c_block == 16ull * a.s_block && a.c_pos == 16 * a.s_pos));
 #define SB_FEW(DT, D)                                                                           \
   {                                                                                             \
-    if (q4) SB_LAUNCH("paged_decode", (paged_decode_kernel<DT, D, true>), grid, block, st, b);  \
-    else SB_LAUNCH("paged_decode", (paged_decode_kernel<DT, D, false>), grid, block, st, b);    \
+    if (q4 && uniform)                                                                          \
+      SB_LAUNCH("paged_decode", (paged_decode_kernel<DT, D, true, true>), grid, block, st, b);  \
+    else if (q4)                                                                                \
+      SB_LAUNCH("paged_decode", (paged_decode_kernel<DT, D, true, false>), grid, block, st, b); \
+    else if (uniform)                                                                           \
+      SB_LAUNCH("paged_decode", (paged_decode_kernel<DT, D, false, true>), grid, block, st, b); \
+    else                                                                                        \
+      SB_LAUNCH("paged_decode", (paged_decode_kernel<DT, D, false, false>), grid, block, st, b); \
     SB_MERGE(DT, D, kDecodeRows, 32, b, pl.few)                                                 \
   }
 #define SB_FEW_BF16(D) SB_FEW(SB_DTYPE_BF16, D)

@@ -67,10 +67,22 @@ class QuantizedKVCache:
             raise ValueError("codes and scales need unit last strides")
         if codes.device != scales.device:
             raise RuntimeError("codes and scales on different devices")
-        self.codes, self.scales = codes, scales
+        self._codes, self._scales = codes, scales
         nb, _, heads, bs, half = codes.shape
         self.shape = (nb, 2, heads, bs, 2 * half)
         self.device = codes.device
+        # what every call passes of it (the tensors are held, so their addresses stay theirs)
+        self._args = (self.shape, codes.data_ptr(), scales.data_ptr(),
+                      _stride_array(codes.stride()), _stride_array(scales.stride()),
+                      _lib.SB_DTYPE_MXFP4)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
 
     @classmethod
     def allocate(cls, num_blocks: int, num_kv_heads: int, block_size: int, head_dim: int,
@@ -83,23 +95,30 @@ class QuantizedKVCache:
                    torch.zeros((*shape, head_dim // 32), dtype=torch.uint8, device=device))
 
 
-def _cache_args(kv_cache, dtype: torch.dtype):
-    """(device, shape, base, scale base, strides, scale strides, dtype code) of either cache."""
+def _cache_args(kv_cache, dtype: torch.dtype, *rows):
+    """(device, shape, base, scale base, strides, scale strides, dtype code) of either cache; the
+    ``rows`` tensors must be on its device."""
     if isinstance(kv_cache, QuantizedKVCache):
-        dev = _lib.require_device(kv_cache.codes, kv_cache.scales)
-        return (dev, kv_cache.shape, kv_cache.codes.data_ptr(), kv_cache.scales.data_ptr(),
-                _stride_array(kv_cache.codes.stride()),
-                _stride_array(kv_cache.scales.stride()), _lib.SB_DTYPE_MXFP4)
-    dev = _lib.require_device(kv_cache)
-    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2:
+        return (_lib.require_device(kv_cache._codes, *rows), *kv_cache._args)
+    dev = _lib.require_device(kv_cache, *rows)
+    shape, strides = tuple(kv_cache.shape), kv_cache.stride()
+    if len(shape) != 5 or shape[1] != 2:
         raise ValueError("kv_cache must be [num_blocks, 2, num_kv_heads, block_size, head_dim]")
     if kv_cache.dtype != dtype:
         raise TypeError("the rows and kv_cache must share a dtype (or kv_cache be a "
                         "QuantizedKVCache)")
-    if kv_cache.stride(4) != 1:
+    if strides[4] != 1:
         raise ValueError("kv_cache needs a unit last stride")
-    return (dev, tuple(kv_cache.shape), kv_cache.data_ptr(), None, _stride_array(kv_cache.stride()), None,
+    return (dev, shape, kv_cache.data_ptr(), None, _stride_array(strides), None,
             _lib.dtype_code(kv_cache))
+
+
+def _index(t, dev) -> torch.Tensor:
+    """``_lib.as_index`` with the usual case (already a device index array) first."""
+    if type(t) is torch.Tensor and t.dtype == torch.int32 and t.device == dev and t.dim() == 1 \
+            and t.is_contiguous():
+        return t
+    return _lib.as_index(t, dev)
 
 
 def _batch_args(dev, num_rows: int, block_tables, positions, row_starts):
@@ -111,19 +130,19 @@ def _batch_args(dev, num_rows: int, block_tables, positions, row_starts):
     if bt.dim() == 1:
         if row_starts is not None:
             raise ValueError("row_starts goes with block_tables [num_requests, max_blocks]")
-        bt = _lib.as_index(bt, dev).unsqueeze(0)
+        bt = _index(bt, dev).unsqueeze(0)
     elif bt.dim() != 2:
         raise ValueError("block_tables must be [num_requests, max_blocks], or [max_blocks] for "
                          "one request")
-    elif bt.device != dev or bt.dtype != torch.int32 or (bt.shape[1] > 1 and bt.stride(1) != 1):
+    elif bt.dtype != torch.int32 or bt.device != dev or (bt.shape[1] > 1 and bt.stride(1) != 1):
         shape = bt.shape
-        bt = _lib.as_index(bt.reshape(-1), dev).view(shape)
-    pos = _lib.as_index(positions, dev)
+        bt = _index(bt.reshape(-1), dev).view(shape)
+    pos = _index(positions, dev)
     if pos.shape[0] != num_rows:
         raise ValueError("positions must have one entry per row")
     requests = bt.shape[0]
     if row_starts is not None:
-        row_starts = _lib.as_index(row_starts, dev)
+        row_starts = _index(row_starts, dev)
         if row_starts.shape[0] != requests + 1:
             raise ValueError("row_starts must have num_requests + 1 entries")
     elif num_rows > requests != 1:
@@ -170,8 +189,8 @@ def append_kv_paged(
     Extension with no reference counterpart (``partial_prefill`` writes its new K/V into
     contiguous caches, semblend_core/triton_kernels.py:904-909).
     """
-    dev, shape, base, sbase, st, sst, code = _cache_args(kv_cache, key.dtype)
-    _lib.require_device(key, value, query, query_out, *_tensors(kv_cache))
+    dev, shape, base, sbase, st, sst, code = _cache_args(kv_cache, key.dtype, key, value, query,
+                                                         query_out)
     _, _, heads, bs, d = shape
     if value.dtype != key.dtype or (query is not None and query.dtype != key.dtype):
         raise TypeError("key, value and query must share a dtype")
@@ -189,7 +208,8 @@ def append_kv_paged(
     if query is not None:
         q = _rows3(query, "query", num, d)
         if query_out is None:
-            query_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            query_out = (torch.empty_like(q) if q.is_contiguous()
+                         else torch.empty(q.shape, dtype=q.dtype, device=dev))
         elif query_out.shape != q.shape or query_out.dtype != q.dtype or query_out.stride(2) != 1:
             raise ValueError("query_out must be like query, with a unit last stride")
     elif query_out is not None:
@@ -199,7 +219,7 @@ def append_kv_paged(
     bt, pos, starts, requests = _batch_args(dev, num, block_tables, positions, row_starts)
     rot = None
     if rotations is not None:
-        rot = _lib.as_index(rotations, dev)
+        rot = _index(rotations, dev)
         if rot.shape[0] != num:
             raise ValueError("rotations must have one entry per token")
     inv = inv_freq_table(rope_base, d, dev) if rope_base is not None else None
@@ -215,11 +235,6 @@ def append_kv_paged(
             _lib.stream_handle(dev),
         )
     return query_out
-
-
-def _tensors(kv_cache):
-    return ((kv_cache.codes, kv_cache.scales) if isinstance(kv_cache, QuantizedKVCache)
-            else (kv_cache,))
 
 
 def gather_kv_paged(
@@ -243,10 +258,10 @@ def gather_kv_paged(
         dtype = torch.bfloat16 if quant else kv_cache.dtype
     dev, shape, base, sbase, st, sst, code = _cache_args(kv_cache, dtype)
     _, _, heads, bs, d = shape
-    bt = _lib.as_index(block_table, dev)
+    bt = _index(block_table, dev)
     pos = None
     if positions is not None:
-        pos = _lib.as_index(positions, dev)
+        pos = _index(positions, dev)
         if num_rows is not None and num_rows != pos.shape[0]:
             raise ValueError("num_rows and positions differ")
         num_rows = pos.shape[0]
@@ -305,8 +320,7 @@ def paged_attention(
     """
     if query.dim() != 3:
         raise ValueError("query must be [rows, num_q_heads, head_dim]")
-    dev, shape, base, sbase, st, sst, code = _cache_args(kv_cache, query.dtype)
-    _lib.require_device(query, out, *_tensors(kv_cache))
+    dev, shape, base, sbase, st, sst, code = _cache_args(kv_cache, query.dtype, query, out)
     num, hq, d = query.shape
     nb, _, heads, bs, hd = shape
     if hd != d:
@@ -321,7 +335,8 @@ def paged_attention(
     if scale is None:
         scale = 1.0 / math.sqrt(d)
     if out is None:
-        out = torch.empty((num, hq, d), dtype=query.dtype, device=dev)
+        out = (torch.empty_like(q) if q.is_contiguous()
+               else torch.empty((num, hq, d), dtype=q.dtype, device=dev))
     elif out.shape != query.shape or out.dtype != query.dtype or out.stride(2) != 1:
         raise ValueError("out must be like query, with a unit last stride")
     dt = _lib.dtype_code(q)
