@@ -645,7 +645,8 @@ int64_t sb_paged_attention_workspace_size(int64_t num_rows, int64_t num_requests
                                           int64_t max_rows, int64_t num_q_heads,
                                           int64_t num_kv_heads, int64_t head_dim,
                                           int64_t block_size, int64_t num_blocks_per_seq,
-                                          int64_t window, int64_t sinks, int32_t dtype);
+                                          int64_t window, int64_t sinks, int32_t dtype,
+                                          int32_t cache_dtype);
 int sb_paged_attention(void* out, const void* q, const void* kv_cache, const void* kv_scales,
                        const int32_t* block_tables, int64_t table_stride,
                        const int32_t* positions, const int32_t* row_starts, void* workspace,

@@ -138,7 +138,7 @@ SIZE_QUERIES: dict[str, list] = {
     "sb_masked_qkv_projection_workspace_size": [_i64],
     "sb_qkv_projection_paged_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i32],
     "sb_paged_attention_workspace_size": [_i64, _i64, _i32, _i64, _i64, _i64, _i64, _i64, _i64,
-                                          _i64, _i64, _i32],
+                                          _i64, _i64, _i32, _i32],
 }
 
 # Python index lists to host arrays (csrc/sb_host.cpp): None until first wanted, False where it

@@ -432,6 +432,8 @@ __device__ __forceinline__ void join_waves(const PagedArgs& a, const float* area
 // lies in one page, so its offset is a scalar: the offsets of 32 steps are looked up at once, two
 // per step in the lanes, and read from there (the scale bytes' are a sixteenth of the codes', as a
 // row's bytes are). Other block sizes and strides look every lane's keys up.
+// Four waves: a CU takes in about 40 GB/s whatever it runs, so a workgroup of eight is no faster
+// (one row of 1000, 14 / 2 heads x 64: 9.1 against 7.8 us); few long rows are split instead.
 template <int DT, int D, bool Q4, bool UNIFORM>
 __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_kernel(const PagedArgs a) {
   using M = Mma<DT>;
@@ -1773,26 +1775,31 @@ struct PagedPlan {
 constexpr int kFewRows = 32;       // 16-bit arithmetic: two row tiles of 16
 constexpr int kRowsMinTiles = 4;   // fewest 64-key tiles of a split of the rows kernel
 
-// Splits of each of `items` row tiles over `tiles` key tiles, `waves` of a workgroup taking a share
-// of them each: those that a launch of `slots` workgroups at a time takes the fewest rounds x (key
-// tiles of a wave + a workgroup's fixed cost, in key tiles) for. With more than one, the merge
-// launch counts `merge` and the partials `parts` key tiles a round.
-int split_for(int64_t items, int64_t slots, int64_t tiles, int waves, int min_tiles, int fixed,
-              int merge, int parts) {
+// Splits of each of `items` row tiles over `tiles` key tiles: those that 256 CUs take the shortest
+// for, in rounds of a workgroup's fixed time and its tiles' (which two workgroups of a CU share),
+// and with more than one split the merge's, and `part` for a split's partials.
+int split_for(int64_t items, int64_t tiles, int min_tiles, int64_t tile_ns, int64_t fixed_ns,
+              int64_t merge_ns, int64_t part_ns) {
+  constexpr int64_t kCus = 256;
   int64_t best = 1, cost = 0;
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(tiles / min_tiles, 128));
-  for (int64_t n = 1; n <= most && items * (n - 1) < 2 * slots; ++n) {
-    const int64_t rounds = (items * n + slots - 1) / slots;
-    const int64_t c = rounds * ((tiles + n * waves - 1) / (n * waves) + fixed) +
-                      (n > 1 ? merge + rounds * parts + items * n * parts / slots : 0);
+  for (int64_t n = 1; n <= most && items * (n - 1) < 2 * kCus; ++n) {
+    const int64_t rounds = (items * n + kCus - 1) / kCus;
+    const int64_t c = rounds * ((tiles + n - 1) / n * tile_ns + fixed_ns) +
+                      (n > 1 ? merge_ns + rounds * part_ns + items * n * part_ns / kCus : 0);
     if (n == 1 || c < cost) best = n, cost = c;
   }
   return static_cast<int>(best);
 }
 
+int64_t row_bytes(int64_t head_dim, int32_t dtype, bool q4) {
+  return q4 ? head_dim / 2 + head_dim / 32 : head_dim * elem_size(dtype);
+}
+
 PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_t max_rows,
                      int64_t num_kv_heads, int64_t group, int64_t head_dim, int64_t kv_len,
-                     int64_t window, int64_t sinks, int32_t dtype, bool matrix) {
+                     int64_t window, int64_t sinks, int32_t dtype, int64_t bytes_per_row,
+                     bool matrix) {
   PagedPlan pl = {};
   pl.matrix = matrix && (head_dim == 64 || head_dim == 128);
   if (!pl.matrix) return pl;
@@ -1814,22 +1821,24 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
                                          : std::min<int64_t>(tiles_bound, flat);
     const int64_t key_tiles = (keys + (f32 ? 15 : 31)) / (f32 ? 16 : 32);
     const int64_t items = pl.few.tiles * num_kv_heads;
+    const int kt = f32 ? 16 : 32;
+    const int64_t most_tiles =  // of any row
+        std::min<int64_t>((kv_len + kt - 1) / kt,
+                          (std::min(window, kv_len) + kt - 2) / kt + 1 + (sinks + kt - 1) / kt);
     pl.few.min_tiles = kFewMinTiles;
-    pl.few.nsplit = split_for(items, kFewSlots, key_tiles, kDecodeWaves, kFewMinTiles, 8, 10, 1);
+    // (a workgroup's start and end take about 4 us, the merge launch 5)
+    const int64_t tile_ns = std::max<int64_t>(110, 2 * kt * bytes_per_row / 40);
+    pl.few.nsplit = split_for(items, key_tiles, kFewMinTiles, tile_ns, 4000, 5000, 0);
     if (!ragged || num_rows == 1) {
       // Balanced items, unless there are enough of them as they are and none is long.
       const bool split = pl.few.nsplit > 1 || key_tiles > kLongTiles;
       pl.few.target = split ? kFewTarget : 0;
       pl.few.nsplit = 1;
     }
-    const int kt = f32 ? 16 : 32;
-    const int64_t most_tiles =  // of any row
-        std::min<int64_t>((kv_len + kt - 1) / kt,
-                          (std::min(window, kv_len) + kt - 2) / kt + 1 + (sinks + kt - 1) / kt);
     // (a row of t tiles has at most t / size + 1 items, of `size` tiles, and all tiles are at most
     // target * size)
     pl.few.grid = pl.few.target > 0
-                      ? items + std::min<int64_t>(kFewTarget, items * (most_tiles / kFewMinTiles))
+                      ? items + std::min<int64_t>(kFewTarget, items * (most_tiles / pl.few.min_tiles))
                       : items * pl.few.nsplit;
     const int64_t slots =
         pl.few.target > 0 || pl.few.nsplit > 1 ? pl.few.grid * kDecodeRows : 0;
@@ -1841,8 +1850,10 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
     pl.rows.tiles = std::min<int64_t>(flat / kRowsTile + num_requests,
                                       (flat + kFewRows - 1) / kFewRows);
     pl.rows.min_tiles = kRowsMinTiles;
-    pl.rows.nsplit = split_for(((flat + kRowsTile - 1) / kRowsTile) * num_kv_heads, 256,
-                               (keys + 63) / 64, 1, kRowsMinTiles, 5, 2, 3);
+    // (a tile takes about 2.2 us at head_dim 128, a workgroup's start and end about 10)
+    const int64_t tile_ns = 2200 * head_dim / 128;
+    pl.rows.nsplit = split_for(((flat + kRowsTile - 1) / kRowsTile) * num_kv_heads,
+                               (keys + 63) / 64, kRowsMinTiles, tile_ns, 10000, 5000, 6000);
     pl.rows.grid = pl.rows.tiles * num_kv_heads * pl.rows.nsplit;
     const int64_t slots = pl.rows.nsplit > 1 ? pl.rows.grid * kRowsTile : 0;
     pl.rows.o_floats = slots * head_dim;
@@ -1860,7 +1871,8 @@ extern "C" int64_t sb_paged_attention_workspace_size(int64_t num_rows, int64_t n
                                                      int64_t num_q_heads, int64_t num_kv_heads,
                                                      int64_t head_dim, int64_t block_size,
                                                      int64_t num_blocks_per_seq, int64_t window,
-                                                     int64_t sinks, int32_t dtype) {
+                                                     int64_t sinks, int32_t dtype,
+                                                     int32_t cache_dtype) {
   using namespace sb;
   if (num_rows <= 0 || num_requests <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
       num_q_heads % num_kv_heads || block_size <= 0 || num_blocks_per_seq <= 0 || window < 0 ||
@@ -1870,7 +1882,8 @@ extern "C" int64_t sb_paged_attention_workspace_size(int64_t num_rows, int64_t n
   return plan_paged(num_rows, num_requests, has_starts != 0,
                     max_rows > 0 && max_rows < num_rows ? max_rows : num_rows, num_kv_heads,
                     num_q_heads / num_kv_heads, head_dim, kv_len,
-                    window > 0 ? window : kNoWindow, sinks, dtype, true)
+                    window > 0 ? window : kNoWindow, sinks, dtype,
+                    row_bytes(head_dim, dtype, cache_dtype == SB_DTYPE_MXFP4), true)
       .bytes;
 }
 
@@ -1966,7 +1979,7 @@ extern "C" int sb_paged_attention(
   const PagedPlan pl = plan_paged(num_rows, num_requests, row_starts != nullptr,
                                   max_rows > 0 && max_rows < num_rows ? max_rows : num_rows,
                                   num_kv_heads, group, head_dim, a.kv_len, a.window, a.sinks,
-                                  dtype, matrix);
+                                  dtype, row_bytes(head_dim, dtype, q4), matrix);
   if (pl.bytes > workspace_bytes || (pl.bytes && !workspace))
     return fail(fn, "workspace too small");
   if (workspace && addr(workspace) % 16) return fail(fn, "workspace must be 16-byte aligned");
@@ -2044,16 +2057,14 @@ extern "C" int sb_paged_attention(
     // (a lane's offset inside a group of 16 keys is 32 bits there)
     const bool uniform = block_size % 16 == 0 && a.c_pos >= 0 && a.c_pos < (1 << 27) &&
                          (!q4 || (a.c_block == 16ull * a.s_block && a.c_pos == 16 * a.s_pos));
+#define SB_FEW_K(DT, D, Q4, U)                                                                  \
+  { SB_LAUNCH("paged_decode", (paged_decode_kernel<DT, D, Q4, U>), grid, block, st, b); }
 #define SB_FEW(DT, D)                                                                           \
   {                                                                                             \
-    if (q4 && uniform)                                                                          \
-      SB_LAUNCH("paged_decode", (paged_decode_kernel<DT, D, true, true>), grid, block, st, b);  \
-    else if (q4)                                                                                \
-      SB_LAUNCH("paged_decode", (paged_decode_kernel<DT, D, true, false>), grid, block, st, b); \
-    else if (uniform)                                                                           \
-      SB_LAUNCH("paged_decode", (paged_decode_kernel<DT, D, false, true>), grid, block, st, b); \
-    else                                                                                        \
-      SB_LAUNCH("paged_decode", (paged_decode_kernel<DT, D, false, false>), grid, block, st, b); \
+    if (q4 && uniform) SB_FEW_K(DT, D, true, true)                                              \
+    else if (q4) SB_FEW_K(DT, D, true, false)                                                   \
+    else if (uniform) SB_FEW_K(DT, D, false, true)                                              \
+    else SB_FEW_K(DT, D, false, false)                                                          \
     SB_MERGE(DT, D, kDecodeRows, 32, b, pl.few)                                                 \
   }
 #define SB_FEW_BF16(D) SB_FEW(SB_DTYPE_BF16, D)

@@ -346,7 +346,7 @@ def paged_attention(
     most = num if max_rows is None else max(1, int(max_rows))
     win = 0 if window is None else min(int(window), 0x7fffffff)
     ws_bytes = _workspace_bytes(num, requests, int(starts is not None), most, hq, heads, d, bs,
-                                bt.shape[1], win, int(sinks), dt)
+                                bt.shape[1], win, int(sinks), dt, code)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     with _lib.on_device(dev):
         _lib.call(

@@ -621,18 +621,21 @@ def test_graph_decode_step(dev, quant):
     k, v, q = (torch.zeros((3, h, d), dtype=BF16, device="cuda") for h in (hkv, hkv, hq))
     pos = torch.tensor([5, 6, 7], dtype=torch.int32).cuda()
 
-    def step(c):
+    def step(c, outs=(None, None)):
         qr = pc.append_kv_paged(c, k, v, t, pos, rope_base=1e6, query=q)
-        return (pc.paged_attention(qr, c, t, pos),
-                pc.paged_attention(qr, c, t, pos, window=100, sinks=4))
+        return (pc.paged_attention(qr, c, t, pos, out=outs[0]),
+                pc.paged_attention(qr, c, t, pos, window=100, sinks=4, out=outs[1]))
 
     step(copy), step(cache)      # (both caches hold this step's tokens; nothing is captured yet)
     torch.cuda.synchronize()
     graphs = []
     for _ in range(2):
+        # (outputs of the caller's: memory that a graph allocates serves it for other things, so
+        # padding rows could not be seen to stay as they were)
+        out = (torch.empty_like(q), torch.empty_like(q))
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            out = step(cache)
+            step(cache, out)
         graphs.append((g, out))
     for r in range(4):
         for x, s in ((k, 1), (v, 2), (q, 3)):

@@ -188,11 +188,11 @@ def test_empty_calls():
 def test_workspace_query():
     size = lambda *a: _lib.size_query("sb_paged_attention_workspace_size", *a)
     # one row over a long context is split; 512 of them over short ones are not
-    assert size(1, 1, 0, 1, 28, 4, 128, 16, 1000, 0, 0, 2) > 0
-    assert size(512, 512, 0, 1, 32, 8, 128, 16, 100, 0, 0, 2) == 0
-    assert size(1, 1, 0, 1, 28, 4, 96, 16, 1000, 0, 0, 2) == 0      # not on the matrix cores
-    assert size(0, 1, 0, 1, 28, 4, 128, 16, 1000, 0, 0, 2) == 0
-    assert size(4, 1, 0, 1, 28, 3, 128, 16, 1000, 0, 0, 2) == 0
+    assert size(1, 1, 0, 1, 28, 4, 128, 16, 1000, 0, 0, 2, 2) > 0
+    assert size(512, 512, 0, 1, 32, 8, 128, 16, 100, 0, 0, 2, 2) == 0
+    assert size(1, 1, 0, 1, 28, 4, 96, 16, 1000, 0, 0, 2, 2) == 0      # not on the matrix cores
+    assert size(0, 1, 0, 1, 28, 4, 128, 16, 1000, 0, 0, 2, 3) == 0
+    assert size(4, 1, 0, 1, 28, 3, 128, 16, 1000, 0, 0, 2, 2) == 0
 
 
 def test_reference_quantiser():
