@@ -10,11 +10,14 @@
 //
 // Arithmetic: the angle p * f_i is formed and reduced in 64 bits (f_i the fp32 frequencies): its
 // fp32 product is off by 2^-11 at position 16384, a quarter of a bf16 rounding. 16-bit pages take
-// the rotation itself in fp32 with one rounding. fp32 and 4-bit pages take it in 64 bits, the
-// latter because a value next to a border between two codes must fall on the right side: the
-// 64-bit result is rounded to fp32 to odd, which keeps every comparison with a border (borders
-// have few bits, an odd last bit never equals one), then scaled and rounded to nearest even by
-// v_cvt_scalef32_pk_fp4_f32.
+// the rotation itself in fp32 with one rounding, fp32 pages in 64 bits. For 4-bit pages a value
+// next to a border between two codes must fall on the side where its 64-bit value lies: blocks
+// are rotated in fp32 and rounded to nearest even by v_cvt_scalef32_pk_fp4_f32, and again with
+// the error's bound added and taken off; where the three agree on codes and scale the 64-bit
+// result has the same ones. The others (one block in some thousands) are rotated in 64 bits and
+// rounded to fp32 to odd, which keeps every comparison with a border (borders have few bits, an
+// odd last bit never equals one), then rounded the same way. (All blocks in 64 bits: 16000 tokens
+// of 8 heads x 128 32 us.)
 //
 // What bounds it: bytes for prompts, the launch and one dependent chain (position, table entry,
 // row) for decode steps. One workgroup takes a few tokens with all their heads, so that each
@@ -98,9 +101,11 @@ template <int DT, int VEC> struct RowVec {
   }
   __device__ __forceinline__ void store(char* p) const {
     if constexpr (kWide) {
-      uint4 w;
+      // (nontemporal: append of 4602 tokens of 32 / 8 heads x 128 24.4 -> 21.1 us)
+      typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+      u32x4 w;
       __builtin_memcpy(&w, e, 16);
-      *reinterpret_cast<uint4*>(p) = w;
+      __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p));
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) reinterpret_cast<T*>(p)[i] = e[i];
@@ -118,6 +123,47 @@ __device__ __forceinline__ float round_to_odd(double x) {
   return __uint_as_float(u);
 }
 
+// The scale byte of a block whose largest magnitude is `top`, a number: top in
+// [4, 8) * 2^(E - 2 - 127), and one power more above 7 (mantissa above 1.75).
+__device__ __forceinline__ int scale_byte(float top) {
+  const uint32_t u = __float_as_uint(top);
+  return max(static_cast<int>(u >> 23) - 2 + ((u & 0x7fffffu) > 0x600000u), 0);
+}
+template <int VEC>
+__device__ __forceinline__ uint32_t pack_codes(const float (&f)[VEC], float scale) {
+  uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0], f[1], scale, 0);
+  if constexpr (VEC >= 4) w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[2], f[3], scale, 1);
+  if constexpr (VEC >= 8) {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[4], f[5], scale, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[6], f[7], scale, 3);
+  }
+  return w;
+}
+// VEC values of a block of 32 (the lanes' others are 32 / VEC neighbours') as codes; a block that
+// holds an infinity or a NaN is marked as one by scale byte 255.
+template <int VEC> struct Block {
+  uint32_t codes;
+  int byte;
+  float top, scale;
+};
+template <int VEC>
+__device__ __forceinline__ Block<VEC> quantize(const float (&f)[VEC]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = 16 / VEC; o >= 1; o >>= 1)
+    top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, 64)));
+  Block<VEC> b;
+  b.top = __uint_as_float(top);
+  const bool bad = top >= 0x7f800000u;
+  b.byte = bad ? 255 : scale_byte(b.top);
+  // (byte 0 is 2^-127, below fp32's normal numbers)
+  b.scale = __uint_as_float(b.byte > 0 && !bad ? static_cast<uint32_t>(b.byte) << 23 : 0x00400000u);
+  b.codes = bad ? 0u : pack_codes(f, b.scale);
+  return b;
+}
+
 // A thread takes vector tid % vpr of rows tid / vpr + k rpi (K, V, then query heads, token after
 // token), kRowsInFlight of them at a time. (Requesting the first ones before the positions, table
 // entries and sines are known was slower for prompts: 28.5 against 24.3 us for 4602 tokens of
@@ -125,10 +171,11 @@ __device__ __forceinline__ float round_to_odd(double x) {
 constexpr int kRowsInFlight = 4;
 template <int DT, int VEC, bool Q4>
 __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendArgs a) {
-  constexpr bool kWide64 = Q4 || DT == SB_DTYPE_F32;  // rotate in 64 bits
-  using CS = std::conditional_t<kWide64, double, float>;
+  using CS = std::conditional_t<DT == SB_DTYPE_F32, double, float>;
+  constexpr bool kBoth = Q4 && DT != SB_DTYPE_F32;         // 64-bit sines and cosines besides
   constexpr int ES = sizeof(typename Elem<DT>::T);
-  __shared__ CS cs[2 * kTableEntries];
+  __shared__ CS cs[2 * kTableEntries];                    // cosine, sine of each (token, pair)
+  __shared__ double cs64[kBoth ? 2 * kTableEntries : 1];
   __shared__ int64_t tok_c[kTokensMax];  // page and slot byte offset in the cache, -1: no slot
   __shared__ int64_t tok_s[kTokensMax];  // ... and in the scale bytes
   __shared__ int tok_live[kTokensMax];
@@ -194,6 +241,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
       sincos_cw(static_cast<double>(p) * static_cast<double>(a.inv_freq[f]), &s, &c);
       cs[2 * i] = static_cast<CS>(c);
       cs[2 * i + 1] = static_cast<CS>(s);
+      if constexpr (kBoth) cs64[2 * i] = c, cs64[2 * i + 1] = s;
     }
   }
   __syncthreads();
@@ -217,15 +265,8 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
         const CS e = Elem<DT>::get(x[u].e[i]), o = Elem<DT>::get(x[u].e[i + 1]);
         if (turn) {
           const CS c = trig[i], s = trig[i + 1];
-          const CS r0 = e * c - o * s, r1 = e * s + o * c;
-          if constexpr (Q4) {
-            // (a query is not quantised: its one rounding is from the 64-bit value)
-            f[i] = j < hk ? round_to_odd(r0) : static_cast<float>(r0);
-            f[i + 1] = j < hk ? round_to_odd(r1) : static_cast<float>(r1);
-          } else {
-            f[i] = static_cast<float>(r0);
-            f[i + 1] = static_cast<float>(r1);
-          }
+          f[i] = static_cast<float>(e * c - o * s);
+          f[i + 1] = static_cast<float>(e * s + o * c);
         } else {
           f[i] = static_cast<float>(e);
           f[i + 1] = static_cast<float>(o);
@@ -233,29 +274,36 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
       }
       if (Q4 && j < 2 * hk) {
         const int kv = j >= hk, h = j - kv * hk;
-        uint32_t top = 0;
+        Block<VEC> b = quantize(f);
+        if (turn) {
+          // A rotated fp32 value is off by at most 2^-22 of its pair's norm (products and sum
+          // 2^-24 each, sine and cosine 2^-24): 2^-21 of the block's largest magnitude, which is
+          // below 2^-18 of the scale.
+          bool unsure = b.byte == 255 || scale_byte(b.top * (1.f - 0x1p-20f)) !=
+                                             scale_byte(b.top * (1.f + 0x1p-20f));
+          const float off = b.scale * 0x1p-18f;
+          float lo[VEC], hi[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+          for (int i = 0; i < VEC; ++i) lo[i] = f[i] - off, hi[i] = f[i] + off;
+          unsure |= pack_codes(lo, b.scale) != pack_codes(hi, b.scale);
+          int any = unsure;
 #pragma unroll
-        for (int o = 16 / VEC; o >= 1; o >>= 1)  // the 32 / VEC lanes of the block
-          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, 64)));
-        // top in [4, 8) * 2^(E - 2 - 127); one power more above 7 (mantissa above 1.75). A
-        // block that holds an infinity or a NaN is marked as one: scale byte 255.
-        const bool bad = top >= 0x7f800000u;
-        const int e = static_cast<int>(top >> 23) - 2 + ((top & 0x7fffffu) > 0x600000u);
-        const int sb = bad ? 255 : max(e, 0);
-        const float scale = __uint_as_float(sb > 0 && !bad ? static_cast<uint32_t>(sb) << 23
-                                                           : 0x00400000u);
-        uint32_t w = 0;
-        if (!bad) {
-          w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[0], f[1], scale, 0);
-          if constexpr (VEC >= 4)
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[2], f[3], scale, 1);
-          if constexpr (VEC >= 8) {
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[4], f[5], scale, 2);
-            w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[6], f[7], scale, 3);
+          for (int o = 16 / VEC; o >= 1; o >>= 1) any |= __shfl_xor(any, o, 64);
+          if (any) {
+            const double* t64;
+            if constexpr (kBoth) t64 = cs64 + 2 * (tok * half + vec * (VEC / 2));
+            else t64 = reinterpret_cast<const double*>(trig);
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) {
+              const double e = Elem<DT>::get(x[u].e[i]), o = Elem<DT>::get(x[u].e[i + 1]);
+              f[i] = round_to_odd(e * t64[i] - o * t64[i + 1]);
+              f[i + 1] = round_to_odd(e * t64[i + 1] + o * t64[i]);
+            }
+            b = quantize(f);
           }
         }
+        const uint32_t w = b.codes;
+        const int sb = b.byte;
         char* dst = a.cache + oc + kv * a.c_kv + h * a.c_head + vec * (VEC / 2);
         if constexpr (VEC == 8) *reinterpret_cast<uint32_t*>(dst) = w;
         else if constexpr (VEC == 4) *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(w);

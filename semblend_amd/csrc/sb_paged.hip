@@ -298,11 +298,13 @@ struct Item {
 };
 
 // Items of even splits: every row tile has its keys split nsplit ways (fewer if they are few); KV
-// head fastest, then row tile, then split. (nsplit is filled in once the tile's positions are read.)
+// head fastest, then row tile (the last one, which sees most, first), then split. (nsplit is filled
+// in once the tile's positions are read.)
 template <int TR>
 __device__ __forceinline__ Item even_item(const PagedArgs& a, int b) {
   const int rest = b / a.num_kv_heads, split = rest / a.num_tiles;
-  const int tile_idx = rest - split * a.num_tiles, kvh = b - rest * a.num_kv_heads;
+  const int kvh = b - rest * a.num_kv_heads;
+  const int tile_idx = a.num_tiles - 1 - (rest - split * a.num_tiles);
   return {kvh, 1, split,
           (static_cast<int64_t>(tile_idx) * a.num_kv_heads + kvh) * a.nsplit + split,
           find_tile<TR>(a, tile_idx)};
@@ -547,8 +549,12 @@ __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_ke
         asm volatile("" : "+s"(kg), "+s"(vg));
 #pragma unroll
         for (int s = 0; s < RAW; ++s) {
-          st.k[h][s] = *(const SB_GLOBAL raw_t*)(kg + lane_row + 64 * s);
-          st.v[h][s] = *(const SB_GLOBAL raw_t*)(vg + lane_row + 64 * s);
+          // (nontemporal for 4-bit rows: 32 requests of up to 32K tokens 119 -> 107 us; 16-bit
+          // ones lose by it, 64 requests under a window of 4096 170 -> 181 us)
+          const SB_GLOBAL raw_t* kr = (const SB_GLOBAL raw_t*)(kg + lane_row + 64 * s);
+          const SB_GLOBAL raw_t* vr = (const SB_GLOBAL raw_t*)(vg + lane_row + 64 * s);
+          st.k[h][s] = Q4 ? __builtin_nontemporal_load(kr) : *kr;
+          st.v[h][s] = Q4 ? __builtin_nontemporal_load(vr) : *vr;
         }
         if constexpr (Q4) {
           const SB_GLOBAL char* ksg = (const SB_GLOBAL char*)(ksb + (off >> 4));
@@ -1828,7 +1834,9 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
     pl.few.min_tiles = kFewMinTiles;
     // (a workgroup's start and end take about 4 us, the merge launch 5)
     const int64_t tile_ns = std::max<int64_t>(110, 2 * kt * bytes_per_row / 40);
-    pl.few.nsplit = split_for(items, key_tiles, kFewMinTiles, tile_ns, 4000, 5000, 0);
+    // (beside the rows kernel most of `tiles` are empty: one a request, about)
+    pl.few.nsplit = split_for(rows_kernel ? std::min(items, num_requests * num_kv_heads) : items,
+                              key_tiles, kFewMinTiles, tile_ns, 4000, 5000, 0);
     if (!ragged || num_rows == 1) {
       // Balanced items, unless there are enough of them as they are and none is long.
       const bool split = pl.few.nsplit > 1 || key_tiles > kLongTiles;
