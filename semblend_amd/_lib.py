@@ -246,9 +246,14 @@ def call(name: str, *args) -> None:
     """Invoke an entry point and turn a nonzero status into RuntimeError."""
     rc = getattr(lib(), name)(*args)
     if rc != SB_OK:
-        msg = lib().sb_last_error_string().decode()
-        kind = "invalid argument" if rc == SB_ERR_INVALID_ARGUMENT else f"hip error {rc}"
-        raise RuntimeError(f"{name} failed ({kind}): {msg}")
+        raise_status(name, rc)
+
+
+def raise_status(name: str, rc: int) -> None:
+    """RuntimeError for the nonzero status of an entry point."""
+    msg = lib().sb_last_error_string().decode()
+    kind = "invalid argument" if rc == SB_ERR_INVALID_ARGUMENT else f"hip error {rc}"
+    raise RuntimeError(f"{name} failed ({kind}): {msg}")
 
 
 # ------------------------------------------------------------------------------------------
@@ -330,6 +335,21 @@ def on_device(device: torch.device):
     if _current_index is not None and _current_index() == _index(device):
         return contextlib.nullcontext()
     return torch.cuda.device(device)
+
+
+def launch(device: torch.device, name: str, *args) -> None:
+    """Invoke an entry point whose last argument is the stream on ``device``'s current stream,
+    with ``device`` current (``call`` within ``on_device``, for callers that launch a kernel of a
+    few microseconds)."""
+    fn = getattr(_lib or _load(), name)
+    index = device.index
+    if _raw_stream is not None and _current_index is not None and _current_index() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with on_device(device):
+            rc = fn(*args, stream_handle(device))
+    if rc != SB_OK:
+        raise_status(name, rc)
 
 
 # Pinned staging buffers of host-to-device copies recorded into a HIP graph: every replay

@@ -101,7 +101,7 @@ def _cache_args(kv_cache, dtype: torch.dtype, *rows):
     if isinstance(kv_cache, QuantizedKVCache):
         return (_lib.require_device(kv_cache._codes, *rows), *kv_cache._args)
     dev = _lib.require_device(kv_cache, *rows)
-    shape, strides = tuple(kv_cache.shape), kv_cache.stride()
+    shape, strides = kv_cache.shape, kv_cache.stride()
     if len(shape) != 5 or shape[1] != 2:
         raise ValueError("kv_cache must be [num_blocks, 2, num_kv_heads, block_size, head_dim]")
     if kv_cache.dtype != dtype:
@@ -153,13 +153,6 @@ def _batch_args(dev, num_rows: int, block_tables, positions, row_starts):
     return bt, pos, row_starts, requests
 
 
-def _rows3(t: torch.Tensor, name: str, num_rows: int | None, head_dim: int) -> torch.Tensor:
-    if t.dim() != 3 or t.shape[2] != head_dim or (num_rows is not None and t.shape[0] != num_rows):
-        raise ValueError(f"{name} must be [rows, heads, head_dim], one row per token, with the "
-                         "cache's head_dim")
-    return t if t.stride(2) == 1 else t.contiguous()
-
-
 def append_kv_paged(
     kv_cache,
     key: torch.Tensor,
@@ -189,15 +182,19 @@ def append_kv_paged(
     Extension with no reference counterpart (``partial_prefill`` writes its new K/V into
     contiguous caches, semblend_core/triton_kernels.py:904-909).
     """
-    dev, shape, base, sbase, st, sst, code = _cache_args(kv_cache, key.dtype, key, value, query,
+    dtype = key.dtype
+    dev, shape, base, sbase, st, sst, code = _cache_args(kv_cache, dtype, key, value, query,
                                                          query_out)
     _, _, heads, bs, d = shape
-    if value.dtype != key.dtype or (query is not None and query.dtype != key.dtype):
+    if value.dtype != dtype or (query is not None and query.dtype != dtype):
         raise TypeError("key, value and query must share a dtype")
+    if key.dim() != 3 or key.shape[1:] != (heads, d) or value.shape != key.shape:
+        raise ValueError("key and value must be [tokens, num_kv_heads, head_dim] with the "
+                         "cache's heads and head_dim")
     num = key.shape[0]
-    k, v = _rows3(key, "key", num, d), _rows3(value, "value", num, d)
-    if k.shape[1] != heads or v.shape[1] != heads:
-        raise ValueError("key and value must have the cache's heads")
+    k = key if key.stride(2) == 1 else key.contiguous()
+    v = value if value.stride(2) == 1 else value.contiguous()
+    dt = _lib.dtype_code(key)
     if rope_base is None and (rotations is not None or query is not None):
         raise ValueError("rotations and query go with rope_base")
     if rope_base is not None and not rope_base >= 1.0:
@@ -206,7 +203,9 @@ def append_kv_paged(
         raise ValueError("head_dim must be even")
     q = None
     if query is not None:
-        q = _rows3(query, "query", num, d)
+        if query.dim() != 3 or query.shape[0] != num or query.shape[2] != d:
+            raise ValueError("query must be [tokens, num_q_heads, head_dim]")
+        q = query if query.stride(2) == 1 else query.contiguous()
         if query_out is None:
             query_out = (torch.empty_like(q) if q.is_contiguous()
                          else torch.empty(q.shape, dtype=q.dtype, device=dev))
@@ -223,17 +222,14 @@ def append_kv_paged(
         if rot.shape[0] != num:
             raise ValueError("rotations must have one entry per token")
     inv = inv_freq_table(rope_base, d, dev) if rope_base is not None else None
-    with _lib.on_device(dev):
-        _lib.call(
-            "sb_append_kv_paged",
-            base, sbase, k.data_ptr(), v.data_ptr(), _lib.ptr(q),
-            None if q is None else query_out.data_ptr(), bt.data_ptr(), bt.stride(0),
-            pos.data_ptr(), _lib.ptr(rot), _lib.ptr(starts), _lib.ptr(inv), num, requests, heads,
-            0 if q is None else q.shape[1], d, bs, shape[0], bt.shape[1], _stride_array(k.stride()),
-            _stride_array(v.stride()), None if q is None else _stride_array(q.stride()),
-            None if q is None else _stride_array(query_out.stride()), st, sst, _lib.dtype_code(k), code,
-            _lib.stream_handle(dev),
-        )
+    _lib.launch(
+        dev, "sb_append_kv_paged",
+        base, sbase, k.data_ptr(), v.data_ptr(), _lib.ptr(q),
+        None if q is None else query_out.data_ptr(), bt.data_ptr(), bt.stride(0), pos.data_ptr(),
+        _lib.ptr(rot), _lib.ptr(starts), _lib.ptr(inv), num, requests, heads,
+        0 if q is None else q.shape[1], d, bs, shape[0], bt.shape[1], _stride_array(k.stride()),
+        _stride_array(v.stride()), None if q is None else _stride_array(q.stride()),
+        None if q is None else _stride_array(query_out.stride()), st, sst, dt, code)
     return query_out
 
 
@@ -280,10 +276,9 @@ def gather_kv_paged(
         return out
     if bt.shape[0] == 0:
         return out.zero_()
-    with _lib.on_device(dev):
-        _lib.call("sb_gather_kv_paged", out.data_ptr(), base, sbase, bt.data_ptr(),
-                  _lib.ptr(pos), num_rows, heads, d, bs, shape[0], bt.shape[0],
-                  _stride_array(out.stride()), st, sst, dt, code, _lib.stream_handle(dev))
+    _lib.launch(dev, "sb_gather_kv_paged", out.data_ptr(), base, sbase, bt.data_ptr(),
+                _lib.ptr(pos), num_rows, heads, d, bs, shape[0], bt.shape[0],
+                _stride_array(out.stride()), st, sst, dt, code)
     return out
 
 
@@ -348,12 +343,10 @@ def paged_attention(
     ws_bytes = _workspace_bytes(num, requests, int(starts is not None), most, hq, heads, d, bs,
                                 bt.shape[1], win, int(sinks), dt, code)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    with _lib.on_device(dev):
-        _lib.call(
-            "sb_paged_attention",
-            out.data_ptr(), q.data_ptr(), base, sbase, bt.data_ptr(), bt.stride(0),
-            pos.data_ptr(), _lib.ptr(starts), _lib.ptr(ws), ws_bytes, num, requests, most, hq,
-            heads, d, bs, nb, bt.shape[1], win, int(sinks), float(scale), _stride_array(q.stride()),
-            _stride_array(out.stride()), st, sst, dt, code, _lib.stream_handle(dev),
-        )
+    _lib.launch(
+        dev, "sb_paged_attention",
+        out.data_ptr(), q.data_ptr(), base, sbase, bt.data_ptr(), bt.stride(0), pos.data_ptr(),
+        _lib.ptr(starts), _lib.ptr(ws), ws_bytes, num, requests, most, hq, heads, d, bs, nb,
+        bt.shape[1], win, int(sinks), float(scale), _stride_array(q.stride()),
+        _stride_array(out.stride()), st, sst, dt, code)
     return out

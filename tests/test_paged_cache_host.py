@@ -54,9 +54,7 @@ def on_cpu(monkeypatch):
     cpu = torch.device("cpu")
     monkeypatch.setattr(_lib, "require_device", lambda *t: cpu)
     monkeypatch.setattr(_lib, "as_index", lambda t, d: torch.as_tensor(t).to(torch.int32).reshape(-1))
-    monkeypatch.setattr(_lib, "on_device", lambda d: __import__("contextlib").nullcontext())
-    monkeypatch.setattr(_lib, "stream_handle", lambda d: 0)
-    monkeypatch.setattr(_lib, "call", lambda name, *a: calls.append((name, a)))
+    monkeypatch.setattr(_lib, "launch", lambda dev, name, *a: calls.append((name, a)))
     return calls
 
 
