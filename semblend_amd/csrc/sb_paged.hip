@@ -1498,24 +1498,45 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
   const float l_tot = l_run + xor32(l_run);
   const int other_seen = __shfl_xor(static_cast<int>(seen), 32, 64);  // (by every lane)
   const bool row_seen = seen || other_seen != 0;
-  if (p < 0) return;
+  // The rows go out through LDS, a wave's 32 of them through its eighth of the tiles' memory, so
+  // that a store instruction writes whole rows instead of eight bytes of each: 64 rows of 8 bytes
+  // take 64 cycles of address processing, 16 KB 4 us of a CU (8192 rows of a window of 1: 64 -> 58 us).
+  // 16-byte chunks XOR-swizzled by row.
+  constexpr int kWaveBytes = 32 * D * 2;
+  static_assert(sizeof(Ks) == kRowsWaves / 2 * kWaveBytes, "each of K and V holds half the waves");
+  char* stage = (wave < kRowsWaves / 2 ? reinterpret_cast<char*>(Ks) : reinterpret_cast<char*>(Vs)) +
+                wave % (kRowsWaves / 2) * kWaveBytes;
   if (nsplit > 1) {
-    const int64_t slot = it.slot * kRowsTile + wave * 32 + lq;
-    float* po = a.part_o + slot * D;
+    // fp32 partials, in two halves of the dims
+    const int64_t slot = it.slot * kRowsTile + wave * 32;
+    constexpr int PCH = D / 8;  // chunks of half a row
 #pragma unroll
-    for (int d = 0; d < NDT; ++d)
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<float4*>(po + 32 * d + 8 * e + 4 * lg) =
-            make_float4(o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]);
+      for (int d = 0; d < NDT / 2; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int dd = half * (NDT / 2) + d;
+          const int c = (32 * d + 8 * e + 4 * lg) / 4;
+          *reinterpret_cast<float4*>(stage + lq * (D * 2) + 16 * (c ^ (lq & (PCH - 1)))) =
+              make_float4(o[dd][4 * e], o[dd][4 * e + 1], o[dd][4 * e + 2], o[dd][4 * e + 3]);
+        }
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int k = 0; k < 32 * PCH / 64; ++k) {
+        const int r = (k * 64 + lane) / PCH, c = (k * 64 + lane) % PCH;
+        *reinterpret_cast<float4*>(a.part_o + (slot + r) * D + half * (D / 2) + 4 * c) =
+            *reinterpret_cast<const float4*>(stage + r * (D * 2) + 16 * (c ^ (r & (PCH - 1))));
+      }
+      asm volatile("" ::: "memory");
+    }
     if (lg == 0)
-      *reinterpret_cast<float2*>(a.part_ml + slot * 2) =
-          make_float2(seeded ? m_ref : row_seen ? kSeenNothing : -INFINITY, l_tot);
+      *reinterpret_cast<float2*>(a.part_ml + (slot + lq) * 2) =
+          make_float2(seeded && p >= 0 ? m_ref : row_seen ? kSeenNothing : -INFINITY, l_tot);
     return;
   }
   const float out_scale = Q4 ? static_cast<float>(1 << H::kShift) : 1.f;
   const float inv = !row_seen ? 0.f : out_scale / l_tot;
-  char* op = a.o + (t.row0 + pi) * a.o_row + head * a.o_head;
 #pragma unroll
   for (int d = 0; d < NDT; ++d)
 #pragma unroll
@@ -1524,10 +1545,28 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] = o[d][8 * h + e] * inv;
       const u32x4_t w = __builtin_bit_cast(u32x4_t, M::cvt8(f));
-      const int d0 = 32 * d + 16 * h + 4 * lg;
-      *reinterpret_cast<uint2*>(op + d0 * 2) = make_uint2(w.x, w.y);
-      *reinterpret_cast<uint2*>(op + (d0 + 8) * 2) = make_uint2(w.z, w.w);
+      const int c = 4 * d + 2 * h;  // dims 8 c + 4 lg + 0..3 and 8 (c + 1) + 4 lg + 0..3
+      char* at = stage + lq * (D * 2) + 8 * lg;
+      *reinterpret_cast<uint2*>(at + 16 * (c ^ (lq & (CH - 1)))) = make_uint2(w.x, w.y);
+      *reinterpret_cast<uint2*>(at + 16 * ((c + 1) ^ (lq & (CH - 1)))) = make_uint2(w.z, w.w);
     }
+  asm volatile("" ::: "memory");
+  const int64_t row_at = p < 0 ? -1 : (t.row0 + pi) * a.o_row + head * a.o_head;
+  const bool wide = (reinterpret_cast<uintptr_t>(a.o) | a.o_row | a.o_head) % 16 == 0;
+#pragma unroll
+  for (int k = 0; k < 32 * CH / 64; ++k) {
+    const int r = (k * 64 + lane) / CH, c = (k * 64 + lane) % CH;
+    const int64_t at = __shfl(row_at, r, 64);
+    const uint4 w = *reinterpret_cast<const uint4*>(stage + r * (D * 2) + 16 * (c ^ (r & (CH - 1))));
+    if (at < 0) continue;
+    char* dst = a.o + at + 16 * c;
+    if (wide) {
+      *reinterpret_cast<uint4*>(dst) = w;
+    } else {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(w.x, w.y);
+      *reinterpret_cast<uint2*>(dst + 8) = make_uint2(w.z, w.w);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------

@@ -71,10 +71,6 @@ class QuantizedKVCache:
         nb, _, heads, bs, half = codes.shape
         self.shape = (nb, 2, heads, bs, 2 * half)
         self.device = codes.device
-        # what every call passes of it (the tensors are held, so their addresses stay theirs)
-        self._args = (self.shape, codes.data_ptr(), scales.data_ptr(),
-                      _stride_array(codes.stride()), _stride_array(scales.stride()),
-                      _lib.SB_DTYPE_MXFP4)
 
     @property
     def codes(self) -> torch.Tensor:
@@ -99,7 +95,10 @@ def _cache_args(kv_cache, dtype: torch.dtype, *rows):
     """(device, shape, base, scale base, strides, scale strides, dtype code) of either cache; the
     ``rows`` tensors must be on its device."""
     if isinstance(kv_cache, QuantizedKVCache):
-        return (_lib.require_device(kv_cache._codes, *rows), *kv_cache._args)
+        codes, scales = kv_cache._codes, kv_cache._scales
+        return (_lib.require_device(codes, *rows), kv_cache.shape, codes.data_ptr(),
+                scales.data_ptr(), _stride_array(codes.stride()), _stride_array(scales.stride()),
+                _lib.SB_DTYPE_MXFP4)
     dev = _lib.require_device(kv_cache, *rows)
     shape, strides = kv_cache.shape, kv_cache.stride()
     if len(shape) != 5 or shape[1] != 2:
