@@ -585,9 +585,10 @@ int sb_partial_attention_paged_varlen(void* out, const void* q, const void* kv_c
  *
  * Shared by the three entries:
  *   - Rows (tokens) of num_requests requests lie back to back: request r's are row_starts[r] ..
- *     row_starts[r + 1] - 1 (device int32, num_requests + 1 entries, ascending). row_starts NULL:
- *     row i is request i's only one, or, with num_requests 1, all rows are that one's. Rows from row_starts[num_requests] on, and rows with a
- *     negative position, are padding: nothing is read, appended or written for them.
+ *     row_starts[r + 1] - 1 (device int32, num_requests + 1 entries, ascending). row_starts
+ *     NULL: row i is request i's only one, or, with num_requests 1, all rows are that one's. Rows
+ *     of no request and rows with a negative position are padding: nothing is appended or written
+ *     for them.
  *   - block_tables: row r (table_stride entries apart) names request r's pages; entries that are
  *     no page of the pool ([0, num_blocks_total)) take no token, and their keys are not seen.
  *   - cache_dtype is the cache's type: the tensors' dtype, with kv_strides[5] = (block, kv, head,
@@ -600,8 +601,8 @@ int sb_partial_attention_paged_varlen(void* out, const void* q, const void* kv_c
 
 /* Writes K and V of num_tokens tokens (key, value [num_tokens, num_kv_heads, head_dim], strides
  * token, head, dim in elements) to the slots of their positions. With inv_freq (device fp32
- * [head_dim / 2], 1 / base^(2i/head_dim) <= 1), K is rotated in interleaved pairs by rotations[t] (or, NULL,
- * positions[t]) * inv_freq[i], the product and its sine and cosine in 64 bits; and query
+ * [head_dim / 2], 1 / base^(2i/head_dim) <= 1), K is rotated in interleaved pairs by rotations[t]
+ * (or, NULL, positions[t]) * inv_freq[i], the product and its sine and cosine in 64 bits; and query
  * (NULL: none; [num_tokens, num_q_heads, head_dim]) likewise into query_out. One rounding to the
  * cache's type. 4-bit blocks: 2^e is the smallest power with max |x| <= 7 * 2^e (e >= -127),
  * x / 2^e rounds to the nearest 4-bit value, ties to even; a block with an infinity or a NaN is

@@ -56,9 +56,10 @@ struct AppendArgs {
   int tokens_per_wg, rows_per_y;
 };
 
-// Request of row t, or -1 behind the last one: the last r with row_starts[r] <= t.
+// Request of row t, or -1 before the first and behind the last one: the last r with
+// row_starts[r] <= t.
 __device__ __forceinline__ int request_of(const int32_t* row_starts, int num_requests, int t) {
-  if (t >= row_starts[num_requests]) return -1;
+  if (t < row_starts[0] || t >= row_starts[num_requests]) return -1;
   int lo = 0, hi = num_requests;  // row_starts[lo] <= t < row_starts[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;

@@ -1876,7 +1876,7 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
     // (beside the rows kernel most of `tiles` are empty: one a request, about)
     pl.few.nsplit = split_for(rows_kernel ? std::min(items, num_requests * num_kv_heads) : items,
                               key_tiles, kFewMinTiles, tile_ns, 4000, 5000, 0);
-    if (!ragged || num_rows == 1) {
+    if (!starts && (num_requests > 1 || num_rows == 1)) {  // row i is request i's
       // Balanced items, unless there are enough of them as they are and none is long.
       const bool split = pl.few.nsplit > 1 || key_tiles > kLongTiles;
       pl.few.target = split ? kFewTarget : 0;
@@ -1923,13 +1923,13 @@ extern "C" int64_t sb_paged_attention_workspace_size(int64_t num_rows, int64_t n
   using namespace sb;
   if (num_rows <= 0 || num_requests <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 ||
       num_q_heads % num_kv_heads || block_size <= 0 || num_blocks_per_seq <= 0 || window < 0 ||
-      sinks < 0)
+      sinks < 0 || block_size > 0x7fffffff || num_blocks_per_seq > 0x7fffffff)
     return 0;
   const int64_t kv_len = std::min<int64_t>(block_size * num_blocks_per_seq, 0x7fff0000);
   return plan_paged(num_rows, num_requests, has_starts != 0,
                     max_rows > 0 && max_rows < num_rows ? max_rows : num_rows, num_kv_heads,
                     num_q_heads / num_kv_heads, head_dim, kv_len,
-                    window > 0 ? window : kNoWindow, sinks, dtype,
+                    window > 0 && window <= kNoWindow ? window : kNoWindow, sinks, dtype,
                     row_bytes(head_dim, dtype, cache_dtype == SB_DTYPE_MXFP4), true)
       .bytes;
 }
@@ -2007,8 +2007,10 @@ extern "C" int sb_paged_attention(
   a.bs_magic = static_cast<uint32_t>(((1ull << a.bs_shift) + block_size - 1) / block_size);
   a.num_blocks_total = static_cast<int>(num_blocks_total);
   a.kv_len = static_cast<int>(std::min<int64_t>(block_size * num_blocks_per_seq, 0x7fff0000));
-  a.window = window > 0 ? static_cast<int>(std::min<int64_t>(window, kNoWindow)) : kNoWindow;
-  a.sinks = static_cast<int>(std::min<int64_t>(sinks, a.kv_len));
+  // (no window: the last position's would end behind key 0, so every key is a first one as well)
+  const bool windowed = window > 0 && window <= kNoWindow;
+  a.window = windowed ? static_cast<int>(window) : kNoWindow;
+  a.sinks = windowed ? static_cast<int>(std::min<int64_t>(sinks, a.kv_len)) : a.kv_len;
   a.scale = scale;
   const double sl = static_cast<double>(scale) * 1.4426950408889634;
   a.scale_log2 = static_cast<float>(sl);
@@ -2067,7 +2069,7 @@ extern "C" int sb_paged_attention(
   if (head_dim == 64) { X(64) }     \
   else { X(128) }
 #define SB_MERGE(DT, D, TR, KT, B, P)                                                           \
-  if ((P).nsplit > 1 || (P).target > 0) {                                                                         \
+  if ((P).nsplit > 1 || (P).target > 0) {                                                       \
     constexpr int rpw = TR == kDecodeRows ? 1 : 1024 / D;                                       \
     const int live = (P).target > 0 ? std::min<int>(TR, static_cast<int>(group)) : TR;          \
     const dim3 mg(static_cast<unsigned>((P).tiles * num_kv_heads), (live + rpw - 1) / rpw);     \

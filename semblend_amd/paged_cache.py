@@ -17,9 +17,9 @@ extensions with no reference counterpart, on the same caches, block tables and p
 
 Batches: ``row_starts`` [num_requests + 1] (int32, on the device) says where each request's rows
 begin; without it row i is request i's only one, as in a decode step, or, with one request, all
-rows are that one's. Rows behind the last request and rows with a negative position are padding and
-left as they are. All metadata is read on the
-device, so a step can be captured into a HIP graph once and replayed with new positions.
+rows are that one's. Rows of no request and rows with a negative position are padding and left as
+they are. All metadata is read on the device, so a step can be captured into a HIP graph once and
+replayed with new positions.
 """
 
 from __future__ import annotations
@@ -337,15 +337,16 @@ def paged_attention(
     if num == 0:
         return out
     bt, pos, starts, requests = _batch_args(dev, num, block_tables, positions, row_starts)
-    most = num if max_rows is None else max(1, int(max_rows))
-    win = 0 if window is None else min(int(window), 0x7fffffff)
+    most = num if max_rows is None else min(max(1, int(max_rows)), num)
+    win = 0 if window is None or window > 0x7fffffff else int(window)
+    sinks = min(int(sinks), 0x7fffffff)
     ws_bytes = _workspace_bytes(num, requests, int(starts is not None), most, hq, heads, d, bs,
-                                bt.shape[1], win, int(sinks), dt, code)
+                                bt.shape[1], win, sinks, dt, code)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     _lib.launch(
         dev, "sb_paged_attention",
         out.data_ptr(), q.data_ptr(), base, sbase, bt.data_ptr(), bt.stride(0), pos.data_ptr(),
         _lib.ptr(starts), _lib.ptr(ws), ws_bytes, num, requests, most, hq, heads, d, bs, nb,
-        bt.shape[1], win, int(sinks), float(scale), _stride_array(q.stride()),
+        bt.shape[1], win, sinks, float(scale), _stride_array(q.stride()),
         _stride_array(out.stride()), st, sst, dt, code)
     return out

@@ -569,6 +569,104 @@ def test_many_requests(dev):
         _attend_case(dtype, d, hq, hkv, bs, lens, rows, 50, 2, quant)
 
 
+@pytest.mark.parametrize("dtype,quant", FORMATS)
+def test_one_row_of_several_requests(dev, dtype, quant):
+    """A batch of one row whose request is not the first, and one whose only row is padding: the
+    context is long enough to be split."""
+    _attend_case(dtype, 64, 4, 2, 16, [10, 6000, 10], [0, 1, 0], None, 0, quant)
+    _attend_case(dtype, 64, 40, 1, 16, [10, 6000, 10], [0, 1, 0], None, 0, quant)
+    _attend_case(dtype, 64, 4, 2, 16, [6000], [0], None, 0, quant,
+                 positions=torch.tensor([5999], dtype=torch.int32))
+
+
+@pytest.mark.parametrize("dtype,quant", FORMATS)
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1, 0), (5, 4), (2 ** 31 + 5, 2 ** 40)])
+def test_largest_position(dev, dtype, quant, window, sinks):
+    """Rows at 2^31 - 1 see the whole table, or the first tokens, or nothing."""
+    for rows in (1, 60):
+        pos = torch.full((rows,), 2 ** 31 - 1, dtype=torch.int32)
+        pos[rows // 2:] -= torch.arange(rows - rows // 2, dtype=torch.int32)
+        for d in (64, 96):
+            _attend_case(dtype, d, 4, 2, 16, [100], [rows], window, sinks, quant, positions=pos)
+
+
+@pytest.mark.parametrize("dtype,quant", FORMATS)
+def test_output_in_place_of_the_query(dev, dtype, quant):
+    d, hq, hkv, bs = 64, 14, 2, 16
+    tables, nb = _tables([3000, 90], bs, 1)
+    cache = _quant_cache(nb, hkv, bs, d, 2)[2] if quant else _cache(nb, hkv, bs, d, dtype, 2)[1]
+    for rows in (None, [70, 1]):
+        lens = rows or [1, 1]
+        pos = torch.cat([torch.arange(n - r, n) for n, r in zip([3000, 90], lens)]).int().cuda()
+        rs = None if rows is None else torch.tensor(_starts(rows), dtype=torch.int32).cuda()
+        q = randn((pos.numel(), hq, d), dtype, 3).cuda()
+        want = pc.paged_attention(q, cache, tables.cuda(), pos, rs)
+        got = pc.paged_attention(q, cache, tables.cuda(), pos, rs, out=q)
+        assert got is q
+        assert_bit_exact(got, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("pad", [0, 12])
+def test_codes_and_scales_in_one_row(dev, dtype, pad):
+    """Codes and scale bytes of a row side by side (rows of 68 bytes, or padded to 80, so that the
+    codes stay aligned), pages apart: strides that are no multiples of each other."""
+    d, hq, hkv, bs = 128, 28, 4, 16
+    tables, nb = _tables([400, 33], bs, 1)
+    codes, scales, cache = _quant_cache(nb, hkv, bs, d, 2)
+    width = d // 2 + d // 32 + pad
+    both = torch.zeros((nb, 3, hkv, bs, width), dtype=torch.uint8, device="cuda")[:, :2]
+    other = pc.QuantizedKVCache(both[..., :d // 2], both[..., d // 2:d // 2 + d // 32])
+    other.codes.copy_(codes)
+    other.scales.copy_(scales)
+    t = tables.cuda()
+    for rows in ([1, 1], [100, 3]):
+        pos = torch.cat([torch.arange(n - r, n) for n, r in zip([400, 33], rows)]).int().cuda()
+        rs = torch.tensor(_starts(rows), dtype=torch.int32).cuda()
+        k, v = (randn((pos.numel(), hkv, d), dtype, s).cuda() for s in (3, 4))
+        q = randn((pos.numel(), hq, d), dtype, 5).cuda()
+        for c in (cache, other):
+            pc.append_kv_paged(c, k, v, t, pos, rs, rope_base=1e4)
+        assert torch.equal(cache.codes, other.codes) and torch.equal(cache.scales, other.scales)
+        want, mass, serr = ref.attention(q.cpu(), ref.dequantize(cache.codes.cpu(),
+                                                                 cache.scales.cpu()), tables,
+                                         pos.cpu(), _starts(rows), 50, 4, d ** -0.5)
+        got = pc.paged_attention(q, other, t, pos, rs, window=50, sinks=4).cpu()
+        assert ((got.double() - want).abs() <= ref.attention_bound(want, mass, serr, dtype,
+                                                                   400)).all()
+    assert_bit_exact(pc.gather_kv_paged(other, t[0]), pc.gather_kv_paged(cache, t[0]))
+    if pad:
+        assert (both[..., d // 2 + d // 32:] == 0).all()
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_append_tokens_of_no_request_or_slot(dev, quant):
+    """Tokens before the first request's and behind the last one's are left out, and so are slots
+    behind the table, up to position 2^31 - 1 (whose query is rotated all the same)."""
+    d, hq, hkv, bs = 64, 4, 2, 16
+    tables, nb = _tables([64, 64], bs, 1)
+    cache = _quant_cache(nb, hkv, bs, d, 2)[2] if quant else _cache(nb, hkv, bs, d, BF16, 2)[1]
+    parts = (cache.codes, cache.scales) if quant else (cache,)
+    before = [p.clone() for p in parts]
+    pos = torch.tensor([3, 4, 2 ** 31 - 1, 64, 5, 6], dtype=torch.int32)
+    q = randn((6, hq, d), BF16, 3)
+    out = torch.full(q.shape, 3.0, dtype=BF16).cuda()
+    got = pc.append_kv_paged(cache, randn((6, hkv, d), BF16, 4).cuda(),
+                             randn((6, hkv, d), BF16, 5).cuda(), tables.cuda(), pos.cuda(),
+                             torch.tensor([2, 3, 4], dtype=torch.int32).cuda(), rope_base=1e4,
+                             query=q.cuda(), query_out=out).cpu()
+    for p, b in zip(parts, before):
+        assert torch.equal(p.cpu(), b.cpu())
+    rows = [0, 1, 4, 5]
+    assert (got[rows] == 3.0).all()
+    # (interleaved sums of two products in fp32, 2^-22 of the pair's norm, and one rounding)
+    want = ref.rotate(q, pos, 1e4)
+    norm = q.double().unflatten(-1, (-1, 2)).norm(dim=-1).repeat_interleave(2, -1)
+    err = (got.double() - want).abs()
+    bound = want.abs() * ref.half_step(BF16) + norm * 2.0 ** -21
+    assert (err <= bound)[2:4].all()
+
+
 # ---- together, captured, on other streams -----------------------------------------------------
 
 @pytest.mark.parametrize("quant", [False, True])
