@@ -1601,34 +1601,36 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedA
           static_cast<int64_t>(TR)));
   const int row_base = blockIdx.y * RPW;
   if (row_base >= nflat) return;
-  // the tile's key range, as the attention kernel saw it
-  int pmin = 0x7fffffff, pmax = -1;
-  static_assert(TR <= kMergeThreads, "one row per thread");
-  if (static_cast<int>(threadIdx.x) < nflat) {
-    const int p = a.positions[t.row0 + (t.tile * TR + static_cast<int>(threadIdx.x)) / a.group];
-    if (p >= 0) pmin = p;
-    pmax = p;
-  }
-  pmin = wave_min_i(pmin);
-  pmax = wave_max_i(pmax);
-  if ((threadIdx.x & 63) == 0) {
-    red[0][threadIdx.x >> 6] = pmin;
-    red[1][threadIdx.x >> 6] = pmax;
-  }
-  __syncthreads();
+  int nsplit = it.nsplit;
+  if (nsplit == 0) {  // even splits: the tile's key range, as the attention kernel saw it
+    int pmin = 0x7fffffff, pmax = -1;
+    static_assert(TR <= kMergeThreads, "one row per thread");
+    if (static_cast<int>(threadIdx.x) < nflat) {
+      const int p = a.positions[t.row0 + (t.tile * TR + static_cast<int>(threadIdx.x)) / a.group];
+      if (p >= 0) pmin = p;
+      pmax = p;
+    }
+    pmin = wave_min_i(pmin);
+    pmax = wave_max_i(pmax);
+    if ((threadIdx.x & 63) == 0) {
+      red[0][threadIdx.x >> 6] = pmin;
+      red[1][threadIdx.x >> 6] = pmax;
+    }
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kMergeThreads / 64; ++w) {
-    pmin = min(pmin, red[0][w]);
-    pmax = max(pmax, red[1][w]);
+    for (int w = 0; w < kMergeThreads / 64; ++w) {
+      pmin = min(pmin, red[0][w]);
+      pmax = max(pmax, red[1][w]);
+    }
+    if (pmax < 0) return;
+    nsplit = split_count(a, key_tiles<KT>(a, pmin, pmax).total);
   }
-  if (pmax < 0) return;
-  const int nsplit =
-      it.nsplit > 0 ? it.nsplit : split_count(a, key_tiles<KT>(a, pmin, pmax).total);
   if (nsplit <= 1) return;
   const int lane = threadIdx.x % VPR, row_in = threadIdx.x / VPR % RPW;
   const int grp = threadIdx.x / (VPR * RPW);
   const int row = min(row_base + row_in, nflat - 1), d = lane * 4;
   const int flat = t.tile * TR + row, pi = flat / a.group;
+  const int p = a.positions[t.row0 + pi];
   const int64_t slot0 = it.slot * TR + row;
   const int64_t step = static_cast<int64_t>(slot_step(a)) * TR;
   float m = -INFINITY, l = 0.f;
@@ -1680,7 +1682,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedA
     }
     m = mb;
   }
-  if (row_base + row_in >= nflat || a.positions[t.row0 + pi] < 0) return;
+  if (row_base + row_in >= nflat || p < 0) return;
   const float inv = m == -INFINITY ? 0.f : out_scale / l;
   char* op = a.o + (t.row0 + pi) * a.o_row + (kvh * a.group + flat - pi * a.group) * a.o_head;
   if constexpr (DT == SB_DTYPE_F32) {
