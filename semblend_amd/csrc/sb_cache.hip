@@ -22,7 +22,9 @@
 // What bounds it: bytes for prompts, the launch and one dependent chain (position, table entry,
 // row) for decode steps. One workgroup takes a few tokens with all their heads, so that each
 // (token, frequency) pair's sine and cosine (about 45 fp64 instructions) is evaluated once and
-// shared through LDS by the K and query heads.
+// shared through LDS by the K and query heads. Measured: 4602 tokens of 32 / 8 heads x 128, 113 MB
+// in 21 us (5.3 TB/s; a large copy reaches 6.6); 16 tokens 4 us; 4099 tokens of 4 heads into 4-bit
+// pages 9 us, reading 16384 of 8 heads back 18.6 us (85 MB, 4.6 TB/s).
 #include "sb_common.h"
 
 #include <algorithm>
