@@ -91,15 +91,28 @@ class QuantizedKVCache:
                    torch.zeros((*shape, head_dim // 32), dtype=torch.uint8, device=device))
 
 
+# A call's checks cost as much host time as its launch, so the usual cases come first below and a
+# tensor's shape and strides are read once.
+def _device(first: torch.Tensor, rest) -> torch.device:
+    """``_lib.require_device`` of all of them, by their device numbers."""
+    index = first.get_device()
+    if index < 0:
+        return _lib.require_device(first, *rest)
+    for t in rest:
+        if t is not None and t.get_device() != index:
+            return _lib.require_device(first, *rest)
+    return first.device
+
+
 def _cache_args(kv_cache, dtype: torch.dtype, *rows):
     """(device, shape, base, scale base, strides, scale strides, dtype code) of either cache; the
     ``rows`` tensors must be on its device."""
     if isinstance(kv_cache, QuantizedKVCache):
         codes, scales = kv_cache._codes, kv_cache._scales
-        return (_lib.require_device(codes, *rows), kv_cache.shape, codes.data_ptr(),
+        return (_device(codes, rows), kv_cache.shape, codes.data_ptr(),
                 scales.data_ptr(), _stride_array(codes.stride()), _stride_array(scales.stride()),
                 _lib.SB_DTYPE_MXFP4)
-    dev = _lib.require_device(kv_cache, *rows)
+    dev = _device(kv_cache, rows)
     shape, strides = kv_cache.shape, kv_cache.stride()
     if len(shape) != 5 or shape[1] != 2:
         raise ValueError("kv_cache must be [num_blocks, 2, num_kv_heads, block_size, head_dim]")
@@ -114,15 +127,15 @@ def _cache_args(kv_cache, dtype: torch.dtype, *rows):
 
 def _index(t, dev) -> torch.Tensor:
     """``_lib.as_index`` with the usual case (already a device index array) first."""
-    if type(t) is torch.Tensor and t.dtype == torch.int32 and t.device == dev and t.dim() == 1 \
-            and t.is_contiguous():
+    if type(t) is torch.Tensor and t.dtype is torch.int32 and t.get_device() == dev.index \
+            and t.dim() == 1 and t.is_contiguous():
         return t
     return _lib.as_index(t, dev)
 
 
 def _batch_args(dev, num_rows: int, block_tables, positions, row_starts):
-    """(tables, positions, row_starts, number of requests) checked and on the device. A 1-D table
-    is one request's, and all rows are that request's."""
+    """(tables, positions, row_starts, number of requests, entries of a table) checked and on the
+    device. A 1-D table is one request's, and all rows are that request's."""
     bt = block_tables
     if not isinstance(bt, torch.Tensor):
         bt = torch.as_tensor(bt, dtype=torch.int32)
@@ -133,13 +146,14 @@ def _batch_args(dev, num_rows: int, block_tables, positions, row_starts):
     elif bt.dim() != 2:
         raise ValueError("block_tables must be [num_requests, max_blocks], or [max_blocks] for "
                          "one request")
-    elif bt.dtype != torch.int32 or bt.device != dev or (bt.shape[1] > 1 and bt.stride(1) != 1):
+    elif bt.dtype is not torch.int32 or bt.get_device() != dev.index or (
+            bt.stride(1) != 1 and bt.shape[1] > 1):
         shape = bt.shape
         bt = _index(bt.reshape(-1), dev).view(shape)
     pos = _index(positions, dev)
     if pos.shape[0] != num_rows:
         raise ValueError("positions must have one entry per row")
-    requests = bt.shape[0]
+    requests, width = bt.shape
     if row_starts is not None:
         row_starts = _index(row_starts, dev)
         if row_starts.shape[0] != requests + 1:
@@ -147,9 +161,26 @@ def _batch_args(dev, num_rows: int, block_tables, positions, row_starts):
     elif num_rows > requests != 1:
         raise ValueError("without row_starts there is one row per request: "
                          f"{num_rows} rows, {requests} block tables")
-    if bt.shape[1] == 0 or requests == 0:
+    if width == 0 or requests == 0:
         raise ValueError("block_tables is empty")
-    return bt, pos, row_starts, requests
+    return bt, pos, row_starts, requests, width
+
+
+def _rows(t: torch.Tensor):
+    """(t, its strides), copied where its last dimension is not contiguous."""
+    st = t.stride()
+    if st[2] != 1:
+        t = t.contiguous()
+        st = t.stride()
+    return t, st
+
+
+def _like(t: torch.Tensor, strides):
+    """(a new dense tensor of t's shape and dtype, its strides)."""
+    if t.is_contiguous():
+        return torch.empty_like(t), strides
+    new = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return new, new.stride()
 
 
 def append_kv_paged(
@@ -187,12 +218,13 @@ def append_kv_paged(
     _, _, heads, bs, d = shape
     if value.dtype != dtype or (query is not None and query.dtype != dtype):
         raise TypeError("key, value and query must share a dtype")
-    if key.dim() != 3 or key.shape[1:] != (heads, d) or value.shape != key.shape:
+    kshape = key.shape
+    if len(kshape) != 3 or kshape[1] != heads or kshape[2] != d or value.shape != kshape:
         raise ValueError("key and value must be [tokens, num_kv_heads, head_dim] with the "
                          "cache's heads and head_dim")
-    num = key.shape[0]
-    k = key if key.stride(2) == 1 else key.contiguous()
-    v = value if value.stride(2) == 1 else value.contiguous()
+    num = kshape[0]
+    k, kst = _rows(key)
+    v, vst = _rows(value)
     dt = _lib.dtype_code(key)
     if rope_base is None and (rotations is not None or query is not None):
         raise ValueError("rotations and query go with rope_base")
@@ -200,21 +232,24 @@ def append_kv_paged(
         raise ValueError("rope_base must be at least 1")
     if d % 2:
         raise ValueError("head_dim must be even")
-    q = None
+    q, qst, ost, hq = None, None, None, 0
     if query is not None:
-        if query.dim() != 3 or query.shape[0] != num or query.shape[2] != d:
+        qshape = query.shape
+        if len(qshape) != 3 or qshape[0] != num or qshape[2] != d:
             raise ValueError("query must be [tokens, num_q_heads, head_dim]")
-        q = query if query.stride(2) == 1 else query.contiguous()
+        hq = qshape[1]
+        q, qst = _rows(query)
         if query_out is None:
-            query_out = (torch.empty_like(q) if q.is_contiguous()
-                         else torch.empty(q.shape, dtype=q.dtype, device=dev))
-        elif query_out.shape != q.shape or query_out.dtype != q.dtype or query_out.stride(2) != 1:
-            raise ValueError("query_out must be like query, with a unit last stride")
+            query_out, ost = _like(q, qst)
+        else:
+            ost = query_out.stride()
+            if query_out.shape != qshape or query_out.dtype != dtype or ost[2] != 1:
+                raise ValueError("query_out must be like query, with a unit last stride")
     elif query_out is not None:
         raise ValueError("query_out goes with query")
     if num == 0:
         return query_out
-    bt, pos, starts, requests = _batch_args(dev, num, block_tables, positions, row_starts)
+    bt, pos, starts, requests, width = _batch_args(dev, num, block_tables, positions, row_starts)
     rot = None
     if rotations is not None:
         rot = _index(rotations, dev)
@@ -225,10 +260,9 @@ def append_kv_paged(
         dev, "sb_append_kv_paged",
         base, sbase, k.data_ptr(), v.data_ptr(), _lib.ptr(q),
         None if q is None else query_out.data_ptr(), bt.data_ptr(), bt.stride(0), pos.data_ptr(),
-        _lib.ptr(rot), _lib.ptr(starts), _lib.ptr(inv), num, requests, heads,
-        0 if q is None else q.shape[1], d, bs, shape[0], bt.shape[1], _stride_array(k.stride()),
-        _stride_array(v.stride()), None if q is None else _stride_array(q.stride()),
-        None if q is None else _stride_array(query_out.stride()), st, sst, dt, code)
+        _lib.ptr(rot), _lib.ptr(starts), _lib.ptr(inv), num, requests, heads, hq, d, bs, shape[0],
+        width, _stride_array(kst), _stride_array(vst), None if q is None else _stride_array(qst),
+        None if q is None else _stride_array(ost), st, sst, dt, code)
     return query_out
 
 
@@ -312,10 +346,11 @@ def paged_attention(
     are). Extension with no reference counterpart: the reference's attention is MHA over
     contiguous K/V (semblend_core/triton_kernels.py:655-734), without window.
     """
-    if query.dim() != 3:
+    qshape, dtype = query.shape, query.dtype
+    if len(qshape) != 3:
         raise ValueError("query must be [rows, num_q_heads, head_dim]")
-    dev, shape, base, sbase, st, sst, code = _cache_args(kv_cache, query.dtype, query, out)
-    num, hq, d = query.shape
+    dev, shape, base, sbase, st, sst, code = _cache_args(kv_cache, dtype, query, out)
+    num, hq, d = qshape
     nb, _, heads, bs, hd = shape
     if hd != d:
         raise ValueError("query and kv_cache head_dim differ")
@@ -325,28 +360,28 @@ def paged_attention(
         raise ValueError("window must be at least 1 (None: no window)")
     if sinks < 0:
         raise ValueError("sinks must not be negative")
-    q = query if query.stride(2) == 1 else query.contiguous()
+    q, qst = _rows(query)
     if scale is None:
         scale = 1.0 / math.sqrt(d)
     if out is None:
-        out = (torch.empty_like(q) if q.is_contiguous()
-               else torch.empty((num, hq, d), dtype=q.dtype, device=dev))
-    elif out.shape != query.shape or out.dtype != query.dtype or out.stride(2) != 1:
-        raise ValueError("out must be like query, with a unit last stride")
+        out, ost = _like(q, qst)
+    else:
+        ost = out.stride()
+        if out.shape != qshape or out.dtype != dtype or ost[2] != 1:
+            raise ValueError("out must be like query, with a unit last stride")
     dt = _lib.dtype_code(q)
     if num == 0:
         return out
-    bt, pos, starts, requests = _batch_args(dev, num, block_tables, positions, row_starts)
+    bt, pos, starts, requests, width = _batch_args(dev, num, block_tables, positions, row_starts)
     most = num if max_rows is None else min(max(1, int(max_rows)), num)
     win = 0 if window is None or window > 0x7fffffff else int(window)
     sinks = min(int(sinks), 0x7fffffff)
     ws_bytes = _workspace_bytes(num, requests, int(starts is not None), most, hq, heads, d, bs,
-                                bt.shape[1], win, sinks, dt, code)
+                                width, win, sinks, dt, code)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     _lib.launch(
         dev, "sb_paged_attention",
         out.data_ptr(), q.data_ptr(), base, sbase, bt.data_ptr(), bt.stride(0), pos.data_ptr(),
         _lib.ptr(starts), _lib.ptr(ws), ws_bytes, num, requests, most, hq, heads, d, bs, nb,
-        bt.shape[1], win, sinks, float(scale), _stride_array(q.stride()),
-        _stride_array(out.stride()), st, sst, dt, code)
+        width, win, sinks, float(scale), _stride_array(qst), _stride_array(ost), st, sst, dt, code)
     return out
