@@ -35,6 +35,7 @@ namespace {
 constexpr int kAppendThreads = 256;
 constexpr int kTableEntries = 512;   // (token, frequency) pairs of one workgroup
 constexpr int kTokensMax = 8;
+constexpr int kRowsMax = 256;        // rows (K, V and query heads of its tokens) of one workgroup
 
 struct AppendArgs {
   const char* k;
@@ -56,6 +57,8 @@ struct AppendArgs {
   int64_t num_blocks_total, num_blocks_per_seq;
   int num_requests, num_kv_heads, num_q_heads, head_dim, block_size;
   int tokens_per_wg, rows_per_y;
+  uint32_t row_magic;                     // row / rows of a token = (row * row_magic) >> row_shift
+  int row_shift;
 };
 
 // Request of row t, or -1 before the first and behind the last one: the last r with
@@ -71,22 +74,33 @@ __device__ __forceinline__ int request_of(const int32_t* row_starts, int num_req
   return lo;
 }
 
+// An element's value, and two values rounded to elements.
 template <int DT> struct Elem;
 template <> struct Elem<SB_DTYPE_F32> {
   using T = float;
   __device__ static float get(float x) { return x; }
-  __device__ static float put(float x) { return x; }
+  __device__ static void put2(float a, float b, float* e) { e[0] = a, e[1] = b; }
 };
 template <> struct Elem<SB_DTYPE_F16> {
   using T = uint16_t;
   __device__ static float get(uint16_t x) { return f16_to_f32(x); }
-  __device__ static uint16_t put(float x) { return f32_to_f16(x); }
+  __device__ static void put2(float a, float b, uint16_t* e) {
+    e[0] = f32_to_f16(a), e[1] = f32_to_f16(b);
+  }
 };
 template <> struct Elem<SB_DTYPE_BF16> {
   using T = uint16_t;
   __device__ static float get(uint16_t x) { return bf16_to_f32(x); }
-  __device__ static uint16_t put(float x) { return f32_to_bf16(x); }
+  __device__ static void put2(float a, float b, uint16_t* e) {
+    const uint32_t w = pack2_bf16(a, b);
+    e[0] = static_cast<uint16_t>(w), e[1] = static_cast<uint16_t>(w >> 16);
+  }
 };
+
+// Device memory (a pointer that went through LDS would be taken for any kind, and its loads wait
+// with LDS's).
+#define SB_GLOBAL __attribute__((address_space(1)))
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 // VEC elements of a row: 16 bytes, or (VEC 2) a pair, element by element at any alignment.
 template <int DT, int VEC> struct RowVec {
@@ -95,23 +109,22 @@ template <int DT, int VEC> struct RowVec {
   T e[VEC];
   __device__ __forceinline__ void load(const char* p) {
     if constexpr (kWide) {
-      const uint4 w = *reinterpret_cast<const uint4*>(p);
+      const u32x4_t w = *(const SB_GLOBAL u32x4_t*)p;
       __builtin_memcpy(e, &w, 16);
     } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) e[i] = reinterpret_cast<const T*>(p)[i];
+      for (int i = 0; i < VEC; ++i) e[i] = ((const SB_GLOBAL T*)p)[i];
     }
   }
   __device__ __forceinline__ void store(char* p) const {
     if constexpr (kWide) {
       // (nontemporal: append of 4602 tokens of 32 / 8 heads x 128 24.4 -> 21.1 us)
-      typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-      u32x4 w;
+      u32x4_t w;
       __builtin_memcpy(&w, e, 16);
-      __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p));
+      __builtin_nontemporal_store(w, (SB_GLOBAL u32x4_t*)p);
     } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) reinterpret_cast<T*>(p)[i] = e[i];
+      for (int i = 0; i < VEC; ++i) ((SB_GLOBAL T*)p)[i] = e[i];
     }
   }
 };
@@ -167,10 +180,17 @@ __device__ __forceinline__ Block<VEC> quantize(const float (&f)[VEC]) {
   return b;
 }
 
+// One thread per row works out where the row comes from and goes to, for all lanes of it: worked out
+// by every lane, that (selects, divisions, 64-bit products) was most of the kernel's instructions.
+struct RowRef {
+  const char* src;  // nullptr: left out (padding, or no slot)
+  char* dst;
+  char* sdst;       // scale bytes of a 4-bit row
+  uint32_t info;    // index of the token's sines and cosines << 2 | a 4-bit row << 1 | rotated
+  uint32_t pad;
+};
 // A thread takes vector tid % vpr of rows tid / vpr + k rpi (K, V, then query heads, token after
-// token), kRowsInFlight of them at a time. (Requesting the first ones before the positions, table
-// entries and sines are known was slower for prompts: 28.5 against 24.3 us for 4602 tokens of
-// 32 / 8 heads x 128; the workgroups' phases then overlap less.)
+// token), kRowsInFlight of them at a time.
 constexpr int kRowsInFlight = 4;
 template <int DT, int VEC, bool Q4>
 __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendArgs a) {
@@ -179,9 +199,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
   constexpr int ES = sizeof(typename Elem<DT>::T);
   __shared__ CS cs[2 * kTableEntries];                    // cosine, sine of each (token, pair)
   __shared__ double cs64[kBoth ? 2 * kTableEntries : 1];
-  __shared__ int64_t tok_c[kTokensMax];  // page and slot byte offset in the cache, -1: no slot
-  __shared__ int64_t tok_s[kTokensMax];  // ... and in the scale bytes
-  __shared__ int tok_live[kTokensMax];
+  __shared__ __align__(16) RowRef rows[kRowsMax];
   const int tid = threadIdx.x;
   const int half = a.head_dim >> 1;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens_per_wg;
@@ -193,51 +211,40 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
   const int hk = a.num_kv_heads;
   const int nrows = 2 * hk + a.num_q_heads;     // rows of a token
   const int j0 = blockIdx.y * a.rows_per_y;     // (with several, a workgroup has one token)
-  const int j1 = min(j0 + a.rows_per_y, ntok * nrows);
-  RowVec<DT, VEC> x[kRowsInFlight];
-  auto fetch = [&](int jb) {
-#pragma unroll
-    for (int u = 0; u < kRowsInFlight; ++u) {
-      const int r = min(jb + u * rpi, j1 - 1);
-      const int tok = static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(nrows));
-      const int j = r - tok * nrows;
-      const int64_t t = t0 + tok;
-      const char* src = j < hk       ? a.k + t * a.k_tok + j * a.k_head
-                        : j < 2 * hk ? a.v + t * a.v_tok + (j - hk) * a.v_head
-                                     : a.q + t * a.q_tok + (j - 2 * hk) * a.q_head;
-      x[u].load(src + static_cast<int64_t>(vec) * VEC * ES);
-    }
-  };
-  const bool works = rsub < rpi && j0 + rsub < j1;
+  const int n = min(a.rows_per_y, ntok * nrows - j0);
 
-  if (tid < ntok) {
-    const int64_t t = t0 + tid;
+  if (tid < n) {
+    const int r0 = j0 + tid;
+    const int tok = static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(r0)) * a.row_magic) >>
+                                     a.row_shift);
+    const int j = r0 - tok * nrows;
+    const int64_t t = t0 + tok;
     const int p = a.positions[t];
-    int64_t oc = -1, os = -1;
-    int live = 0;
-    if (p >= 0) {
-      const int r = a.row_starts ? request_of(a.row_starts, a.num_requests, static_cast<int>(t))
-                    : a.num_requests == 1 ? 0 : static_cast<int>(t);
-      if (r >= 0) {
-        live = 1;
-        const int lb = p / a.block_size, slot = p - lb * a.block_size;
-        if (lb < a.num_blocks_per_seq) {
-          const int64_t pb = a.tables[r * a.table_stride + lb];
-          if (pb >= 0 && pb < a.num_blocks_total) {
-            oc = pb * a.c_block + slot * a.c_pos;
-            os = pb * a.s_block + slot * a.s_pos;
-          }
-        }
+    RowRef ref = {nullptr, nullptr, nullptr, 0, 0};
+    const int r = p < 0 ? -1
+                  : a.row_starts ? request_of(a.row_starts, a.num_requests, static_cast<int>(t))
+                  : a.num_requests == 1 ? 0 : static_cast<int>(t);
+    if (r >= 0 && j >= 2 * hk) {
+      ref.src = a.q + t * a.q_tok + (j - 2 * hk) * a.q_head;
+      ref.dst = a.q_out + t * a.qo_tok + (j - 2 * hk) * a.qo_head;
+    } else if (r >= 0) {
+      const int kv = j >= hk, h = j - kv * hk;
+      const int lb = p / a.block_size, slot = p - lb * a.block_size;
+      const int64_t pb = lb < a.num_blocks_per_seq ? a.tables[r * a.table_stride + lb] : -1;
+      if (pb >= 0 && pb < a.num_blocks_total) {
+        ref.src = kv ? a.v + t * a.v_tok + h * a.v_head : a.k + t * a.k_tok + h * a.k_head;
+        ref.dst = a.cache + pb * a.c_block + slot * a.c_pos + kv * a.c_kv + h * a.c_head;
+        if (Q4) ref.sdst = a.scales + pb * a.s_block + slot * a.s_pos + kv * a.s_kv + h * a.s_head;
       }
     }
-    tok_c[tid] = oc;
-    tok_s[tid] = os;
-    tok_live[tid] = live;
+    const bool turn = a.inv_freq && (j < hk || j >= 2 * hk);
+    ref.info = static_cast<uint32_t>(2 * tok * half) << 2 | (Q4 && j < 2 * hk ? 2u : 0u) |
+               (turn ? 1u : 0u);
+    rows[tid] = ref;
   }
   if (a.inv_freq) {
-    // (from the last wave down: the first one looks the pages up)
-    const int n = ntok * half;
-    for (int i = kAppendThreads - 1 - tid; i < n; i += kAppendThreads) {
+    // (from the last wave down: the first ones look the pages up)
+    for (int i = kAppendThreads - 1 - tid; i < ntok * half; i += kAppendThreads) {
       const int tok = i / half, f = i - tok * half;
       const int p = (a.rotations ? a.rotations : a.positions)[t0 + tok];
       double s, c;
@@ -248,20 +255,22 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
     }
   }
   __syncthreads();
-  if (!works) return;
+  if (rsub >= rpi) return;
 
-  for (int jb = j0 + rsub; jb < j1; jb += kRowsInFlight * rpi) {
-    fetch(jb);
+  for (int ib = rsub; ib < n; ib += kRowsInFlight * rpi) {
+    RowVec<DT, VEC> x[kRowsInFlight];
 #pragma unroll
     for (int u = 0; u < kRowsInFlight; ++u) {
-      const int r = jb + u * rpi;
-      if (r >= j1) break;
-      const int tok = static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(nrows));
-      const int j = r - tok * nrows;
-      const int64_t t = t0 + tok, oc = tok_c[tok];
-      if (!tok_live[tok] || (j < 2 * hk && oc < 0)) continue;
-      const CS* trig = cs + 2 * (tok * half + vec * (VEC / 2));
-      const bool turn = a.inv_freq && (j < hk || j >= 2 * hk);
+      const char* src = rows[min(ib + u * rpi, n - 1)].src;
+      if (src) x[u].load(src + vec * (VEC * ES));
+    }
+#pragma unroll
+    for (int u = 0; u < kRowsInFlight; ++u) {
+      if (ib + u * rpi >= n) break;
+      const RowRef ref = rows[ib + u * rpi];
+      if (!ref.src) continue;
+      const CS* trig = cs + (ref.info >> 2) + vec * VEC;
+      const bool turn = ref.info & 1u;
       float f[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; i += 2) {
@@ -275,8 +284,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
           f[i + 1] = static_cast<float>(o);
         }
       }
-      if (Q4 && j < 2 * hk) {
-        const int kv = j >= hk, h = j - kv * hk;
+      if (Q4 && (ref.info & 2u)) {
         Block<VEC> b = quantize(f);
         if (turn) {
           // A rotated fp32 value is off by at most 2^-22 of its pair's norm (products and sum
@@ -294,7 +302,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
           for (int o = 16 / VEC; o >= 1; o >>= 1) any |= __shfl_xor(any, o, 64);
           if (any) {
             const double* t64;
-            if constexpr (kBoth) t64 = cs64 + 2 * (tok * half + vec * (VEC / 2));
+            if constexpr (kBoth) t64 = cs64 + (ref.info >> 2) + vec * VEC;
             else t64 = reinterpret_cast<const double*>(trig);
 #pragma unroll
             for (int i = 0; i < VEC; i += 2) {
@@ -307,26 +315,18 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
         }
         const uint32_t w = b.codes;
         const int sb = b.byte;
-        char* dst = a.cache + oc + kv * a.c_kv + h * a.c_head + vec * (VEC / 2);
-        if constexpr (VEC == 8) *reinterpret_cast<uint32_t*>(dst) = w;
-        else if constexpr (VEC == 4) *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(w);
-        else *reinterpret_cast<uint8_t*>(dst) = static_cast<uint8_t>(w);
+        char* dst = ref.dst + vec * (VEC / 2);
+        if constexpr (VEC == 8) *(SB_GLOBAL uint32_t*)dst = w;
+        else if constexpr (VEC == 4) *(SB_GLOBAL uint16_t*)dst = static_cast<uint16_t>(w);
+        else *(SB_GLOBAL uint8_t*)dst = static_cast<uint8_t>(w);
         if ((vec & (32 / VEC - 1)) == 0)
-          a.scales[tok_s[tok] + kv * a.s_kv + h * a.s_head + vec * VEC / 32] =
-              static_cast<char>(sb);
+          ((SB_GLOBAL char*)ref.sdst)[vec / (32 / VEC)] = static_cast<char>(sb);
       } else {
         if (turn) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) x[u].e[i] = Elem<DT>::put(f[i]);
+          for (int i = 0; i < VEC; i += 2) Elem<DT>::put2(f[i], f[i + 1], x[u].e + i);
         }
-        char* dst;
-        if (j < 2 * hk) {
-          const int kv = j >= hk;
-          dst = a.cache + oc + kv * a.c_kv + (j - kv * hk) * a.c_head;
-        } else {
-          dst = a.q_out + t * a.qo_tok + (j - 2 * hk) * a.qo_head;
-        }
-        x[u].store(dst + static_cast<int64_t>(vec) * VEC * ES);
+        x[u].store(ref.dst + vec * (VEC * ES));
       }
     }
   }
@@ -351,6 +351,24 @@ struct GatherArgs {
 };
 
 constexpr int kGatherThreads = 256;
+
+// VEC values of a word of codes; one instruction converts two (fp16: and rounds them).
+template <int DT, int VEC>
+__device__ __forceinline__ void unpack_codes(uint32_t w, float scale, typename Elem<DT>::T* e) {
+  auto put = [&](int i, auto pair) { __builtin_memcpy(e + 2 * i, &pair, sizeof(pair)); };
+#define SB_UNPACK(I)                                                                      \
+  if constexpr (2 * I < VEC) {                                                            \
+    if constexpr (DT == SB_DTYPE_F32) put(I, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, I)); \
+    else if constexpr (DT == SB_DTYPE_F16)                                                \
+      put(I, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, I));                      \
+    else put(I, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, I));                  \
+  }
+  SB_UNPACK(0)
+  SB_UNPACK(1)
+  SB_UNPACK(2)
+  SB_UNPACK(3)
+#undef SB_UNPACK
+}
 
 // A thread takes VEC elements of one position and some of its 2 Hkv rows, four in flight: the
 // position and its table entry are read once. Positions without a page give zeros.
@@ -412,15 +430,7 @@ __global__ __launch_bounds__(kGatherThreads) void gather_kv_kernel(const GatherA
       if constexpr (Q4) {
         if (oc >= 0) {
           // (the exponent field alone is the scale: byte 0 is 2^-127, byte 255 gives NaN)
-          const float scale = __uint_as_float(sb[u] << 23);
-          typedef float f32x2 __attribute__((ext_vector_type(2)));
-          f32x2 r[4];
-          r[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], scale, 0);
-          r[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], scale, 1);
-          r[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], scale, 2);
-          r[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], scale, 3);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) x[u].e[e] = Elem<DT>::put(r[e / 2][e & 1]);
+          unpack_codes<DT, VEC>(w[u], __uint_as_float(sb[u] << 23), x[u].e);
         }
       }
       x[u].store(dst + kv * a.o_kv + h * a.o_head);
@@ -528,14 +538,19 @@ extern "C" int sb_append_kv_paged(
   const int nrows = 2 * a.num_kv_heads + a.num_q_heads;
   const int rpi = kAppendThreads / (a.head_dim / vec);
   const int fit = std::min(kTokensMax, std::max(1, kTableEntries / (a.head_dim / 2)));
-  const int full = std::max(1, std::min(fit, kRowsInFlight * rpi / nrows));
+  const int full = std::max(1, std::min(fit, std::min(kRowsInFlight * rpi, kRowsMax) / nrows));
   a.tokens_per_wg = num_tokens >= 512 * static_cast<int64_t>(full) ? full : 1;
   const int64_t gx = (num_tokens + a.tokens_per_wg - 1) / a.tokens_per_wg;
   const int all = a.tokens_per_wg * nrows;
   const int steps = (all + rpi - 1) / rpi;
   const int ny = a.tokens_per_wg > 1
                      ? 1 : static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, 512 / gx), steps));
-  a.rows_per_y = (steps + ny - 1) / ny * rpi;
+  a.rows_per_y = std::min((steps + ny - 1) / ny, kRowsMax / rpi) * rpi;
+  // (exact for rows below 2^31: T. Granlund and P. Montgomery, 1994)
+  int log2_up = 0;
+  while ((1 << log2_up) < nrows) ++log2_up;
+  a.row_shift = 31 + log2_up;
+  a.row_magic = static_cast<uint32_t>(((1ull << a.row_shift) + nrows - 1) / nrows);
   const dim3 grid(static_cast<unsigned>(gx),
                   static_cast<unsigned>((all + a.rows_per_y - 1) / a.rows_per_y));
   const hipStream_t st = static_cast<hipStream_t>(stream);

@@ -569,6 +569,29 @@ def test_many_requests(dev):
         _attend_case(dtype, d, hq, hkv, bs, lens, rows, 50, 2, quant)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("hkv,hq,d,num", [(150, 300, 4, 3), (1, 1, 2, 700), (130, 1, 512, 2),
+                                          (7, 3, 32, 5000)])
+def test_append_many_heads_or_tokens(dev, dtype, hkv, hq, d, num):
+    """Tokens of more rows than a workgroup takes, and rows of a few bytes: V exactly, K and the
+    query rotated (two products and a sum in fp32 at most, and one rounding)."""
+    bs = 16
+    tables, nb = _tables([num], bs, 1)
+    _, cache = _cache(nb, hkv, bs, d, dtype, 2)
+    k, v = (randn((num, hkv, d), dtype, s) for s in (3, 4))
+    q = randn((num, hq, d), dtype, 5)
+    pos = torch.randperm(num, generator=gen(6)).to(torch.int32)
+    got_q = pc.append_kv_paged(cache, k.cuda(), v.cuda(), tables[0].cuda(), pos.cuda(),
+                               rope_base=1e4, query=q.cuda()).cpu()
+    rows = cache.cpu()[tables[0].long()[(pos // bs).long()], :, :, (pos % bs).long()]
+    assert_bit_exact(rows[:, 1], v)
+    for got, x in ((rows[:, 0], k), (got_q, q)):
+        want = ref.rotate(x, pos, 1e4)
+        norm = x.double().unflatten(-1, (-1, 2)).norm(dim=-1).repeat_interleave(2, -1)
+        bound = want.abs() * ref.half_step(dtype) + norm * 2.0 ** -21
+        assert ((got.double() - want).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("dtype,quant", FORMATS)
 def test_one_row_of_several_requests(dev, dtype, quant):
     """A batch of one row whose request is not the first, and one whose only row is padding: the
