@@ -16,15 +16,16 @@
 // the error's bound added and taken off; where the three agree on codes and scale the 64-bit
 // result has the same ones. The others (one block in some thousands) are rotated in 64 bits and
 // rounded to fp32 to odd, which keeps every comparison with a border (borders have few bits, an
-// odd last bit never equals one), then rounded the same way. (All blocks in 64 bits: 16000 tokens
-// of 8 heads x 128 32 us.)
+// odd last bit never equals one), then rounded the same way. (16000 tokens of 8 heads x 128:
+// 25.9 us.)
 //
 // What bounds it: bytes for prompts, the launch and one dependent chain (position, table entry,
 // row) for decode steps. One workgroup takes a few tokens with all their heads, so that each
 // (token, frequency) pair's sine and cosine (about 45 fp64 instructions) is evaluated once and
 // shared through LDS by the K and query heads. Measured: 4602 tokens of 32 / 8 heads x 128, 113 MB
-// in 21 us (5.3 TB/s; a large copy reaches 6.6); 16 tokens 4 us; 4099 tokens of 4 heads into 4-bit
-// pages 9 us, reading 16384 of 8 heads back 18.6 us (85 MB, 4.6 TB/s).
+// in 20.7 us (5.4 TB/s; a large copy reaches 6.6); 16 tokens 4 us; 4099 tokens of 4 heads into 4-bit
+// pages 8.4 us, 16000 of 8 heads 25.9 (instructions: a third sines and cosines, the rest rotation,
+// scales and codes); reading 16384 of 8 heads back 18.6 us (85 MB, 4.6 TB/s).
 #include "sb_common.h"
 
 #include <algorithm>
@@ -36,6 +37,22 @@ constexpr int kAppendThreads = 256;
 constexpr int kTableEntries = 512;   // (token, frequency) pairs of one workgroup
 constexpr int kTokensMax = 8;
 constexpr int kRowsMax = 256;        // rows (K, V and query heads of its tokens) of one workgroup
+
+// x / d for 0 <= x < 2^31: with l = ceil(log2 d) and m = ceil(2^(31+l) / d), m d - 2^(31+l) < d <=
+// 2^l, so x * m >> (31 + l) is exact (T. Granlund and P. Montgomery, "Division by invariant integers
+// using multiplication", 1994).
+struct Divisor {
+  uint32_t magic;
+  int shift;
+  static Divisor by(int d) {
+    int shift = 31;
+    while ((1ll << (shift - 31)) < d) ++shift;
+    return {static_cast<uint32_t>(((1ull << shift) + d - 1) / d), shift};
+  }
+  __device__ __forceinline__ int of(int x) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(x)) * magic) >> shift);
+  }
+};
 
 struct AppendArgs {
   const char* k;
@@ -57,8 +74,7 @@ struct AppendArgs {
   int64_t num_blocks_total, num_blocks_per_seq;
   int num_requests, num_kv_heads, num_q_heads, head_dim, block_size;
   int tokens_per_wg, rows_per_y;
-  uint32_t row_magic;                     // row / rows of a token = (row * row_magic) >> row_shift
-  int row_shift;
+  Divisor row_div, half_div;              // by the rows of a token, by head_dim / 2
 };
 
 // Request of row t, or -1 before the first and behind the last one: the last r with
@@ -155,33 +171,43 @@ __device__ __forceinline__ uint32_t pack_codes(const float (&f)[VEC], float scal
   }
   return w;
 }
-// VEC values of a block of 32 (the lanes' others are 32 / VEC neighbours') as codes; a block that
-// holds an infinity or a NaN is marked as one by scale byte 255.
-template <int VEC> struct Block {
-  uint32_t codes;
+// Largest of the 32 / VEC lanes that share a block of 32 values, in all of them: neighbours inside
+// four lanes, then the mirror image inside eight and sixteen (DPP moves, no trip through LDS; with the
+// two packings below instead of three, 16000 tokens of 8 heads 27.3 -> 25.9 us).
+template <int VEC>
+__device__ __forceinline__ uint32_t block_max(uint32_t v) {
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xb1, 15, 15, true)));
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4e, 15, 15, true)));
+  if constexpr (VEC <= 4)
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x141, 15, 15, true)));
+  if constexpr (VEC <= 2)
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x140, 15, 15, true)));
+  return v;
+}
+// The scale of a block; one that holds an infinity or a NaN is marked as one by scale byte 255.
+struct Scale {
   int byte;
-  float top, scale;
+  bool bad;
+  float top, value;
 };
 template <int VEC>
-__device__ __forceinline__ Block<VEC> quantize(const float (&f)[VEC]) {
+__device__ __forceinline__ Scale block_scale(const float (&f)[VEC]) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-#pragma unroll
-  for (int o = 16 / VEC; o >= 1; o >>= 1)
-    top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, 64)));
-  Block<VEC> b;
+  top = block_max<VEC>(top);
+  Scale b;
   b.top = __uint_as_float(top);
-  const bool bad = top >= 0x7f800000u;
-  b.byte = bad ? 255 : scale_byte(b.top);
+  b.bad = top >= 0x7f800000u;
+  b.byte = b.bad ? 255 : scale_byte(b.top);
   // (byte 0 is 2^-127, below fp32's normal numbers)
-  b.scale = __uint_as_float(b.byte > 0 && !bad ? static_cast<uint32_t>(b.byte) << 23 : 0x00400000u);
-  b.codes = bad ? 0u : pack_codes(f, b.scale);
+  b.value = __uint_as_float(b.byte > 0 && !b.bad ? static_cast<uint32_t>(b.byte) << 23 : 0x00400000u);
   return b;
 }
 
 // One thread per row works out where the row comes from and goes to, for all lanes of it: worked out
-// by every lane, that (selects, divisions, 64-bit products) was most of the kernel's instructions.
+// by every lane, that (selects, divisions, 64-bit products) was most of the kernel's instructions: 4602 tokens of 32 / 8
+// heads x 128 22.9 -> 20.9 us, 16000 of 8 heads into 4-bit pages 31.2 -> 27.0.
 struct RowRef {
   const char* src;  // nullptr: left out (padding, or no slot)
   char* dst;
@@ -215,8 +241,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
 
   if (tid < n) {
     const int r0 = j0 + tid;
-    const int tok = static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(r0)) * a.row_magic) >>
-                                     a.row_shift);
+    const int tok = a.row_div.of(r0);
     const int j = r0 - tok * nrows;
     const int64_t t = t0 + tok;
     const int p = a.positions[t];
@@ -245,7 +270,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
   if (a.inv_freq) {
     // (from the last wave down: the first ones look the pages up)
     for (int i = kAppendThreads - 1 - tid; i < ntok * half; i += kAppendThreads) {
-      const int tok = i / half, f = i - tok * half;
+      const int tok = a.half_div.of(i), f = i - tok * half;
       const int p = (a.rotations ? a.rotations : a.positions)[t0 + tok];
       double s, c;
       sincos_cw(static_cast<double>(p) * static_cast<double>(a.inv_freq[f]), &s, &c);
@@ -285,22 +310,21 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
         }
       }
       if (Q4 && (ref.info & 2u)) {
-        Block<VEC> b = quantize(f);
+        Scale b = block_scale(f);
+        uint32_t w;
         if (turn) {
           // A rotated fp32 value is off by at most 2^-22 of its pair's norm (products and sum
           // 2^-24 each, sine and cosine 2^-24): 2^-21 of the block's largest magnitude, which is
-          // below 2^-18 of the scale.
-          bool unsure = b.byte == 255 || scale_byte(b.top * (1.f - 0x1p-20f)) !=
-                                             scale_byte(b.top * (1.f + 0x1p-20f));
-          const float off = b.scale * 0x1p-18f;
+          // below 2^-18 of the scale. Codes that agree at both ends agree between.
+          uint32_t unsure = b.bad || scale_byte(b.top * (1.f - 0x1p-20f)) !=
+                                         scale_byte(b.top * (1.f + 0x1p-20f));
+          const float off = b.value * 0x1p-18f;
           float lo[VEC], hi[VEC];
 #pragma unroll
           for (int i = 0; i < VEC; ++i) lo[i] = f[i] - off, hi[i] = f[i] + off;
-          unsure |= pack_codes(lo, b.scale) != pack_codes(hi, b.scale);
-          int any = unsure;
-#pragma unroll
-          for (int o = 16 / VEC; o >= 1; o >>= 1) any |= __shfl_xor(any, o, 64);
-          if (any) {
+          w = pack_codes(lo, b.value);
+          unsure |= w ^ pack_codes(hi, b.value);
+          if (block_max<VEC>(unsure)) {
             const double* t64;
             if constexpr (kBoth) t64 = cs64 + (ref.info >> 2) + vec * VEC;
             else t64 = reinterpret_cast<const double*>(trig);
@@ -310,17 +334,18 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
               f[i] = round_to_odd(e * t64[i] - o * t64[i + 1]);
               f[i + 1] = round_to_odd(e * t64[i + 1] + o * t64[i]);
             }
-            b = quantize(f);
+            b = block_scale(f);
+            w = b.bad ? 0u : pack_codes(f, b.value);
           }
+        } else {
+          w = b.bad ? 0u : pack_codes(f, b.value);
         }
-        const uint32_t w = b.codes;
-        const int sb = b.byte;
         char* dst = ref.dst + vec * (VEC / 2);
         if constexpr (VEC == 8) *(SB_GLOBAL uint32_t*)dst = w;
         else if constexpr (VEC == 4) *(SB_GLOBAL uint16_t*)dst = static_cast<uint16_t>(w);
         else *(SB_GLOBAL uint8_t*)dst = static_cast<uint8_t>(w);
         if ((vec & (32 / VEC - 1)) == 0)
-          ((SB_GLOBAL char*)ref.sdst)[vec / (32 / VEC)] = static_cast<char>(sb);
+          ((SB_GLOBAL char*)ref.sdst)[vec / (32 / VEC)] = static_cast<char>(b.byte);
       } else {
         if (turn) {
 #pragma unroll
@@ -546,11 +571,8 @@ extern "C" int sb_append_kv_paged(
   const int ny = a.tokens_per_wg > 1
                      ? 1 : static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, 512 / gx), steps));
   a.rows_per_y = std::min((steps + ny - 1) / ny, kRowsMax / rpi) * rpi;
-  // (exact for rows below 2^31: T. Granlund and P. Montgomery, 1994)
-  int log2_up = 0;
-  while ((1 << log2_up) < nrows) ++log2_up;
-  a.row_shift = 31 + log2_up;
-  a.row_magic = static_cast<uint32_t>(((1ull << a.row_shift) + nrows - 1) / nrows);
+  a.row_div = Divisor::by(nrows);
+  a.half_div = Divisor::by(a.head_dim / 2);
   const dim3 grid(static_cast<unsigned>(gx),
                   static_cast<unsigned>((all + a.rows_per_y - 1) / a.rows_per_y));
   const hipStream_t st = static_cast<hipStream_t>(stream);
