@@ -206,6 +206,8 @@ def _load_host() -> ctypes.PyDLL:
         lib.sb_host_rotation_counts.restype = _i64
         lib.sb_host_rotation_counts.argtypes = [ctypes.py_object, _i64, _i64, _i64, _vp, _vp,
                                                 _i64p]
+        lib.sb_host_entry.restype = ctypes.py_object
+        lib.sb_host_entry.argtypes = [ctypes.c_char_p, _vp]
     except AttributeError as exc:
         raise OSError(f"{HOST_LIB_PATH} does not export the expected functions ({exc})") from exc
     return lib
@@ -337,11 +339,26 @@ def on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
+_entries: dict = {}
+
+
+def _entry(name: str):
+    """An entry point as a callable of Python values, strides as tuples: the host library's where it
+    loads, which costs a microsecond less per call than ctypes."""
+    fn = getattr(lib(), name)
+    host = host_lib()
+    quick = host and host.sb_host_entry(name.encode(), ctypes.cast(fn, _vp).value)
+    return quick or (lambda *args: fn(*[(_i64 * len(a))(*a) if type(a) is tuple else a
+                                        for a in args]))
+
+
 def launch(device: torch.device, name: str, *args) -> None:
     """Invoke an entry point whose last argument is the stream on ``device``'s current stream,
     with ``device`` current (``call`` within ``on_device``, for callers that launch a kernel of a
-    few microseconds)."""
-    fn = getattr(_lib or _load(), name)
+    few microseconds); strides are given as tuples."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = _entry(name)
     index = device.index
     if _raw_stream is not None and _current_index is not None and _current_index() == index:
         rc = fn(*args, _raw_stream(index))

@@ -24,7 +24,6 @@ replayed with new positions.
 
 from __future__ import annotations
 
-import ctypes
 import functools
 import math
 
@@ -34,13 +33,6 @@ from . import _lib
 from .rope_correction import inv_freq_table
 
 __all__ = ["QuantizedKVCache", "append_kv_paged", "gather_kv_paged", "paged_attention"]
-
-
-@functools.lru_cache(maxsize=1024)
-def _stride_array(strides: tuple[int, ...]):
-    """Host array of strides for the library, which only reads it (the same few layouts come back
-    in every call: building the array takes about a microsecond)."""
-    return (ctypes.c_int64 * len(strides))(*strides)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -110,7 +102,7 @@ def _cache_args(kv_cache, dtype: torch.dtype, *rows):
     if isinstance(kv_cache, QuantizedKVCache):
         codes, scales = kv_cache._codes, kv_cache._scales
         return (_device(codes, rows), kv_cache.shape, codes.data_ptr(),
-                scales.data_ptr(), _stride_array(codes.stride()), _stride_array(scales.stride()),
+                scales.data_ptr(), codes.stride(), scales.stride(),
                 _lib.SB_DTYPE_MXFP4)
     dev = _device(kv_cache, rows)
     shape, strides = kv_cache.shape, kv_cache.stride()
@@ -121,7 +113,7 @@ def _cache_args(kv_cache, dtype: torch.dtype, *rows):
                         "QuantizedKVCache)")
     if strides[4] != 1:
         raise ValueError("kv_cache needs a unit last stride")
-    return (dev, shape, kv_cache.data_ptr(), None, _stride_array(strides), None,
+    return (dev, shape, kv_cache.data_ptr(), None, strides, None,
             _lib.dtype_code(kv_cache))
 
 
@@ -261,8 +253,7 @@ def append_kv_paged(
         base, sbase, k.data_ptr(), v.data_ptr(), _lib.ptr(q),
         None if q is None else query_out.data_ptr(), bt.data_ptr(), bt.stride(0), pos.data_ptr(),
         _lib.ptr(rot), _lib.ptr(starts), _lib.ptr(inv), num, requests, heads, hq, d, bs, shape[0],
-        width, _stride_array(kst), _stride_array(vst), None if q is None else _stride_array(qst),
-        None if q is None else _stride_array(ost), st, sst, dt, code)
+        width, kst, vst, qst, ost, st, sst, dt, code)
     return query_out
 
 
@@ -311,7 +302,7 @@ def gather_kv_paged(
         return out.zero_()
     _lib.launch(dev, "sb_gather_kv_paged", out.data_ptr(), base, sbase, bt.data_ptr(),
                 _lib.ptr(pos), num_rows, heads, d, bs, shape[0], bt.shape[0],
-                _stride_array(out.stride()), st, sst, dt, code)
+                out.stride(), st, sst, dt, code)
     return out
 
 
@@ -383,5 +374,5 @@ def paged_attention(
         dev, "sb_paged_attention",
         out.data_ptr(), q.data_ptr(), base, sbase, bt.data_ptr(), bt.stride(0), pos.data_ptr(),
         _lib.ptr(starts), _lib.ptr(ws), ws_bytes, num, requests, most, hq, heads, d, bs, nb,
-        width, win, sinks, float(scale), _stride_array(qst), _stride_array(ost), st, sst, dt, code)
+        width, win, sinks, float(scale), qst, ost, st, sst, dt, code)
     return out

@@ -204,3 +204,55 @@ def test_reference_quantiser():
     assert scale.tolist() == [[128]] and code[0, 8].item() == 6
     packed = torch.tensor([[0x21] * 16], dtype=torch.uint8)
     assert ref.dequantize(packed, torch.tensor([[128]], dtype=torch.uint8))[0, :2].tolist() == [1.0, 2.0]
+
+
+@pytest.mark.parametrize("host", [True, False])
+def test_entries_called_with_python_values(host, monkeypatch):
+    """Both forms of a call with Python values (through the host library, or ctypes without it)
+    reach the entry point with the same arguments: its refusals say which one was wrong."""
+    if not host:
+        monkeypatch.setattr(_lib, "_host", False)
+    strides = dict(ks=(128, 64, 1), vs=(128, 64, 1), cs=(4096, 2048, 1024, 64, 1))
+    refusals = [(_append, strides | dict(cdt=1), "dtype"),
+                (_append, strides | dict(k=None), "null"),
+                (_append, strides | dict(ks=(128, 64, 2)), "contiguous"),
+                (_append, strides | dict(n=1 << 32), "32 bits"),
+                (_append, strides | dict(d=48, cdt=3, scales=FAKE, ss=(8, 4, 2, 1, 1)), "of 32"),
+                (_gather, dict(os=(1, 1, 1, 2), cs=strides["cs"]), "contiguous"),
+                (_gather, dict(os=(384, 192, 64, 1), cs=strides["cs"], nb=0), "positive"),
+                (_attend, dict(qs=(256, 64, 1), os=(256, 64, 1), cs=(1 << 33, 2048, 1024, 64, 1)),
+                 "4 GiB"),
+                (_attend, dict(qs=(256, 64, 2), os=(256, 64, 1), cs=strides["cs"]), "contiguous"),
+                (_attend, dict(qs=(256, 64, 1), os=(256, 64, 1), cs=strides["cs"], win=-1),
+                 "negative")]
+    names = {_append: "sb_append_kv_paged", _gather: "sb_gather_kv_paged",
+             _attend: "sb_paged_attention"}
+    for call, over, words in refusals:
+        entry = _lib._entry(names[call])
+        assert (type(entry).__name__ == "builtin_function_or_method") == host
+        with monkeypatch.context() as m:  # (the same argument list, given to the callable)
+            m.setattr(_lib, "lib", lambda entry=entry, name=names[call]:
+                      type("entries", (), {name: staticmethod(entry)}))
+            assert call(**over) == _lib.SB_ERR_INVALID_ARGUMENT
+        assert words in _lib.lib().sb_last_error_string().decode()
+    # nothing to do: every argument is accepted
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "lib", lambda entry=entry: type("entries", (), {
+            "sb_paged_attention": staticmethod(entry)}))
+        assert _attend(n=0, qs=(256, 64, 1), os=(256, 64, 1), cs=strides["cs"]) == _lib.SB_OK
+
+
+def test_entries_refuse_other_values():
+    entry = _lib._entry("sb_gather_kv_paged")
+    good = [FAKE, FAKE, None, FAKE, None, 0, 2, 64, 16, 8, 4, (1, 1, 1, 1), (1, 1, 1, 1, 1), None,
+            2, 2, None]
+    assert entry(*good) == _lib.SB_OK                     # no rows: nothing is read
+    for i, bad in ((0, "x"), (0, 1.5), (5, 2.5), (5, None), (5, 1 << 64), (11, [1, 1, 1, 1]),
+                   (11, (1,) * 6), (11, (1, 1, 1, "1")), (14, 1 << 40), (14, None)):
+        args = list(good)
+        args[i] = bad
+        with pytest.raises((TypeError, OverflowError)):
+            entry(*args)
+    with pytest.raises(TypeError):
+        entry(*good[:-1])
+    assert _lib.host_lib().sb_host_entry(b"sb_version", FAKE) is None
