@@ -171,10 +171,16 @@ __device__ __forceinline__ int block_of(const PagedArgs& a, int key) {
                           a.bs_shift);
 }
 // Page of a key: its number in the pool, or -1 (outside the table, or no page of the pool).
+// In two parts where it is requested ahead of its use: behind a branch, or compared at once, the load
+// would be waited for, and with it all that were issued before it.
+__device__ __forceinline__ int page_entry(const PagedArgs& a, const int32_t* table, int key) {
+  return table[block_of(a, min(key, a.kv_len - 1))];
+}
+__device__ __forceinline__ int page_in(const PagedArgs& a, int entry, int key) {
+  return key < a.kv_len && entry >= 0 && entry < a.num_blocks_total ? entry : -1;
+}
 __device__ __forceinline__ int page_of(const PagedArgs& a, const int32_t* table, int key) {
-  if (key >= a.kv_len) return -1;
-  const int pb = table[block_of(a, key)];
-  return pb >= 0 && pb < a.num_blocks_total ? pb : -1;
+  return page_in(a, page_entry(a, table, key), key);
 }
 // Byte offset of a key's row from its plane and head (page given; no page: page 0, masked later).
 __device__ __forceinline__ int64_t row_offset(const PagedArgs& a, int key, int pb, uint32_t s_block,
@@ -518,7 +524,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_ke
   const uint32_t lane_scale = static_cast<uint32_t>(lq * a.s_pos) + lg * (D / 32) / 4;
   int64_t group_off = 0;                   // UNIFORM: of group lane & 1 of step lane / 2
   uint64_t group_live = 0;
-  int page[2] = {-1, -1};                  // else: of keys lq and lq + 16 of the next step
+  int entry[2] = {-1, -1};                 // else: of keys lq and lq + 16 of the next step
   auto lookup = [&](int idx) {
     if constexpr (UNIFORM) {
       if (((idx - i0) & 31) != 0 || idx >= i1) return;
@@ -530,7 +536,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_ke
     } else {
       const int k0 = tile_key<KT>(kt, min(idx, i1 - 1));
 #pragma unroll
-      for (int h = 0; h < 2; ++h) page[h] = page_of(a, table, k0 + 16 * h + lq);
+      for (int h = 0; h < 2; ++h) entry[h] = page_entry(a, table, k0 + 16 * h + lq);
     }
   };
   auto lane64 = [](int64_t v, int l) -> int64_t {
@@ -569,6 +575,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_ke
       }
     } else {
       const int k0 = tile_key<KT>(kt, idx);
+      const int page[2] = {page_in(a, entry[0], k0 + lq), page_in(a, entry[1], k0 + 16 + lq)};
       st.live = static_cast<uint32_t>(__ballot(page[0] >= 0) & 0xffffu) |
                 static_cast<uint32_t>(__ballot(page[1] >= 0) & 0xffffu) << 16;
 #pragma unroll
@@ -846,18 +853,25 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
     }
   }
   struct Stage {
-    f32x4 k[NC];
-    int64_t off;
-    int page;
+    f32x4 k[NC], v[4][NU];
+    int entry, page;
   };
   auto lookup = [&](int idx) -> int {
-    return page_of(a, table, tile_key<KT>(kt, min(idx, i1 - 1)) + lq);
+    return page_entry(a, table, tile_key<KT>(kt, min(idx, i1 - 1)) + lq);
   };
   auto fetch = [&](int idx, Stage& st) {
     const int k0 = tile_key<KT>(kt, idx);
-    st.off = row_offset(a, k0 + lq, st.page, a.c_block, a.c_pos);
+    st.page = page_in(a, st.entry, k0 + lq);
+    const int64_t off = row_offset(a, k0 + lq, st.page, a.c_block, a.c_pos);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) st.k[c] = *reinterpret_cast<const f32x4*>(kbase + st.off + 64 * c);
+    for (int c = 0; c < NC; ++c) st.k[c] = *reinterpret_cast<const f32x4*>(kbase + off + 64 * c);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {  // the offset of key 4 lg + x is lane 4 lg + x's
+      const int64_t vo = __shfl(off, 4 * lg + x, 64);
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+        st.v[x][u] = *reinterpret_cast<const f32x4*>(vbase + vo + 256 * u);
+    }
   };
   float m_ref = -INFINITY, negm = 0.f, l_run = 0.f;
   bool seen = false;
@@ -869,15 +883,9 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
   const float c_hi = a.scale_log2, c_lo = a.scale_log2_lo;
 
   int odd_first = 0x7fffffff, odd_last = -1;
-  auto step = [&](int idx, const Stage& st, Stage& ahead) {
+  auto step = [&](int idx, Stage& st, Stage& ahead) {
     const int k0 = tile_key<KT>(kt, idx);
-    f32x4 v[4][NU];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {  // the offset of key 4 lg + x is lane 4 lg + x's
-      const int64_t vo = __shfl(st.off, 4 * lg + x, 64);
-#pragma unroll
-      for (int u = 0; u < NU; ++u) v[x][u] = *reinterpret_cast<const f32x4*>(vbase + vo + 256 * u);
-    }
+    auto& v = st.v;
     fetch(min(idx + 1, i1 - 1), ahead);
     f32x4 sc[2] = {f32x4{}, f32x4{}};  // two chains
 #pragma unroll
@@ -944,20 +952,20 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
           o[u][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[x][u][e], w[x], o[u][e], 0, 0, 0);
   };
 
-  // K one step ahead in registers, the pages two; V is requested before the scores are formed.
-  // (Loads past the end are those of the last step again, as in paged_decode_kernel.)
+  // K and V one step ahead in registers, the pages two. (Loads past the end are those of the last
+  // step again, as in paged_decode_kernel.)
   Stage st[2];
   if (i0 < i1) {
-    st[0].page = lookup(i0);
+    st[0].entry = lookup(i0);
     fetch(i0, st[0]);
-    st[1].page = lookup(i0 + 1);
+    st[1].entry = lookup(i0 + 1);
     int i = i0;
     for (; i + 1 < i1; i += 2) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int page = lookup(i + u + 2);
+        const int entry = lookup(i + u + 2);
         step(i + u, st[u], st[u ^ 1]);
-        st[u].page = page;
+        st[u].entry = entry;
       }
     }
     if (i < i1) step(i, st[0], st[1]);
