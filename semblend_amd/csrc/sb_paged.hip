@@ -435,6 +435,12 @@ __device__ __forceinline__ void join_waves(const PagedArgs& a, const float* area
   }
 }
 
+__device__ __forceinline__ int64_t lane64(int64_t v, int l) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), l);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), l);
+  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
 // UNIFORM: pages of whole groups of 16 keys (block_size a multiple of 16). A group of 16 keys then
 // lies in one page, so its offset is a scalar: the offsets of 32 steps are looked up at once, two
 // per step in the lanes, and read from there (the scale bytes' are a sixteenth of the codes', as a
@@ -524,7 +530,9 @@ __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_ke
   const uint32_t lane_scale = static_cast<uint32_t>(lq * a.s_pos) + lg * (D / 32) / 4;
   int64_t group_off = 0;                   // UNIFORM: of group lane & 1 of step lane / 2
   uint64_t group_live = 0;
-  int entry[2] = {-1, -1};                 // else: of keys lq and lq + 16 of the next step
+  // else the table's entries for keys lq and lq + 16 of the step that is fetched next, and of the one
+  // behind it (requested before that fetch, whose loads need not be waited for then)
+  int entry[2] = {-1, -1}, entry_next[2] = {-1, -1};
   auto lookup = [&](int idx) {
     if constexpr (UNIFORM) {
       if (((idx - i0) & 31) != 0 || idx >= i1) return;
@@ -536,13 +544,11 @@ __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_ke
     } else {
       const int k0 = tile_key<KT>(kt, min(idx, i1 - 1));
 #pragma unroll
-      for (int h = 0; h < 2; ++h) entry[h] = page_entry(a, table, k0 + 16 * h + lq);
+      for (int h = 0; h < 2; ++h) {
+        entry[h] = entry_next[h];
+        entry_next[h] = page_entry(a, table, k0 + 16 * h + lq);
+      }
     }
-  };
-  auto lane64 = [](int64_t v, int l) -> int64_t {
-    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), l);
-    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), l);
-    return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
   };
   auto fetch = [&](int idx, Stage& st) {  // (behind lookup(idx))
     if constexpr (UNIFORM) {
@@ -738,16 +744,15 @@ __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_ke
     lookup(i0);
 #pragma unroll
     for (int x = 0; x < PD; ++x) {
-      fetch(min(i0 + x, i1 - 1), st[x]);
       if (!UNIFORM) lookup(i0 + x + 1);
+      fetch(min(i0 + x, i1 - 1), st[x]);
     }
     int i = i0;
     for (; i + PD < i1; i += PD + 1) {
 #pragma unroll
       for (int u = 0; u <= PD; ++u) {
-        if (UNIFORM) lookup(i + u + PD);
+        lookup(UNIFORM ? i + u + PD : i + u + PD + 1);
         fetch(min(i + u + PD, i1 - 1), st[(u + PD) % (PD + 1)]);
-        if (!UNIFORM) lookup(i + u + PD + 1);
         step(i + u, st[u]);
       }
     }
@@ -803,8 +808,9 @@ __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_ke
 // 16 c + 4 lg + e), and of V rows 4 lg + s the dims 64 u + 4 lq + 0..3: element e of them is the A
 // operand of output tile (u, e), whose row m is dim 64 u + 4 m + e, so V needs no transposition.
 // Weight s of a lane is key 4 lg + s, as the scores leave it. (154 rows of a context of 1024, 14 / 2
-// heads x 64, window 300: 12 us, the chain of latencies above and five key tiles per wave.)
-template <int D>
+// heads x 64, window 300: 10.5 us, the chain of latencies above and five key tiles per wave; with
+// every lane looking its keys up, as for pages that are no multiple of 16 tokens, 11.2.)
+template <int D, bool UNIFORM>
 __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const PagedArgs a) {
   constexpr int KT = 16;
   constexpr int NC = D / 16, NU = D / 64;
@@ -839,8 +845,8 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
   const int i1 = static_cast<int>(kt.total * (share + 1) / shares);
 
   const int32_t* table = a.tables + t.request * a.table_stride;
-  const char* kbase = a.k + kvh * a.c_head + 16 * lg;
-  const char* vbase = a.v + kvh * a.c_head + 16 * lq;
+  const char* kbase = a.k + kvh * a.c_head;
+  const char* vbase = a.v + kvh * a.c_head;
   f32x4 qf[NC];
   {
     const char* qp = a.q + (t.row0 + pi) * a.q_row +
@@ -854,23 +860,58 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
   }
   struct Stage {
     f32x4 k[NC], v[4][NU];
-    int entry, page;
+    uint32_t live;  // which of the step's keys have a page
   };
-  auto lookup = [&](int idx) -> int {
-    return page_entry(a, table, tile_key<KT>(kt, min(idx, i1 - 1)) + lq);
+  // UNIFORM (as in paged_decode_kernel): the offsets of 64 steps, looked up at once, one per lane;
+  // else the table's entries for key lq of the step that is fetched next and of the one behind it
+  // (requested before that fetch, whose loads need not be waited for then).
+  int64_t group_off = 0;
+  uint64_t group_live = 0;
+  int entry = -1, entry_next = -1;
+  auto lookup = [&](int idx) {
+    if constexpr (UNIFORM) {
+      if (((idx - i0) & 63) != 0 || idx >= i1) return;
+      const int key = tile_key<KT>(kt, min(idx + lane, i1 - 1));
+      const int pb = page_of(a, table, key);
+      group_off = row_offset(a, key, pb, a.c_block, a.c_pos);
+      group_live = __ballot(pb >= 0);
+    } else {
+      entry = entry_next;
+      entry_next = page_entry(a, table, tile_key<KT>(kt, min(idx, i1 - 1)) + lq);
+    }
   };
-  auto fetch = [&](int idx, Stage& st) {
-    const int k0 = tile_key<KT>(kt, idx);
-    st.page = page_in(a, st.entry, k0 + lq);
-    const int64_t off = row_offset(a, k0 + lq, st.page, a.c_block, a.c_pos);
+  const uint32_t lane_k = static_cast<uint32_t>(lq * a.c_pos) + 16 * lg;
+  auto fetch = [&](int idx, Stage& st) {  // (behind lookup(idx))
+    if constexpr (UNIFORM) {
+      const int at = (idx - i0) & 63;
+      st.live = (group_live >> at & 1u) ? 0xffffu : 0u;
+      const int64_t off = lane64(group_off, at);
+      const SB_GLOBAL char* kg = (const SB_GLOBAL char*)(kbase + off);
+      const SB_GLOBAL char* vg = (const SB_GLOBAL char*)(vbase + off);
+      asm volatile("" : "+s"(kg), "+s"(vg));
 #pragma unroll
-    for (int c = 0; c < NC; ++c) st.k[c] = *reinterpret_cast<const f32x4*>(kbase + off + 64 * c);
+      for (int c = 0; c < NC; ++c) st.k[c] = *(const SB_GLOBAL f32x4*)(kg + lane_k + 64 * c);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {  // the offset of key 4 lg + x is lane 4 lg + x's
-      const int64_t vo = __shfl(off, 4 * lg + x, 64);
+      for (int x = 0; x < 4; ++x) {
+        const uint32_t lane_v = static_cast<uint32_t>((4 * lg + x) * a.c_pos) + 16 * lq;
 #pragma unroll
-      for (int u = 0; u < NU; ++u)
-        st.v[x][u] = *reinterpret_cast<const f32x4*>(vbase + vo + 256 * u);
+        for (int u = 0; u < NU; ++u) st.v[x][u] = *(const SB_GLOBAL f32x4*)(vg + lane_v + 256 * u);
+      }
+    } else {
+      const int key = tile_key<KT>(kt, idx) + lq;
+      const int page = page_in(a, entry, key);
+      st.live = static_cast<uint32_t>(__ballot(page >= 0) & 0xffffu);
+      const int64_t off = row_offset(a, key, page, a.c_block, a.c_pos);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        st.k[c] = *reinterpret_cast<const f32x4*>(kbase + off + 16 * lg + 64 * c);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {  // the offset of key 4 lg + x is lane 4 lg + x's
+        const int64_t vo = __shfl(off, 4 * lg + x, 64);
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+          st.v[x][u] = *reinterpret_cast<const f32x4*>(vbase + vo + 16 * lq + 256 * u);
+      }
     }
   };
   float m_ref = -INFINITY, negm = 0.f, l_run = 0.f;
@@ -886,6 +927,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
   auto step = [&](int idx, Stage& st, Stage& ahead) {
     const int k0 = tile_key<KT>(kt, idx);
     auto& v = st.v;
+    lookup(UNIFORM ? idx + 1 : idx + 2);
     fetch(min(idx + 1, i1 - 1), ahead);
     f32x4 sc[2] = {f32x4{}, f32x4{}};  // two chains
 #pragma unroll
@@ -894,7 +936,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
       for (int e = 0; e < 4; ++e)
         sc[c & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(st.k[c][e], qf[c][e], sc[c & 1], 0, 0, 0);
     f32x4 s = sc[0] + sc[1];
-    const uint32_t live = static_cast<uint32_t>(__ballot(st.page >= 0) & 0xffffu);
+    const uint32_t live = st.live;
     const bool whole = live == 0xffffu && k0 + KT - 1 <= pmin &&
                        (k0 > pmax - a.window || k0 + KT - 1 < a.sinks);
     if (whole) {
@@ -956,17 +998,13 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
   // step again, as in paged_decode_kernel.)
   Stage st[2];
   if (i0 < i1) {
-    st[0].entry = lookup(i0);
+    lookup(i0);
+    if (!UNIFORM) lookup(i0 + 1);
     fetch(i0, st[0]);
-    st[1].entry = lookup(i0 + 1);
     int i = i0;
     for (; i + 1 < i1; i += 2) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int entry = lookup(i + u + 2);
-        step(i + u, st[u], st[u ^ 1]);
-        st[u].entry = entry;
-      }
+      step(i, st[0], st[1]);
+      step(i + 1, st[1], st[0]);
     }
     if (i < i1) step(i, st[0], st[1]);
   }
@@ -2140,7 +2178,8 @@ extern "C" int sb_paged_attention(
 #define SB_FEW_F16(D) SB_FEW(SB_DTYPE_F16, D)
 #define SB_FEW_F32(D)                                                                           \
   {                                                                                             \
-    SB_LAUNCH("paged_f32", (paged_f32_kernel<D>), grid, block, st, b);                          \
+    if (uniform) SB_LAUNCH("paged_f32", (paged_f32_kernel<D, true>), grid, block, st, b);       \
+    else SB_LAUNCH("paged_f32", (paged_f32_kernel<D, false>), grid, block, st, b);              \
     SB_MERGE(SB_DTYPE_F32, D, kDecodeRows, 16, b, pl.few)                                       \
   }
     if (dtype == SB_DTYPE_BF16) { SB_D(SB_FEW_BF16) }
