@@ -2,8 +2,9 @@
 
 Compiles every ``csrc/*.hip`` translation unit with hipcc for gfx950 only and links them into
 ``semblend_amd/libsemblend_hip.so``, next to the Python package that loads it. Object files
-go to ``_build/`` at the repository root (git-ignored). ``csrc/sb_host.cpp`` (Python index lists and call arguments to
-host arrays, against the interpreter's own headers) becomes ``libsemblend_host.so`` beside it.
+go to ``_build/`` at the repository root (git-ignored). ``csrc/sb_host.cpp`` (Python index lists to
+host arrays and Python values to call arguments, against the interpreter's own headers) becomes
+``libsemblend_host.so`` beside it.
 
 Usage: ``python -m semblend_amd._build`` or ``semblend_amd._build.build()``.
 """
