@@ -41,6 +41,7 @@ constexpr int kFewTarget = 1536;   // balanced items of a launch
 constexpr int kFewMinTiles = 8;    // fewest key tiles of an item (two per wave)
 constexpr int kShortItem = 24;     // key tiles of an item up to which one round is cut
 constexpr int64_t kLongTiles = 256;
+constexpr int kBalancedRows = 2048;  // most rows of balanced items
 constexpr int kDecodeAhead4 = 1;  // steps of 4-bit rows in flight per wave
 constexpr int kRowsTile = 256;
 constexpr int kRowsWaves = 8;
@@ -75,6 +76,7 @@ struct PagedArgs {
                                           // row per request), instead of nsplit per row tile
   float* part_o;                          // [tile][kv head][split][row][D]
   float* part_ml;                         // [tile][kv head][split][row][2]
+  int2* part_item;                        // balanced items: [tile][kv head] first slot and splits
 };
 
 __device__ __forceinline__ int wave_sum_i(int v) {
@@ -317,11 +319,11 @@ __device__ __forceinline__ Item even_item(const PagedArgs& a, int b) {
 
 // Items of one row per request, whose lengths may differ widely: all requests' key tiles together
 // are cut into items of about 1 / target of them, so a long request has many and a short one has
-// one. `c` counts the items of a KV head; with `merge`, it counts the row tiles, and the item
-// returned is the row tile's first. Every wave goes through all positions (a load and two lane
-// scans for 64 requests).
+// one. `c` counts the items of a KV head. Every wave goes through all positions (a load and two lane
+// scans for 64 requests); a row tile's first item leaves its place for the merge, which would have to
+// do the same (256 requests of up to 8300 tokens, 14 / 2 heads x 64: 17 us of merge, 1024: 112).
 template <int KT>
-__device__ __forceinline__ Item balanced_item(const PagedArgs& a, int c, int kvh, bool merge) {
+__device__ __forceinline__ Item balanced_item(const PagedArgs& a, int c, int kvh) {
   const int lane = threadIdx.x & 63;
   const int per = (a.group + kDecodeRows - 1) / kDecodeRows;  // row tiles of a request
   auto tiles_of = [&](int r) -> int {
@@ -341,7 +343,7 @@ __device__ __forceinline__ Item balanced_item(const PagedArgs& a, int c, int kvh
     size64 = max((all + a.target - 1) / a.target, static_cast<int64_t>(kShortItem));
   const int size = static_cast<int>(max(size64, static_cast<int64_t>(a.min_tiles)));
   Item it = {kvh, 0, 0, 0, {-1, 0, 0, 0}};
-  int base = 0, row_base = 0;  // items, row tiles before this block of requests
+  int base = 0;  // items before this block of requests
   for (int r0 = 0; r0 < a.num_rows; r0 += 64) {
     const int tiles = r0 == 0 ? first : tiles_of(r0 + lane);
     const int n = tiles < 0 ? 0 : max((tiles + size - 1) / size, 1);  // items of a row tile
@@ -352,24 +354,23 @@ __device__ __forceinline__ Item balanced_item(const PagedArgs& a, int c, int kvh
       if (lane >= d) incl += y;
     }
     const int before = incl - n * per;
-    const uint64_t past =
-        __ballot(merge ? c < row_base + (lane + 1) * per : c < base + incl);
+    const uint64_t past = __ballot(c < base + incl);
     if (past) {
       const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
       const int r = r0 + l;
-      if (r >= a.num_rows) return it;
       const int nl = __builtin_amdgcn_readfirstlane(__shfl(n, l, 64));
       const int start = base + __builtin_amdgcn_readfirstlane(__shfl(before, l, 64));
-      const int in = merge ? (c - row_base - l * per) * nl : c - start;
-      if (nl == 0) return it;  // (a padding row of the merge)
+      const int in = c - start;
       it.nsplit = nl;
       it.t = {r, r, 1, in / nl};
       it.split = in - it.t.tile * nl;
       it.slot = static_cast<int64_t>(start + in) * a.num_kv_heads + kvh;
+      if (it.split == 0 && threadIdx.x == 0)
+        a.part_item[(static_cast<int64_t>(r) * per + it.t.tile) * a.num_kv_heads + kvh] =
+            make_int2(static_cast<int>(it.slot), nl);
       return it;
     }
     base += __builtin_amdgcn_readfirstlane(__shfl(incl, 63, 64));
-    row_base += 64 * per;
   }
   return it;
 }
@@ -381,7 +382,7 @@ template <int KT>
 __device__ __forceinline__ Item decode_item(const PagedArgs& a, int b) {
   if (a.target > 0) {
     const int c = b / a.num_kv_heads;
-    return balanced_item<KT>(a, c, b - c * a.num_kv_heads, false);
+    return balanced_item<KT>(a, c, b - c * a.num_kv_heads);
   }
   return even_item<kDecodeRows>(a, b);
 }
@@ -1643,7 +1644,10 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedA
   const int kvh = blockIdx.x - tile_idx * a.num_kv_heads;
   Item it;
   if (TR == kDecodeRows && a.target > 0) {
-    it = balanced_item<KT>(a, tile_idx, kvh, true);
+    const int per = (a.group + TR - 1) / TR, r = tile_idx / per;
+    if (r >= a.num_rows || a.positions[r] < 0) return;  // (no item, nothing written for it)
+    const int2 first = a.part_item[blockIdx.x];
+    it = {kvh, first.y, 0, first.x, {r, r, 1, tile_idx - r * per}};
   } else {
     it = {kvh, 0, 0, (static_cast<int64_t>(tile_idx) * a.num_kv_heads + kvh) * a.nsplit,
           find_tile<TR>(a, tile_idx)};
@@ -1866,7 +1870,7 @@ struct PartPlan {  // one attention launch
   bool on;
   int64_t tiles, grid;
   int nsplit, min_tiles, target;
-  int64_t o_floats, ml_floats;
+  int64_t o_floats, ml_floats, items;
 };
 struct PagedPlan {
   bool matrix;          // the matrix-core kernels (else the VALU kernel)
@@ -1908,6 +1912,7 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
   if (!pl.matrix) return pl;
   const bool f32 = dtype == SB_DTYPE_F32;
   const bool ragged = starts || num_requests == 1;  // else one row per request
+  const bool one_each = !starts && (num_requests > 1 || num_rows == 1);  // row i is request i's
   // keys that a row may see, tables taken as full
   const int64_t keys = std::min(kv_len, std::min<int64_t>(window, kv_len) + sinks + 64);
   const int64_t per_few = (group + kDecodeRows - 1) / kDecodeRows;
@@ -1919,8 +1924,8 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
   pl.few.on = !rows_kernel || num_requests > 1;
   if (pl.few.on) {
     // with both kernels a `few` request has two tiles at most
-    pl.few.tiles = !ragged ? num_rows * per_few
-                           : rows_kernel ? std::min<int64_t>(tiles_bound, 2 * num_requests)
+    pl.few.tiles = one_each ? num_rows * per_few
+                            : rows_kernel ? std::min<int64_t>(tiles_bound, 2 * num_requests)
                                          : std::min<int64_t>(tiles_bound, flat);
     const int64_t key_tiles = (keys + (f32 ? 15 : 31)) / (f32 ? 16 : 32);
     const int64_t items = pl.few.tiles * num_kv_heads;
@@ -1934,9 +1939,12 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
     // (beside the rows kernel most of `tiles` are empty: one a request, about)
     pl.few.nsplit = split_for(rows_kernel ? std::min(items, num_requests * num_kv_heads) : items,
                               key_tiles, kFewMinTiles, tile_ns, 4000, 5000, 0);
-    if (!starts && (num_requests > 1 || num_rows == 1)) {  // row i is request i's
-      // Balanced items, unless there are enough of them as they are and none is long.
-      const bool split = pl.few.nsplit > 1 || key_tiles > kLongTiles;
+    if (one_each) {
+      // Balanced items, unless there are enough of them as they are and none is long, or so many rows
+      // that going through their positions costs more: 14 / 2 heads x 64, rows of up to 8300 tokens,
+      // balanced against one item each: 128 rows 66 and 73 us, 256 119 and 121, 1024 428 and 409,
+      // 4096 1788 and 1546 (lengths spread evenly; a long row among short ones is one item's else).
+      const bool split = (pl.few.nsplit > 1 || key_tiles > kLongTiles) && num_rows <= kBalancedRows;
       pl.few.target = split ? kFewTarget : 0;
       pl.few.nsplit = 1;
     }
@@ -1949,6 +1957,7 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
         pl.few.target > 0 || pl.few.nsplit > 1 ? pl.few.grid * kDecodeRows : 0;
     pl.few.o_floats = slots * head_dim;
     pl.few.ml_floats = slots * 2;
+    pl.few.items = pl.few.target > 0 ? (items + 1) / 2 * 2 : 0;  // (keeps what follows aligned)
   }
   pl.rows.on = rows_kernel;
   if (rows_kernel) {
@@ -1964,7 +1973,8 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
     pl.rows.o_floats = slots * head_dim;
     pl.rows.ml_floats = slots * 2;
   }
-  pl.bytes = 4 * (pl.few.o_floats + pl.few.ml_floats + pl.rows.o_floats + pl.rows.ml_floats);
+  pl.bytes = 4 * (pl.few.o_floats + pl.few.ml_floats + pl.rows.o_floats + pl.rows.ml_floats) +
+             8 * pl.few.items;
   return pl;
 }
 
@@ -2120,7 +2130,8 @@ extern "C" int sb_paged_attention(
     b.target = p.target;
     b.part_o = ws;
     b.part_ml = ws + p.o_floats;
-    ws += p.o_floats + p.ml_floats;
+    b.part_item = reinterpret_cast<int2*>(ws + p.o_floats + p.ml_floats);
+    ws += p.o_floats + p.ml_floats + 2 * p.items;
     return b;
   };
 #define SB_D(X)                     \

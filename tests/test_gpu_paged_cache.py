@@ -690,6 +690,18 @@ def test_append_tokens_of_no_request_or_slot(dev, quant):
     assert (err <= bound)[2:4].all()
 
 
+@pytest.mark.parametrize("n", [2048, 2049])
+@pytest.mark.parametrize("dtype,quant", [(BF16, False), (FP16, True), (FP32, False)])
+def test_very_many_single_rows(dev, dtype, quant, n):
+    """Decode steps on both sides of the most rows whose items are balanced, with tables of 9600
+    keys: padding rows, one long row, the others short."""
+    lens = [1 + (37 * i) % 40 for i in range(n)]
+    lens[n // 2] = 5000
+    pos = torch.tensor([-1 if i % 5 == 3 else x - 1 for i, x in enumerate(lens)], dtype=torch.int32)
+    pos[n // 2] = 4999
+    _attend_case(dtype, 64, 3, 1, 16, lens, None, None, 0, quant, positions=pos, width=600)
+
+
 # ---- together, captured, on other streams -----------------------------------------------------
 
 @pytest.mark.parametrize("quant", [False, True])
