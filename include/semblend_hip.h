@@ -636,7 +636,7 @@ int sb_gather_kv_paged(void* out, const void* kv_cache, const void* kv_scales,
  * j < sinks, inside the table and in a page of the pool; zeros for a row that sees none. Pages
  * between the sinks and the window are not read. fp32 scores, weights' sums and outputs; weights
  * rounded to dtype for their product with V (16-bit dtypes).
- * max_rows: no request has more rows (0: unknown). It chooses kernels (with max_rows * group <= 32
+ * max_rows: no request has more rows (0: unknown). It chooses kernels (with max_rows * group <= 48
  * only the single-token one is launched); any value gives the same rows.
  * q, out [num_rows, num_q_heads, head_dim] by strides (row, head, dim). head_dim at most 512;
  * 64 and 128 with 16-byte aligned rows (fp32 queries: over fp32 pages) run on the matrix cores.

@@ -337,6 +337,8 @@ __device__ __forceinline__ Item balanced_item(const PagedArgs& a, int c, int kvh
   for (int o = 32; o >= 1; o >>= 1) all += __shfl_xor(all, o, 64);
   // Key tiles of an item: one round of kFewSlots items while those are short, because there a
   // workgroup's fixed cost weighs; else `target` items, of which late ones make up for early ones.
+  // (32 / 8 heads x 128, one round and 1536 items: 4 requests of up to 8300 tokens 18.7 and 23.5 us,
+  // 32 requests 116 and 105, 32 of up to 32K over 4-bit pages 117 and 105.)
   all *= per * a.num_kv_heads;
   int64_t size64 = (all + kFewSlots - 1) / kFewSlots;
   if (size64 > kShortItem)
@@ -1879,7 +1881,14 @@ struct PagedPlan {
   int64_t bytes;
 };
 
-constexpr int kFewRows = 32;       // 16-bit arithmetic: two row tiles of 16
+// Flattened rows up to which all requests take the decode kernel (16-bit arithmetic): three tiles, which
+// read a request's keys three times. (Requests of 4000 tokens, 32 / 8 heads x 128, decode and rows
+// kernel: 48 rows 4 requests 41 and 52 us, 32 requests 183 and 205; 64 rows 53 and 52, 234 and 192.)
+constexpr int kFewRows = 48;
+// The same for a request of a call that launches the rows kernel anyway: one tile (40 requests of 700
+// rows and up to 6000 tokens, 28 / 4 heads x 128: 177 us, with 32 rows 189; nine requests of 1801 rows,
+// 32 / 8 heads, window 700: 57, with 32 rows 57, with 48 63).
+constexpr int kFewBeside = kDecodeRows;
 constexpr int kRowsMinTiles = 4;   // fewest 64-key tiles of a split of the rows kernel
 
 // Splits of each of `items` row tiles over `tiles` key tiles: those that 256 CUs take the shortest
@@ -1919,13 +1928,13 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
   const int64_t flat = num_rows * group;
   pl.few_max = 0x7fffffff;
   const bool rows_kernel = !f32 && ragged && max_rows * group > kFewRows;
-  if (rows_kernel) pl.few_max = num_requests == 1 ? 0 : kFewRows;
+  if (rows_kernel) pl.few_max = num_requests == 1 ? 0 : kFewBeside;
   const int64_t tiles_bound = (flat + kDecodeRows - 1) / kDecodeRows + num_requests;
   pl.few.on = !rows_kernel || num_requests > 1;
   if (pl.few.on) {
-    // with both kernels a `few` request has two tiles at most
+    // with both kernels a `few` request has one tile
     pl.few.tiles = one_each ? num_rows * per_few
-                            : rows_kernel ? std::min<int64_t>(tiles_bound, 2 * num_requests)
+                            : rows_kernel ? std::min<int64_t>(tiles_bound, num_requests)
                                          : std::min<int64_t>(tiles_bound, flat);
     const int64_t key_tiles = (keys + (f32 ? 15 : 31)) / (f32 ? 16 : 32);
     const int64_t items = pl.few.tiles * num_kv_heads;
@@ -1962,7 +1971,7 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
   pl.rows.on = rows_kernel;
   if (rows_kernel) {
     pl.rows.tiles = std::min<int64_t>(flat / kRowsTile + num_requests,
-                                      (flat + kFewRows - 1) / kFewRows);
+                                      (flat + kFewBeside - 1) / kFewBeside);
     pl.rows.min_tiles = kRowsMinTiles;
     // (a tile takes about 2.2 us at head_dim 128, a workgroup's start and end about 10)
     const int64_t tile_ns = 2200 * head_dim / 128;

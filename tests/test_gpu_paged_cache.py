@@ -363,6 +363,19 @@ def test_max_rows_is_a_hint(dev, dtype, quant, rows, max_rows):
 
 
 @pytest.mark.parametrize("dtype,quant", FORMATS)
+@pytest.mark.parametrize("hq,hkv", [(28, 4), (8, 2), (20, 1)])
+def test_requests_of_a_few_rows(dev, dtype, quant, hq, hkv):
+    """Requests on both sides of where their rows change kernels (48 rows and heads of a group), of
+    one to three row tiles of 16 each, without and with others of many rows."""
+    for extra in ([], [70]):
+        rows = [7, 6, 5, 1, 12, 13, 2, 3, 0, 7] + extra
+        _attend_case(dtype, 64, hq, hkv, 16, [30 + 41 * i for i in range(len(rows))], rows, None, 0,
+                     quant)
+        _attend_case(dtype, 128, hq, hkv, 16, [30 + 41 * i for i in range(len(rows))], rows, 50, 3,
+                     quant, max_rows=max(rows))
+
+
+@pytest.mark.parametrize("dtype,quant", FORMATS)
 def test_long_context_is_split(dev, dtype, quant):
     """Few items over a long context: the key ranges are split and joined."""
     _attend_case(dtype, 64, 4, 2, 16, [6000], None, None, 0, quant)
