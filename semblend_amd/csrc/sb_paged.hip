@@ -208,6 +208,8 @@ template <int DT> struct Half;  // 16-bit arithmetic beyond Mma<DT>
 template <> struct Half<SB_DTYPE_BF16> {
   static constexpr uint32_t kExp = 0x7f80u, kOne = 0x3f80u;
   static constexpr int kShift = 0;  // powers of two taken off 4-bit values
+  // The first scale byte whose block can hold a value that converts to an infinity (4 * 2^126).
+  static constexpr uint32_t kInfByte = 253;
   __device__ __forceinline__ static float to_f32(uint32_t x) { return bf16_to_f32(x); }
   __device__ __forceinline__ static f32x4 mma16(bf16x8_t a, bf16x8_t b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -223,6 +225,7 @@ template <> struct Half<SB_DTYPE_BF16> {
 template <> struct Half<SB_DTYPE_F16> {
   static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u;
   static constexpr int kShift = 2;
+  static constexpr uint32_t kInfByte = 143;  // (4 * 2^(143 - 127 - 2) = 65536)
   __device__ __forceinline__ static float to_f32(uint32_t x) { return f16_to_f32(x); }
   __device__ __forceinline__ static f32x4 mma16(f16x8_t a, f16x8_t b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -248,6 +251,13 @@ __device__ __forceinline__ u32x4_t fp4x8(uint32_t w, float scale) {
   const u32x4_t r = {H::template fp4<0>(w, scale), H::template fp4<1>(w, scale),
                      H::template fp4<2>(w, scale), H::template fp4<3>(w, scale)};
   return r;
+}
+
+// 4 values (16 bits of codes).
+template <int DT>
+__device__ __forceinline__ uint2 fp4x4(uint32_t w, float scale) {
+  using H = Half<DT>;
+  return make_uint2(H::template fp4<0>(w, scale), H::template fp4<1>(w, scale));
 }
 
 // Bits 15 and 31 of the result are set where a packed 16-bit value is infinite or NaN: adding one
@@ -626,13 +636,12 @@ __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_ke
     const uint32_t live = st.live;
     const bool whole = live == 0xffffffffu && k0 + KT - 1 <= pmin &&
                        (k0 > pmax - a.window || k0 + KT - 1 < a.sinks);
+    bool taken = false;  // (wave-uniform) some of this tile's V is not finite and is taken out
     if (!whole) {  // values that are not finite are taken out of V, and added where they are seen
       bool odd;
       if constexpr (Q4) {
-        odd = st.sv[0] == 255 || st.sv[1] == 255;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (st.sv[h] == 255) st.v[h][0] = raw_t{}, st.sv[h] = 0;
+        // (the scale byte decides: the values are looked at below, where they are converted)
+        odd = st.sv[0] >= H::kInfByte || st.sv[1] >= H::kInfByte;
       } else {
         uint32_t bits = 0;
 #pragma unroll
@@ -647,7 +656,8 @@ __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_ke
             for (int s = 0; s < NKS; ++s) st.v[h][s] = finite_part<DT>(st.v[h][s]);
         }
       }
-      if (__any(odd)) {
+      taken = __any(odd);
+      if (taken) {
         odd_first = min(odd_first, idx);
         odd_last = idx;
       }
@@ -662,6 +672,12 @@ __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_ke
         for (int s = 0; s < NKS; ++s)
           *reinterpret_cast<u32x4_t*>(vst + vchunk(row, lg * NKS + s)) =
               fp4x8<DT>(st.v[h][0][s], sc);
+        if (taken) {
+#pragma unroll
+          for (int s = 0; s < NKS; ++s)
+            *reinterpret_cast<u32x4_t*>(vst + vchunk(row, lg * NKS + s)) =
+                finite_part<DT>(fp4x8<DT>(st.v[h][0][s], sc));
+        }
       } else {
 #pragma unroll
         for (int s = 0; s < NKS; ++s)
@@ -780,7 +796,11 @@ __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_ke
 #pragma unroll
       for (int d = 0; d < NDT; ++d) {
         if constexpr (Q4) {
-          if (on && static_cast<uint8_t>(sr[d / 2]) == 255) o[d] += __builtin_nanf("");
+          const uint32_t byte = static_cast<uint8_t>(sr[d / 2]);
+          if (on && byte >= H::kInfByte) {
+            const uint32_t c = *reinterpret_cast<const uint16_t*>(row + 8 * d + 2 * lg);
+            add_not_finite<DT>(fp4x4<DT>(c, scale_of<H::kShift>(byte)), o[d], 0);
+          }
         } else {
           const uint2 w = *reinterpret_cast<const uint2*>(row + 2 * (16 * d + 4 * lg));
           if (on) add_not_finite<DT>(w, o[d], 0);
@@ -1206,8 +1226,16 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
     if (!in_part(key_of(i), paged[slot])) return;
     bool odd = false;
     if constexpr (Q4) {
-      odd = scale == 255;
-      if (odd) unpack(Codes{}, Vs[stage], IsV{});  // zeros
+      odd = scale >= H::kInfByte;
+      if (odd) {
+        const int row = tid4 >> 3, part = tid4 & 7;
+#pragma unroll
+        for (int x = 0; x < NW; ++x) {
+          u32x4_t* at = reinterpret_cast<u32x4_t*>(reinterpret_cast<char*>(Vs[stage]) + row * (D * 2) +
+                                                   16 * vswz<CH>(row, part * NW + x));
+          *at = finite_part<DT>(*at);
+        }
+      }
     } else {
 #pragma unroll
       for (int q = 0; q < NLD; ++q) {
@@ -1538,7 +1566,15 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
         const char* sr = vsb + row_offset(a, key, page, a.s_block, a.s_pos);
 #pragma unroll
         for (int d = 0; d < NDT; ++d)
-          if (on && static_cast<uint8_t>(sr[d]) == 255) o[d] += __builtin_nanf("");
+        {
+          const uint32_t byte = static_cast<uint8_t>(sr[d]);
+          if (!on || byte < H::kInfByte) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t c = *reinterpret_cast<const uint16_t*>(row + 16 * d + 4 * e + 2 * lg);
+            add_not_finite<DT>(fp4x4<DT>(c, scale_of<H::kShift>(byte)), o[d], 4 * e);
+          }
+        }
       } else {
 #pragma unroll
         for (int d = 0; d < NDT; ++d)

@@ -838,3 +838,77 @@ def test_repeated_calls_are_bit_identical(dev):
     want = pc.paged_attention(q, cache, tables.cuda(), pos)
     for _ in range(3):
         assert_bit_exact(pc.paged_attention(q, cache, tables.cuda(), pos), want)
+
+
+# ---- 4-bit blocks of any scale ----------------------------------------------------------------
+
+def _any_scale_case(dtype, d, rows, byte, bad_at, minus_page):
+    """Blocks of scale byte `byte` with random codes in K and V of the positions `bad_at`, and in
+    page 0, which is no page of the request (a table entry of -1 in the middle)."""
+    hq, hkv, bs, n, window, sinks = 14, 2, 16, 150, 20, 3
+    tables = torch.randperm(10, generator=gen(1))[None].to(torch.int32) + 1
+    if minus_page:
+        tables[0, (n - 10) // bs] = -1
+    codes, scales, _ = _quant_cache(11, hkv, bs, d, 2)
+    x = torch.tensor(bad_at)
+    page, slot = tables[0].long()[x // bs], x % bs
+    scales[page, :, :, slot] = byte
+    scales[0] = byte
+    cache = pc.QuantizedKVCache(codes.cuda(), scales.cuda())
+    pos = torch.arange(n - rows, n, dtype=torch.int32)
+    q = randn((rows, hq, d), dtype, 4)
+    want, mass, serr = ref.attention(q, ref.dequantize(codes, scales), tables, pos, [0, rows], window,
+                                     sinks, .125)
+    got = pc.paged_attention(q.cuda(), cache, tables[0].cuda(), pos.cuda(), window=window,
+                             sinks=sinks, scale=.125).cpu()
+    clean = ~torch.tensor([[bool(ref.visible(int(p), torch.tensor([b]), window, sinks))
+                            for b in bad_at] for p in pos]).any(1)
+    assert clean.any()
+    assert got[clean].isfinite().all()
+    bound = ref.attention_bound(want, mass, serr, dtype, n)
+    assert ((got.double() - want).abs()[clean] <= bound[clean]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [1, 3, 90])
+@pytest.mark.parametrize("byte", [142, 143, 200, 252, 253, 254, 255])
+def test_masked_4bit_blocks_of_any_scale(dev, dtype, d, rows, byte):
+    """Blocks that a row does not see may have any scale byte, those whose values are infinite in
+    the query's type (fp16 from 143 on, bf16 from 253 on) among them."""
+    n = 150
+    _any_scale_case(dtype, d, rows, byte, [n, n + 3], False)
+    _any_scale_case(dtype, d, rows, byte, [n + 1], True)
+    if rows < 90:
+        _any_scale_case(dtype, d, rows, byte, [5, 70], False)
+    if rows > 1:
+        _any_scale_case(dtype, d, rows, byte, [n - 1], False)
+
+
+@pytest.mark.parametrize("dtype,byte", [(BF16, 253), (BF16, 254), (FP16, 143)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [1, 60])
+def test_seen_4bit_values_beside_infinite_ones(dev, dtype, byte, d, rows):
+    """A block of V that holds an infinity in the query's type (one column of each block here), seen
+    whole or in part: an infinity of its sign there, the sums of the other columns as ever."""
+    hq, hkv, bs, n = 8, 2, 16, 200
+    tables, nb = _tables([n], bs, 1)
+    codes, scales, _ = _quant_cache(nb, hkv, bs, d, 2)
+    small = 1 if byte == 254 else 5                      # up to 2^126, 3 * 2^126, 3 * 2^16
+    for at in (40, n - 3 - rows):
+        c, s = codes.clone(), scales.clone()
+        page, slot = int(tables[0, at // bs]), at % bs
+        v = torch.randint(0, small + 1, (hkv, d), generator=gen(3)) + 8 * (torch.arange(d) % 2)
+        v[:, 3::32], v[:, 8::32] = 7, 15                 # 6 and -6 times the power
+        c[page, 1, :, slot] = (v[:, 0::2] | v[:, 1::2] << 4).to(torch.uint8)
+        s[page, 1, :, slot] = byte
+        q = randn((rows, hq, d), dtype, 4) * .25
+        pos = torch.arange(n - rows, n, dtype=torch.int32)
+        want, mass, serr = ref.attention(q, ref.dequantize(c, s), tables, pos, [0, rows], None, 0,
+                                         .01)
+        got = pc.paged_attention(q.cuda(), pc.QuantizedKVCache(c.cuda(), s.cuda()), tables[0].cuda(),
+                                 pos.cuda(), scale=.01).cpu()
+        assert (got[..., 3::32] == math.inf).all() and (got[..., 8::32] == -math.inf).all()
+        rest = [i for i in range(d) if i % 32 not in (3, 8)]
+        bound = ref.attention_bound(want, mass, serr, dtype, n)
+        assert ((got.double() - want).abs() <= bound)[..., rest].all()
