@@ -672,17 +672,20 @@ __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_ke
         for (int s = 0; s < NKS; ++s)
           *reinterpret_cast<u32x4_t*>(vst + vchunk(row, lg * NKS + s)) =
               fp4x8<DT>(st.v[h][0][s], sc);
-        if (taken) {
-#pragma unroll
-          for (int s = 0; s < NKS; ++s)
-            *reinterpret_cast<u32x4_t*>(vst + vchunk(row, lg * NKS + s)) =
-                finite_part<DT>(fp4x8<DT>(st.v[h][0][s], sc));
-        }
       } else {
 #pragma unroll
         for (int s = 0; s < NKS; ++s)
           *reinterpret_cast<u32x4_t*>(vst + vchunk(row, 4 * s + lg)) = st.v[h][s];
       }
+    }
+    if (Q4 && taken) {  // (the stage read back by words: values held in registers would spill)
+      asm volatile("" ::: "memory");
+#pragma unroll 1
+      for (int c = 0; c < KT * D / 2; c += 64) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(vst) + c + lane;
+        *at = finite_part<DT>(*at);
+      }
+      asm volatile("" ::: "memory");
     }
     // S^T = K Q^T: lane (lq, lg) gets row lq's scores of keys 16 h + 4 lg + 0..3
     f32x4 sc[2];
