@@ -1871,7 +1871,8 @@ __global__ __launch_bounds__(64) void paged_valu_kernel(const PagedArgs a) {
     seen |= __any(on) != 0;
     const float mt = fmaxf(m, wave_max(s));
     const float f = mt == -INFINITY || m == -INFINITY ? 0.f : expf(m - mt);
-    const float w = !on || (mt == -INFINITY) ? 0.f : expf(s - mt);
+    // (a NaN score has a NaN weight, also while no other score is above -inf)
+    const float w = !on || s == -INFINITY ? 0.f : expf(s - mt);
     l = l * f + wave_sum(w);
     m = mt;
     __syncthreads();

@@ -912,3 +912,26 @@ def test_seen_4bit_values_beside_infinite_ones(dev, dtype, byte, d, rows):
         rest = [i for i in range(d) if i % 32 not in (3, 8)]
         bound = ref.attention_bound(want, mass, serr, dtype, n)
         assert ((got.double() - want).abs() <= bound)[..., rest].all()
+
+
+@pytest.mark.parametrize("dtype,quant", FORMATS)
+@pytest.mark.parametrize("d", [64, 96])
+@pytest.mark.parametrize("rows", [1, 60])
+def test_seen_nan_score_before_finite_ones(dev, dtype, quant, d, rows):
+    """A first key whose score is NaN, alone in the first key tile that a row sees (later tiles hold
+    finite scores): the row is NaN, whichever kernel takes the call."""
+    hq, hkv, bs, n = 14, 2, 16, 700
+    tables, nb = _tables([n], bs, 1)
+    pos = torch.arange(n - rows, n, dtype=torch.int32)
+    if quant:
+        codes, scales, _ = _quant_cache(nb, hkv, bs, d, 2)
+        scales[int(tables[0, 0]), 0, :, 0] = 255
+        cache = pc.QuantizedKVCache(codes.cuda(), scales.cuda())
+    else:
+        host, _ = _cache(nb, hkv, bs, d, dtype, 2)
+        host[int(tables[0, 0]), 0, :, 0] = math.nan
+        cache = host.cuda()
+    q = randn((rows, hq, d), dtype, 4).cuda()
+    for window, sinks, nan in ((20, 1, True), (300, 3, True), (20, 0, False)):
+        got = pc.paged_attention(q, cache, tables[0].cuda(), pos.cuda(), window=window, sinks=sinks)
+        assert got.isnan().all() if nan else got.isfinite().all()
