@@ -635,7 +635,10 @@ int sb_gather_kv_paged(void* out, const void* kv_cache, const void* kv_scales,
  * num_kv_heads), over the keys j <= p_r = positions[r] with (window > 0) j > p_r - window or
  * j < sinks, inside the table and in a page of the pool; zeros for a row that sees none. Pages
  * between the sinks and the window are not read. fp32 scores, weights' sums and outputs; weights
- * rounded to dtype for their product with V (16-bit dtypes).
+ * rounded to dtype for their product with V (16-bit dtypes; with fp16 a weight below 2^-25 of the
+ * row's largest may round to zero).
+ * fp16 queries over 4-bit pages: values of 2^18 and more (scale bytes from 143 on; pages of fp16
+ * tokens hold none) are infinite to the matrix-core kernels, and bits below 2^-22 are rounded off.
  * max_rows: no request has more rows (0: unknown). It chooses kernels (with max_rows * group <= 48
  * only the single-token one is launched); any value gives the same rows.
  * q, out [num_rows, num_q_heads, head_dim] by strides (row, head, dim). head_dim at most 512;

@@ -220,8 +220,9 @@ template <> struct Half<SB_DTYPE_BF16> {
   }
 };
 // fp16: 4-bit values are taken times 2^-2 and the scores and outputs times 2^2, so that a block
-// whose largest value rounds to 65536 (its fp16 source was at most 65504) stays finite. Values are
-// exact from 2^-22 to 2^17; below that the last bits of a block are lost, at most 2^-23 of a value.
+// whose largest value rounds to 65536 (its fp16 source was at most 65504) stays finite. Values below
+// 2^18 are finite (larger ones, of pages written from wider tokens, become infinite), and exact where
+// they have no bits below 2^-22; others are off by at most 2^-23.
 template <> struct Half<SB_DTYPE_F16> {
   static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u;
   static constexpr int kShift = 2;

@@ -332,7 +332,10 @@ def paged_attention(
     (NaN included) does not reach it. A row that sees no key gets zeros.
     ``max_rows``: no request has more rows than this; it only helps to choose kernels (a decode
     step of several rows a request runs as one launch fewer). Scores, sums and outputs are fp32,
-    rounded once; 16-bit calls round the weights to their dtype for the product with V.
+    rounded once; 16-bit calls round the weights to their dtype for the product with V (fp16: a
+    weight below 2^-25 of the row's largest may be zero there). fp16 queries take 4-bit values
+    below 2^18, as pages of fp16 tokens hold them: a page written from wider tokens may hold larger
+    ones, which are infinite to such a query.
     Returns [R, num_q_heads, head_dim] (``out`` if given; padding rows of it are left as they
     are). Extension with no reference counterpart: the reference's attention is MHA over
     contiguous K/V (semblend_core/triton_kernels.py:655-734), without window.

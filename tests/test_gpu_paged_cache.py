@@ -935,3 +935,28 @@ def test_seen_nan_score_before_finite_ones(dev, dtype, quant, d, rows):
     for window, sinks, nan in ((20, 1, True), (300, 3, True), (20, 0, False)):
         got = pc.paged_attention(q, cache, tables[0].cuda(), pos.cuda(), window=window, sinks=sinks)
         assert got.isnan().all() if nan else got.isfinite().all()
+
+
+@pytest.mark.parametrize("plane", [0, 1])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [1, 60])
+def test_largest_4bit_values_of_fp16_queries(dev, plane, d, rows):
+    """fp16 queries over 4-bit pages take values below 2^18: every fourth key's K or V has blocks of
+    scale byte 142 (up to 6 * 2^15), and rows see them in whole tiles and in part."""
+    hq, hkv, bs, n = 8, 2, 16, 200
+    tables, nb = _tables([n], bs, 1)
+    codes, scales, _ = _quant_cache(nb, hkv, bs, d, 2)
+    at = torch.arange(0, n, 4)
+    scales[tables[0].long()[at // bs], plane, :, at % bs] = 142
+    cache = pc.QuantizedKVCache(codes.cuda(), scales.cuda())
+    pos = torch.arange(n - rows, n, dtype=torch.int32)
+    q = randn((rows, hq, d), FP16, 4)
+    scale = 1e-6 if plane == 0 else .01
+    for window, sinks in ((None, 0), (90, 4)):
+        want, mass, serr = ref.attention(q, ref.dequantize(codes, scales), tables, pos, [0, rows],
+                                         window, sinks, scale)
+        assert want.abs().amax() < 65504 * (1 if plane else 2 ** -8)
+        got = pc.paged_attention(q.cuda(), cache, tables[0].cuda(), pos.cuda(), window=window,
+                                 sinks=sinks, scale=scale).cpu()
+        bound = ref.attention_bound(want, mass, serr, FP16, n)
+        assert ((got.double() - want).abs() <= bound).all()
