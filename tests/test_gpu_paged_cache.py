@@ -960,3 +960,112 @@ def test_largest_4bit_values_of_fp16_queries(dev, plane, d, rows):
                                  sinks=sinks, scale=scale).cpu()
         bound = ref.attention_bound(want, mass, serr, FP16, n)
         assert ((got.double() - want).abs() <= bound).all()
+
+
+# ---- prompt chunks whose keys are split ---------------------------------------------------------
+
+HALVES = [f for f in FORMATS if f[0] != FP32]
+
+
+def _planned_bytes(rows, requests, hq, hkv, d, bs, width, window, sinks, dtype, quant):
+    from semblend_amd import _lib
+
+    return _lib.size_query("sb_paged_attention_workspace_size", rows, requests, int(requests > 1),
+                           rows, hq, hkv, d, bs, width, window or 0, sinks, _lib.SB_DTYPE[dtype],
+                           _lib.SB_DTYPE_MXFP4 if quant else _lib.SB_DTYPE[dtype])
+
+
+@pytest.mark.parametrize("dtype,quant", HALVES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (2900, 33)])
+def test_chunk_over_a_long_context_is_split(dev, dtype, quant, d, window, sinks):
+    """Chunks on the rows kernel, of one row tile and of three (the last not full), whose key lists
+    are cut into several parts: alone, beside a single token, and with padding between their rows."""
+    hq, hkv, bs, n = 4, 2, 16, 6000
+    for rows in (70, 300):
+        tiles = -(-rows * 2 // 256)
+        part = 4 * (d + 2) * 256 * tiles * hkv    # bytes of one part of every row tile
+        planned = _planned_bytes(rows, 1, hq, hkv, d, bs, n // bs, window, sinks, dtype, quant)
+        assert planned >= 3 * part, (planned, part)
+        pos = torch.arange(n - rows, n, dtype=torch.int32)
+        _attend_case(dtype, d, hq, hkv, bs, [n], [rows], window, sinks, quant, positions=pos)
+        pos = torch.cat([pos, torch.tensor([2], dtype=torch.int32)])
+        pos[3:9], pos[rows - 1] = -1, -1
+        _attend_case(dtype, d, hq, hkv, bs, [n, 3], [rows, 1], window, sinks, quant, positions=pos)
+
+
+@pytest.mark.parametrize("dtype,quant", HALVES)
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (28, 4)])
+def test_chunks_among_many_single_rows(dev, dtype, quant, hq, hkv):
+    """One or several long chunks in a batch of many requests, most of them of one row or none: the
+    chunks' keys are split."""
+    d, bs, n = 64, 16, 140
+    lens = [1 + (37 * i) % 400 for i in range(n)]
+    for chunks in ({100: 90}, {0: 33, 70: 150, 71: 64, 139: 20}):
+        rows = [chunks.get(i, 0 if i % 5 == 0 else 1) for i in range(n)]
+        ctx = [4000 + i if i in chunks else x for i, x in enumerate(lens)]
+        assert _planned_bytes(sum(rows), n, hq, hkv, d, bs, 259, None, 0, dtype, quant) > 0
+        _attend_case(dtype, d, hq, hkv, bs, ctx, rows, None, 0, quant, width=259)
+        _attend_case(dtype, d, hq, hkv, bs, ctx, rows, 3000, 5, quant, width=259)
+
+
+@pytest.mark.parametrize("dtype,quant", HALVES)
+def test_tables_much_wider_than_the_contexts(dev, dtype, quant):
+    """A captured step's tables are as wide as the longest context it may meet: chunks and single
+    tokens of a few hundred keys under tables of 128K."""
+    for d, rows in ((64, [90]), (128, [90]), (64, [90, 1, 40]), (128, [1, 300, 1])):
+        _attend_case(dtype, d, 14, 2, 16, [700, 40, 333][:len(rows)] if rows[0] > 1 else
+                     [30, 700, 64], rows, None, 0, quant, width=8192)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_graph_of_a_mixed_batch(dev, quant):
+    """A captured call of a chunk beside single tokens (both kernels and their merges), replayed with
+    other positions, rows per request and pages, eager calls between the replays."""
+    d, hq, hkv, bs, n = 128, 28, 4, 16, 4000
+    tables, nb = _tables([n, n, 90], bs, 1)
+    cache = _quant_cache(nb, hkv, bs, d, 2)[2] if quant else _cache(nb, hkv, bs, d, BF16, 2)[1]
+    num = 90
+    t = tables.cuda()
+    pos = torch.zeros(num, dtype=torch.int32, device="cuda")
+    starts = torch.zeros(4, dtype=torch.int32, device="cuda")
+    q = torch.zeros((num, hq, d), dtype=BF16, device="cuda")
+    out = torch.empty_like(q)
+
+    def step(o):
+        return pc.paged_attention(q, cache, t, pos, starts, window=3500, sinks=4, out=o)
+
+    step(torch.empty_like(q))
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(out)
+    for r, rows in enumerate(([80, 1, 1], [1, 60, 20], [0, 88, 2], [80, 1, 1])):
+        starts.copy_(torch.tensor(_starts(rows), dtype=torch.int32).cuda())
+        ctx = [n - 7 * r, n - 9, 90 - r]
+        p = torch.cat([torch.arange(c - x, c) for c, x in zip(ctx, rows)])
+        pos.copy_(torch.cat([p, torch.full((num - len(p),), 5)]).to(torch.int32).cuda())
+        q.copy_(randn((num, hq, d), BF16, 10 + r).cuda())
+        t.copy_(tables.flip(1) if r == 2 else tables)
+        out.fill_(2.0)
+        want = torch.full_like(q, 2.0)
+        g.replay()
+        step(want)
+        torch.cuda.synchronize()
+        assert_bit_exact(out, want)
+        assert (out[len(p):] == 2.0).all()
+        assert not (out[:len(p)] == 2.0).all(-1).any()
+
+
+@pytest.mark.parametrize("dtype,quant", HALVES)
+def test_repeated_mixed_calls_are_bit_identical(dev, dtype, quant):
+    d, hq, hkv, bs, rows = 128, 32, 8, 16, [200, 1, 1, 30]
+    tables, nb = _tables([5000, 300, 4000, 90], bs, 1)
+    cache = _quant_cache(nb, hkv, bs, d, 2)[2] if quant else _cache(nb, hkv, bs, d, dtype, 2)[1]
+    starts = torch.tensor(_starts(rows), dtype=torch.int32).cuda()
+    pos = torch.cat([torch.arange(n - r, n) for n, r in zip([5000, 300, 4000, 90], rows)])
+    q = randn((sum(rows), hq, d), dtype, 3).cuda()
+    args = (q, cache, tables.cuda(), pos.int().cuda(), starts)
+    want = pc.paged_attention(*args)
+    for _ in range(3):
+        assert_bit_exact(pc.paged_attention(*args), want)
