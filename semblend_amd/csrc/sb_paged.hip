@@ -72,6 +72,8 @@ struct PagedArgs {
   int flat_min, flat_max;                 // flattened rows of the requests this launch takes
   int num_tiles;                          // row tiles of the launch (bound)
   int nsplit, min_tiles;                  // key splits of a row tile; fewest key tiles of one
+  int slots;                              // > 0: places of partials; nsplit is the most that they
+                                          // allow the row tiles there are (counted on the device)
   int target;                             // > 0: items of about 1 / target of all key tiles (one
                                           // row per request), instead of nsplit per row tile
   float* part_o;                          // [tile][kv head][split][row][D]
@@ -83,6 +85,22 @@ __device__ __forceinline__ int wave_sum_i(int v) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
+}
+
+// First row, number of rows and number of row tiles of request r (with row_starts).
+struct RequestRows {
+  int start, rows, tiles;
+};
+template <int TR>
+__device__ __forceinline__ RequestRows request_rows(const PagedArgs& a, int r) {
+  RequestRows q = {0, 0, 0};
+  if (r < a.num_requests) {
+    q.start = min(max(a.row_starts[r], 0), a.num_rows);
+    q.rows = max(min(a.row_starts[r + 1], a.num_rows) - q.start, 0);
+    const int64_t flat = static_cast<int64_t>(q.rows) * a.group;
+    if (flat > a.flat_min && flat <= a.flat_max) q.tiles = static_cast<int>((flat + TR - 1) / TR);
+  }
+  return q;
 }
 
 // Row tile `idx` of a launch: its request and which tile of TR flattened rows of it.
@@ -107,15 +125,8 @@ __device__ __forceinline__ TileRef find_tile(const PagedArgs& a, int idx) {
   const int lane = threadIdx.x & 63;
   int base = 0;
   for (int c = 0; c < a.num_requests; c += 64) {
-    const int r = c + lane;
-    int s = 0, n = 0, tiles = 0;
-    if (r < a.num_requests) {
-      s = min(max(a.row_starts[r], 0), a.num_rows);
-      n = max(min(a.row_starts[r + 1], a.num_rows) - s, 0);
-      const int64_t flat = static_cast<int64_t>(n) * a.group;
-      if (flat > a.flat_min && flat <= a.flat_max) tiles = static_cast<int>((flat + TR - 1) / TR);
-    }
-    int incl = tiles;
+    const RequestRows q = request_rows<TR>(a, c + lane);
+    int incl = q.tiles;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int y = __shfl_up(incl, d, 64);
@@ -125,15 +136,39 @@ __device__ __forceinline__ TileRef find_tile(const PagedArgs& a, int idx) {
     if (past) {
       const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
       t.request = c + l;
-      t.row0 = __builtin_amdgcn_readfirstlane(__shfl(s, l, 64));
-      t.rows = __builtin_amdgcn_readfirstlane(__shfl(n, l, 64));
+      t.row0 = __builtin_amdgcn_readfirstlane(__shfl(q.start, l, 64));
+      t.rows = __builtin_amdgcn_readfirstlane(__shfl(q.rows, l, 64));
       t.tile = idx - base -
-               __builtin_amdgcn_readfirstlane(__shfl(incl, l, 64) - __shfl(tiles, l, 64));
+               __builtin_amdgcn_readfirstlane(__shfl(incl, l, 64) - __shfl(q.tiles, l, 64));
       return t;
     }
     base += __builtin_amdgcn_readfirstlane(__shfl(incl, 63, 64));
   }
   return t;
+}
+
+// Row tiles of a launch and the most parts that the keys of one are cut into. The host knows how
+// many row tiles a batch may have, and what its rows would fill if they were one request's; between
+// the two lie factors of ten (one chunk among hundreds of single tokens). Partials are kept for
+// `slots` (row tile, KV head, part) places, and the parts of a tile follow from the number of tiles
+// that row_starts gives: one scan more per workgroup, of the launches that split only. (Bounds
+// alone: 256 requests with a chunk of 512 rows, 32 / 8 heads x 128, up to 8192 tokens: 1022 MB of
+// partials and 234 us of rows kernel and merge, 68 MB and 134 with the scan.)
+struct Parts {
+  int tiles, most;
+};
+template <int TR>
+__device__ __forceinline__ Parts parts_of(const PagedArgs& a) {
+  if constexpr (TR == kRowsTile) {
+    if (a.slots > 0) {
+      int n = 0;
+      for (int c = 0; c < a.num_requests; c += 64)
+        n += request_rows<TR>(a, c + (threadIdx.x & 63)).tiles;
+      n = max(__builtin_amdgcn_readfirstlane(wave_sum_i(n)), 1);
+      return {n, max(min(a.nsplit, a.slots / (n * a.num_kv_heads)), 1)};
+    }
+  }
+  return {a.num_tiles, a.nsplit};
 }
 
 // The key tiles (of KT keys) that rows at positions [pmin, pmax] see: n_sink tiles from 0 on,
@@ -161,8 +196,8 @@ template <int KT>
 __device__ __forceinline__ int tile_key(const KeyTiles& t, int i) {
   return (i < t.n_sink ? i : t.lo + i - t.n_sink) * KT;
 }
-__device__ __forceinline__ int split_count(const PagedArgs& a, int total) {
-  return max(1, min(a.nsplit, total / a.min_tiles));
+__device__ __forceinline__ int split_count(const PagedArgs& a, int most, int total) {
+  return max(1, min(most, total / a.min_tiles));
 }
 
 // Quotient of a key (31 bits) by the block size d: with l = ceil(log2 d) and m = ceil(2^(31+l) / d),
@@ -316,15 +351,17 @@ struct Item {
 };
 
 // Items of even splits: every row tile has its keys split nsplit ways (fewer if they are few); KV
-// head fastest, then row tile (the last one, which sees most, first), then split. (nsplit is filled
-// in once the tile's positions are read.)
+// head fastest, then row tile (the last one, which sees most, first), then split. (nsplit is the most
+// here; the tile's own follows once its positions are read.)
 template <int TR>
 __device__ __forceinline__ Item even_item(const PagedArgs& a, int b) {
-  const int rest = b / a.num_kv_heads, split = rest / a.num_tiles;
+  const Parts n = parts_of<TR>(a);
+  const int rest = b / a.num_kv_heads, split = rest / n.tiles;
   const int kvh = b - rest * a.num_kv_heads;
-  const int tile_idx = a.num_tiles - 1 - (rest - split * a.num_tiles);
-  return {kvh, 1, split,
-          (static_cast<int64_t>(tile_idx) * a.num_kv_heads + kvh) * a.nsplit + split,
+  if (TR == kRowsTile && split >= n.most) return {kvh, n.most, split, 0, {-1, 0, 0, 0}};
+  const int tile_idx = n.tiles - 1 - (rest - split * n.tiles);
+  return {kvh, n.most, split,
+          (static_cast<int64_t>(tile_idx) * a.num_kv_heads + kvh) * n.most + split,
           find_tile<TR>(a, tile_idx)};
 }
 
@@ -503,7 +540,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64, Q4 ? 3 : 2) void paged_decode_ke
   pmax = __builtin_amdgcn_readfirstlane(pmax);
   if (pmax < 0) return;
   const KeyTiles kt = key_tiles<KT>(a, pmin, pmax);
-  const int nsplit = a.target > 0 ? it.nsplit : split_count(a, kt.total);
+  const int nsplit = a.target > 0 ? it.nsplit : split_count(a, it.nsplit, kt.total);
   if (it.split >= nsplit) return;
   // this wave's share of the split's tiles
   const int64_t share = static_cast<int64_t>(it.split) * kDecodeWaves + wave;
@@ -864,7 +901,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
   pmax = __builtin_amdgcn_readfirstlane(pmax);
   if (pmax < 0) return;
   const KeyTiles kt = key_tiles<KT>(a, pmin, pmax);
-  const int nsplit = a.target > 0 ? it.nsplit : split_count(a, kt.total);
+  const int nsplit = a.target > 0 ? it.nsplit : split_count(a, it.nsplit, kt.total);
   if (it.split >= nsplit) return;
   const int64_t share = static_cast<int64_t>(it.split) * kDecodeWaves + wave;
   const int64_t shares = static_cast<int64_t>(nsplit) * kDecodeWaves;
@@ -1131,7 +1168,7 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
   tmax = __builtin_amdgcn_readfirstlane(tmax);
   if (tmax < 0) return;  // uniform
   const KeyTiles kt = key_tiles<KT>(a, tmin, tmax);
-  const int nsplit = split_count(a, kt.total);
+  const int nsplit = split_count(a, it.nsplit, kt.total);
   if (it.split >= nsplit) return;  // uniform
   const int i0 = static_cast<int>(static_cast<int64_t>(kt.total) * it.split / nsplit);
   const int i1 = static_cast<int>(static_cast<int64_t>(kt.total) * (it.split + 1) / nsplit);
@@ -1685,13 +1722,16 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedA
   const int tile_idx = blockIdx.x / a.num_kv_heads;
   const int kvh = blockIdx.x - tile_idx * a.num_kv_heads;
   Item it;
+  int most = 0;  // even splits: the most parts of a row tile
   if (TR == kDecodeRows && a.target > 0) {
     const int per = (a.group + TR - 1) / TR, r = tile_idx / per;
     if (r >= a.num_rows || a.positions[r] < 0) return;  // (no item, nothing written for it)
     const int2 first = a.part_item[blockIdx.x];
     it = {kvh, first.y, 0, first.x, {r, r, 1, tile_idx - r * per}};
   } else {
-    it = {kvh, 0, 0, (static_cast<int64_t>(tile_idx) * a.num_kv_heads + kvh) * a.nsplit,
+    most = parts_of<TR>(a).most;
+    if (most <= 1) return;
+    it = {kvh, 0, 0, (static_cast<int64_t>(tile_idx) * a.num_kv_heads + kvh) * most,
           find_tile<TR>(a, tile_idx)};
   }
   const TileRef& t = it.t;
@@ -1723,7 +1763,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(const PagedA
       pmax = max(pmax, red[1][w]);
     }
     if (pmax < 0) return;
-    nsplit = split_count(a, key_tiles<KT>(a, pmin, pmax).total);
+    nsplit = split_count(a, most, key_tiles<KT>(a, pmin, pmax).total);
   }
   if (nsplit <= 1) return;
   const int lane = threadIdx.x % VPR, row_in = threadIdx.x / VPR % RPW;
@@ -1913,6 +1953,8 @@ struct PartPlan {  // one attention launch
   bool on;
   int64_t tiles, grid;
   int nsplit, min_tiles, target;
+  int64_t slots;        // > 0: places of partials that row tiles counted on the device share
+  int64_t merge_tiles;  // row tiles that may be split
   int64_t o_floats, ml_floats, items;
 };
 struct PagedPlan {
@@ -1931,6 +1973,9 @@ constexpr int kFewRows = 48;
 // 32 / 8 heads, window 700: 57, with 32 rows 57, with 48 63).
 constexpr int kFewBeside = kDecodeRows;
 constexpr int kRowsMinTiles = 4;   // fewest 64-key tiles of a split of the rows kernel
+// Places of partials of a batch of several requests: two rounds of workgroups, one per CU (40 requests
+// of 17 rows, 28 / 4 heads x 128, up to 6000 tokens: 129 us, with one round 165; 68 MB at 128 dims).
+constexpr int64_t kRowsSlots = 512;
 
 // Splits of each of `items` row tiles over `tiles` key tiles: those that 256 CUs take the shortest
 // for, in rounds of a workgroup's fixed time and its tiles' (which two workgroups of a CU share),
@@ -2008,20 +2053,32 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
     pl.few.o_floats = slots * head_dim;
     pl.few.ml_floats = slots * 2;
     pl.few.items = pl.few.target > 0 ? (items + 1) / 2 * 2 : 0;  // (keeps what follows aligned)
+    pl.few.merge_tiles = pl.few.tiles;
   }
   pl.rows.on = rows_kernel;
   if (rows_kernel) {
-    pl.rows.tiles = std::min<int64_t>(flat / kRowsTile + num_requests,
-                                      (flat + kFewBeside - 1) / kFewBeside);
+    const int64_t filled = (flat + kRowsTile - 1) / kRowsTile;  // row tiles of one request's rows
+    pl.rows.tiles = num_requests == 1 ? filled
+                                      : std::min<int64_t>(flat / kRowsTile + num_requests,
+                                                          (flat + kFewBeside - 1) / kFewBeside);
     pl.rows.min_tiles = kRowsMinTiles;
     // (a tile takes about 2.2 us at head_dim 128, a workgroup's start and end about 10)
     const int64_t tile_ns = 2200 * head_dim / 128;
-    pl.rows.nsplit = split_for(((flat + kRowsTile - 1) / kRowsTile) * num_kv_heads,
-                               (keys + 63) / 64, kRowsMinTiles, tile_ns, 10000, 5000, 6000);
-    pl.rows.grid = pl.rows.tiles * num_kv_heads * pl.rows.nsplit;
-    const int64_t slots = pl.rows.nsplit > 1 ? pl.rows.grid * kRowsTile : 0;
-    pl.rows.o_floats = slots * head_dim;
-    pl.rows.ml_floats = slots * 2;
+    const int64_t items = filled * num_kv_heads, most_items = pl.rows.tiles * num_kv_heads;
+    pl.rows.nsplit = split_for(items, (keys + 63) / 64, kRowsMinTiles, tile_ns, 10000, 5000, 6000);
+    int64_t slots = 0;
+    if (pl.rows.nsplit > 1) {
+      // What the parts of `filled` tiles take, or kRowsSlots if that is more (rows of several requests
+      // fill their tiles less), and no more than all parts of all tiles.
+      slots = std::min(std::max<int64_t>(items * pl.rows.nsplit, kRowsSlots),
+                       most_items * pl.rows.nsplit);
+      if (num_requests > 1) pl.rows.slots = slots;
+    }
+    pl.rows.grid = std::max(most_items, slots);
+    // (of more tiles than half the places none is split)
+    pl.rows.merge_tiles = std::min(pl.rows.tiles, slots / (2 * num_kv_heads));
+    pl.rows.o_floats = slots * kRowsTile * head_dim;
+    pl.rows.ml_floats = slots * kRowsTile * 2;
   }
   pl.bytes = 4 * (pl.few.o_floats + pl.few.ml_floats + pl.rows.o_floats + pl.rows.ml_floats) +
              8 * pl.few.items;
@@ -2177,6 +2234,7 @@ extern "C" int sb_paged_attention(
     b.num_tiles = static_cast<int>(p.tiles);
     b.nsplit = p.nsplit;
     b.min_tiles = p.min_tiles;
+    b.slots = static_cast<int>(p.slots);
     b.target = p.target;
     b.part_o = ws;
     b.part_ml = ws + p.o_floats;
@@ -2191,7 +2249,7 @@ extern "C" int sb_paged_attention(
   if ((P).nsplit > 1 || (P).target > 0) {                                                       \
     constexpr int rpw = TR == kDecodeRows ? 1 : 1024 / D;                                       \
     const int live = (P).target > 0 ? std::min<int>(TR, static_cast<int>(group)) : TR;          \
-    const dim3 mg(static_cast<unsigned>((P).tiles * num_kv_heads), (live + rpw - 1) / rpw);     \
+    const dim3 mg(static_cast<unsigned>((P).merge_tiles * num_kv_heads), (live + rpw - 1) / rpw); \
     SB_LAUNCH("paged_merge", (paged_merge_kernel<DT, D, TR, KT, rpw>), mg, dim3(kMergeThreads), \
               st, B, out_scale);                                                                \
   }

@@ -1069,3 +1069,15 @@ def test_repeated_mixed_calls_are_bit_identical(dev, dtype, quant):
     want = pc.paged_attention(*args)
     for _ in range(3):
         assert_bit_exact(pc.paged_attention(*args), want)
+
+
+@pytest.mark.parametrize("dtype,quant", HALVES)
+@pytest.mark.parametrize("chunks", [2, 6, 20, 70])
+def test_row_tiles_share_the_partials(dev, dtype, quant, chunks):
+    """Requests of a few more rows than the decode kernel takes: many row tiles that are little
+    filled, so that the parts of each go from the most to one; empty requests between them."""
+    d, hq, hkv, bs = 64, 28, 4, 16
+    rows = [3 + i % 2 if i % 2 else 0 for i in range(2 * chunks)]
+    lens = [1500 + 31 * i for i in range(2 * chunks)]
+    for window, sinks in ((None, 0), (700, 70)):
+        _attend_case(dtype, d, hq, hkv, bs, lens, rows, window, sinks, quant, width=400)

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import random
 
 import pytest
 import torch
@@ -256,3 +257,26 @@ def test_entries_refuse_other_values():
     with pytest.raises(TypeError):
         entry(*good[:-1])
     assert _lib.host_lib().sb_host_entry(b"sb_version", FAKE) is None
+
+
+def test_workspace_of_many_requests():
+    """A chunk or several among many requests: the partials of split key ranges go by what a round or
+    two of workgroups can hold, not by the row tiles that such a batch might have."""
+    size = lambda *a: _lib.size_query("sb_paged_attention_workspace_size", *a)
+    # (rows, requests, query and KV heads, pages of a table)
+    for rows, requests, hq, hkv, width in ((767, 256, 32, 8, 512), (300, 128, 32, 8, 512),
+                                           (575, 64, 32, 8, 512), (127, 64, 28, 4, 512),
+                                           (511, 256, 28, 4, 2048), (4000, 1000, 32, 8, 2048)):
+        for dt, cdt in ((2, 2), (1, 1), (2, 3)):
+            got = size(rows, requests, 1, rows, hq, hkv, 128, 16, width, 0, 0, dt, cdt)
+            assert got <= 100e6, (rows, requests, got)
+    # (a launch of n items is split while (n - 1) of them are below two rounds of 256)
+    rng = random.Random(1)
+    for _ in range(2000):
+        hkv = rng.choice((1, 2, 4, 8, 16, 32))
+        requests, d = int(2 ** rng.uniform(0, 11)), rng.choice((64, 128))
+        rows = requests + int(2 ** rng.uniform(0, 12))
+        got = size(rows, requests, 1, rng.choice((0, rows)), hkv * rng.choice((1, 4, 7)), hkv, d, 16,
+                   int(2 ** rng.uniform(0, 14)), rng.choice((0, 1, 700, 40000)), rng.choice((0, 4)),
+                   rng.choice((1, 2)), rng.choice((1, 2, 3)))
+        assert got <= 4 * (d + 2) * 1024 * (256 + 16), (rows, requests, hkv, got)
