@@ -20,6 +20,10 @@ begin; without it row i is request i's only one, as in a decode step, or, with o
 rows are that one's. Rows of no request and rows with a negative position are padding and left as
 they are. All metadata is read on the device, so a step can be captured into a HIP graph once and
 replayed with new positions.
+
+These are a server's calls and have no backward pass: a result that torch would differentiate
+through (an input requires a gradient, in grad mode) raises when its gradient is asked for. Rows
+written into a cache, ``out`` or ``query_out`` leave no record there.
 """
 
 from __future__ import annotations
@@ -175,6 +179,26 @@ def _like(t: torch.Tensor, strides):
     return new, new.stride()
 
 
+class _NoBackward(torch.autograd.Function):
+    """``out`` as a function of ``inputs`` that cannot be differentiated."""
+
+    @staticmethod
+    def forward(ctx, name, out, *inputs):
+        ctx.name = name
+        ctx.mark_dirty(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name} has no backward pass; call it under torch.no_grad(), or on "
+                           "detached tensors")
+
+
+def _recorded(name: str, out: torch.Tensor, *inputs: torch.Tensor) -> torch.Tensor:
+    """A new result, so that a gradient of it raises instead of missing these inputs."""
+    return _NoBackward.apply(name, out, *inputs) if torch.is_grad_enabled() else out
+
+
 def append_kv_paged(
     kv_cache,
     key: torch.Tensor,
@@ -225,6 +249,7 @@ def append_kv_paged(
     if d % 2:
         raise ValueError("head_dim must be even")
     q, qst, ost, hq = None, None, None, 0
+    new = query is not None and query_out is None
     if query is not None:
         qshape = query.shape
         if len(qshape) != 3 or qshape[0] != num or qshape[2] != d:
@@ -254,6 +279,8 @@ def append_kv_paged(
         None if q is None else query_out.data_ptr(), bt.data_ptr(), bt.stride(0), pos.data_ptr(),
         _lib.ptr(rot), _lib.ptr(starts), _lib.ptr(inv), num, requests, heads, hq, d, bs, shape[0],
         width, kst, vst, qst, ost, st, sst, dt, code)
+    if new and query.requires_grad:
+        return _recorded("append_kv_paged", query_out, query)
     return query_out
 
 
@@ -357,7 +384,8 @@ def paged_attention(
     q, qst = _rows(query)
     if scale is None:
         scale = 1.0 / math.sqrt(d)
-    if out is None:
+    new = out is None
+    if new:
         out, ost = _like(q, qst)
     else:
         ost = out.stride()
@@ -378,4 +406,6 @@ def paged_attention(
         out.data_ptr(), q.data_ptr(), base, sbase, bt.data_ptr(), bt.stride(0), pos.data_ptr(),
         _lib.ptr(starts), _lib.ptr(ws), ws_bytes, num, requests, most, hq, heads, d, bs, nb,
         width, win, sinks, float(scale), qst, ost, st, sst, dt, code)
+    if new and (query.requires_grad or sbase is None and kv_cache.requires_grad):
+        return _recorded("paged_attention", out, query, *(() if sbase else (kv_cache,)))
     return out

@@ -280,3 +280,34 @@ def test_workspace_of_many_requests():
                    int(2 ** rng.uniform(0, 14)), rng.choice((0, 1, 700, 40000)), rng.choice((0, 4)),
                    rng.choice((1, 2)), rng.choice((1, 2, 3)))
         assert got <= 4 * (d + 2) * 1024 * (256 + 16), (rows, requests, hkv, got)
+
+
+def test_gradients_are_refused_not_lost(on_cpu):
+    """A result whose gradient torch would ask for raises there; others carry no record."""
+    kv = torch.zeros((4, 2, 2, 16, 64))
+    q4 = pc.QuantizedKVCache.allocate(4, 2, 16, 64, "cpu")
+    bt = torch.zeros((3, 4), dtype=torch.int32)
+    pos = [0, 1, 2]
+    x = torch.zeros((3, 2, 64))
+    w = torch.ones(64, requires_grad=True)
+    calls = {
+        "paged_attention": lambda q, out=None, c=kv: pc.paged_attention(q, c, bt, pos, out=out),
+        "append_kv_paged": lambda q, out=None, c=kv: pc.append_kv_paged(
+            c, x, x, bt, pos, rope_base=1e4, query=q, query_out=out),
+    }
+    for name, call in calls.items():
+        for cache in (kv, q4):
+            for q in (torch.zeros((3, 6, 64), requires_grad=True), torch.ones((3, 6, 64)) * w,
+                      (torch.ones((3, 64, 6)) * w[None, :, None]).transpose(1, 2)):
+                got = call(q, c=cache)
+                assert got.requires_grad and got.shape == q.shape
+                with pytest.raises(RuntimeError, match=f"{name} has no backward"):
+                    (got * 2).sum().backward()
+                with torch.no_grad():
+                    assert not call(q, c=cache).requires_grad
+                assert not call(q.detach(), c=cache).requires_grad
+                out = torch.zeros(q.shape)
+                assert call(q, out, cache) is out and not out.requires_grad
+    got = pc.paged_attention(x, kv.clone().requires_grad_(), bt, pos)
+    with pytest.raises(RuntimeError, match="no backward"):
+        got.sum().backward()
