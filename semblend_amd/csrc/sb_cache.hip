@@ -22,7 +22,7 @@
 // What bounds it: bytes for prompts, the launch and one dependent chain (position, table entry,
 // row) for decode steps. One workgroup takes a few tokens with all their heads, so that each
 // (token, frequency) pair's sine and cosine (about 45 fp64 instructions) is evaluated once and
-// shared through LDS by the K and query heads. Measured: 4602 tokens of 32 / 8 heads x 128, 113 MB
+// shared through LDS by the K and query heads. Measured: 4587 tokens of 32 / 8 heads x 128, 113 MB
 // in 20.7 us (5.4 TB/s; a large copy reaches 6.6); 16 tokens 4 us; 4099 tokens of 4 heads into 4-bit
 // pages 8.4 us, 16000 of 8 heads 25.9 (instructions: a third sines and cosines, the rest rotation,
 // scales and codes); reading 16384 of 8 heads back 18.6 us (85 MB, 4.6 TB/s).
@@ -134,7 +134,7 @@ template <int DT, int VEC> struct RowVec {
   }
   __device__ __forceinline__ void store(char* p) const {
     if constexpr (kWide) {
-      // (nontemporal: append of 4602 tokens of 32 / 8 heads x 128 24.4 -> 21.1 us)
+      // (nontemporal: append of 4587 tokens of 32 / 8 heads x 128 24.4 -> 21.1 us)
       u32x4_t w;
       __builtin_memcpy(&w, e, 16);
       __builtin_nontemporal_store(w, (SB_GLOBAL u32x4_t*)p);
@@ -206,7 +206,7 @@ __device__ __forceinline__ Scale block_scale(const float (&f)[VEC]) {
 }
 
 // One thread per row works out where the row comes from and goes to, for all lanes of it: worked out
-// by every lane, that (selects, divisions, 64-bit products) was most of the kernel's instructions: 4602 tokens of 32 / 8
+// by every lane, that (selects, divisions, 64-bit products) was most of the kernel's instructions: 4587 tokens of 32 / 8
 // heads x 128 22.9 -> 20.9 us, 16000 of 8 heads into 4-bit pages 31.2 -> 27.0.
 struct RowRef {
   const char* src;  // nullptr: left out (padding, or no slot)
@@ -236,7 +236,9 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
   const int rsub = tid / vpr, vec = tid - rsub * vpr;
   const int hk = a.num_kv_heads;
   const int nrows = 2 * hk + a.num_q_heads;     // rows of a token
-  const int j0 = blockIdx.y * a.rows_per_y;     // (with several, a workgroup has one token)
+  // First of this workgroup's rows. (Several in y: of one token with many rows, or, where the rows of
+  // a step do not divide kRowsMax, of tokens whose last rows a second workgroup takes.)
+  const int j0 = blockIdx.y * a.rows_per_y;
   const int n = min(a.rows_per_y, ntok * nrows - j0);
 
   if (tid < n) {

@@ -1123,7 +1123,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64, 2) void paged_f32_kernel(const P
 // and O^T += V^T P^T with v_mfma_f32_32x32x16 (a lane owns one row), V through transposing reads.
 // Bound by instruction issue: 2.1 us a key tile at 28 / 4 heads x 128 (1.8 GHz under this load), of
 // which the products take 1.1, and by the three dependent loads in front of a workgroup's first
-// tile and its output, 10 us together (8192 rows under a window of 1024: 174-195 us by card, 18
+// tile and its output, 10 us together (8192 rows under a window of 1024: 170-195 us by card, 18
 // tiles a workgroup; 512 rows over 16384 keys of 4-bit pages: 144 us).
 template <int DT, int D, bool Q4>
 __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const PagedArgs a) {
@@ -1707,7 +1707,8 @@ __global__ __launch_bounds__(kRowsWaves * 64, 1) void paged_rows_kernel(const Pa
 // Joins the partials of row tiles whose keys were split: blockIdx.x = (tile, KV head), blockIdx.y
 // = which RPW rows of the tile. D / 4 lanes take a row, and the groups of them that RPW rows leave
 // share the row's splits: a decode row of 60 splits is then one batch of loads each for 8 groups
-// instead of eight batches in turn (28 / 4 heads x 128, one row of 16000: 8.5 -> 5.4 us).
+// instead of eight batches in turn (28 / 4 heads x 128, one row of 16000: 8.5 -> 5.4 us; 4.0 since the
+// places of balanced items are read instead of scanned for).
 // ---------------------------------------------------------------------------------------
 constexpr int kMergeThreads = 256;
 template <int DT, int D, int TR, int KT, int RPW>
@@ -1966,7 +1967,11 @@ struct PagedPlan {
 
 // Flattened rows up to which all requests take the decode kernel (16-bit arithmetic): three tiles, which
 // read a request's keys three times. (Requests of 4000 tokens, 32 / 8 heads x 128, decode and rows
-// kernel: 48 rows 4 requests 41 and 52 us, 32 requests 183 and 205; 64 rows 53 and 52, 234 and 192.)
+// kernel: 48 rows 4 requests 41 and 52 us, 32 requests 183 and 205; 64 rows 53 and 52, 234 and 192.
+// One request alone crosses later, by its rows and its keys: 448 rows over 1000 tokens, 28 / 4 heads,
+// 18.5 and 22.8 us; 1078 over 1024, 14 / 2 heads x 64, 11.2 and 16.8; 280 over 4096 29.3 and 32; 800
+// over 2000, 32 / 8 heads, 42.8 and 26.7. The rule stays at the batches' figure; a caller that knows
+// its rows to be few has max_rows.)
 constexpr int kFewRows = 48;
 // The same for a request of a call that launches the rows kernel anyway: one tile (40 requests of 700
 // rows and up to 6000 tokens, 28 / 4 heads x 128: 177 us, with 32 rows 189; nine requests of 1801 rows,
@@ -2008,7 +2013,9 @@ PagedPlan plan_paged(int64_t num_rows, int64_t num_requests, bool starts, int64_
   const bool f32 = dtype == SB_DTYPE_F32;
   const bool ragged = starts || num_requests == 1;  // else one row per request
   const bool one_each = !starts && (num_requests > 1 || num_rows == 1);  // row i is request i's
-  // keys that a row may see, tables taken as full
+  // Keys that a row may see, tables taken as full: the host does not know the contexts. Parts that a
+  // short key list has no tiles for end at once. (512 rows of 2000 tokens, 32 / 8 heads x 128: 35.5 us
+  // under a table of 2000 keys, 34.5 under one of 131072.)
   const int64_t keys = std::min(kv_len, std::min<int64_t>(window, kv_len) + sinks + 64);
   const int64_t per_few = (group + kDecodeRows - 1) / kDecodeRows;
   const int64_t flat = num_rows * group;

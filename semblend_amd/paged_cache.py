@@ -18,8 +18,10 @@ extensions with no reference counterpart, on the same caches, block tables and p
 Batches: ``row_starts`` [num_requests + 1] (int32, on the device) says where each request's rows
 begin; without it row i is request i's only one, as in a decode step, or, with one request, all
 rows are that one's. Rows of no request and rows with a negative position are padding and left as
-they are. All metadata is read on the device, so a step can be captured into a HIP graph once and
-replayed with new positions.
+they are. A decode step of one row per request is best given without ``row_starts``: attention
+then deals the keys of all requests out evenly (64 rows, one over 32768 keys and the others over
+300, 32 / 8 heads x 128: 48 us, with ``row_starts`` 453). All metadata is read on the device, so a
+step can be captured into a HIP graph once and replayed with new positions.
 
 These are a server's calls and have no backward pass: a result that torch would differentiate
 through (an input requires a gradient, in grad mode) raises when its gradient is asked for. Rows
@@ -358,14 +360,20 @@ def paged_attention(
     are not read, and their entries may hold anything. What lies in keys that a row does not see
     (NaN included) does not reach it. A row that sees no key gets zeros.
     ``max_rows``: no request has more rows than this; it only helps to choose kernels (a decode
-    step of several rows a request runs as one launch fewer). Scores, sums and outputs are fp32,
-    rounded once; 16-bit calls round the weights to their dtype for the product with V (fp16: a
-    weight below 2^-25 of the row's largest may be zero there). fp16 queries take 4-bit values
-    below 2^18, as pages of fp16 tokens hold them: a page written from wider tokens may hold larger
-    ones, which are infinite to such a query.
+    step of several rows a request runs as one launch fewer, and a few dozen rows over at most a
+    thousand keys are faster on the single-token kernel, which 1 asks for). Scores, sums and
+    outputs are fp32, rounded once; 16-bit calls round the weights to their dtype for the product
+    with V (fp16: a weight below 2^-25 of the row's largest may be zero there). fp16 queries take
+    4-bit values below 2^18, as pages of fp16 tokens hold them: a page written from wider tokens may
+    hold larger ones, which are infinite to such a query.
     Returns [R, num_q_heads, head_dim] (``out`` if given; padding rows of it are left as they
-    are). Extension with no reference counterpart: the reference's attention is MHA over
-    contiguous K/V (semblend_core/triton_kernels.py:655-734), without window.
+    are). Over one request's 16-bit or fp32 pages without a window
+    ``triton_kernels.partial_prefill_attention_paged`` computes the same; this call takes ragged
+    batches described on the device, that one splits a chunk over a few thousand keys better (28 / 4
+    heads x 128, this call against that one: 1 row of 4096 keys 14 and 18 us, 40 of 4096 32 and 27,
+    614 of 4096 52 and 41, 2458 of 16384 317 and 312; fp32, 32 / 8 heads, 500 of 4096 187 and 245).
+    Extension with no reference counterpart: the reference's attention is MHA over contiguous K/V
+    (semblend_core/triton_kernels.py:655-734), without window.
     """
     qshape, dtype = query.shape, query.dtype
     if len(qshape) != 3:
