@@ -330,14 +330,19 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
             const double* t64;
             if constexpr (kBoth) t64 = cs64 + (ref.info >> 2) + vec * VEC;
             else t64 = reinterpret_cast<const double*>(trig);
+            // (a sum of two values of the largest fp32 exponent may pass fp32, but not 7 * 2^126: such a
+            // block, not finite above, is taken times 2^-2)
+            const double down = b.bad ? 0.25 : 1.0;
+            const int up = b.bad ? 2 : 0;
 #pragma unroll
             for (int i = 0; i < VEC; i += 2) {
-              const double e = Elem<DT>::get(x[u].e[i]), o = Elem<DT>::get(x[u].e[i + 1]);
+              const double e = Elem<DT>::get(x[u].e[i]) * down, o = Elem<DT>::get(x[u].e[i + 1]) * down;
               f[i] = round_to_odd(e * t64[i] - o * t64[i + 1]);
               f[i + 1] = round_to_odd(e * t64[i + 1] + o * t64[i]);
             }
             b = block_scale(f);
             w = b.bad ? 0u : pack_codes(f, b.value);
+            if (!b.bad) b.byte += up;
           }
         } else {
           w = b.bad ? 0u : pack_codes(f, b.value);

@@ -1081,3 +1081,27 @@ def test_row_tiles_share_the_partials(dev, dtype, quant, chunks):
     lens = [1500 + 31 * i for i in range(2 * chunks)]
     for window, sinks in ((None, 0), (700, 70)):
         _attend_case(dtype, d, hq, hkv, bs, lens, rows, window, sinks, quant, width=400)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_append_4bit_largest_rotated_keys(dev, dtype):
+    """Rotated keys of the dtype's largest values, whose pairs' sums may pass fp32: codes and scale
+    bytes are the 64-bit quantiser's; blocks with an infinity or a NaN beside them are NaN."""
+    bs, heads, d, num, base = 16, 2, 64, 70, 1e4
+    tables, nb = _tables([num], bs, 1)
+    codes, scales, cache = _quant_cache(nb, heads, bs, d, 2)
+    top = torch.finfo(dtype).max
+    k = (torch.rand((num, heads, d), generator=gen(3)) * 2 - 1).double()
+    k[:, :, ::5] = k[:, :, ::5].sign()                  # +-max, in some blocks beside small values
+    k[40:, 0, 1::2] *= 1e-3
+    k = (k * top).to(dtype)
+    k[50, 0, 3], k[51, 1, 40], k[52, 0, 63] = math.inf, math.nan, -math.inf
+    v = randn((num, heads, d), dtype, 4)
+    at = torch.arange(num, dtype=torch.int32)
+    pc.append_kv_paged(cache, k.cuda(), v.cuda(), tables[0].cuda(), at.cuda(), rope_base=base)
+    page, slot = tables[0].long()[at.long() // bs], at.long() % bs
+    c, s = ref.quantize(ref.rotate(k, at, base))
+    assert (s == 255).any(-1).sum() == 3 and (dtype == FP16 or (s == 253).sum() > 100)
+    assert torch.equal(cache.scales.cpu()[page, 0, :, slot].long(), s)
+    assert torch.equal(cache.codes.cpu()[page, 0, :, slot],
+                       (c[..., 0::2] | c[..., 1::2] << 4).to(torch.uint8))
