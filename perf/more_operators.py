@@ -219,14 +219,16 @@ def _inputs(case, seed: int) -> dict:
 def prepare(case, seed: int) -> dict:
     s = _inputs(case, seed)
     if own and case["kind"] == "w4":
-        from semblend_amd.quantized import QuantizedLinear
+        from semblend_amd import quantized
 
-        s["handle"] = QuantizedLinear(s["codes"], s["scales"], s["zeros"])
+        s["api"] = quantized
+        s["handle"] = quantized.QuantizedLinear(s["codes"], s["scales"], s["zeros"])
     elif own:
-        from semblend_amd.rotary import RotaryEmbedding
+        from semblend_amd import paged_cache, rope_correction, rotary
 
-        s["rotary"] = RotaryEmbedding(s["freq"], case["d"], layout=case["pairs"],
-                                      factor=case["factor"])
+        s["api"] = {"rotate": rotary, "append": paged_cache}.get(case["kind"], rope_correction)
+        s["rotary"] = rotary.RotaryEmbedding(s["freq"], case["d"], layout=case["pairs"],
+                                             factor=case["factor"])
         if "caches" in s:
             s["layers"] = [x.permute(1, 0, 3, 2, 4) for x in s["caches"].unbind(0)]
         if "donors" in s:
@@ -237,27 +239,22 @@ def prepare(case, seed: int) -> dict:
 # ---- one pass ------------------------------------------------------------------------------
 
 def _run_own(s):
-    from semblend_amd import paged_cache as pc
-    from semblend_amd import rope_correction as rc
-    from semblend_amd.quantized import quantized_linear
-    from semblend_amd.rotary import apply_rotary
-
-    kind = s["case"]["kind"]
+    api, kind = s["api"], s["case"]["kind"]
     if kind == "w4":
-        return quantized_linear(s["x"], s["handle"], bias=s["bias"])
+        return api.quantized_linear(s["x"], s["handle"], bias=s["bias"])
     if kind == "rotate":
-        return apply_rotary(s["q"], s["pos"], s["rotary"], key=s["k"])
+        return api.apply_rotary(s["q"], s["pos"], s["rotary"], key=s["k"])
     if kind == "append":
-        q = pc.append_kv_paged(s["cache"], s["k"], s["v"], s["tables"], s["pos"],
-                               row_starts=None if s["single"] else s["starts"],
-                               rotary=s["rotary"], query=s["q"])
+        q = api.append_kv_paged(s["cache"], s["k"], s["v"], s["tables"], s["pos"],
+                                row_starts=None if s["single"] else s["starts"],
+                                rotary=s["rotary"], query=s["q"])
         return q, s["cache"]
     if kind == "scatter":
-        rc.rope_correct_scatter_paged_layers(s["layers"], s["donor_layers"], s["tables"][0],
-                                             s["from"], s["to"], rotary=s["rotary"])
+        api.rope_correct_scatter_paged_layers(s["layers"], s["donor_layers"], s["tables"][0],
+                                              s["from"], s["to"], rotary=s["rotary"])
     else:
-        rc.apply_rope_deltas_inplace_layers(s["layers"], s["tables"][0], s["pos"], s["delta"],
-                                            layout="standard", rotary=s["rotary"])
+        api.apply_rope_deltas_inplace_layers(s["layers"], s["tables"][0], s["pos"], s["delta"],
+                                             layout="standard", rotary=s["rotary"])
     return s["caches"]
 
 
