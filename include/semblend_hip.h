@@ -37,6 +37,10 @@ extern "C" {
 #define SB_DTYPE_BF16 2
 #define SB_DTYPE_MXFP4 3 /* caches of sb_append_kv_paged, sb_gather_kv_paged, sb_paged_attention */
 
+/* Pairs of a rotary embedding: interleaved (2i, 2i + 1), or half (i, i + pairs). */
+#define SB_ROTARY_INTERLEAVED 0
+#define SB_ROTARY_HALF 1
+
 /* Flags of the multi-layer scatters (sb_*_paged_layers, sb_composite_scatter_paged_layers).
  * SB_SCATTER_REPEATED_DONOR_ROWS: a donor row may be the source of several pairs (one
  * donor position mapped to several targets). The launch then reads the donor through the
@@ -619,6 +623,24 @@ int sb_append_kv_paged(void* kv_cache, void* kv_scales, const void* key, const v
                        const int64_t* scale_strides, int32_t dtype, int32_t cache_dtype,
                        void* stream);
 
+/* sb_append_kv_paged with a model's own rotary embedding (required here): the first 2 * pairs
+ * elements of K and query rows are rotated, in interleaved pairs (2i, 2i + 1) or half pairs (i, i +
+ * pairs; an even number of them), by rotations[t] (or positions[t]) * inv_freq[i], inv_freq [pairs]
+ * of at most 1; cosine and sine are multiplied by factor. 4-bit pages: whole blocks of 32 values in
+ * what is rotated and in what is not (half pairs: in either half of both). */
+int sb_append_kv_rotary_paged(void* kv_cache, void* kv_scales, const void* key, const void* value,
+                              const void* query, void* query_out, const int32_t* block_tables,
+                              int64_t table_stride, const int32_t* positions,
+                              const int32_t* rotations, const int32_t* row_starts,
+                              const float* inv_freq, int64_t num_tokens, int64_t num_requests,
+                              int64_t num_kv_heads, int64_t num_q_heads, int64_t head_dim,
+                              int64_t block_size, int64_t num_blocks_total,
+                              int64_t num_blocks_per_seq, const int64_t* k_strides,
+                              const int64_t* v_strides, const int64_t* q_strides,
+                              const int64_t* qo_strides, const int64_t* kv_strides,
+                              const int64_t* scale_strides, int64_t pairs, int32_t layout,
+                              double factor, int32_t dtype, int32_t cache_dtype, void* stream);
+
 /* out[kv, h, i, :] = the cache's row of position positions[i] (NULL: i) of one request, in dtype
  * (a 4-bit value is exact in bf16 and fp32, rounded once to fp16); zeros where the position has
  * no page. out [2, num_kv_heads, num_rows, head_dim] by o_strides[4] in elements: the donor
@@ -663,6 +685,59 @@ int sb_paged_attention(void* out, const void* q, const void* kv_cache, const voi
                        int32_t cache_dtype, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * A model's own rotary embedding (no reference counterparts: the reference rotates interleaved
+ * pairs of whole heads by plain frequencies)
+ *
+ * Shared by the entries, and by sb_append_kv_rotary_paged: the first 2 * pairs elements of a row
+ * are turned and the others kept; layout SB_ROTARY_INTERLEAVED, or SB_ROTARY_HALF with an even number of pairs;
+ * inv_freq: device fp32 [pairs], at most 1. Angles, sines and cosines in 64 bits, one rounding to
+ * dtype. head_dim even, at most 512.
+ * ---------------------------------------------------------------------------------------- */
+
+/* query_out[t, h] = query[t, h] turned by positions[t] (any int32), and key likewise (NULL: none):
+ * [num_tokens, heads, head_dim] by strides (token, head, dim) in elements. cosine and sine are
+ * multiplied by factor. An output may be its input; it must not overlap it otherwise. */
+int sb_apply_rotary(void* query_out, const void* query, void* key_out, const void* key,
+                    const int32_t* positions, const float* inv_freq, int64_t num_tokens,
+                    int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                    const int64_t* q_strides, const int64_t* qo_strides, const int64_t* k_strides,
+                    const int64_t* ko_strides, int64_t pairs, int32_t layout, double factor,
+                    int32_t dtype, void* stream);
+
+/* sb_rope_correct_scatter_paged_layers with K turned by (t - d) as the embedding has it (a cached
+ * K holds the factor already). Pairs out of range are skipped; targets are distinct. */
+int sb_rotary_scatter_paged_layers(const uint64_t* kv_layer_ptrs,
+                                   const uint64_t* donor_layer_ptrs, int64_t num_layers,
+                                   const int32_t* block_table, const int32_t* donor_pos,
+                                   const int32_t* target_pos, const float* inv_freq,
+                                   int64_t num_pairs, int64_t num_heads, int64_t block_size,
+                                   int64_t head_dim, int64_t donor_seq_len,
+                                   int64_t num_blocks_total, int64_t num_blocks_per_seq,
+                                   const int64_t* kv_strides, const int64_t* d_strides,
+                                   int64_t pairs, int32_t layout, int32_t dtype, int32_t flags,
+                                   void* stream);
+
+/* K at positions[i] of every layer turned in place by deltas[i]; V untouched. Positions are
+ * distinct; those outside the table, and deltas of 0, are skipped. kv_strides[4] = (block, head,
+ * pos, dim) in elements. _host: positions and deltas in HOST memory, at most
+ * SB_INLINE_POSITIONS_MAX, carried in the launch. */
+int sb_rotary_shift_paged_layers(const uint64_t* kv_layer_ptrs, int64_t num_layers,
+                                 const int32_t* block_table, const int32_t* positions,
+                                 const int32_t* deltas, int64_t num_positions,
+                                 const float* inv_freq, int64_t num_heads, int64_t block_size,
+                                 int64_t head_dim, int64_t num_blocks_total,
+                                 int64_t num_blocks_per_seq, const int64_t* kv_strides,
+                                 int64_t pairs, int32_t layout, int32_t dtype, void* stream);
+int sb_rotary_shift_paged_layers_host(const uint64_t* kv_layer_ptrs, int64_t num_layers,
+                                      const int32_t* block_table, const int32_t* positions,
+                                      const int32_t* deltas, int64_t num_positions,
+                                      const float* inv_freq, int64_t num_heads,
+                                      int64_t block_size, int64_t head_dim,
+                                      int64_t num_blocks_total, int64_t num_blocks_per_seq,
+                                      const int64_t* kv_strides, int64_t pairs, int32_t layout,
+                                      int32_t dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Flat device copy (measurement reference; no reference counterpart)
  * ---------------------------------------------------------------------------------------- */
 
@@ -682,7 +757,7 @@ int sb_device_copy(void* dst, const void* src, int64_t num_bytes, void* stream);
  * (the log stays readable). At most 65536 launches are logged. Kernel names:
  * "move_rows", "rope_rows", "rope_index", "fill_i32", "attn_mfma", "attn_valu", "attn_merge",
  * "mask_compact", "zero_rows", "copy", "append_kv", "gather_kv", "paged_decode", "paged_f32",
- * "paged_rows", "paged_valu", "paged_merge". */
+ * "paged_rows", "paged_valu", "paged_merge", "rotary_rows". */
 int sb_kernel_timing_enable(int32_t enable);
 
 /* Sum of the logged durations (ms) and number of logged launches of one kernel. Waits for the

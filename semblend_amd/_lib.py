@@ -33,12 +33,15 @@ SB_GROUPED_PAIR_ALIGN = 256
 MAX_ROPE_DELTA = 1 << 31
 # Cache type of 4-bit pages (append, gather and attention of semblend_amd.paged_cache).
 SB_DTYPE_MXFP4 = 3
+# Pairs of a rotary embedding (semblend_amd.rotary).
+SB_ROTARY = {"interleaved": 0, "half": 1}
 SB_DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _i64p = ctypes.POINTER(ctypes.c_int64)
 _i32p = ctypes.POINTER(ctypes.c_int32)
 I32P = _i32p  # host int32 arrays passed by address (numpy: arr.ctypes.data_as(I32P))
@@ -115,6 +118,18 @@ SIGNATURES: dict[str, list] = {
     "sb_append_kv_paged": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64,
                            _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p, _i64p,
                            _i64p, _i64p, _i32, _i32, _vp],
+    "sb_append_kv_rotary_paged": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp,
+                                  _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64p, _i64p,
+                                  _i64p, _i64p, _i64p, _i64p, _i64, _i32, _f64, _i32, _i32, _vp],
+    "sb_apply_rotary": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p,
+                        _i64p, _i64, _i32, _f64, _i32, _vp],
+    "sb_rotary_scatter_paged_layers": [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                                       _i64, _i64, _i64, _i64p, _i64p, _i64, _i32, _i32, _i32,
+                                       _vp],
+    "sb_rotary_shift_paged_layers": [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64,
+                                     _i64, _i64p, _i64, _i32, _i32, _vp],
+    "sb_rotary_shift_paged_layers_host": [_vp, _i64, _vp, _i32p, _i32p, _i64, _vp, _i64, _i64,
+                                          _i64, _i64, _i64, _i64p, _i64, _i32, _i32, _vp],
     "sb_gather_kv_paged": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64p,
                            _i64p, _i64p, _i32, _i32, _vp],
     "sb_paged_attention": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64,

@@ -26,33 +26,10 @@
 // in 20.7 us (5.4 TB/s; a large copy reaches 6.6); 16 tokens 4 us; 4099 tokens of 4 heads into 4-bit
 // pages 8.4 us, 16000 of 8 heads 25.9 (instructions: a third sines and cosines, the rest rotation,
 // scales and codes); reading 16384 of 8 heads back 18.6 us (85 MB, 4.6 TB/s).
-#include "sb_common.h"
-
-#include <algorithm>
+#include "sb_rows.h"
 
 namespace sb {
 namespace {
-
-constexpr int kAppendThreads = 256;
-constexpr int kTableEntries = 512;   // (token, frequency) pairs of one workgroup
-constexpr int kTokensMax = 8;
-constexpr int kRowsMax = 256;        // rows (K, V and query heads of its tokens) of one workgroup
-
-// x / d for 0 <= x < 2^31: with l = ceil(log2 d) and m = ceil(2^(31+l) / d), m d - 2^(31+l) < d <=
-// 2^l, so x * m >> (31 + l) is exact (T. Granlund and P. Montgomery, "Division by invariant integers
-// using multiplication", 1994).
-struct Divisor {
-  uint32_t magic;
-  int shift;
-  static Divisor by(int d) {
-    int shift = 31;
-    while ((1ll << (shift - 31)) < d) ++shift;
-    return {static_cast<uint32_t>(((1ull << shift) + d - 1) / d), shift};
-  }
-  __device__ __forceinline__ int of(int x) const {
-    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(x)) * magic) >> shift);
-  }
-};
 
 struct AppendArgs {
   const char* k;
@@ -74,166 +51,27 @@ struct AppendArgs {
   int64_t num_blocks_total, num_blocks_per_seq;
   int num_requests, num_kv_heads, num_q_heads, head_dim, block_size;
   int tokens_per_wg, rows_per_y;
-  Divisor row_div, half_div;              // by the rows of a token, by head_dim / 2
+  int pairs;                              // pairs of a row that are turned
+  double factor;                          // of the cosines and sines
+  RowSplit split;
+  Divisor row_div, half_div;              // by the rows of a token, by pairs
 };
 
-// Request of row t, or -1 before the first and behind the last one: the last r with
-// row_starts[r] <= t.
-__device__ __forceinline__ int request_of(const int32_t* row_starts, int num_requests, int t) {
-  if (t < row_starts[0] || t >= row_starts[num_requests]) return -1;
-  int lo = 0, hi = num_requests;  // row_starts[lo] <= t < row_starts[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (row_starts[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
-// An element's value, and two values rounded to elements.
-template <int DT> struct Elem;
-template <> struct Elem<SB_DTYPE_F32> {
-  using T = float;
-  __device__ static float get(float x) { return x; }
-  __device__ static void put2(float a, float b, float* e) { e[0] = a, e[1] = b; }
-};
-template <> struct Elem<SB_DTYPE_F16> {
-  using T = uint16_t;
-  __device__ static float get(uint16_t x) { return f16_to_f32(x); }
-  __device__ static void put2(float a, float b, uint16_t* e) {
-    e[0] = f32_to_f16(a), e[1] = f32_to_f16(b);
-  }
-};
-template <> struct Elem<SB_DTYPE_BF16> {
-  using T = uint16_t;
-  __device__ static float get(uint16_t x) { return bf16_to_f32(x); }
-  __device__ static void put2(float a, float b, uint16_t* e) {
-    const uint32_t w = pack2_bf16(a, b);
-    e[0] = static_cast<uint16_t>(w), e[1] = static_cast<uint16_t>(w >> 16);
-  }
-};
-
-// Device memory (a pointer that went through LDS would be taken for any kind, and its loads wait
-// with LDS's).
-#define SB_GLOBAL __attribute__((address_space(1)))
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-
-// VEC elements of a row: 16 bytes, or (VEC 2) a pair, element by element at any alignment.
-template <int DT, int VEC> struct RowVec {
-  using T = typename Elem<DT>::T;
-  static constexpr bool kWide = VEC * sizeof(T) == 16;
-  T e[VEC];
-  __device__ __forceinline__ void load(const char* p) {
-    if constexpr (kWide) {
-      const u32x4_t w = *(const SB_GLOBAL u32x4_t*)p;
-      __builtin_memcpy(e, &w, 16);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) e[i] = ((const SB_GLOBAL T*)p)[i];
-    }
-  }
-  __device__ __forceinline__ void store(char* p) const {
-    if constexpr (kWide) {
-      // (nontemporal: append of 4587 tokens of 32 / 8 heads x 128 24.4 -> 21.1 us)
-      u32x4_t w;
-      __builtin_memcpy(&w, e, 16);
-      __builtin_nontemporal_store(w, (SB_GLOBAL u32x4_t*)p);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) ((SB_GLOBAL T*)p)[i] = e[i];
-    }
-  }
-};
-
-// x rounded to fp32 to odd: the result's comparisons with fp32 values of an even last bit are x's.
-__device__ __forceinline__ float round_to_odd(double x) {
-  const float f = static_cast<float>(x);
-  uint32_t u = __float_as_uint(f);
-  const double back = static_cast<double>(f);
-  if (back != x && (u & 1u) == 0 && (u & 0x7fffffffu) < 0x7f800000u)
-    u += (fabs(x) > fabs(back)) ? 1u : 0xffffffffu;  // (toward x; f = 0 only moves outwards)
-  return __uint_as_float(u);
-}
-
-// The scale byte of a block whose largest magnitude is `top`, a number: top in
-// [4, 8) * 2^(E - 2 - 127), and one power more above 7 (mantissa above 1.75).
-__device__ __forceinline__ int scale_byte(float top) {
-  const uint32_t u = __float_as_uint(top);
-  return max(static_cast<int>(u >> 23) - 2 + ((u & 0x7fffffu) > 0x600000u), 0);
-}
-template <int VEC>
-__device__ __forceinline__ uint32_t pack_codes(const float (&f)[VEC], float scale) {
-  uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0], f[1], scale, 0);
-  if constexpr (VEC >= 4) w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[2], f[3], scale, 1);
-  if constexpr (VEC >= 8) {
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[4], f[5], scale, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[6], f[7], scale, 3);
-  }
-  return w;
-}
-// Largest of the 32 / VEC lanes that share a block of 32 values, in all of them: neighbours inside
-// four lanes, then the mirror image inside eight and sixteen (DPP moves, no trip through LDS; with the
-// two packings below instead of three, 16000 tokens of 8 heads 27.3 -> 25.9 us).
-template <int VEC>
-__device__ __forceinline__ uint32_t block_max(uint32_t v) {
-  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xb1, 15, 15, true)));
-  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4e, 15, 15, true)));
-  if constexpr (VEC <= 4)
-    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x141, 15, 15, true)));
-  if constexpr (VEC <= 2)
-    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x140, 15, 15, true)));
-  return v;
-}
-// The scale of a block; one that holds an infinity or a NaN is marked as one by scale byte 255.
-struct Scale {
-  int byte;
-  bool bad;
-  float top, value;
-};
-template <int VEC>
-__device__ __forceinline__ Scale block_scale(const float (&f)[VEC]) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-  top = block_max<VEC>(top);
-  Scale b;
-  b.top = __uint_as_float(top);
-  b.bad = top >= 0x7f800000u;
-  b.byte = b.bad ? 255 : scale_byte(b.top);
-  // (byte 0 is 2^-127, below fp32's normal numbers)
-  b.value = __uint_as_float(b.byte > 0 && !b.bad ? static_cast<uint32_t>(b.byte) << 23 : 0x00400000u);
-  return b;
-}
-
-// One thread per row works out where the row comes from and goes to, for all lanes of it: worked out
-// by every lane, that (selects, divisions, 64-bit products) was most of the kernel's instructions: 4587 tokens of 32 / 8
-// heads x 128 22.9 -> 20.9 us, 16000 of 8 heads into 4-bit pages 31.2 -> 27.0.
-struct RowRef {
-  const char* src;  // nullptr: left out (padding, or no slot)
-  char* dst;
-  char* sdst;       // scale bytes of a 4-bit row
-  uint32_t info;    // index of the token's sines and cosines << 2 | a 4-bit row << 1 | rotated
-  uint32_t pad;
-};
-// A thread takes vector tid % vpr of rows tid / vpr + k rpi (K, V, then query heads, token after
-// token), kRowsInFlight of them at a time.
-constexpr int kRowsInFlight = 4;
-template <int DT, int VEC, bool Q4>
-__global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendArgs a) {
+template <int DT, int VEC, bool Q4, bool HALF>
+__global__ __launch_bounds__(kRowThreads) void append_kv_kernel(const AppendArgs a) {
   using CS = std::conditional_t<DT == SB_DTYPE_F32, double, float>;
   constexpr bool kBoth = Q4 && DT != SB_DTYPE_F32;         // 64-bit sines and cosines besides
-  constexpr int ES = sizeof(typename Elem<DT>::T);
   __shared__ CS cs[2 * kTableEntries];                    // cosine, sine of each (token, pair)
   __shared__ double cs64[kBoth ? 2 * kTableEntries : 1];
   __shared__ __align__(16) RowRef rows[kRowsMax];
   const int tid = threadIdx.x;
-  const int half = a.head_dim >> 1;
+  const int half = a.pairs;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens_per_wg;
   const int ntok = static_cast<int>(min(static_cast<int64_t>(a.tokens_per_wg), a.num_tokens - t0));
 
-  const int vpr = a.head_dim / VEC;             // vectors per row (at most kAppendThreads)
-  const int rpi = kAppendThreads / vpr;         // rows per step of the workgroup
-  const int rsub = tid / vpr, vec = tid - rsub * vpr;
+  const int upr = a.split.units;                // threads per row (at most kRowThreads)
+  const int rpi = kRowThreads / upr;            // rows per step of the workgroup
+  const int rsub = tid / upr, unit = tid - rsub * upr;
   const int hk = a.num_kv_heads;
   const int nrows = 2 * hk + a.num_q_heads;     // rows of a token
   // First of this workgroup's rows. (Several in y: of one token with many rows, or, where the rows of
@@ -271,11 +109,12 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
   }
   if (a.inv_freq) {
     // (from the last wave down: the first ones look the pages up)
-    for (int i = kAppendThreads - 1 - tid; i < ntok * half; i += kAppendThreads) {
+    for (int i = kRowThreads - 1 - tid; i < ntok * half; i += kRowThreads) {
       const int tok = a.half_div.of(i), f = i - tok * half;
       const int p = (a.rotations ? a.rotations : a.positions)[t0 + tok];
       double s, c;
       sincos_cw(static_cast<double>(p) * static_cast<double>(a.inv_freq[f]), &s, &c);
+      c *= a.factor, s *= a.factor;
       cs[2 * i] = static_cast<CS>(c);
       cs[2 * i + 1] = static_cast<CS>(s);
       if constexpr (kBoth) cs64[2 * i] = c, cs64[2 * i + 1] = s;
@@ -284,84 +123,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(const AppendA
   __syncthreads();
   if (rsub >= rpi) return;
 
-  for (int ib = rsub; ib < n; ib += kRowsInFlight * rpi) {
-    RowVec<DT, VEC> x[kRowsInFlight];
-#pragma unroll
-    for (int u = 0; u < kRowsInFlight; ++u) {
-      const char* src = rows[min(ib + u * rpi, n - 1)].src;
-      if (src) x[u].load(src + vec * (VEC * ES));
-    }
-#pragma unroll
-    for (int u = 0; u < kRowsInFlight; ++u) {
-      if (ib + u * rpi >= n) break;
-      const RowRef ref = rows[ib + u * rpi];
-      if (!ref.src) continue;
-      const CS* trig = cs + (ref.info >> 2) + vec * VEC;
-      const bool turn = ref.info & 1u;
-      float f[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; i += 2) {
-        const CS e = Elem<DT>::get(x[u].e[i]), o = Elem<DT>::get(x[u].e[i + 1]);
-        if (turn) {
-          const CS c = trig[i], s = trig[i + 1];
-          f[i] = static_cast<float>(e * c - o * s);
-          f[i + 1] = static_cast<float>(e * s + o * c);
-        } else {
-          f[i] = static_cast<float>(e);
-          f[i + 1] = static_cast<float>(o);
-        }
-      }
-      if (Q4 && (ref.info & 2u)) {
-        Scale b = block_scale(f);
-        uint32_t w;
-        if (turn) {
-          // A rotated fp32 value is off by at most 2^-22 of its pair's norm (products and sum
-          // 2^-24 each, sine and cosine 2^-24): 2^-21 of the block's largest magnitude, which is
-          // below 2^-18 of the scale. Codes that agree at both ends agree between.
-          uint32_t unsure = b.bad || scale_byte(b.top * (1.f - 0x1p-20f)) !=
-                                         scale_byte(b.top * (1.f + 0x1p-20f));
-          const float off = b.value * 0x1p-18f;
-          float lo[VEC], hi[VEC];
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) lo[i] = f[i] - off, hi[i] = f[i] + off;
-          w = pack_codes(lo, b.value);
-          unsure |= w ^ pack_codes(hi, b.value);
-          if (block_max<VEC>(unsure)) {
-            const double* t64;
-            if constexpr (kBoth) t64 = cs64 + (ref.info >> 2) + vec * VEC;
-            else t64 = reinterpret_cast<const double*>(trig);
-            // (a sum of two values of the largest fp32 exponent may pass fp32, but not 7 * 2^126: such a
-            // block, not finite above, is taken times 2^-2)
-            const double down = b.bad ? 0.25 : 1.0;
-            const int up = b.bad ? 2 : 0;
-#pragma unroll
-            for (int i = 0; i < VEC; i += 2) {
-              const double e = Elem<DT>::get(x[u].e[i]) * down, o = Elem<DT>::get(x[u].e[i + 1]) * down;
-              f[i] = round_to_odd(e * t64[i] - o * t64[i + 1]);
-              f[i + 1] = round_to_odd(e * t64[i + 1] + o * t64[i]);
-            }
-            b = block_scale(f);
-            w = b.bad ? 0u : pack_codes(f, b.value);
-            if (!b.bad) b.byte += up;
-          }
-        } else {
-          w = b.bad ? 0u : pack_codes(f, b.value);
-        }
-        char* dst = ref.dst + vec * (VEC / 2);
-        if constexpr (VEC == 8) *(SB_GLOBAL uint32_t*)dst = w;
-        else if constexpr (VEC == 4) *(SB_GLOBAL uint16_t*)dst = static_cast<uint16_t>(w);
-        else *(SB_GLOBAL uint8_t*)dst = static_cast<uint8_t>(w);
-        if ((vec & (32 / VEC - 1)) == 0)
-          ((SB_GLOBAL char*)ref.sdst)[vec / (32 / VEC)] = static_cast<char>(b.byte);
-      } else {
-        if (turn) {
-#pragma unroll
-          for (int i = 0; i < VEC; i += 2) Elem<DT>::put2(f[i], f[i + 1], x[u].e + i);
-        }
-        x[u].store(ref.dst + vec * (VEC * ES));
-      }
-    }
-  }
+  turn_rows<DT, VEC, Q4, HALF, false>(rows, n, cs, cs64, a.split, a.head_dim, a.pairs, rsub, rpi, unit);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -470,10 +232,6 @@ __global__ __launch_bounds__(kGatherThreads) void gather_kv_kernel(const GatherA
   }
 }
 
-bool valid_dtype(int32_t dt) {
-  return dt == SB_DTYPE_F32 || dt == SB_DTYPE_F16 || dt == SB_DTYPE_BF16;
-}
-
 // Byte strides of a cache given in elements (4 bit: codes in bytes, scales in bytes).
 struct CacheStrides {
   int64_t block, kv, head, pos;
@@ -485,17 +243,19 @@ CacheStrides cache_strides(const int64_t* s, int64_t es) {
 }  // namespace
 }  // namespace sb
 
-extern "C" int sb_append_kv_paged(
-    void* kv_cache, void* kv_scales, const void* key, const void* value, const void* query,
+namespace sb {
+namespace {
+
+// Both append entries; `pairs` pairs of a row are turned (0: all of it).
+int append_kv(
+    const char* fn, void* kv_cache, void* kv_scales, const void* key, const void* value, const void* query,
     void* query_out, const int32_t* block_tables, int64_t table_stride, const int32_t* positions,
     const int32_t* rotations, const int32_t* row_starts, const float* inv_freq,
     int64_t num_tokens, int64_t num_requests, int64_t num_kv_heads, int64_t num_q_heads,
     int64_t head_dim, int64_t block_size, int64_t num_blocks_total, int64_t num_blocks_per_seq,
     const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides,
     const int64_t* qo_strides, const int64_t* kv_strides, const int64_t* scale_strides,
-    int32_t dtype, int32_t cache_dtype, void* stream) {
-  using namespace sb;
-  const char* fn = "sb_append_kv_paged";
+    int64_t pairs, int32_t layout, double factor, int32_t dtype, int32_t cache_dtype, void* stream) {
   clear_error();
   if (num_tokens == 0) return SB_OK;
   if (!valid_dtype(dtype)) return fail(fn, "invalid dtype");
@@ -515,6 +275,15 @@ extern "C" int sb_append_kv_paged(
   if (head_dim <= 0 || head_dim % 2 || head_dim > 512)
     return fail(fn, "head_dim must be even and at most 512");
   if (q4 && head_dim % 32) return fail(fn, "4-bit pages need a head_dim that is a multiple of 32");
+  const bool half = inv_freq && layout == SB_ROTARY_HALF;
+  if (inv_freq) {
+    if (const char* why = rotary_fault(head_dim, pairs, layout, factor)) return fail(fn, why);
+    if (q4 && (half ? pairs % 32 || (head_dim - 2 * pairs) % 64 : pairs % 16))
+      return fail(fn, "4-bit pages need whole blocks of 32 values in each half of what is rotated and of "
+                      "what is not");
+  } else {
+    pairs = head_dim / 2;
+  }
   if (!row_starts && num_requests > 1 && num_tokens > num_requests)
     return fail(fn, "without row_starts there is one token per request");
   if (k_strides[2] != 1 || v_strides[2] != 1 || kv_strides[4] != 1 ||
@@ -546,6 +315,8 @@ extern "C" int sb_append_kv_paged(
   a.rotations = rotations;
   a.row_starts = row_starts;
   a.inv_freq = inv_freq;
+  a.pairs = static_cast<int>(pairs);
+  a.factor = factor;
   a.num_tokens = num_tokens;
   a.num_requests = static_cast<int>(num_requests);
   a.num_kv_heads = static_cast<int>(num_kv_heads);
@@ -557,7 +328,8 @@ extern "C" int sb_append_kv_paged(
 
   const auto addr = [](const void* p) { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)); };
   int vb = vec_bytes({addr(key), addr(value), addr(query), addr(query_out), a.k_tok, a.k_head,
-                      a.v_tok, a.v_head, a.q_tok, a.q_head, a.qo_tok, a.qo_head, head_dim * es});
+                      a.v_tok, a.v_head, a.q_tok, a.q_head, a.qo_tok, a.qo_head, head_dim * es,
+                      (half ? pairs : 2 * pairs) * es});
   const int64_t cells[] = {addr(kv_cache), c.block, c.kv, c.head, c.pos};
   const int64_t cell = q4 ? 16 / es / 2 : 16;  // bytes of the cache that 16 bytes of a row become
   for (int64_t x : cells)
@@ -568,8 +340,9 @@ extern "C" int sb_append_kv_paged(
   // and cosines takes). Few tokens: one, and its rows spread over workgroups until there are 512
   // (each repeats the sines and cosines).
   const int nrows = 2 * a.num_kv_heads + a.num_q_heads;
-  const int rpi = kAppendThreads / (a.head_dim / vec);
-  const int fit = std::min(kTokensMax, std::max(1, kTableEntries / (a.head_dim / 2)));
+  a.split = RowSplit::of(a.head_dim, a.pairs, vec, half);
+  const int rpi = kRowThreads / a.split.units;
+  const int fit = std::min(kTokensMax, std::max(1, kTableEntries / a.pairs));
   const int full = std::max(1, std::min(fit, std::min(kRowsInFlight * rpi, kRowsMax) / nrows));
   a.tokens_per_wg = num_tokens >= 512 * static_cast<int64_t>(full) ? full : 1;
   const int64_t gx = (num_tokens + a.tokens_per_wg - 1) / a.tokens_per_wg;
@@ -579,16 +352,22 @@ extern "C" int sb_append_kv_paged(
                      ? 1 : static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, 512 / gx), steps));
   a.rows_per_y = std::min((steps + ny - 1) / ny, kRowsMax / rpi) * rpi;
   a.row_div = Divisor::by(nrows);
-  a.half_div = Divisor::by(a.head_dim / 2);
+  a.half_div = Divisor::by(a.pairs);
   const dim3 grid(static_cast<unsigned>(gx),
                   static_cast<unsigned>((all + a.rows_per_y - 1) / a.rows_per_y));
   const hipStream_t st = static_cast<hipStream_t>(stream);
-#define SB_APPEND(DT, VEC)                                                                      \
-  if (dtype == DT && vec == VEC) {                                                              \
-    if (q4)                                                                                     \
-      SB_LAUNCH("append_kv", (append_kv_kernel<DT, VEC, true>), grid, dim3(kAppendThreads), st, a); \
-    else                                                                                        \
-      SB_LAUNCH("append_kv", (append_kv_kernel<DT, VEC, false>), grid, dim3(kAppendThreads), st, a); \
+#define SB_APPEND_(DT, VEC, Q4, HALF)                                                            \
+  SB_LAUNCH("append_kv", (append_kv_kernel<DT, VEC, Q4, HALF>), grid, dim3(kRowThreads), st, a)
+#define SB_APPEND(DT, VEC)                  \
+  if (dtype == DT && vec == VEC) {          \
+    if (q4 && half)                         \
+      SB_APPEND_(DT, VEC, true, true);      \
+    else if (q4)                            \
+      SB_APPEND_(DT, VEC, true, false);     \
+    else if (half)                          \
+      SB_APPEND_(DT, VEC, false, true);     \
+    else                                    \
+      SB_APPEND_(DT, VEC, false, false);    \
   }
   SB_APPEND(SB_DTYPE_F32, 4)
   SB_APPEND(SB_DTYPE_F32, 2)
@@ -597,7 +376,47 @@ extern "C" int sb_append_kv_paged(
   SB_APPEND(SB_DTYPE_BF16, 8)
   SB_APPEND(SB_DTYPE_BF16, 2)
 #undef SB_APPEND
+#undef SB_APPEND_
   return check_launch(fn);
+}
+
+}  // namespace
+}  // namespace sb
+
+extern "C" int sb_append_kv_paged(
+    void* kv_cache, void* kv_scales, const void* key, const void* value, const void* query,
+    void* query_out, const int32_t* block_tables, int64_t table_stride, const int32_t* positions,
+    const int32_t* rotations, const int32_t* row_starts, const float* inv_freq,
+    int64_t num_tokens, int64_t num_requests, int64_t num_kv_heads, int64_t num_q_heads,
+    int64_t head_dim, int64_t block_size, int64_t num_blocks_total, int64_t num_blocks_per_seq,
+    const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides,
+    const int64_t* qo_strides, const int64_t* kv_strides, const int64_t* scale_strides,
+    int32_t dtype, int32_t cache_dtype, void* stream) {
+  return sb::append_kv("sb_append_kv_paged", kv_cache, kv_scales, key, value, query, query_out,
+                       block_tables, table_stride, positions, rotations, row_starts, inv_freq,
+                       num_tokens, num_requests, num_kv_heads, num_q_heads, head_dim, block_size,
+                       num_blocks_total, num_blocks_per_seq, k_strides, v_strides, q_strides,
+                       qo_strides, kv_strides, scale_strides, head_dim / 2, SB_ROTARY_INTERLEAVED,
+                       1.0, dtype, cache_dtype, stream);
+}
+
+extern "C" int sb_append_kv_rotary_paged(
+    void* kv_cache, void* kv_scales, const void* key, const void* value, const void* query,
+    void* query_out, const int32_t* block_tables, int64_t table_stride, const int32_t* positions,
+    const int32_t* rotations, const int32_t* row_starts, const float* inv_freq,
+    int64_t num_tokens, int64_t num_requests, int64_t num_kv_heads, int64_t num_q_heads,
+    int64_t head_dim, int64_t block_size, int64_t num_blocks_total, int64_t num_blocks_per_seq,
+    const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides,
+    const int64_t* qo_strides, const int64_t* kv_strides, const int64_t* scale_strides,
+    int64_t pairs, int32_t layout, double factor, int32_t dtype, int32_t cache_dtype, void* stream) {
+  if (!inv_freq && num_tokens != 0)
+    return sb::fail("sb_append_kv_rotary_paged", "null pointer");
+  return sb::append_kv("sb_append_kv_rotary_paged", kv_cache, kv_scales, key, value, query, query_out,
+                       block_tables, table_stride, positions, rotations, row_starts, inv_freq,
+                       num_tokens, num_requests, num_kv_heads, num_q_heads, head_dim, block_size,
+                       num_blocks_total, num_blocks_per_seq, k_strides, v_strides, q_strides,
+                       qo_strides, kv_strides, scale_strides, pairs, layout, factor, dtype, cache_dtype,
+                       stream);
 }
 
 extern "C" int sb_gather_kv_paged(void* out, const void* kv_cache, const void* kv_scales,

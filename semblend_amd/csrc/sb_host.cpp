@@ -156,6 +156,14 @@ template <> struct Arg<float> {
   }
   float get() const { return v; }
 };
+template <> struct Arg<double> {
+  double v = 0.0;
+  bool take(PyObject* o) {
+    v = PyFloat_AsDouble(o);
+    return v != -1.0 || !PyErr_Occurred();
+  }
+  double get() const { return v; }
+};
 template <typename T> struct Arg<T*> {  // an address, or None
   void* v = nullptr;
   bool take(PyObject* o) {
@@ -218,6 +226,8 @@ PyMethodDef method(const char* name) {
 }
 PyMethodDef entries[] = {
     method<decltype(&sb_append_kv_paged)>("sb_append_kv_paged"),
+    method<decltype(&sb_append_kv_rotary_paged)>("sb_append_kv_rotary_paged"),
+    method<decltype(&sb_apply_rotary)>("sb_apply_rotary"),
     method<decltype(&sb_gather_kv_paged)>("sb_gather_kv_paged"),
     method<decltype(&sb_paged_attention)>("sb_paged_attention"),
 };

@@ -212,6 +212,7 @@ def append_kv_paged(
     rotations: torch.Tensor | None = None,
     query: torch.Tensor | None = None,
     query_out: torch.Tensor | None = None,
+    rotary=None,
 ) -> torch.Tensor | None:
     """K and V of new tokens into the cache slots of their positions, in one launch.
 
@@ -225,6 +226,10 @@ def append_kv_paged(
     the path's fp32 frequencies, the product and its sine and cosine in 64 bits.
     ``rotations``: [T], the positions to rotate by instead (a donor's K, rotated already at d and
     appended at t: t - d).
+    ``rotary``: a :class:`semblend_amd.rotary.RotaryEmbedding` instead of ``rope_base``: half pairs,
+    part of the head, scaled frequencies, its factor on cosine and sine (not with ``rotations``: that
+    K holds it already; a query then needs a factor of 1). 4-bit pages take embeddings whose turned
+    elements (half layout: either half of them, and of the others) are whole blocks of 32.
     Tokens whose position has no page are not appended (their query is rotated still); padding
     rows are left out altogether. Two tokens with one slot race: slots must be distinct.
     Extension with no reference counterpart (``partial_prefill`` writes its new K/V into
@@ -244,8 +249,14 @@ def append_kv_paged(
     k, kst = _rows(key)
     v, vst = _rows(value)
     dt = _lib.dtype_code(key)
-    if rope_base is None and (rotations is not None or query is not None):
-        raise ValueError("rotations and query go with rope_base")
+    if rotary is not None:
+        if rope_base is not None:
+            raise ValueError("rope_base and rotary are alternatives")
+        if rotations is not None and query is not None and rotary.factor != 1.0:
+            raise ValueError("with rotations the factor of rotary applies to no row: a query needs "
+                             "a factor of 1")
+    elif rope_base is None and (rotations is not None or query is not None):
+        raise ValueError("rotations and query go with rope_base or rotary")
     if rope_base is not None and not rope_base >= 1.0:
         raise ValueError("rope_base must be at least 1")
     if d % 2:
@@ -274,13 +285,19 @@ def append_kv_paged(
         rot = _index(rotations, dev)
         if rot.shape[0] != num:
             raise ValueError("rotations must have one entry per token")
-    inv = inv_freq_table(rope_base, d, dev) if rope_base is not None else None
+    entry, more = "sb_append_kv_paged", ()
+    if rotary is not None:
+        inv = rotary._table(dev, d)
+        entry = "sb_append_kv_rotary_paged"
+        more = (inv.shape[0], rotary._code, 1.0 if rot is not None else rotary._factor)
+    else:
+        inv = inv_freq_table(rope_base, d, dev) if rope_base is not None else None
     _lib.launch(
-        dev, "sb_append_kv_paged",
+        dev, entry,
         base, sbase, k.data_ptr(), v.data_ptr(), _lib.ptr(q),
         None if q is None else query_out.data_ptr(), bt.data_ptr(), bt.stride(0), pos.data_ptr(),
         _lib.ptr(rot), _lib.ptr(starts), _lib.ptr(inv), num, requests, heads, hq, d, bs, shape[0],
-        width, kst, vst, qst, ost, st, sst, dt, code)
+        width, kst, vst, qst, ost, st, sst, *more, dt, code)
     if new and query.requires_grad:
         return _recorded("append_kv_paged", query_out, query)
     return query_out
