@@ -738,6 +738,36 @@ int sb_rotary_shift_paged_layers_host(const uint64_t* kv_layer_ptrs, int64_t num
                                       int32_t dtype, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Products with 4-bit weights (no reference counterparts: the reference leaves them to its host
+ * engines)
+ *
+ * w[n, k] = (codes[n, k] - zeros[n, k / group]) * scales[n, k / group]: codes and zeros of 0 to 15,
+ * scales in bf16 or fp16 (scale_dtype), group a multiple of 32 that divides in_features. Packed
+ * weights are two buffers, 16-byte aligned, of sb_w4_codes_size and sb_w4_table_size bytes.
+ * ---------------------------------------------------------------------------------------- */
+int64_t sb_w4_codes_size(int64_t out_features, int64_t in_features);
+int64_t sb_w4_table_size(int64_t out_features, int64_t in_features, int64_t group);
+
+/* Packs codes [out_features, in_features] (a byte each, row stride codes_stride), scales and zeros
+ * (NULL: 8) [out_features, in_features / group] by row strides in elements. */
+int sb_w4_pack(void* packed, void* table, const uint8_t* codes, const void* scales,
+               const uint8_t* zeros, int64_t out_features, int64_t in_features, int64_t group,
+               int64_t codes_stride, int64_t scales_stride, int64_t zeros_stride, void* stream);
+
+/* out [out_features, in_features] (row stride out_stride) = the weights, rounded once to dtype. */
+int sb_w4_dequantize(void* out, const void* packed, const void* table, int64_t out_features,
+                     int64_t in_features, int64_t group, int64_t out_stride, int32_t scale_dtype,
+                     int32_t dtype, void* stream);
+
+/* y [num_rows, out_features] = x [num_rows, in_features] w^T + bias (NULL: none), rows by strides
+ * in elements, x 16-byte aligned in base and stride, all in dtype (bf16 or fp16): exact weights,
+ * fp32 sums, one rounding. */
+int sb_w4_linear(void* y, const void* x, const void* packed, const void* table, const void* bias,
+                 int64_t num_rows, int64_t out_features, int64_t in_features, int64_t group,
+                 int64_t x_stride, int64_t y_stride, int32_t scale_dtype, int32_t dtype,
+                 void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Flat device copy (measurement reference; no reference counterpart)
  * ---------------------------------------------------------------------------------------- */
 
@@ -757,7 +787,8 @@ int sb_device_copy(void* dst, const void* src, int64_t num_bytes, void* stream);
  * (the log stays readable). At most 65536 launches are logged. Kernel names:
  * "move_rows", "rope_rows", "rope_index", "fill_i32", "attn_mfma", "attn_valu", "attn_merge",
  * "mask_compact", "zero_rows", "copy", "append_kv", "gather_kv", "paged_decode", "paged_f32",
- * "paged_rows", "paged_valu", "paged_merge", "rotary_rows". */
+ * "paged_rows", "paged_valu", "paged_merge", "rotary_rows",
+ * "w4_pack", "w4_unpack", "w4_rows". */
 int sb_kernel_timing_enable(int32_t enable);
 
 /* Sum of the logged durations (ms) and number of logged launches of one kernel. Waits for the

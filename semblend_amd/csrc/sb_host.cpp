@@ -230,6 +230,7 @@ PyMethodDef entries[] = {
     method<decltype(&sb_apply_rotary)>("sb_apply_rotary"),
     method<decltype(&sb_gather_kv_paged)>("sb_gather_kv_paged"),
     method<decltype(&sb_paged_attention)>("sb_paged_attention"),
+    method<decltype(&sb_w4_linear)>("sb_w4_linear"),
 };
 
 }  // namespace
