@@ -137,7 +137,8 @@ SIGNATURES: dict[str, list] = {
                            _i64p, _i64p, _i32, _i32, _vp],
     "sb_w4_pack": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp],
     "sb_w4_dequantize": [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _vp],
-    "sb_w4_linear": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _vp],
+    "sb_w4_linear": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i32,
+                     _i32, _vp],
     "sb_device_copy": [_vp, _vp, _i64, _vp],
     "sb_kernel_timing_enable": [_i32],
     "sb_kernel_timing_read": [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double), _i64p],
@@ -156,6 +157,7 @@ SIZE_QUERIES: dict[str, list] = {
     "sb_masked_qkv_projection_workspace_size": [_i64],
     "sb_qkv_projection_paged_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i32],
     "sb_w4_codes_size": [_i64, _i64],
+    "sb_w4_linear_workspace_size": [_i64, _i64, _i64, _i64],
     "sb_w4_table_size": [_i64, _i64, _i64],
     "sb_paged_attention_workspace_size": [_i64, _i64, _i32, _i64, _i64, _i64, _i64, _i64, _i64,
                                           _i64, _i64, _i32, _i32],

@@ -78,6 +78,10 @@ struct W4Args {
   int64_t num_rows;
   int n, k, k_tiles;
   bool scales_f16;
+  // many rows
+  const char* sums;       // [rows][sum_blocks][4][32] bf16
+  int sum_blocks;
+  bool wide_out;          // rows of y take 16-byte stores
 };
 
 // A workgroup takes 16 features and 16 MI rows; its waves take every kWaves'th tile of inputs and add
@@ -155,6 +159,239 @@ __global__ __launch_bounds__(64 * kWaves) void w4_rows_kernel(const W4Args a) {
     if (row < a.num_rows && f < a.n) {
       if (a.bias) v += T::value(a.bias[f]);
       reinterpret_cast<uint16_t*>(a.y + row * a.y_row)[f] = T::round(v);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Many rows. A workgroup of four waves takes 128 rows x 128 features, each wave all the rows and 32
+// features, so that a code is unpacked once for 128 rows and weights never pass through LDS: a wave
+// loads its 32 x 128 codes of a step straight into registers, a step ahead. Rows go global -> LDS, 128
+// inputs a step, two stages. A group's sum P of one 32 x 32 block is a chain of matrix instructions from
+// zero, then acc += scale P. The offsets' share, sum over groups of S (16 + zero) scale, is a product
+// over the groups: S as three bf16 values and (16 + zero) scale as two (exact: 5 bits times 11 at
+// most), the five largest of their six products, 2^-24 of the largest left out. w4_sums_kernel writes the
+// S of 32 groups as one more step of 128 columns of a row ([part][group], the last quarter unused).
+// ---------------------------------------------------------------------------------------
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+template <int DT>
+__device__ __forceinline__ f32x16_t mma32(typename W4<DT>::vec8 a, typename W4<DT>::vec8 b, f32x16_t c) {
+  if constexpr (DT == SB_DTYPE_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// x as three bf16 values that add up to it.
+__device__ __forceinline__ void split3(float x, uint16_t* p) {
+  p[0] = f32_to_bf16(x);
+  const float r = x - bf16_to_f32(p[0]);
+  p[1] = f32_to_bf16(r);
+  p[2] = f32_to_bf16(r - bf16_to_f32(p[1]));
+}
+
+// sums [rows][blocks of 32 groups][4][32]: thread (row, group of `step` inputs). 8 lanes a group and up.
+template <int DT, int STEP>
+__global__ __launch_bounds__(256) void w4_sums_kernel(uint16_t* sums, const char* x, int64_t x_row,
+                                                      int64_t num_rows, int k, int blocks) {
+  constexpr int kLanes = STEP / 8;  // lanes of a group, 8 values each
+  const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t per = static_cast<int64_t>(blocks) * 32 * kLanes;
+  const int64_t row = idx / per;
+  const int64_t rest = idx - row * per;
+  const int64_t k0 = rest * 8;
+  float v = 0.f;
+  if (row < num_rows && k0 < k) {
+    const u32x4_t w = *reinterpret_cast<const u32x4_t*>(x + row * x_row + k0 * 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v += W4<DT>::value(static_cast<uint16_t>(w[i])) + W4<DT>::value(static_cast<uint16_t>(w[i] >> 16));
+  }
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) v += __shfl_xor(v, o, 64);
+  if (row >= num_rows) return;
+  const int64_t g = rest / kLanes;
+  uint16_t p[3];
+  split3(v, p);
+  uint16_t* out = sums + (row * blocks + g / 32) * 128 + g % 32;
+  // (lanes of the group share the stores: parts, and zeros behind them)
+  const int sub = static_cast<int>(rest % kLanes);
+  if (sub < 4) out[sub * 32] = sub == 0 ? p[0] : sub == 1 ? p[1] : sub == 2 ? p[2] : 0;
+}
+
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// One 16-byte global -> LDS copy per lane, lane i's chunk to lds_wave + 16 i; assembly so that the
+// compiler does not order later LDS reads behind it (the kernel waits before its barriers).
+__device__ __forceinline__ void w4_dma(const char* src, uint32_t lds_wave) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, off"
+      :
+      : "s"(lds_wave), "v"(src)
+      : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t w4_lds_addr(const void* p) {
+  using lds_ptr = __attribute__((address_space(3))) const void*;
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)p));
+}
+#pragma clang diagnostic pop
+
+constexpr int kXcds = 8;
+constexpr int kBand = 8;       // row tiles of a band of the tile order
+constexpr int kBM = 128, kBN = 128;
+
+// Tile of workgroup b: workgroups go round-robin to the XCDs, each of which gets a contiguous range of
+// an order that walks bands of kBand row tiles, feature tile by feature tile, so that the workgroups of
+// an XCD share rows and weights in its L2.
+__device__ __forceinline__ void w4_tile(uint32_t b, uint32_t n_ft, uint32_t n_rt, uint32_t* ft, uint32_t* rt) {
+  const uint32_t total = n_ft * n_rt, x = b % kXcds, i = b / kXcds;
+  const uint32_t q = x * (total / kXcds) + min(x, total % kXcds) + i;
+  const uint32_t band = q / (kBand * n_ft), in_band = q - band * kBand * n_ft;
+  const uint32_t rows_in_band = min<uint32_t>(kBand, n_rt - band * kBand);
+  *rt = band * kBand + in_band % rows_in_band;
+  *ft = in_band / rows_in_band;
+}
+
+template <int DT, int GPT>
+__global__ __launch_bounds__(256, 2) void w4_tiles_kernel(const W4Args a) {
+  using T = W4<DT>;
+  using vec8 = typename T::vec8;
+  constexpr int kLoads = kBM * 16 / 256;  // 16-byte copies of a thread a step
+  __shared__ __align__(16) uint16_t ring[2][kBM * kTileK];
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, lq = lane & 31, lg = lane >> 5;
+  const uint32_t n_ft = (a.n + kBN - 1) / kBN;
+  const uint32_t n_rt = static_cast<uint32_t>((a.num_rows + kBM - 1) / kBM);
+  uint32_t ft, rt;
+  w4_tile(blockIdx.x, n_ft, n_rt, &ft, &rt);
+  const int64_t m0 = static_cast<int64_t>(rt) * kBM;
+  const int64_t f0 = static_cast<int64_t>(ft) * kBN;
+  const int steps = a.k_tiles + a.sum_blocks;
+
+  // Copies: slot q * 256 + tid of a stage is row (slot / 16), position slot % 16, and holds chunk
+  // position ^ (row & 15) of the row: the 16-byte reads of 16 consecutive rows fall on all banks. Rows
+  // behind the last are the last one's, chunks behind the last input too (their scale is 0).
+  const int chunk = (tid & 15) ^ ((tid >> 4) & 15);
+  auto copy = [&](int stage, int kt, int q) {
+    const int64_t row = min(m0 + q * 16 + (tid >> 4), a.num_rows - 1);
+    const char* src;
+    if (kt < a.k_tiles)
+      src = a.x + row * a.x_row + static_cast<int64_t>(min(kt * 16 + chunk, a.k / 8 - 1)) * 16;
+    else
+      src = a.sums + (row * a.sum_blocks + (kt - a.k_tiles)) * 256 + chunk * 16;
+    w4_dma(src, w4_lds_addr(ring[stage]) + (q * 256 + wave * 64) * 16);
+  };
+  // This wave's features: two tiles of the packed order (past the last one: the last one's).
+  const int64_t tiles_n = (a.n + kTileN - 1) / kTileN;
+  const int64_t nt = min(f0 / kTileN + 2 * wave + (lq >> 4), tiles_n - 1);
+  const u32x4_t* codes = a.codes + nt * a.k_tiles * 64 + (lq & 15) + 16 * lg;
+  const uint32_t* table = a.table + nt * a.k_tiles * GPT * 16 + (lq & 15);
+
+  f32x16_t acc[4] = {};
+  u32x4_t w[2];
+  uint32_t sz[GPT];
+  auto fetch = [&](int kt) {
+    w[0] = codes[static_cast<int64_t>(kt) * 64];
+    w[1] = codes[static_cast<int64_t>(kt) * 64 + 32];
+#pragma unroll
+    for (int g = 0; g < GPT; ++g) sz[g] = table[(static_cast<int64_t>(kt) * GPT + g) * 16];
+  };
+  auto read = [&](int stage, int i, int s) {
+    const int r = 32 * i + lq;
+    return *reinterpret_cast<const vec8*>(ring[stage] + r * kTileK + 8 * ((2 * s + lg) ^ (r & 15)));
+  };
+#pragma unroll
+  for (int q = 0; q < kLoads; ++q) copy(0, 0, q);
+  fetch(0);
+  for (int kt = 0; kt < a.k_tiles; ++kt) {
+    const int stage = kt & 1;
+    vec8 b[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) b[s] = T::values(w[s & 1][s >> 1]);
+    float scale[GPT];
+#pragma unroll
+    for (int g = 0; g < GPT; ++g) scale[g] = scale_of(sz[g], a.scales_f16);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this step's rows have landed
+    __syncthreads();
+    if (kt + 1 < steps) {
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) copy(stage ^ 1, kt + 1, q);
+    }
+    if (kt + 1 < a.k_tiles) fetch(kt + 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int g = 0; g < GPT; ++g) {
+        f32x16_t p = {};
+#pragma unroll
+        for (int s = g * (8 / GPT); s < (g + 1) * (8 / GPT); ++s) p = mma32<DT>(read(stage, i, s), b[s], p);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = fmaf(scale[g], p[r], acc[i][r]);
+      }
+    }
+  }
+  // The offsets' share, 32 groups a step.
+  using B = W4<SB_DTYPE_BF16>;
+  for (int blk = 0; blk < a.sum_blocks; ++blk) {
+    const int kt = a.k_tiles + blk, stage = kt & 1;
+    B::vec8 z[2][2];  // [16 groups][upper, lower part of -(16 + zero) scale]
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int g = blk * 32 + 16 * h + 8 * lg + e;
+        const uint32_t t = table[static_cast<int64_t>(min(g, a.k_tiles * GPT - 1)) * 16];
+        const float v = -offset_of(t) * scale_of(t, a.scales_f16);
+        const uint32_t up = f32_to_bf16(v), low = f32_to_bf16(v - bf16_to_f32(static_cast<uint16_t>(up)));
+        if (e & 1) hi[e >> 1] |= up << 16, lo[e >> 1] |= low << 16;
+        else hi[e >> 1] = up, lo[e >> 1] = low;
+      }
+      const u32x4_t hv = {hi[0], hi[1], hi[2], hi[3]}, lv = {lo[0], lo[1], lo[2], lo[3]};
+      z[h][0] = __builtin_bit_cast(B::vec8, hv);
+      z[h][1] = __builtin_bit_cast(B::vec8, lv);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    __syncthreads();
+    if (kt + 1 < steps) {
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) copy(stage ^ 1, kt + 1, q);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int part = 0; part < 3; ++part)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const auto s = __builtin_bit_cast(B::vec8, read(stage, i, 2 * part + h));
+          acc[i] = mma32<SB_DTYPE_BF16>(s, z[h][0], acc[i]);
+          if (part < 2) acc[i] = mma32<SB_DTYPE_BF16>(s, z[h][1], acc[i]);
+        }
+  }
+
+  // Out: through LDS, so that a row's features are stored together.
+  __syncthreads();
+  uint16_t* tile = ring[0];
+  const int64_t f = f0 + 32 * wave + lq;
+  const float bias = a.bias && f < a.n ? T::value(a.bias[f]) : 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = 32 * i + 8 * (r >> 2) + 4 * lg + (r & 3);
+      tile[row * kBN + 32 * wave + lq] = T::round(acc[i][r] + bias);
+    }
+  __syncthreads();
+  for (int e = tid; e < kBM * kBN / 8; e += 256) {
+    const int row = e / (kBN / 8), c = e % (kBN / 8) * 8;
+    if (m0 + row >= a.num_rows) break;
+    uint16_t* out = reinterpret_cast<uint16_t*>(a.y + (m0 + row) * a.y_row) + f0 + c;
+    if (a.wide_out && f0 + c + 8 <= a.n) {
+      *reinterpret_cast<u32x4_t*>(out) = *reinterpret_cast<const u32x4_t*>(tile + row * kBN + c);
+    } else {
+      for (int j = 0; j < 8 && f0 + c + j < a.n; ++j) out[j] = tile[row * kBN + c + j];
     }
   }
 }
@@ -303,10 +540,26 @@ extern "C" int sb_w4_dequantize(void* out, const void* packed, const void* table
   return check_launch(fn);
 }
 
+namespace sb {
+namespace {
+// Rows from which a call takes 128 x 128 tiles.
+constexpr int64_t kTiledRows = 65;
+int64_t sum_blocks(int64_t k, int64_t group) { return tiles(tiles(k, kTileK) * (kTileK / table_step(group)), 32); }
+}  // namespace
+}  // namespace sb
+
+extern "C" int64_t sb_w4_linear_workspace_size(int64_t num_rows, int64_t out_features, int64_t in_features,
+                                               int64_t group) {
+  using namespace sb;
+  if (num_rows < kTiledRows || shape_fault(out_features, in_features, group)) return 0;
+  return num_rows * sum_blocks(in_features, group) * 256;
+}
+
 extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const void* table,
                             const void* bias, int64_t num_rows, int64_t out_features,
                             int64_t in_features, int64_t group, int64_t x_stride, int64_t y_stride,
-                            int32_t scale_dtype, int32_t dtype, void* stream) {
+                            void* workspace, int64_t workspace_bytes, int32_t scale_dtype,
+                            int32_t dtype, void* stream) {
   using namespace sb;
   const char* fn = "sb_w4_linear";
   clear_error();
@@ -332,12 +585,34 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
   a.k = static_cast<int>(in_features);
   a.k_tiles = static_cast<int>(tiles(in_features, kTileK));
   a.scales_f16 = scale_dtype == SB_DTYPE_F16;
-  const int mi = num_rows <= 16 ? 1 : num_rows <= 32 ? 2 : 4;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
   const int gpt = static_cast<int>(kTileK / table_step(group));
+  if (num_rows >= kTiledRows) {
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
+        workspace_bytes < sb_w4_linear_workspace_size(num_rows, out_features, in_features, group))
+      return fail(fn, "workspace too small or not 16-byte aligned");
+    a.sums = static_cast<const char*>(workspace);
+    a.sum_blocks = static_cast<int>(sum_blocks(in_features, group));
+    a.wide_out = reinterpret_cast<uintptr_t>(y) % 16 == 0 && a.y_row % 16 == 0;
+    const int64_t work = num_rows * a.sum_blocks * 32 * (table_step(group) / 8);
+    const int64_t grid = tiles(num_rows, kBM) * tiles(out_features, kBN);
+    if (tiles(work, 256) > 0x7fffffff || grid > 0x7fffffff) return fail(fn, "grid too large");
+#define SB_W4(DT, GPT)                                                                                \
+  if (dtype == DT && gpt == GPT) {                                                                    \
+    SB_LAUNCH("w4_sums", (w4_sums_kernel<DT, kTileK / GPT>), dim3(static_cast<unsigned>(tiles(work, 256))), \
+              dim3(256), st, static_cast<uint16_t*>(workspace), a.x, a.x_row, a.num_rows, a.k,        \
+              a.sum_blocks);                                                                          \
+    SB_LAUNCH("w4_tiles", (w4_tiles_kernel<DT, GPT>), dim3(static_cast<unsigned>(grid)), dim3(256), st, a); \
+  }
+    SB_W4(SB_DTYPE_BF16, 1) SB_W4(SB_DTYPE_BF16, 2) SB_W4(SB_DTYPE_BF16, 4)
+    SB_W4(SB_DTYPE_F16, 1) SB_W4(SB_DTYPE_F16, 2) SB_W4(SB_DTYPE_F16, 4)
+#undef SB_W4
+    return check_launch(fn);
+  }
+  const int mi = num_rows <= 16 ? 1 : num_rows <= 32 ? 2 : 4;
   const int64_t gy = tiles(num_rows, 16 * mi);
   if (gy > 65535) return fail(fn, "too many rows");
   const dim3 grid(static_cast<unsigned>(tiles(out_features, kTileN)), static_cast<unsigned>(gy));
-  const hipStream_t st = static_cast<hipStream_t>(stream);
 #define SB_W4(DT, MI, GPT)                                                                            \
   if (dtype == DT && mi == MI && gpt == GPT)                                                          \
     SB_LAUNCH("w4_rows", (w4_rows_kernel<DT, MI, GPT>), grid, dim3(64 * kWaves), st, a);

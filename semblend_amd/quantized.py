@@ -14,6 +14,8 @@ A server's calls without a backward pass, as in :mod:`semblend_amd.paged_cache`.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -22,6 +24,11 @@ from .paged_cache import _device, _recorded
 __all__ = ["QuantizedLinear", "quantized_linear"]
 
 _16BIT = (torch.bfloat16, torch.float16)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*sizes: int) -> int:
+    return _lib.size_query("sb_w4_linear_workspace_size", *sizes)
 
 
 class QuantizedLinear:
@@ -154,9 +161,11 @@ def quantized_linear(
             step = k
         if bias is not None and bias.stride(0) != 1:
             bias = bias.contiguous()
+        ws_bytes = _workspace_bytes(num, n, k, weight.group)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         _lib.launch(dev, "sb_w4_linear", out.data_ptr(), rows.data_ptr(), weight._packed.data_ptr(),
                     weight._table.data_ptr(), _lib.ptr(bias), num, n, k, weight.group, step, out_rows,
-                    weight._code, _lib.SB_DTYPE[dtype])
+                    _lib.ptr(ws), ws_bytes, weight._code, _lib.SB_DTYPE[dtype])
     if new and (x.requires_grad or bias is not None and bias.requires_grad):
         return _recorded("quantized_linear", out, x, *(() if bias is None else (bias,)))
     return out

@@ -93,7 +93,8 @@ def test_product_refusals(on_cpu):
 
 
 def _linear(**over):
-    a = dict(y=FAKE, x=FAKE, w=FAKE, t=FAKE, b=None, m=3, n=32, k=128, g=64, xs=128, ys=32, sdt=2, dt=2)
+    a = dict(y=FAKE, x=FAKE, w=FAKE, t=FAKE, b=None, m=3, n=32, k=128, g=64, xs=128, ys=32, ws=None, wsb=0,
+             sdt=2, dt=2)
     a.update(over)
     return _lib.lib().sb_w4_linear(*a.values(), None)
 
@@ -116,6 +117,7 @@ def _unpack(**over):
     (_linear, dict(g=48), b"multiple of 32"), (_linear, dict(k=100), b"multiple of 32"),
     (_linear, dict(x=FAKE + 2), b"aligned"), (_linear, dict(xs=132), b"aligned"),
     (_linear, dict(m=1 << 31), b"32 bits"), (_linear, dict(n=1 << 31), b"32 bits"),
+    (_linear, dict(m=4096), b"workspace"), (_linear, dict(m=4096, ws=FAKE, wsb=100), b"workspace"),
     (_pack, dict(c=None), b"null"), (_pack, dict(g=16), b"multiple of 32"), (_pack, dict(k=0), b"positive"),
     (_pack, dict(w=FAKE + 8), b"aligned"), (_unpack, dict(dt=3), b"invalid dtype"),
     (_unpack, dict(sdt=3), b"scales"), (_unpack, dict(o=None), b"null"),
@@ -132,4 +134,7 @@ def test_sizes():
     assert size("sb_w4_table_size", 16, 128, 128) == 64
     assert size("sb_w4_table_size", 17, 160, 32) == 2 * 8 * 64
     assert size("sb_w4_table_size", 16, 192, 96) == 8 * 64
+    assert size("sb_w4_linear_workspace_size", 4, 32, 128, 64) == 0
+    assert size("sb_w4_linear_workspace_size", 4096, 32, 128, 64) > 0
+    assert size("sb_w4_linear_workspace_size", 4096, 32, 128, 48) == 0
     assert _linear(m=0, x=None) == _lib.SB_OK
