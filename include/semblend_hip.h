@@ -764,7 +764,7 @@ int sb_w4_dequantize(void* out, const void* packed, const void* table, int64_t o
  * fp32 sums, one rounding. workspace: 16-byte aligned, sb_w4_linear_workspace_size bytes (may be
  * NULL where that is 0). */
 int64_t sb_w4_linear_workspace_size(int64_t num_rows, int64_t out_features, int64_t in_features,
-                                    int64_t group);
+                                    int64_t group, int32_t dtype);
 int sb_w4_linear(void* y, const void* x, const void* packed, const void* table, const void* bias,
                  int64_t num_rows, int64_t out_features, int64_t in_features, int64_t group,
                  int64_t x_stride, int64_t y_stride, void* workspace, int64_t workspace_bytes,
@@ -791,7 +791,8 @@ int sb_device_copy(void* dst, const void* src, int64_t num_bytes, void* stream);
  * "move_rows", "rope_rows", "rope_index", "fill_i32", "attn_mfma", "attn_valu", "attn_merge",
  * "mask_compact", "zero_rows", "copy", "append_kv", "gather_kv", "paged_decode", "paged_f32",
  * "paged_rows", "paged_valu", "paged_merge", "rotary_rows",
- * "w4_pack", "w4_unpack", "w4_rows", "w4_sums", "w4_tiles". */
+ * "w4_pack", "w4_unpack", "w4_rows", "w4_sums", "w4_tiles",
+ * "w4_merge". */
 int sb_kernel_timing_enable(int32_t enable);
 
 /* Sum of the logged durations (ms) and number of logged launches of one kernel. Waits for the

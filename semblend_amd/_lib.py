@@ -157,7 +157,7 @@ SIZE_QUERIES: dict[str, list] = {
     "sb_masked_qkv_projection_workspace_size": [_i64],
     "sb_qkv_projection_paged_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i32],
     "sb_w4_codes_size": [_i64, _i64],
-    "sb_w4_linear_workspace_size": [_i64, _i64, _i64, _i64],
+    "sb_w4_linear_workspace_size": [_i64, _i64, _i64, _i64, _i32],
     "sb_w4_table_size": [_i64, _i64, _i64],
     "sb_paged_attention_workspace_size": [_i64, _i64, _i32, _i64, _i64, _i64, _i64, _i64, _i64,
                                           _i64, _i64, _i32, _i32],

@@ -26,20 +26,35 @@ typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kTileN = 16;    // features of a tile
 constexpr int kTileK = 128;   // inputs of a tile
+constexpr int64_t kInputsMax = int64_t{1} << 22;  // inputs, and row stride: 128 rows stay within 2^31 bytes
+
+// A constant that the compiler does not know as one, in a scalar or a vector register: (w & mask) | base
+// is one instruction then, with a literal each they are two.
+__device__ __forceinline__ uint32_t scalar_constant(uint32_t x) {
+  asm("" : "+s"(x));
+  return x;
+}
+__device__ __forceinline__ uint32_t vector_constant(uint32_t x) {
+  asm("" : "+v"(x));
+  return x;
+}
 
 template <int DT> struct W4;
 template <> struct W4<SB_DTYPE_BF16> {
   using vec8 = bf16x8_t;
   static constexpr uint32_t kOnes = 0x3f803f80u;
+  // There is no packed bf16 addition: the values stay 16 + c, and the offset goes to the sums.
+  static constexpr bool kExact = false;
+  __device__ __forceinline__ static vec8 minus(vec8 v, float) { return v; }
   __device__ __forceinline__ static f32x4_t mma(vec8 a, vec8 b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
   // 16 + c for the eight codes of a word: pair p's codes lie at bits 4p + 3 .. 4p + 6 of both halves
   // (modulo 32).
   __device__ __forceinline__ static vec8 values(uint32_t w) {
-    const u32x4_t r = {(w & 0x00780078u) | 0x41804180u, ((w >> 4) & 0x00780078u) | 0x41804180u,
-                       ((w >> 8) & 0x00780078u) | 0x41804180u,
-                       (__builtin_amdgcn_alignbit(w, w, 12) & 0x00780078u) | 0x41804180u};
+    const uint32_t m = scalar_constant(0x00780078u), base = vector_constant(0x41804180u);
+    const u32x4_t r = {((w) & m) | base, ((w >> 4) & m) | base, ((w >> 8) & m) | base,
+                       ((__builtin_amdgcn_alignbit(w, w, 12)) & m) | base};
     return __builtin_bit_cast(vec8, r);
   }
   __device__ __forceinline__ static uint16_t round(float f) { return f32_to_bf16(f); }
@@ -48,13 +63,20 @@ template <> struct W4<SB_DTYPE_BF16> {
 template <> struct W4<SB_DTYPE_F16> {
   using vec8 = f16x8_t;
   static constexpr uint32_t kOnes = 0x3c003c00u;
+  // (16 + c) - (16 + zero) = c - zero, exact: one packed addition for two codes.
+  static constexpr bool kExact = true;
+  __device__ __forceinline__ static vec8 minus(vec8 v, float off) {
+    const _Float16 h = static_cast<_Float16>(off);
+    const vec8 o = {h, h, h, h, h, h, h, h};
+    return v - o;
+  }
   __device__ __forceinline__ static f32x4_t mma(vec8 a, vec8 b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
   __device__ __forceinline__ static vec8 values(uint32_t w) {
-    const u32x4_t r = {((w << 3) & 0x03c003c0u) | 0x4c004c00u, ((w >> 1) & 0x03c003c0u) | 0x4c004c00u,
-                       ((w >> 5) & 0x03c003c0u) | 0x4c004c00u,
-                       (__builtin_amdgcn_alignbit(w, w, 9) & 0x03c003c0u) | 0x4c004c00u};
+    const uint32_t m = scalar_constant(0x03c003c0u), base = vector_constant(0x4c004c00u);
+    const u32x4_t r = {((w << 3) & m) | base, ((w >> 1) & m) | base, ((w >> 5) & m) | base,
+                       ((__builtin_amdgcn_alignbit(w, w, 9)) & m) | base};
     return __builtin_bit_cast(vec8, r);
   }
   __device__ __forceinline__ static uint16_t round(float f) { return f32_to_f16(f); }
@@ -82,81 +104,215 @@ struct W4Args {
   const char* sums;       // [rows][sum_blocks][4][32] bf16
   int sum_blocks;
   bool wide_out;          // rows of y take 16-byte stores
+  // split inputs: slice s of the steps gives its sums to part [splits][rows][n], and no y
+  float* part;
+  int splits, split_steps;
+  uint32_t tiles;         // workgroups of a slice
 };
 
-// A workgroup takes 16 features and 16 MI rows; its waves take every kWaves'th tile of inputs and add
-// their sums up in LDS at the end, in order. GPT: groups of a tile of inputs.
-constexpr int kWaves = 8;
-template <int DT, int MI, int GPT>
-__global__ __launch_bounds__(64 * kWaves) void w4_rows_kernel(const W4Args a) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// Copies global -> LDS without registers, 16 or 4 bytes a lane, lane i's to lds_wave + 16 i (4 i);
+// assembly so that the compiler does not order later LDS reads behind them (the kernels wait
+// themselves: vector memory operations end in order).
+__device__ __forceinline__ void w4_dma(const void* src, uint32_t lds_wave) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, off"
+      :
+      : "s"(lds_wave), "v"(src)
+      : "memory", "m0");
+}
+__device__ __forceinline__ void w4_dma4(const void* src, uint32_t lds_wave) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %1, off"
+      :
+      : "s"(lds_wave), "v"(src)
+      : "memory", "m0");
+}
+// Rows of x: `rows` describes up to 2^32 bytes from a workgroup's first row to the end of the last one
+// (a load behind it gives zeros or nothing), `at` is a lane's offset, `add` one for all lanes. One
+// register where addresses take two for every four rows.
+__device__ __forceinline__ u32x4_t w4_rows_of(const char* first, int64_t bytes) {
+  const uint64_t p = reinterpret_cast<uint64_t>(first);
+  const u32x4_t r = {static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32) & 0xffffu,
+                     static_cast<uint32_t>(min(bytes, static_cast<int64_t>(0xffffffffll))), 0x00020000u};
+  return r;
+}
+__device__ __forceinline__ void w4_dma_row(uint32_t at, u32x4_t rows, uint32_t add, uint32_t lds_wave) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, %3 offen lds"
+      :
+      : "s"(lds_wave), "v"(at), "s"(rows), "s"(add)
+      : "memory", "m0");
+}
+// Until at most N vector memory operations of the wave are under way; later LDS reads stay behind it.
+template <int N>
+__device__ __forceinline__ void w4_wait_vm() {
+  static_assert(N >= 0 && N < 64, "a six-bit count");
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+// Until every LDS read of the wave has its values.
+__device__ __forceinline__ void w4_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
+__device__ __forceinline__ uint32_t w4_lds_addr(const void* p) {
+  using lds_ptr = __attribute__((address_space(3))) const void*;
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)p));
+}
+#pragma clang diagnostic pop
+
+// Few rows. A workgroup takes 16 J features and up to R rows (4, or 16 MI); its WAVES waves take every
+// WAVES'th tile of inputs each for itself, and add their sums up in LDS at the end, in order. What a step
+// needs (codes, table words and the rows' 128 inputs) is copied into a stage of the wave's own LDS, AHEAD
+// steps in flight, with no register and no barrier between. Rows are copied 256 bytes at a time: read by
+// lanes as the matrix operand has them (64 bytes of 16 rows), the rows alone took twice as long as all
+// else (16 rows of 3584 -> 4608: 9.2 us, with one row's address for all of them 4.9). GPT: groups of a
+// tile of inputs.
+constexpr int kRowWaves = 8;
+template <int R, int J, int GPT> struct RowsStage {
+  static constexpr int kMi = R < 16 ? 1 : R / 16;
+  static constexpr int kTableCopies = (J * GPT + 3) / 4;
+  static constexpr int kRowCopies = R / 4;
+  static constexpr int kCopies = J + kTableCopies + kRowCopies;
+  static constexpr int kBytes = J * 1024 + kTableCopies * 256 + R * 256;
+};
+template <int DT, int R, int J, int GPT, int WAVES, int AHEAD>
+__global__ __launch_bounds__(64 * WAVES, 2) void w4_rows_kernel(const W4Args a) {
   using T = W4<DT>;
+  using S = RowsStage<R, J, GPT>;
   using vec8 = typename T::vec8;
-  __shared__ float part[kWaves][MI * 4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t nt = blockIdx.x;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * (16 * MI);
-  const u32x4_t* codes = a.codes + nt * a.k_tiles * 64 + lane;
-  const uint32_t* table = a.table + nt * a.k_tiles * GPT * 16 + (lane & 15);
-  const char* xr[MI];
-  bool live[MI];
+  constexpr int MI = S::kMi;
+  constexpr int kRing = WAVES * AHEAD * S::kBytes, kParts = WAVES * MI * J * 1024;
+  __shared__ __align__(16) char smem[kRing > kParts ? kRing : kParts];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles_n = (a.n + kTileN - 1) / kTileN;
+  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * R;
+  // (tiles of features behind the last one: the last one)
+  const u32x4_t* codes[J];
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const int64_t row = m0 + 16 * i + (lane & 15);
-    live[i] = row < a.num_rows;
-    xr[i] = a.x + (live[i] ? row : 0) * a.x_row + (lane >> 4) * 16;
+  for (int j = 0; j < J; ++j) {
+    const int64_t nt = min(static_cast<int>(blockIdx.x) * J + j, tiles_n - 1);
+    codes[j] = a.codes + nt * a.k_tiles * 64 + lane;
   }
+  const uint32_t* table[S::kTableCopies];
+#pragma unroll
+  for (int t = 0; t < S::kTableCopies; ++t) {
+    const int word = min(lane + 64 * t, J * GPT * 16 - 1);
+    const int64_t nt = min(static_cast<int>(blockIdx.x) * J + word / (GPT * 16), tiles_n - 1);
+    table[t] = a.table + nt * a.k_tiles * GPT * 16 + word % (GPT * 16);
+  }
+  const uint32_t x_row = static_cast<uint32_t>(a.x_row);
+  const u32x4_t rows = w4_rows_of(a.x + m0 * a.x_row, (a.num_rows - 1 - m0) * a.x_row + a.k * 2);
+  const uint32_t row_at = (lane >> 4) * x_row;
+  int chunk[R < 16 ? 1 : 4];  // 16 inputs' place of a row: position ^ row
+#pragma unroll
+  for (int c = 0; c < (R < 16 ? 1 : 4); ++c) chunk[c] = (lane & 15) ^ (4 * c + (lane >> 4));
+  char* mine = smem + wave * (AHEAD * S::kBytes);
+  const uint32_t mine_lds = w4_lds_addr(mine);
+  auto copy = [&](int stage, int kt) {
+    uint32_t at = mine_lds + stage * S::kBytes;
+#pragma unroll
+    for (int j = 0; j < J; ++j, at += 1024) w4_dma(codes[j] + static_cast<int64_t>(kt) * 64, at);
+#pragma unroll
+    for (int t = 0; t < S::kTableCopies; ++t, at += 256)
+      w4_dma4(table[t] + static_cast<int64_t>(kt) * (GPT * 16), at);
+#pragma unroll
+    for (int c = 0; c < S::kRowCopies; ++c, at += 1024) {
+      int k8 = kt * 16 + chunk[c & 3 & (R < 16 ? 0 : 3)];
+      if (GPT > 1) k8 = min(k8, a.k / 8 - 1);  // (behind the last input: the last ones, of scale 0)
+      w4_dma_row(row_at + k8 * 16, rows, 4 * c * x_row, at);
+    }
+  };
   const u32x4_t one4 = {T::kOnes, T::kOnes, T::kOnes, T::kOnes};
   const vec8 ones = __builtin_bit_cast(vec8, one4);
-
-  f32x4_t acc[MI] = {};
-  for (int kt = wave; kt < a.k_tiles; kt += kWaves) {
-    const u32x4_t w = codes[static_cast<int64_t>(kt) * 64];
-    uint32_t sz[GPT];
+  f32x4_t acc[MI][J] = {};
+  auto multiply = [&](int stage) {
+    const char* at = mine + stage * S::kBytes;
+    const char* xs = at + J * 1024 + S::kTableCopies * 256;
+    u32x4_t w[J];
 #pragma unroll
-    for (int g = 0; g < GPT; ++g) sz[g] = table[(static_cast<int64_t>(kt) * GPT + g) * 16];
-    vec8 xv[MI][4];
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        u32x4_t v = {0u, 0u, 0u, 0u};
-        if (live[i] && kt * kTileK + 32 * j < a.k)
-          v = *reinterpret_cast<const u32x4_t*>(xr[i] + (static_cast<int64_t>(kt) * kTileK + 32 * j) * 2);
-        xv[i][j] = __builtin_bit_cast(vec8, v);
-      }
+    for (int j = 0; j < J; ++j) w[j] = *reinterpret_cast<const u32x4_t*>(at + j * 1024 + lane * 16);
     constexpr int kSteps = 4 / GPT;
 #pragma unroll
     for (int g = 0; g < GPT; ++g) {
-      const float s = scale_of(sz[g], a.scales_f16), off = offset_of(sz[g]);
-      f32x4_t p[MI] = {}, sum[MI] = {};
+      float s[J], off[J];
 #pragma unroll
-      for (int j = g * kSteps; j < (g + 1) * kSteps; ++j) {
-        const vec8 b = T::values(w[j]);
+      for (int j = 0; j < J; ++j) {
+        const uint32_t sz =
+            *reinterpret_cast<const uint32_t*>(at + J * 1024 + ((j * GPT + g) * 16 + (lane & 15)) * 4);
+        s[j] = scale_of(sz, a.scales_f16), off[j] = offset_of(sz);
+      }
+      f32x4_t p[MI][J] = {}, sum[MI] = {};
+#pragma unroll
+      for (int q = g * kSteps; q < (g + 1) * kSteps; ++q) {
+        vec8 b[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) b[j] = T::minus(T::values(w[j][q]), off[j]);
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-          p[i] = T::mma(xv[i][j], b, p[i]);
-          sum[i] = T::mma(xv[i][j], ones, sum[i]);
+          const int r = R < 16 ? lane & 3 : 16 * i + (lane & 15);
+          const vec8 x =
+              *reinterpret_cast<const vec8*>(xs + r * 256 + (((4 * q + (lane >> 4)) ^ r) & 15) * 16);
+#pragma unroll
+          for (int j = 0; j < J; ++j) p[i][j] = T::mma(x, b[j], p[i][j]);
+          if (!T::kExact) sum[i] = T::mma(x, ones, sum[i]);
         }
       }
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][r] = fmaf(s, fmaf(-off, sum[i][r], p[i][r]), acc[i][r]);
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            acc[i][j][r] = fmaf(s[j], T::kExact ? p[i][j][r] : fmaf(-off[j], sum[i][r], p[i][j][r]),
+                                acc[i][j][r]);
+      // (64 rows: a group's sums go to the accumulators now; left to the compiler those of all groups
+      // wait behind the next copies, in more registers than there are)
+      if constexpr (MI == 4 && GPT > 1)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < J; ++j) asm volatile("" : "+v"(acc[i][j]));
     }
+  };
+#pragma unroll
+  for (int p = 0; p < AHEAD; ++p)
+    if (wave + p * WAVES < a.k_tiles) copy(p, wave + p * WAVES);
+  int stage = 0;
+  for (int kt = wave; kt < a.k_tiles; kt += WAVES) {
+    // (the last steps wait for all that is left)
+    if (kt + (AHEAD - 1) * WAVES < a.k_tiles) w4_wait_vm<(AHEAD - 1) * S::kCopies>();
+    else w4_wait_vm<0>();
+    multiply(stage);
+    if (kt + AHEAD * WAVES < a.k_tiles) {
+      w4_wait_lds();  // the stage is read before it is written again
+      copy(stage, kt + AHEAD * WAVES);
+    }
+    stage = stage + 1 == AHEAD ? 0 : stage + 1;
   }
+  __syncthreads();
+  float* part = reinterpret_cast<float*>(smem);  // [wave][row tile, feature tile, register][lane]
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) part[wave][4 * i + r][lane] = acc[i][r];
-  __syncthreads();
-  for (int e = threadIdx.x; e < MI * 4 * 64; e += 64 * kWaves) {
-    const int l = e & 63, ir = e >> 6;
-    float v = 0.f;
+    for (int j = 0; j < J; ++j)
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) v += part[w][ir][l];
-    const int64_t row = m0 + 16 * (ir >> 2) + 4 * (l >> 4) + (ir & 3);
-    const int64_t f = nt * kTileN + (l & 15);
-    if (row < a.num_rows && f < a.n) {
+      for (int r = 0; r < 4; ++r)
+        part[((wave * MI + i) * J + j) * 256 + r * 64 + lane] = acc[i][j][r];
+  __syncthreads();
+  for (int e = threadIdx.x; e < MI * J * 256; e += 64 * WAVES) {
+    const int l = e & 63, ir = e >> 6, ij = ir >> 2;
+    const int64_t row = m0 + 16 * (ij / J) + 4 * (l >> 4) + (ir & 3);
+    const int64_t f = (static_cast<int64_t>(blockIdx.x) * J + ij % J) * kTileN + (l & 15);
+    if (row < a.num_rows && f < a.n && row < m0 + R) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) v += part[w * (MI * J * 256) + e];
       if (a.bias) v += T::value(a.bias[f]);
       reinterpret_cast<uint16_t*>(a.y + row * a.y_row)[f] = T::round(v);
     }
@@ -166,12 +322,19 @@ __global__ __launch_bounds__(64 * kWaves) void w4_rows_kernel(const W4Args a) {
 // ---------------------------------------------------------------------------------------
 // Many rows. A workgroup of four waves takes 128 rows x 128 features, each wave all the rows and 32
 // features, so that a code is unpacked once for 128 rows and weights never pass through LDS: a wave
-// loads its 32 x 128 codes of a step straight into registers, a step ahead. Rows go global -> LDS, 128
+// loads its 32 x 128 codes of a step straight into registers, two steps ahead. Rows go global -> LDS, 128
 // inputs a step, two stages. A group's sum P of one 32 x 32 block is a chain of matrix instructions from
-// zero, then acc += scale P. The offsets' share, sum over groups of S (16 + zero) scale, is a product
-// over the groups: S as three bf16 values and (16 + zero) scale as two (exact: 5 bits times 11 at
-// most), the five largest of their six products, 2^-24 of the largest left out. w4_sums_kernel writes the
-// S of 32 groups as one more step of 128 columns of a row ([part][group], the last quarter unused).
+// zero, then acc += scale P. bf16: the offsets' share, sum over groups of S (16 + zero) scale, is a
+// product over the groups: S as three bf16 values and (16 + zero) scale as two (exact: 5 bits times 11 at
+// most), the five largest of their six products, 2^-24 of the largest left out. w4_sums_kernel writes the S of
+// 32 groups as one more step of 128 columns of a row ([part][group], the last quarter unused).
+//
+// What bounds it: the issue of instructions. Of the cycles of a SIMD with one wave, 39% are matrix
+// instructions and 49% the issue of all others (a matrix instruction of 32 cycles comes with two fmas, an
+// LDS read and its wait, and two to three to unpack codes), and little of one runs under the other; a
+// second wave gains a quarter. Waves of 64 x 64 (half the LDS reads, twice the unpacking) were slower
+// (2458 rows of 3584 -> 4608 103 against 95 us), so were copies spread over the step (92-94 against 90);
+// reads 3, 4 and 6 ahead instead of 2 changed nothing, but for groups of 32 (131 -> 128 us).
 // ---------------------------------------------------------------------------------------
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
@@ -218,25 +381,6 @@ __global__ __launch_bounds__(256) void w4_sums_kernel(uint16_t* sums, const char
   if (sub < 4) out[sub * 32] = sub == 0 ? p[0] : sub == 1 ? p[1] : sub == 2 ? p[2] : 0;
 }
 
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-// One 16-byte global -> LDS copy per lane, lane i's chunk to lds_wave + 16 i; assembly so that the
-// compiler does not order later LDS reads behind it (the kernel waits before its barriers).
-__device__ __forceinline__ void w4_dma(const char* src, uint32_t lds_wave) {
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, off"
-      :
-      : "s"(lds_wave), "v"(src)
-      : "memory", "m0");
-}
-__device__ __forceinline__ uint32_t w4_lds_addr(const void* p) {
-  using lds_ptr = __attribute__((address_space(3))) const void*;
-  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)p));
-}
-#pragma clang diagnostic pop
-
 constexpr int kXcds = 8;
 constexpr int kBand = 8;       // row tiles of a band of the tile order
 constexpr int kBM = 128, kBN = 128;
@@ -253,6 +397,56 @@ __device__ __forceinline__ void w4_tile(uint32_t b, uint32_t n_ft, uint32_t n_rt
   *ft = in_band / rows_in_band;
 }
 
+// One wave's 32 x 32 blocks of a slice's sums.
+__device__ __forceinline__ void store_part(const W4Args& a, const f32x16_t (&acc)[4], int slice, int64_t m0,
+                                           int f, int lg) {
+  if (f >= a.n) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int64_t row = m0 + 32 * i + 8 * (r >> 2) + 4 * lg + (r & 3);
+      if (row < a.num_rows) a.part[(slice * a.num_rows + row) * a.n + f] = acc[i][r];
+    }
+}
+
+// y = the slices' sums, in order, + bias. A thread takes VEC features of a row.
+template <int DT, int VEC>
+__global__ __launch_bounds__(256) void w4_merge_kernel(const W4Args a) {
+  const int per = (a.n + VEC - 1) / VEC;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t row = i / per;
+  if (row >= a.num_rows) return;
+  const int f = static_cast<int>(i - row * per) * VEC;
+  const float* p = a.part + row * a.n + f;
+  const int64_t step = a.num_rows * a.n;
+  float v[VEC] = {};
+  for (int s0 = 0; s0 < a.splits; s0 += 4) {
+    float x[4][VEC];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const float* at = p + min(s0 + s, a.splits - 1) * step;
+      if constexpr (VEC == 4) {
+        const f32x4_t w = *reinterpret_cast<const f32x4_t*>(at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[s][e] = w[e];
+      } else {
+        x[s][0] = *at;
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] += s0 + s < a.splits ? x[s][e] : 0.f;
+  }
+  uint16_t h[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) h[e] = W4<DT>::round(v[e] + (a.bias ? W4<DT>::value(a.bias[f + e]) : 0.f));
+  uint16_t* out = reinterpret_cast<uint16_t*>(a.y + row * a.y_row) + f;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) out[e] = h[e];
+}
+
 template <int DT, int GPT>
 __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(const W4Args a) {
   using T = W4<DT>;
@@ -265,23 +459,30 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(const W4Args a) {
   const uint32_t n_ft = (a.n + kBN - 1) / kBN;
   const uint32_t n_rt = static_cast<uint32_t>((a.num_rows + kBM - 1) / kBM);
   uint32_t ft, rt;
-  w4_tile(blockIdx.x, n_ft, n_rt, &ft, &rt);
+  const int slice = static_cast<int>(blockIdx.x / a.tiles);
+  w4_tile(blockIdx.x % a.tiles, n_ft, n_rt, &ft, &rt);
   const int64_t m0 = static_cast<int64_t>(rt) * kBM;
   const int64_t f0 = static_cast<int64_t>(ft) * kBN;
-  const int steps = a.k_tiles + a.sum_blocks;
+  const int begin = slice * a.split_steps, steps = min(begin + a.split_steps, a.k_tiles + a.sum_blocks);
 
   // Copies: slot q * 256 + tid of a stage is row (slot / 16), position slot % 16, and holds chunk
-  // position ^ (row & 15) of the row: the 16-byte reads of 16 consecutive rows fall on all banks. Rows
-  // behind the last are the last one's, chunks behind the last input too (their scale is 0).
+  // position ^ (row & 15) of the row: the 16-byte reads of 16 consecutive rows fall on all banks. Chunks
+  // behind the last input are the last ones (their scale is 0).
   const int chunk = (tid & 15) ^ ((tid >> 4) & 15);
-  auto copy = [&](int stage, int kt, int q) {
-    const int64_t row = min(m0 + q * 16 + (tid >> 4), a.num_rows - 1);
-    const char* src;
-    if (kt < a.k_tiles)
-      src = a.x + row * a.x_row + static_cast<int64_t>(min(kt * 16 + chunk, a.k / 8 - 1)) * 16;
-    else
-      src = a.sums + (row * a.sum_blocks + (kt - a.k_tiles)) * 256 + chunk * 16;
-    w4_dma(src, w4_lds_addr(ring[stage]) + (q * 256 + wave * 64) * 16);
+  const uint32_t x_row = static_cast<uint32_t>(a.x_row), s_row = static_cast<uint32_t>(a.sum_blocks) * 256;
+  const u32x4_t rows = w4_rows_of(a.x + m0 * a.x_row, (a.num_rows - 1 - m0) * a.x_row + a.k * 2);
+  auto copy = [&](int stage, int kt) {
+    const uint32_t to = w4_lds_addr(ring[stage]) + wave * 1024;
+    if (kt < a.k_tiles) {
+      const uint32_t at = (tid >> 4) * x_row + (GPT == 1 ? kt * 16 + chunk : min(kt * 16 + chunk, a.k / 8 - 1)) * 16;
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) w4_dma_row(at, rows, 16 * q * x_row, to + q * 4096);
+    } else {
+      const u32x4_t sums = w4_rows_of(a.sums + m0 * s_row, (a.num_rows - m0) * s_row);
+      const uint32_t at = (tid >> 4) * s_row + (kt - a.k_tiles) * 256 + chunk * 16;
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) w4_dma_row(at, sums, 16 * q * s_row, to + q * 4096);
+    }
   };
   // This wave's features: two tiles of the packed order (past the last one: the last one's).
   const int64_t tiles_n = (a.n + kTileN - 1) / kTileN;
@@ -290,87 +491,116 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(const W4Args a) {
   const uint32_t* table = a.table + nt * a.k_tiles * GPT * 16 + (lq & 15);
 
   f32x16_t acc[4] = {};
-  u32x4_t w[2];
-  uint32_t sz[GPT];
-  auto fetch = [&](int kt) {
-    w[0] = codes[static_cast<int64_t>(kt) * 64];
-    w[1] = codes[static_cast<int64_t>(kt) * 64 + 32];
+  // Codes and table words of step kt: in `next` from the step before it on, in `coming` the one before.
+  struct Codes {
+    u32x4_t w[2];
+    uint32_t sz[GPT];
+  } next, coming;
+  const int last = min(steps, a.k_tiles) - 1;  // (the last step with codes; maybe below begin)
+  auto fetch = [&](Codes& c, int kt) {
+    kt = max(min(kt, last), 0);
+    c.w[0] = codes[static_cast<int64_t>(kt) * 64];
+    c.w[1] = codes[static_cast<int64_t>(kt) * 64 + 32];
 #pragma unroll
-    for (int g = 0; g < GPT; ++g) sz[g] = table[(static_cast<int64_t>(kt) * GPT + g) * 16];
+    for (int g = 0; g < GPT; ++g) c.sz[g] = table[(static_cast<int64_t>(kt) * GPT + g) * 16];
   };
   auto read = [&](int stage, int i, int s) {
     const int r = 32 * i + lq;
     return *reinterpret_cast<const vec8*>(ring[stage] + r * kTileK + 8 * ((2 * s + lg) ^ (r & 15)));
   };
+  fetch(next, begin);
+  copy(begin & 1, begin);
+  fetch(coming, begin + 1);
+  vec8 b[8];
+  float scale[GPT];
+  auto unpack = [&](int s) {
+    b[s] = T::minus(T::values(next.w[s & 1][s >> 1]), offset_of(next.sz[s * GPT / 8]));
+  };
 #pragma unroll
-  for (int q = 0; q < kLoads; ++q) copy(0, 0, q);
-  fetch(0);
-  for (int kt = 0; kt < a.k_tiles; ++kt) {
+  for (int s = 0; s < 8; ++s) unpack(s);
+#pragma unroll
+  for (int g = 0; g < GPT; ++g) scale[g] = scale_of(next.sz[g], a.scales_f16);
+  // A block is a group's chain of matrix instructions for 32 rows. Its sums p go to the accumulators
+  // under the next block's chain, and a step's codes are unpacked for the next step behind their last use,
+  // so that every matrix instruction has its share of vector ones; rows are read kReads ahead.
+  constexpr int kChain = 8 / GPT, kBlocks = 4 * GPT, kReads = GPT == 4 ? 4 : 2;
+  f32x16_t p[2] = {};
+  float p_scale = 0.f;  // of the block whose sums are waiting
+  for (int kt = begin; kt <= last; ++kt) {
     const int stage = kt & 1;
-    vec8 b[8];
-#pragma unroll
-    for (int s = 0; s < 8; ++s) b[s] = T::values(w[s & 1][s >> 1]);
-    float scale[GPT];
-#pragma unroll
-    for (int g = 0; g < GPT; ++g) scale[g] = scale_of(sz[g], a.scales_f16);
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this step's rows have landed
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this step's rows and the next one's codes are here
     __syncthreads();
-    if (kt + 1 < steps) {
+    next = coming;
+    fetch(coming, kt + 2);
+    if (kt + 1 < steps) copy(stage ^ 1, kt + 1);
+    vec8 x[kReads + 1];
 #pragma unroll
-      for (int q = 0; q < kLoads; ++q) copy(stage ^ 1, kt + 1, q);
-    }
-    if (kt + 1 < a.k_tiles) fetch(kt + 1);
+    for (int c = 0; c < kReads; ++c) x[c] = read(stage, 0, c);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int blk = 0; blk < kBlocks; ++blk) {
+      const int i = blk / GPT, g = blk % GPT, prev = (blk + kBlocks - 1) % kBlocks / GPT;
+      f32x16_t q = {};
 #pragma unroll
-      for (int g = 0; g < GPT; ++g) {
-        f32x16_t p = {};
+      for (int c = 0; c < kChain; ++c) {
+        const int s = g * kChain + c, at = blk * kChain + c, ahead = at + kReads;
+        if (ahead < kBlocks * kChain) x[ahead % (kReads + 1)] = read(stage, ahead / 8, ahead % 8);
+        __builtin_amdgcn_sched_barrier(0);
+        q = mma32<DT>(x[at % (kReads + 1)], b[s], q);
 #pragma unroll
-        for (int s = g * (8 / GPT); s < (g + 1) * (8 / GPT); ++s) p = mma32<DT>(read(stage, i, s), b[s], p);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][r] = fmaf(scale[g], p[r], acc[i][r]);
+        for (int r = c * 16 / kChain; r < (c + 1) * 16 / kChain; ++r)
+          acc[prev][r] = fmaf(p_scale, p[(blk & 1) ^ 1][r], acc[prev][r]);
+        if (i == 3) unpack(s);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      p[blk & 1] = q;
+      p_scale = scale[g];
+      if (i == 3) scale[g] = scale_of(next.sz[g], a.scales_f16);
     }
   }
-  // The offsets' share, 32 groups a step.
-  using B = W4<SB_DTYPE_BF16>;
-  for (int blk = 0; blk < a.sum_blocks; ++blk) {
-    const int kt = a.k_tiles + blk, stage = kt & 1;
-    B::vec8 z[2][2];  // [16 groups][upper, lower part of -(16 + zero) scale]
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t hi[4], lo[4];
+  for (int r = 0; r < 16; ++r) acc[3][r] = fmaf(p_scale, p[1][r], acc[3][r]);
+  // bf16: the offsets' share, 32 groups a step.
+  if constexpr (!T::kExact) {
+    using B = W4<SB_DTYPE_BF16>;
+    for (int kt = max(begin, a.k_tiles); kt < steps; ++kt) {
+      const int blk = kt - a.k_tiles, stage = kt & 1;
+      B::vec8 z[2][2];  // [16 groups][upper, lower part of -(16 + zero) scale]
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int g = blk * 32 + 16 * h + 8 * lg + e;
-        const uint32_t t = table[static_cast<int64_t>(min(g, a.k_tiles * GPT - 1)) * 16];
-        const float v = -offset_of(t) * scale_of(t, a.scales_f16);
-        const uint32_t up = f32_to_bf16(v), low = f32_to_bf16(v - bf16_to_f32(static_cast<uint16_t>(up)));
-        if (e & 1) hi[e >> 1] |= up << 16, lo[e >> 1] |= low << 16;
-        else hi[e >> 1] = up, lo[e >> 1] = low;
-      }
-      const u32x4_t hv = {hi[0], hi[1], hi[2], hi[3]}, lv = {lo[0], lo[1], lo[2], lo[3]};
-      z[h][0] = __builtin_bit_cast(B::vec8, hv);
-      z[h][1] = __builtin_bit_cast(B::vec8, lv);
-    }
-    __builtin_amdgcn_s_waitcnt(0x0F70);
-    __syncthreads();
-    if (kt + 1 < steps) {
+      for (int h = 0; h < 2; ++h) {
+        uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int q = 0; q < kLoads; ++q) copy(stage ^ 1, kt + 1, q);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int part = 0; part < 3; ++part)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const auto s = __builtin_bit_cast(B::vec8, read(stage, i, 2 * part + h));
-          acc[i] = mma32<SB_DTYPE_BF16>(s, z[h][0], acc[i]);
-          if (part < 2) acc[i] = mma32<SB_DTYPE_BF16>(s, z[h][1], acc[i]);
+        for (int e = 0; e < 8; ++e) {
+          const int g = blk * 32 + 16 * h + 8 * lg + e;
+          const uint32_t t = table[static_cast<int64_t>(min(g, a.k_tiles * GPT - 1)) * 16];
+          const float v = -offset_of(t) * scale_of(t, a.scales_f16);
+          const uint32_t up = f32_to_bf16(v), low = f32_to_bf16(v - bf16_to_f32(static_cast<uint16_t>(up)));
+          if (e & 1) hi[e >> 1] |= up << 16, lo[e >> 1] |= low << 16;
+          else hi[e >> 1] = up, lo[e >> 1] = low;
         }
+        const u32x4_t hv = {hi[0], hi[1], hi[2], hi[3]}, lv = {lo[0], lo[1], lo[2], lo[3]};
+        z[h][0] = __builtin_bit_cast(B::vec8, hv);
+        z[h][1] = __builtin_bit_cast(B::vec8, lv);
+      }
+      w4_wait_vm<0>();
+      __syncthreads();
+      if (kt + 1 < steps) copy(stage ^ 1, kt + 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int part = 0; part < 3; ++part)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const auto s = __builtin_bit_cast(B::vec8, read(stage, i, 2 * part + h));
+            acc[i] = mma32<SB_DTYPE_BF16>(s, z[h][0], acc[i]);
+            if (part < 2) acc[i] = mma32<SB_DTYPE_BF16>(s, z[h][1], acc[i]);
+          }
+    }
   }
 
+  if (a.part) {  // (uniform)
+    store_part(a, acc, slice, m0, static_cast<int>(f0) + 32 * wave + lq, lg);
+    return;
+  }
   // Out: through LDS, so that a row's features are stored together.
   __syncthreads();
   uint16_t* tile = ring[0];
@@ -472,7 +702,7 @@ int64_t table_step(int64_t group) { return group % 128 == 0 ? 128 : group % 64 =
 
 const char* shape_fault(int64_t n, int64_t k, int64_t group) {
   if (n <= 0 || k <= 0 || group <= 0) return "sizes must be positive";
-  if (n > 0x7fffffe0 || k > 0x7fffff00) return "size past 32 bits";
+  if (n > 0x7fffffe0 || k > kInputsMax) return "size past its limit";
   if (group % 32 || k % group) return "the group must be a multiple of 32 that divides the inputs";
   return nullptr;
 }
@@ -542,17 +772,65 @@ extern "C" int sb_w4_dequantize(void* out, const void* packed, const void* table
 
 namespace sb {
 namespace {
-// Rows from which a call takes 128 x 128 tiles.
-constexpr int64_t kTiledRows = 65;
+
 int64_t sum_blocks(int64_t k, int64_t group) { return tiles(tiles(k, kTileK) * (kTileK / table_step(group)), 32); }
+
+// How a call runs: few rows (workgroups of R rows and 16 J features), or 128 x 128 tiles with the steps
+// (tiles of inputs, and of sums) in `splits` slices.
+struct W4Plan {
+  bool tiled;
+  int r, j;
+  int splits, split_steps, sum_blocks;
+};
+
+// Up to 64 rows take the few-rows kernel: R the smallest that holds them, J = 2 where that leaves enough
+// workgroups. More rows take what the model below says is faster, in us for K inputs on 256 CUs. Few rows,
+// R = 64: 2.5 + rounds (0.5 + 1.5 K / 1024), a round a workgroup per CU. Tiles: 3, the sums' launch 4
+// (bf16), a step 1.08 with one workgroup a CU and 0.85 each with more; slices: the merge's launch 4 and
+// their traffic. Measured, few rows against tiles in their best split: 3584 -> 4608, 128 rows 15.1 and
+// 22.7 us, 256 rows 22.9 and 26.1; 18944 -> 3584 (groups of 64), 128 rows 35.6 and 40.8, 192 rows 63.0
+// and 56.4; 3584 -> 37888, 96 rows 72.1 and 52.8; 896 -> 1152, 256 rows 5.3 and 14.3.
+W4Plan w4_plan(int64_t m, int64_t n, int64_t k, int64_t group, int32_t dtype) {
+  W4Plan p = {};
+  const int64_t nt = tiles(n, kTileN), kt = tiles(k, kTileK);
+  p.r = m <= 4 ? 4 : m <= 16 ? 16 : m <= 32 ? 32 : 64;
+  const int64_t gy = tiles(m, p.r);
+  const auto rounds = [](int64_t wgs) { return tiles(wgs, 256); };
+  // (a workgroup of 32 features takes about a fifth longer than one of 16)
+  p.j = rounds(tiles(nt, 2) * gy) * 1.2 < static_cast<double>(rounds(nt * gy)) ? 2 : 1;
+  p.splits = 1;
+  p.split_steps = static_cast<int>(kt);
+  double best = 0.0;  // us, of more than 64 rows
+  if (m > 64)
+    best = 2.5 + static_cast<double>(rounds(tiles(nt, p.j) * gy)) * (0.5 + 1.5 * static_cast<double>(k) / 1024);
+  const int64_t blocks = dtype == SB_DTYPE_BF16 ? sum_blocks(k, group) : 0;
+  const int64_t steps = kt + blocks, grid = tiles(m, kBM) * tiles(n, kBN);
+  for (int64_t s = 1; m > 64 && s <= 32 && (s == 1 || 2 * s <= steps); ++s) {
+    const int64_t per = tiles(steps, s), slices = tiles(steps, per);
+    if (slices != s) continue;
+    const double load = static_cast<double>(rounds(grid * s));
+    double t = 3.0 + (blocks ? 4.0 : 0.0) + static_cast<double>(per) * (load <= 1.0 ? 1.08 : 0.85 * load);
+    if (s > 1) t += 4.0 + static_cast<double>(s * m * n) * 8.0 / 6e6;
+    if (t >= best) continue;
+    best = t;
+    p.tiled = true;
+    p.splits = static_cast<int>(s);
+    p.split_steps = static_cast<int>(per);
+    p.sum_blocks = static_cast<int>(blocks);
+  }
+  return p;
+}
+int64_t sums_bytes(const W4Plan& p, int64_t m) { return m * p.sum_blocks * 256; }
+
 }  // namespace
 }  // namespace sb
 
 extern "C" int64_t sb_w4_linear_workspace_size(int64_t num_rows, int64_t out_features, int64_t in_features,
-                                               int64_t group) {
+                                               int64_t group, int32_t dtype) {
   using namespace sb;
-  if (num_rows < kTiledRows || shape_fault(out_features, in_features, group)) return 0;
-  return num_rows * sum_blocks(in_features, group) * 256;
+  if (num_rows <= 0 || shape_fault(out_features, in_features, group)) return 0;
+  const W4Plan p = w4_plan(num_rows, out_features, in_features, group, dtype);
+  return sums_bytes(p, num_rows) + (p.splits > 1 ? p.splits * num_rows * out_features * 4 : 0);
 }
 
 extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const void* table,
@@ -569,7 +847,8 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
   if (!y || !x || !packed || !table) return fail(fn, "null pointer");
   if (const char* why = shape_fault(out_features, in_features, group)) return fail(fn, why);
   if (num_rows < 0) return fail(fn, "sizes must be positive");
-  if (num_rows > 0x7fffff00) return fail(fn, "size past 32 bits");
+  if (num_rows > 0x7fffff00) return fail(fn, "size past its limit");
+  if (x_stride < 0 || x_stride > kInputsMax) return fail(fn, "row stride past its limit");
   if (reinterpret_cast<uintptr_t>(x) % 16 || x_stride * 2 % 16)
     return fail(fn, "rows of x must be 16-byte aligned");
   W4Args a = {};
@@ -587,42 +866,67 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
   a.scales_f16 = scale_dtype == SB_DTYPE_F16;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int gpt = static_cast<int>(kTileK / table_step(group));
-  if (num_rows >= kTiledRows) {
-    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
-        workspace_bytes < sb_w4_linear_workspace_size(num_rows, out_features, in_features, group))
-      return fail(fn, "workspace too small or not 16-byte aligned");
-    a.sums = static_cast<const char*>(workspace);
-    a.sum_blocks = static_cast<int>(sum_blocks(in_features, group));
-    a.wide_out = reinterpret_cast<uintptr_t>(y) % 16 == 0 && a.y_row % 16 == 0;
-    const int64_t work = num_rows * a.sum_blocks * 32 * (table_step(group) / 8);
-    const int64_t grid = tiles(num_rows, kBM) * tiles(out_features, kBN);
-    if (tiles(work, 256) > 0x7fffffff || grid > 0x7fffffff) return fail(fn, "grid too large");
+  const W4Plan plan = w4_plan(num_rows, out_features, in_features, group, dtype);
+  const int64_t need = sb_w4_linear_workspace_size(num_rows, out_features, in_features, group, dtype);
+  if (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < need))
+    return fail(fn, "workspace too small or not 16-byte aligned");
+  a.wide_out = reinterpret_cast<uintptr_t>(y) % 16 == 0 && a.y_row % 16 == 0;
+  a.sums = static_cast<const char*>(workspace);
+  a.sum_blocks = plan.sum_blocks;
+  a.splits = plan.splits;
+  a.split_steps = plan.split_steps;
+  if (plan.splits > 1)
+    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + sums_bytes(plan, num_rows));
+  if (!plan.tiled) {
+    const int64_t gy = tiles(num_rows, plan.r);
+    if (gy > 65535) return fail(fn, "too many rows");
+    const int64_t nt = tiles(out_features, kTileN);
+    // Eight waves with two steps in flight where a CU's LDS holds two such workgroups, else one step
+    // (waves of the others run meanwhile).
+#define SB_W4(DT, R, J, GPT)                                                                          \
+  if (dtype == DT && plan.r == R && plan.j == J && gpt == GPT) {                                      \
+    constexpr int kAhead = 2 * kRowWaves * RowsStage<R, J, GPT>::kBytes <= 80 * 1024 ? 2 : 1;         \
+    const dim3 grid(static_cast<unsigned>(tiles(nt, J)), static_cast<unsigned>(gy));                  \
+    SB_LAUNCH("w4_rows", (w4_rows_kernel<DT, R, J, GPT, kRowWaves, kAhead>), grid, dim3(64 * kRowWaves), \
+              st, a);                                                                                 \
+  }
+#define SB_W4_(DT, J)                                          \
+  SB_W4(DT, 4, J, 1) SB_W4(DT, 4, J, 2) SB_W4(DT, 4, J, 4)     \
+  SB_W4(DT, 16, J, 1) SB_W4(DT, 16, J, 2) SB_W4(DT, 16, J, 4)  \
+  SB_W4(DT, 32, J, 1) SB_W4(DT, 32, J, 2) SB_W4(DT, 32, J, 4)  \
+  SB_W4(DT, 64, J, 1) SB_W4(DT, 64, J, 2) SB_W4(DT, 64, J, 4)
+    SB_W4_(SB_DTYPE_BF16, 1) SB_W4_(SB_DTYPE_BF16, 2)
+    SB_W4_(SB_DTYPE_F16, 1) SB_W4_(SB_DTYPE_F16, 2)
+#undef SB_W4_
+#undef SB_W4
+    return check_launch(fn);
+  }
+  const int64_t grid_tiles = tiles(num_rows, kBM) * tiles(out_features, kBN);
+  const int64_t grid = grid_tiles * plan.splits;
+  if (grid > 0x7fffffff) return fail(fn, "grid too large");
+  a.tiles = static_cast<uint32_t>(grid_tiles);
+  const int64_t work = num_rows * a.sum_blocks * 32 * (table_step(group) / 8);
+  if (tiles(work, 256) > 0x7fffffff) return fail(fn, "grid too large");
 #define SB_W4(DT, GPT)                                                                                \
   if (dtype == DT && gpt == GPT) {                                                                    \
-    SB_LAUNCH("w4_sums", (w4_sums_kernel<DT, kTileK / GPT>), dim3(static_cast<unsigned>(tiles(work, 256))), \
+    if (a.sum_blocks)                                                                                 \
+      SB_LAUNCH("w4_sums", (w4_sums_kernel<DT, kTileK / GPT>), dim3(static_cast<unsigned>(tiles(work, 256))), \
               dim3(256), st, static_cast<uint16_t*>(workspace), a.x, a.x_row, a.num_rows, a.k,        \
               a.sum_blocks);                                                                          \
     SB_LAUNCH("w4_tiles", (w4_tiles_kernel<DT, GPT>), dim3(static_cast<unsigned>(grid)), dim3(256), st, a); \
   }
-    SB_W4(SB_DTYPE_BF16, 1) SB_W4(SB_DTYPE_BF16, 2) SB_W4(SB_DTYPE_BF16, 4)
-    SB_W4(SB_DTYPE_F16, 1) SB_W4(SB_DTYPE_F16, 2) SB_W4(SB_DTYPE_F16, 4)
+  SB_W4(SB_DTYPE_BF16, 1) SB_W4(SB_DTYPE_BF16, 2) SB_W4(SB_DTYPE_BF16, 4)
+  SB_W4(SB_DTYPE_F16, 1) SB_W4(SB_DTYPE_F16, 2) SB_W4(SB_DTYPE_F16, 4)
 #undef SB_W4
-    return check_launch(fn);
+  if (plan.splits > 1) {
+    const int vec = out_features % 4 == 0 ? 4 : 1;
+    const int64_t gx = tiles(num_rows * tiles(out_features, vec), 256);
+    if (gx > 0x7fffffff) return fail(fn, "grid too large");
+#define SB_W4(DT, VEC)                                                                                \
+  if (dtype == DT && vec == VEC)                                                                      \
+    SB_LAUNCH("w4_merge", (w4_merge_kernel<DT, VEC>), dim3(static_cast<unsigned>(gx)), dim3(256), st, a);
+    SB_W4(SB_DTYPE_BF16, 4) SB_W4(SB_DTYPE_BF16, 1) SB_W4(SB_DTYPE_F16, 4) SB_W4(SB_DTYPE_F16, 1)
+#undef SB_W4
   }
-  const int mi = num_rows <= 16 ? 1 : num_rows <= 32 ? 2 : 4;
-  const int64_t gy = tiles(num_rows, 16 * mi);
-  if (gy > 65535) return fail(fn, "too many rows");
-  const dim3 grid(static_cast<unsigned>(tiles(out_features, kTileN)), static_cast<unsigned>(gy));
-#define SB_W4(DT, MI, GPT)                                                                            \
-  if (dtype == DT && mi == MI && gpt == GPT)                                                          \
-    SB_LAUNCH("w4_rows", (w4_rows_kernel<DT, MI, GPT>), grid, dim3(64 * kWaves), st, a);
-#define SB_W4_(DT)                                    \
-  SB_W4(DT, 1, 1) SB_W4(DT, 1, 2) SB_W4(DT, 1, 4)     \
-  SB_W4(DT, 2, 1) SB_W4(DT, 2, 2) SB_W4(DT, 2, 4)     \
-  SB_W4(DT, 4, 1) SB_W4(DT, 4, 2) SB_W4(DT, 4, 4)
-  SB_W4_(SB_DTYPE_BF16)
-  SB_W4_(SB_DTYPE_F16)
-#undef SB_W4_
-#undef SB_W4
   return check_launch(fn);
 }

@@ -23,6 +23,7 @@ from .paged_cache import _device, _recorded
 
 __all__ = ["QuantizedLinear", "quantized_linear"]
 
+_ROW_STRIDE_MAX = 1 << 22  # elements (the C ABI's limit, and that of in_features)
 _16BIT = (torch.bfloat16, torch.float16)
 
 
@@ -156,16 +157,17 @@ def quantized_linear(
         out_rows = flat.stride(0)
     if num:
         step = rows.stride(0)
-        if rows.stride(1) != 1 or step % 8 or rows.data_ptr() % 16:
+        if rows.stride(1) != 1 or step % 8 or step > _ROW_STRIDE_MAX or rows.data_ptr() % 16:
             rows = rows.clone(memory_format=torch.contiguous_format)
             step = k
         if bias is not None and bias.stride(0) != 1:
             bias = bias.contiguous()
-        ws_bytes = _workspace_bytes(num, n, k, weight.group)
+        dt = _lib.SB_DTYPE[dtype]
+        ws_bytes = _workspace_bytes(num, n, k, weight.group, dt)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         _lib.launch(dev, "sb_w4_linear", out.data_ptr(), rows.data_ptr(), weight._packed.data_ptr(),
                     weight._table.data_ptr(), _lib.ptr(bias), num, n, k, weight.group, step, out_rows,
-                    _lib.ptr(ws), ws_bytes, weight._code, _lib.SB_DTYPE[dtype])
+                    _lib.ptr(ws), ws_bytes, weight._code, dt)
     if new and (x.requires_grad or bias is not None and bias.requires_grad):
         return _recorded("quantized_linear", out, x, *(() if bias is None else (bias,)))
     return out

@@ -116,8 +116,10 @@ def _unpack(**over):
     (_linear, dict(t=None), b"null"), (_linear, dict(m=-1), b"positive"), (_linear, dict(n=0), b"positive"),
     (_linear, dict(g=48), b"multiple of 32"), (_linear, dict(k=100), b"multiple of 32"),
     (_linear, dict(x=FAKE + 2), b"aligned"), (_linear, dict(xs=132), b"aligned"),
-    (_linear, dict(m=1 << 31), b"32 bits"), (_linear, dict(n=1 << 31), b"32 bits"),
-    (_linear, dict(m=4096), b"workspace"), (_linear, dict(m=4096, ws=FAKE, wsb=100), b"workspace"),
+    (_linear, dict(m=1 << 31), b"limit"), (_linear, dict(n=1 << 31), b"limit"),
+    (_linear, dict(k=(1 << 22) + 64), b"limit"), (_linear, dict(xs=(1 << 22) + 8), b"limit"),
+    (_linear, dict(m=4096, n=8192, k=1024, xs=1024), b"workspace"),
+    (_linear, dict(m=4096, n=8192, k=1024, xs=1024, ws=FAKE, wsb=100), b"workspace"),
     (_pack, dict(c=None), b"null"), (_pack, dict(g=16), b"multiple of 32"), (_pack, dict(k=0), b"positive"),
     (_pack, dict(w=FAKE + 8), b"aligned"), (_unpack, dict(dt=3), b"invalid dtype"),
     (_unpack, dict(sdt=3), b"scales"), (_unpack, dict(o=None), b"null"),
@@ -134,7 +136,7 @@ def test_sizes():
     assert size("sb_w4_table_size", 16, 128, 128) == 64
     assert size("sb_w4_table_size", 17, 160, 32) == 2 * 8 * 64
     assert size("sb_w4_table_size", 16, 192, 96) == 8 * 64
-    assert size("sb_w4_linear_workspace_size", 4, 32, 128, 64) == 0
-    assert size("sb_w4_linear_workspace_size", 4096, 32, 128, 64) > 0
-    assert size("sb_w4_linear_workspace_size", 4096, 32, 128, 48) == 0
+    assert size("sb_w4_linear_workspace_size", 4, 32, 128, 64, 2) == 0
+    assert size("sb_w4_linear_workspace_size", 4096, 8192, 1024, 64, 2) > 0
+    assert size("sb_w4_linear_workspace_size", 4096, 32, 128, 48, 2) == 0
     assert _linear(m=0, x=None) == _lib.SB_OK
