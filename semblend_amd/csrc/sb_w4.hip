@@ -39,23 +39,28 @@ __device__ __forceinline__ uint32_t vector_constant(uint32_t x) {
   return x;
 }
 
+// The eight codes of a word as 16-bit floats kBase + c: pair p's lie at bits 4p + 3 .. 4p + 6 of both
+// halves (modulo 32) and go to bits 3 .. 6 of kBase.
+__device__ __forceinline__ u32x4_t w4_words(uint32_t w, uint32_t base_bits) {
+  const uint32_t m = scalar_constant(0x00780078u), base = vector_constant(base_bits);
+  const u32x4_t r = {(w & m) | base, ((w >> 4) & m) | base, ((w >> 8) & m) | base,
+                     (__builtin_amdgcn_alignbit(w, w, 12) & m) | base};
+  return r;
+}
+
 template <int DT> struct W4;
 template <> struct W4<SB_DTYPE_BF16> {
   using vec8 = bf16x8_t;
   static constexpr uint32_t kOnes = 0x3f803f80u;
   // There is no packed bf16 addition: the values stay 16 + c, and the offset goes to the sums.
+  static constexpr float kBase = 16.f;
   static constexpr bool kExact = false;
   __device__ __forceinline__ static vec8 minus(vec8 v, float) { return v; }
   __device__ __forceinline__ static f32x4_t mma(vec8 a, vec8 b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
-  // 16 + c for the eight codes of a word: pair p's codes lie at bits 4p + 3 .. 4p + 6 of both halves
-  // (modulo 32).
   __device__ __forceinline__ static vec8 values(uint32_t w) {
-    const uint32_t m = scalar_constant(0x00780078u), base = vector_constant(0x41804180u);
-    const u32x4_t r = {((w) & m) | base, ((w >> 4) & m) | base, ((w >> 8) & m) | base,
-                       ((__builtin_amdgcn_alignbit(w, w, 12)) & m) | base};
-    return __builtin_bit_cast(vec8, r);
+    return __builtin_bit_cast(vec8, w4_words(w, 0x41804180u));
   }
   __device__ __forceinline__ static uint16_t round(float f) { return f32_to_bf16(f); }
   __device__ __forceinline__ static float value(uint16_t h) { return bf16_to_f32(h); }
@@ -63,7 +68,9 @@ template <> struct W4<SB_DTYPE_BF16> {
 template <> struct W4<SB_DTYPE_F16> {
   using vec8 = f16x8_t;
   static constexpr uint32_t kOnes = 0x3c003c00u;
-  // (16 + c) - (16 + zero) = c - zero, exact: one packed addition for two codes.
+  // Ten bits of mantissa: the same bits are 128 + c. (128 + c) - (128 + zero) is exact too, one packed
+  // addition for two codes.
+  static constexpr float kBase = 128.f;
   static constexpr bool kExact = true;
   __device__ __forceinline__ static vec8 minus(vec8 v, float off) {
     const _Float16 h = static_cast<_Float16>(off);
@@ -74,21 +81,20 @@ template <> struct W4<SB_DTYPE_F16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
   __device__ __forceinline__ static vec8 values(uint32_t w) {
-    const uint32_t m = scalar_constant(0x03c003c0u), base = vector_constant(0x4c004c00u);
-    const u32x4_t r = {((w << 3) & m) | base, ((w >> 1) & m) | base, ((w >> 5) & m) | base,
-                       ((__builtin_amdgcn_alignbit(w, w, 9)) & m) | base};
-    return __builtin_bit_cast(vec8, r);
+    return __builtin_bit_cast(vec8, w4_words(w, 0x58005800u));
   }
   __device__ __forceinline__ static uint16_t round(float f) { return f32_to_f16(f); }
   __device__ __forceinline__ static float value(uint16_t h) { return f16_to_f32(h); }
 };
 
-// The scale and 16 + zero of a table word.
+// The scale of a table word, and DT's kBase + zero.
 __device__ __forceinline__ float scale_of(uint32_t w, bool f16) {
   const float h = f16_to_f32(static_cast<uint16_t>(w));
   return f16 ? h : __uint_as_float(w << 16);
 }
-__device__ __forceinline__ float offset_of(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+template <int DT> __device__ __forceinline__ float offset_of(uint32_t w) {
+  return __uint_as_float(w & 0xffff0000u) + (W4<DT>::kBase - 16.f);
+}
 
 struct W4Args {
   char* y;
@@ -120,6 +126,15 @@ __device__ __forceinline__ void w4_dma(const void* src, uint32_t lds_wave) {
       "s_mov_b32 m0, %0\n\t"
       "s_nop 0\n\t"
       "global_load_lds_dwordx4 %1, off"
+      :
+      : "s"(lds_wave), "v"(src)
+      : "memory", "m0");
+}
+__device__ __forceinline__ void w4_dma_once(const void* src, uint32_t lds_wave) {  // nontemporal
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, off nt"
       :
       : "s"(lds_wave), "v"(src)
       : "memory", "m0");
@@ -172,7 +187,6 @@ __device__ __forceinline__ uint32_t w4_lds_addr(const void* p) {
 // lanes as the matrix operand has them (64 bytes of 16 rows), the rows alone took twice as long as all
 // else (16 rows of 3584 -> 4608: 9.2 us, with one row's address for all of them 4.9). GPT: groups of a
 // tile of inputs.
-constexpr int kRowWaves = 8;
 template <int R, int J, int GPT> struct RowsStage {
   static constexpr int kMi = R < 16 ? 1 : R / 16;
   static constexpr int kTableCopies = (J * GPT + 3) / 4;
@@ -180,12 +194,16 @@ template <int R, int J, int GPT> struct RowsStage {
   static constexpr int kCopies = J + kTableCopies + kRowCopies;
   static constexpr int kBytes = J * 1024 + kTableCopies * 256 + R * 256;
 };
-template <int DT, int R, int J, int GPT, int WAVES, int AHEAD>
+// ONCE: codes nontemporal.
+template <int DT, int R, int J, int GPT, int WAVES, int AHEAD, bool ONCE>
 __global__ __launch_bounds__(64 * WAVES, 2) void w4_rows_kernel(const W4Args a) {
   using T = W4<DT>;
   using S = RowsStage<R, J, GPT>;
   using vec8 = typename T::vec8;
   constexpr int MI = S::kMi;
+  // (up to 32 rows: the products with ones cost less than the additions of exact differences; one row of
+  // 4096 -> 131072 in fp16 46 against 55-58 us)
+  constexpr bool kExact = T::kExact && MI == 4;
   constexpr int kRing = WAVES * AHEAD * S::kBytes, kParts = WAVES * MI * J * 1024;
   __shared__ __align__(16) char smem[kRing > kParts ? kRing : kParts];
   const int lane = threadIdx.x & 63;
@@ -217,7 +235,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void w4_rows_kernel(const W4Args a) 
   auto copy = [&](int stage, int kt) {
     uint32_t at = mine_lds + stage * S::kBytes;
 #pragma unroll
-    for (int j = 0; j < J; ++j, at += 1024) w4_dma(codes[j] + static_cast<int64_t>(kt) * 64, at);
+    for (int j = 0; j < J; ++j, at += 1024) {
+      if (ONCE) w4_dma_once(codes[j] + static_cast<int64_t>(kt) * 64, at);
+      else w4_dma(codes[j] + static_cast<int64_t>(kt) * 64, at);
+    }
 #pragma unroll
     for (int t = 0; t < S::kTableCopies; ++t, at += 256)
       w4_dma4(table[t] + static_cast<int64_t>(kt) * (GPT * 16), at);
@@ -245,14 +266,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void w4_rows_kernel(const W4Args a) 
       for (int j = 0; j < J; ++j) {
         const uint32_t sz =
             *reinterpret_cast<const uint32_t*>(at + J * 1024 + ((j * GPT + g) * 16 + (lane & 15)) * 4);
-        s[j] = scale_of(sz, a.scales_f16), off[j] = offset_of(sz);
+        s[j] = scale_of(sz, a.scales_f16), off[j] = offset_of<DT>(sz);
       }
       f32x4_t p[MI][J] = {}, sum[MI] = {};
 #pragma unroll
       for (int q = g * kSteps; q < (g + 1) * kSteps; ++q) {
         vec8 b[J];
 #pragma unroll
-        for (int j = 0; j < J; ++j) b[j] = T::minus(T::values(w[j][q]), off[j]);
+        for (int j = 0; j < J; ++j) {
+          b[j] = T::values(w[j][q]);
+          if (kExact) b[j] = T::minus(b[j], off[j]);
+        }
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
           const int r = R < 16 ? lane & 3 : 16 * i + (lane & 15);
@@ -260,7 +284,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void w4_rows_kernel(const W4Args a) 
               *reinterpret_cast<const vec8*>(xs + r * 256 + (((4 * q + (lane >> 4)) ^ r) & 15) * 16);
 #pragma unroll
           for (int j = 0; j < J; ++j) p[i][j] = T::mma(x, b[j], p[i][j]);
-          if (!T::kExact) sum[i] = T::mma(x, ones, sum[i]);
+          if (!kExact) sum[i] = T::mma(x, ones, sum[i]);
         }
       }
 #pragma unroll
@@ -269,7 +293,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void w4_rows_kernel(const W4Args a) 
         for (int j = 0; j < J; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            acc[i][j][r] = fmaf(s[j], T::kExact ? p[i][j][r] : fmaf(-off[j], sum[i][r], p[i][j][r]),
+            acc[i][j][r] = fmaf(s[j], kExact ? p[i][j][r] : fmaf(-off[j], sum[i][r], p[i][j][r]),
                                 acc[i][j][r]);
       // (64 rows: a group's sums go to the accumulators now; left to the compiler those of all groups
       // wait behind the next copies, in more registers than there are)
@@ -514,7 +538,7 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(const W4Args a) {
   vec8 b[8];
   float scale[GPT];
   auto unpack = [&](int s) {
-    b[s] = T::minus(T::values(next.w[s & 1][s >> 1]), offset_of(next.sz[s * GPT / 8]));
+    b[s] = T::minus(T::values(next.w[s & 1][s >> 1]), offset_of<DT>(next.sz[s * GPT / 8]));
   };
 #pragma unroll
   for (int s = 0; s < 8; ++s) unpack(s);
@@ -572,7 +596,7 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(const W4Args a) {
         for (int e = 0; e < 8; ++e) {
           const int g = blk * 32 + 16 * h + 8 * lg + e;
           const uint32_t t = table[static_cast<int64_t>(min(g, a.k_tiles * GPT - 1)) * 16];
-          const float v = -offset_of(t) * scale_of(t, a.scales_f16);
+          const float v = -offset_of<SB_DTYPE_BF16>(t) * scale_of(t, a.scales_f16);
           const uint32_t up = f32_to_bf16(v), low = f32_to_bf16(v - bf16_to_f32(static_cast<uint16_t>(up)));
           if (e & 1) hi[e >> 1] |= up << 16, lo[e >> 1] |= low << 16;
           else hi[e >> 1] = up, lo[e >> 1] = low;
@@ -683,7 +707,7 @@ __global__ __launch_bounds__(256) void w4_unpack_kernel(char* out, const uint32_
   const int lane = static_cast<int>(f - nt * kTileN) + 16 * ((in & 31) >> 3);
   uint32_t w = codes[((nt * k_tiles + kt) * 64 + lane) * 4 + (in >> 5)];
   const uint32_t t = table[((nt * k_tiles + kt) * gpt + in * gpt / kTileK) * 16 + (lane & 15)];
-  const float s = scale_of(t, scales_f16), off = offset_of(t) - 16.f;
+  const float s = scale_of(t, scales_f16), off = offset_of<SB_DTYPE_BF16>(t) - 16.f;
   w = w >> 3 | w << 29;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -785,7 +809,7 @@ struct W4Plan {
 
 // Up to 64 rows take the few-rows kernel: R the smallest that holds them, J = 2 where that leaves enough
 // workgroups. More rows take what the model below says is faster, in us for K inputs on 256 CUs. Few rows,
-// R = 64: 2.5 + rounds (0.5 + 1.5 K / 1024), a round a workgroup per CU. Tiles: 3, the sums' launch 4
+// R = 64: 2.5 + rounds (0.5 + 1.85 K / 1024), a round a workgroup per CU. Tiles: 3, the sums' launch 4
 // (bf16), a step 1.08 with one workgroup a CU and 0.85 each with more; slices: the merge's launch 4 and
 // their traffic. Measured, few rows against tiles in their best split: 3584 -> 4608, 128 rows 15.1 and
 // 22.7 us, 256 rows 22.9 and 26.1; 18944 -> 3584 (groups of 64), 128 rows 35.6 and 40.8, 192 rows 63.0
@@ -802,7 +826,7 @@ W4Plan w4_plan(int64_t m, int64_t n, int64_t k, int64_t group, int32_t dtype) {
   p.split_steps = static_cast<int>(kt);
   double best = 0.0;  // us, of more than 64 rows
   if (m > 64)
-    best = 2.5 + static_cast<double>(rounds(tiles(nt, p.j) * gy)) * (0.5 + 1.5 * static_cast<double>(k) / 1024);
+    best = 2.5 + static_cast<double>(rounds(tiles(nt, p.j) * gy)) * (0.5 + 1.85 * static_cast<double>(k) / 1024);
   const int64_t blocks = dtype == SB_DTYPE_BF16 ? sum_blocks(k, group) : 0;
   const int64_t steps = kt + blocks, grid = tiles(m, kBM) * tiles(n, kBN);
   for (int64_t s = 1; m > 64 && s <= 32 && (s == 1 || 2 * s <= steps); ++s) {
@@ -881,14 +905,29 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
     const int64_t gy = tiles(num_rows, plan.r);
     if (gy > 65535) return fail(fn, "too many rows");
     const int64_t nt = tiles(out_features, kTileN);
-    // Eight waves with two steps in flight where a CU's LDS holds two such workgroups, else one step
-    // (waves of the others run meanwhile).
+    // Up to 16 rows: 16 waves where a workgroup has 16 features (a CU has one or two of them then) and a
+    // tile of inputs for each wave (one row of 18944 -> 3584 9.8 -> 9.1 us, 16 rows 12.9 -> 11.8; of 896 ->
+    // 1152 2.9 and 3.0), and codes read past the caches where these cannot keep them until the next call
+    // (one row of 4096 -> 131072, 268 MB: 47.9 -> 45.2 us; 16 of 3584 -> 37888, 68 MB, 15.3 and 19.6).
+    const bool many = plan.r <= 16 && plan.j == 1 && a.k_tiles > 16;
+    const bool once = plan.r <= 16 && plan.j == 2 &&
+                      sb_w4_codes_size(out_features, in_features) >= (int64_t{192} << 20);
+    // Two steps in flight where a CU's LDS holds two such workgroups, else one (other waves run meanwhile).
+#define SB_W4_L(DT, R, J, GPT, W, ONCE)                                                               \
+  do {                                                                                                \
+    constexpr int kAhead = 2 * W * RowsStage<R, J, GPT>::kBytes <= 80 * 1024 ? 2 : 1;                 \
+    const dim3 grid(static_cast<unsigned>(tiles(nt, J)), static_cast<unsigned>(gy));                  \
+    SB_LAUNCH("w4_rows", (w4_rows_kernel<DT, R, J, GPT, W, kAhead, ONCE>), grid, dim3(64 * W), st, a); \
+  } while (0)
 #define SB_W4(DT, R, J, GPT)                                                                          \
   if (dtype == DT && plan.r == R && plan.j == J && gpt == GPT) {                                      \
-    constexpr int kAhead = 2 * kRowWaves * RowsStage<R, J, GPT>::kBytes <= 80 * 1024 ? 2 : 1;         \
-    const dim3 grid(static_cast<unsigned>(tiles(nt, J)), static_cast<unsigned>(gy));                  \
-    SB_LAUNCH("w4_rows", (w4_rows_kernel<DT, R, J, GPT, kRowWaves, kAhead>), grid, dim3(64 * kRowWaves), \
-              st, a);                                                                                 \
+    if constexpr (R <= 16) {                                                                          \
+      if (J == 1 && many) SB_W4_L(DT, R, 1, GPT, 16, false);                                          \
+      else if (J == 2 && once) SB_W4_L(DT, R, 2, GPT, 8, true);                                       \
+      else SB_W4_L(DT, R, J, GPT, 8, false);                                                          \
+    } else {                                                                                          \
+      SB_W4_L(DT, R, J, GPT, 8, false);                                                               \
+    }                                                                                                 \
   }
 #define SB_W4_(DT, J)                                          \
   SB_W4(DT, 4, J, 1) SB_W4(DT, 4, J, 2) SB_W4(DT, 4, J, 4)     \
@@ -899,6 +938,7 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
     SB_W4_(SB_DTYPE_F16, 1) SB_W4_(SB_DTYPE_F16, 2)
 #undef SB_W4_
 #undef SB_W4
+#undef SB_W4_L
     return check_launch(fn);
   }
   const int64_t grid_tiles = tiles(num_rows, kBM) * tiles(out_features, kBN);
