@@ -15,6 +15,11 @@
 namespace sb {
 namespace {
 
+// Tokens of a dense workgroup (8192 tokens of 32 / 8 heads x 128, bf16 / fp32: 1 31.8 / 61.5 us, 2 27.7 /
+// 62.3, 4 27.7 / 66.2, 8 28.5 / 70.4), rows of a scattering one (28 layers x 6963 pairs of 4 heads x 128: 64
+// 141 us, 128 145, 256 149). Rows in flight of a thread, half pairs: 2 (4: 155 us with 64 rows).
+constexpr int kDenseTokens = 2;
+constexpr int kScatterRows = 64;
 enum RotaryMode : int { ROTARY_DENSE = 0, ROTARY_SCATTER = 1, ROTARY_SHIFT = 2 };
 
 struct RotaryArgs {
@@ -65,6 +70,7 @@ __global__ __launch_bounds__(kRowThreads) void rotary_rows_kernel(
   const int j0 = blockIdx.y * a.rows_per_y;
   const int per = min(a.rows_per_y, a.rows_per_token - j0);
   const int n = per * ntok;
+  bool sines = true;
 
   // The angle of a token: its position, the way from the donor's, or its delta.
   auto angle = [&](int64_t t) -> int {
@@ -76,8 +82,10 @@ __global__ __launch_bounds__(kRowThreads) void rotary_rows_kernel(
   };
 
   if (tid < n) {
-    // neighbours in a step are the same row of consecutive tokens
-    const int jr = tid / ntok, tok = tid - jr * ntok;
+    // rows in the order of memory: a token's heads, or one head (of a layer, of K or V) of all tokens
+    const int major = tid / (MODE == ROTARY_DENSE ? per : ntok);
+    const int minor = tid - major * (MODE == ROTARY_DENSE ? per : ntok);
+    const int jr = MODE == ROTARY_DENSE ? minor : major, tok = MODE == ROTARY_DENSE ? major : minor;
     const int64_t t = t0 + tok;
     const int j = j0 + jr;
     RowRef ref = {nullptr, nullptr, nullptr, 0, 0};
@@ -113,8 +121,13 @@ __global__ __launch_bounds__(kRowThreads) void rotary_rows_kernel(
     ref.info = static_cast<uint32_t>(2 * tok * a.pairs) << 2 | (turn ? 1u : 0u);
     rows[tid] = ref;
   }
+  // (a workgroup of V rows alone turns none)
+  if (MODE == ROTARY_SCATTER) {
+    const int first = a.head_div.of(j0), last = a.head_div.of(j0 + per - 1);
+    sines = first != last || (first & 1) == 0;
+  }
   // (from the last wave down: the first ones work out the rows)
-  for (int i = kRowThreads - 1 - tid; i < ntok * a.pairs; i += kRowThreads) {
+  for (int i = kRowThreads - 1 - tid; sines && i < ntok * a.pairs; i += kRowThreads) {
     const int tok = a.pair_div.of(i), f = i - tok * a.pairs;
     double s, c;
     sincos_cw(static_cast<double>(angle(t0 + tok)) * static_cast<double>(a.inv_freq[f]), &s, &c);
@@ -125,8 +138,8 @@ __global__ __launch_bounds__(kRowThreads) void rotary_rows_kernel(
   const int rpi = kRowThreads / a.split.units;
   const int rsub = tid / a.split.units, unit = tid - rsub * a.split.units;
   if (rsub >= rpi) return;
-  turn_rows<DT, VEC, false, HALF, ONCE>(rows, n, cs, nullptr, a.split, a.head_dim, a.pairs, rsub, rpi,
-                                        unit);
+  turn_rows<DT, VEC, false, HALF, ONCE, HALF ? 2 : 4>(rows, n, cs, nullptr, a.split, a.head_dim,
+                                                       a.pairs, rsub, rpi, unit);
 }
 
 int64_t address(const void* p) { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)); }
@@ -143,11 +156,12 @@ int launch_rotary(const char* fn, RotaryArgs a, int32_t layout, int32_t dtype, i
   // Tokens of a workgroup: as many as its table of sines takes and as leave 1024 workgroups; few
   // tokens: one, and its rows spread over workgroups until there are 512.
   const int rpi = kRowThreads / a.split.units;
-  const int fit = std::min(kTokensMax, std::max(1, kTableEntries / a.pairs));
+  int fit = std::min(MODE == ROTARY_DENSE ? kDenseTokens : kTokensMax, std::max(1, kTableEntries / a.pairs));
+  if (MODE == ROTARY_DENSE) fit = std::max(1, std::min(fit, kRowsMax / a.rows_per_token));
   const int64_t units = a.num_tokens * ((a.rows_per_token + kRowsMax - 1) / kRowsMax);
   a.tokens_per_wg = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(fit, units / 1024)));
   const int64_t gx = (a.num_tokens + a.tokens_per_wg - 1) / a.tokens_per_wg;
-  int per = std::max(1, kRowsMax / a.tokens_per_wg);
+  int per = std::max(1, (MODE == ROTARY_SCATTER ? kScatterRows : kRowsMax) / a.tokens_per_wg);
   if (a.tokens_per_wg == 1) {
     const int steps = (a.rows_per_token + rpi - 1) / rpi;
     const int ny = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, 512 / gx), steps));

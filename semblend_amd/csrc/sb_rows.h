@@ -176,10 +176,6 @@ struct RowRef {
   uint32_t info;    // index of the token's sines and cosines << 2 | a 4-bit row << 1 | rotated
   uint32_t pad;
 };
-// A thread takes one unit of a row (RowSplit) of rows tid / units + k rpi (K, V, then query heads, token
-// after token), kRowsInFlight of them at a time.
-constexpr int kRowsInFlight = 4;
-
 // How a row's vectors fall to threads. Interleaved: thread u takes vector u. Half: u < P (P vectors in
 // a half) takes vectors u and u + P, the others two of the rest (the last of them maybe one).
 struct RowSplit {
@@ -194,9 +190,9 @@ struct RowSplit {
   }
 };
 
-// Rows rows[0 .. n) by a workgroup: thread `unit` of a row takes rows rsub + k rpi, kRowsInFlight of
-// them at a time. cs: cosine and sine of each (token, pair); cs64: the same in 64 bits (4-bit rows).
-template <int DT, int VEC, bool Q4, bool HALF, bool ONCE>
+// Rows rows[0 .. n) by a workgroup: thread `unit` of a row takes rows rsub + k rpi, FLIGHT of them at
+// a time. cs: cosine and sine of each (token, pair); cs64: the same in 64 bits (4-bit rows).
+template <int DT, int VEC, bool Q4, bool HALF, bool ONCE, int FLIGHT>
 __device__ __forceinline__ void turn_rows(
     const RowRef* rows, int n, const std::conditional_t<DT == SB_DTYPE_F32, double, float>* cs,
     const double* cs64, const RowSplit& split, int head_dim, int pairs, int rsub, int rpi, int unit) {
@@ -212,10 +208,10 @@ __device__ __forceinline__ void turn_rows(
   const bool second = HALF && at[NV - 1] * VEC < head_dim;
   const int trig_at = unit * VEC * NV;
 
-  for (int ib = rsub; ib < n; ib += kRowsInFlight * rpi) {
-    RowVec<DT, VEC> x[kRowsInFlight][NV];
+  for (int ib = rsub; ib < n; ib += FLIGHT * rpi) {
+    RowVec<DT, VEC> x[FLIGHT][NV];
 #pragma unroll
-    for (int u = 0; u < kRowsInFlight; ++u) {
+    for (int u = 0; u < FLIGHT; ++u) {
       const char* src = rows[min(ib + u * rpi, n - 1)].src;
       if (src) {
         x[u][0].template load<ONCE>(src + at[0] * (VEC * ES));
@@ -224,7 +220,7 @@ __device__ __forceinline__ void turn_rows(
       }
     }
 #pragma unroll
-    for (int u = 0; u < kRowsInFlight; ++u) {
+    for (int u = 0; u < FLIGHT; ++u) {
       if (ib + u * rpi >= n) break;
       const RowRef ref = rows[ib + u * rpi];
       if (!ref.src) continue;

@@ -638,14 +638,17 @@ __global__ __launch_bounds__(256, 2) void w4_tiles_kernel(const W4Args a) {
       tile[row * kBN + 32 * wave + lq] = T::round(acc[i][r] + bias);
     }
   __syncthreads();
-  for (int e = tid; e < kBM * kBN / 8; e += 256) {
-    const int row = e / (kBN / 8), c = e % (kBN / 8) * 8;
-    if (m0 + row >= a.num_rows) break;
-    uint16_t* out = reinterpret_cast<uint16_t*>(a.y + (m0 + row) * a.y_row) + f0 + c;
-    if (a.wide_out && f0 + c + 8 <= a.n) {
-      *reinterpret_cast<u32x4_t*>(out) = *reinterpret_cast<const u32x4_t*>(tile + row * kBN + c);
-    } else {
-      for (int j = 0; j < 8 && f0 + c + j < a.n; ++j) out[j] = tile[row * kBN + c + j];
+  const int live = static_cast<int>(min(static_cast<int64_t>(kBM), a.num_rows - m0));
+  if (a.wide_out && f0 + kBN <= a.n) {  // (uniform)
+    for (int e = tid; e < live * (kBN / 8); e += 256) {
+      const int row = e / (kBN / 8), c = e % (kBN / 8) * 8;
+      *reinterpret_cast<u32x4_t*>(a.y + (m0 + row) * a.y_row + (f0 + c) * 2) =
+          *reinterpret_cast<const u32x4_t*>(tile + row * kBN + c);
+    }
+  } else {
+    for (int e = tid; e < live * kBN; e += 256) {
+      const int row = e / kBN, c = e % kBN;
+      if (f0 + c < a.n) *reinterpret_cast<uint16_t*>(a.y + (m0 + row) * a.y_row + (f0 + c) * 2) = tile[e];
     }
   }
 }
