@@ -48,15 +48,17 @@ class ReuseRequest:
 
 class KVReuseBatch:
     """Requests sharing per-layer paged caches ``kv_caches`` ([num_blocks, 2, num_kv_heads,
-    block_size, head_dim] each, one per layer)."""
+    block_size, head_dim] each, one per layer). ``rotary``: the model's
+    :class:`semblend_amd.rotary.RotaryEmbedding`, instead of ``rope_base``."""
 
     def __init__(self, kv_caches: Sequence[torch.Tensor], requests: Sequence[ReuseRequest],
-                 rope_base: float = 10000.0):
+                 rope_base: float = 10000.0, rotary=None):
         if not kv_caches:
             raise ValueError("kv_caches is empty")
         self.kv_caches = list(kv_caches)
         self.requests = list(requests)
         self.rope_base = float(rope_base)
+        self.rotary = rotary
         dev = _lib.require_device(*self.kv_caches)
         for r in self.requests:
             if len(r.donor_kvs) != len(self.kv_caches):
@@ -95,7 +97,8 @@ class KVReuseBatch:
         if calls is None:
             calls = [prepare_scatter_paged_layers(
                          self.kv_caches, list(r.donor_kvs), r.block_table, r.donor_positions,
-                         r.target_positions, self.rope_base if rope else None)
+                         r.target_positions, self.rope_base if rope else None,
+                         rotary=self.rotary if rope else None)
                      for r in self.requests]
             calls = [c for c in calls if c is not None]
             self._scatter_calls[rope] = calls

@@ -290,6 +290,7 @@ def qkv_projection_paged(
     rope_base: float | None = None,
     out: torch.Tensor | None = None,
     backend: str = "auto",
+    rotary=None,
 ) -> torch.Tensor:
     """Project only the rows at ``positions`` and write their new K/V into the paged cache.
 
@@ -310,6 +311,11 @@ def qkv_projection_paged(
     26 / 39 at 256, 33 / 36 at 512, 42 / 41.5 at 768, 48.5 / 50.5 at 1024, 76 / 80 at 2048, 89 / 98
     at 2458, 158 / 165 at 4096. The fused form needs no fp32 intermediate of rows x features. Both
     accumulate in fp32 and round once.
+    ``qkv_weight`` may be a :class:`semblend_amd.quantized.QuantizedLinear` of that shape, and
+    ``rotary`` a :class:`semblend_amd.rotary.RotaryEmbedding` instead of ``rope_base``. Either runs in
+    parts (``backend`` "auto"): the rows gathered, their product rounded to the dtype, as such models
+    have it (:func:`semblend_amd.quantized.quantized_linear`, or the library's GEMM), K/V appended and
+    Q and K turned by :func:`semblend_amd.paged_cache.append_kv_paged`, which rounds them once more.
     Fuses the masked projection (semblend_core/triton_kernels.py:451-522) with the K/V write
     of partial_prefill (:904-909), compacted and paged; no reference counterpart.
     """
@@ -317,6 +323,12 @@ def qkv_projection_paged(
 
     if backend not in ("auto", "fused", "library"):
         raise ValueError("backend must be 'auto', 'fused' or 'library'")
+    if rotary is not None or _is_quantized(qkv_weight):
+        if backend != "auto":
+            raise ValueError("quantized weights and rotary run with backend='auto'")
+        return _projection_in_parts(hidden_states, qkv_weight, positions, kv_cache, block_table,
+                                    num_heads, num_kv_heads, head_dim, qkv_bias, rope_base, rotary,
+                                    out)
     dev = _lib.require_device(hidden_states, qkv_weight, kv_cache, qkv_bias)
     dt = hidden_states.dtype
     if dt not in (torch.bfloat16, torch.float16):
@@ -384,6 +396,79 @@ def qkv_projection_paged(
             hidden_states.stride(0), qkv_weight.stride(0), num_heads * head_dim,
             _lib.strides(kv_cache), _lib.dtype_code(hidden_states), _lib.stream_handle(dev),
         )
+    return out
+
+
+def _is_quantized(weight) -> bool:
+    from .quantized import QuantizedLinear
+
+    return isinstance(weight, QuantizedLinear)
+
+
+def _linear(x: torch.Tensor, weight, bias: torch.Tensor | None) -> torch.Tensor:
+    """x @ weight.T + bias for either kind of weight."""
+    from .quantized import quantized_linear
+
+    if _is_quantized(weight):
+        return quantized_linear(x, weight, bias=bias)
+    return torch.nn.functional.linear(x, weight, bias)
+
+
+def _projection_in_parts(hidden_states, qkv_weight, positions, kv_cache, block_table, num_heads,
+                         num_kv_heads, head_dim, qkv_bias, rope_base, rotary,
+                         out) -> torch.Tensor:
+    """:func:`qkv_projection_paged` with a quantized weight or a rotary embedding."""
+    from .paged_cache import append_kv_paged
+
+    quantized = _is_quantized(qkv_weight)
+    dev = _lib.require_device(hidden_states, kv_cache, qkv_bias,
+                              qkv_weight._packed if quantized else qkv_weight)
+    dt = hidden_states.dtype
+    if dt not in (torch.bfloat16, torch.float16):
+        raise TypeError("qkv_projection_paged runs bf16 / fp16 (the MFMA path)")
+    if kv_cache.dtype != dt or (qkv_bias is not None and qkv_bias.dtype != dt) or (
+            not quantized and qkv_weight.dtype != dt):
+        raise TypeError("hidden_states, qkv_weight, qkv_bias and kv_cache must share a dtype")
+    if rotary is not None and rope_base is not None:
+        raise ValueError("rope_base and rotary are alternatives")
+    seq_len, hidden = hidden_states.shape
+    heads = num_heads + 2 * num_kv_heads
+    if tuple(qkv_weight.shape) != (heads * head_dim, hidden):
+        raise ValueError(f"qkv_weight must be [{heads * head_dim}, {hidden}]")
+    if qkv_bias is not None and qkv_bias.shape != (heads * head_dim,):
+        raise ValueError(f"qkv_bias must be [{heads * head_dim}]")
+    nb, two, hkv, bs, d = kv_cache.shape
+    if two != 2 or hkv != num_kv_heads or d != head_dim:
+        raise ValueError("kv_cache must be [num_blocks, 2, num_kv_heads, block_size, head_dim]")
+    if not _mfma_rows_ok(hidden_states) or hidden % 8:
+        raise ValueError("hidden_states needs unit-stride, 16-byte aligned rows of a multiple of 8")
+    pos = _lib.as_index(positions, dev)
+    n = pos.shape[0]
+    if out is not None and (out.shape != (n, num_heads, head_dim) or out.dtype != dt
+                            or not out.is_contiguous() or out.device != dev):
+        raise ValueError("out must be a contiguous [R, Hq, D] tensor of the inputs' dtype and "
+                         "device")
+    # (rows outside the hidden states: zero Q, no K/V; they are padding to the append)
+    if out is None:
+        out = torch.zeros((n, num_heads, head_dim), dtype=dt, device=dev)
+    else:
+        out.zero_()
+    if n == 0:
+        return out
+    rows = torch.empty((n, hidden), dtype=dt, device=dev)
+    with _lib.on_device(dev):
+        _lib.call("sb_qkv_gather_rows", rows.data_ptr(), hidden_states.data_ptr(), pos.data_ptr(), n,
+                  seq_len, hidden, hidden_states.stride(0), None, head_dim, None,
+                  _lib.dtype_code(hidden_states), _lib.stream_handle(dev))
+    proj = _linear(rows, qkv_weight, qkv_bias).view(n, heads, head_dim)
+    q, k, v = proj.split((num_heads, num_kv_heads, num_kv_heads), dim=1)
+    inside = torch.where(pos < seq_len, pos, -1)
+    if rope_base is None and rotary is None:
+        append_kv_paged(kv_cache, k, v, block_table, inside)
+        out.copy_(torch.where((inside >= 0)[:, None, None], q, out))
+    else:
+        append_kv_paged(kv_cache, k, v, block_table, inside, rope_base=rope_base, rotary=rotary,
+                        query=q, query_out=out)
     return out
 
 
@@ -686,6 +771,7 @@ def partial_prefill_layer_paged(
     rope_base: float | None = None,
     scale: float | None = None,
     plan: PagedAttentionPlan | None = None,
+    rotary=None,
 ) -> PagedLayerResult:
     """One attention layer of partial prefill, on the paged cache of that layer.
 
@@ -699,16 +785,19 @@ def partial_prefill_layer_paged(
     the attention rows (torch's GEMM, fp32 accumulation, rounded to the input dtype). A model
     runs this once per layer with that layer's weights and cache; ``plan`` (from
     :func:`plan_partial_attention_paged` for these positions, made once per request) serves
-    every layer's attention.
+    every layer's attention. Either weight may be a
+    :class:`semblend_amd.quantized.QuantizedLinear`, and ``rotary`` a model's
+    :class:`semblend_amd.rotary.RotaryEmbedding` instead of ``rope_base``.
     """
-    dev = _lib.require_device(hidden_states, qkv_weight, output_projection, kv_cache)
+    dev = _lib.require_device(hidden_states, kv_cache, *(
+        w._packed if _is_quantized(w) else w for w in (qkv_weight, output_projection)))
     q = qkv_projection_paged(hidden_states, qkv_weight, compute_positions, kv_cache,
                              block_table, num_heads, num_kv_heads, head_dim, qkv_bias=qkv_bias,
-                             rope_base=rope_base)
+                             rope_base=rope_base, rotary=rotary)
     pos = _lib.as_index(compute_positions, dev)
     attn = partial_prefill_attention_paged(q, kv_cache, block_table, pos, scale=scale, plan=plan)
     flat = attn.reshape(attn.shape[0], num_heads * head_dim)
-    out = torch.nn.functional.linear(flat, output_projection, output_bias)
+    out = _linear(flat, output_projection, output_bias)
     return PagedLayerResult(output=out, query=q, attention=attn)
 
 
