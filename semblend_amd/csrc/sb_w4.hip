@@ -1,11 +1,12 @@
 // Products with 4-bit weights for gfx950: y = x w^T + bias, w[n, k] = (code[n, k] - zero[n, k / g]) *
 // scale[n, k / g] with 16-bit scales, one per group of g inputs.
 //
-// Arithmetic. A code c becomes the 16-bit float 16 + c by putting its four bits at the top of the
-// mantissa of 16.0 (two instructions a pair). For one group, with P = sum x (16 + c) and S = sum x from the
-// matrix cores (S a product with ones), sum x w = scale (P - (16 + zero) S). Nothing is rounded on the
-// way but the fp32 sums, so that the result is that of the 16-bit inputs and the exact weights, rounded
-// once; 16 + c against c - zero costs the sums two or three of their 24 bits.
+// Arithmetic. A code c becomes the 16-bit float B + c by putting its four bits into the mantissa of B
+// (two instructions a pair): B = 16 in bf16, 128 in fp16. For one group, with P = sum x (B + c) and
+// S = sum x from the matrix cores, sum x w = scale (P - (B + zero) S). Nothing is rounded on the way but
+// the fp32 sums, so that the result is that of the 16-bit inputs and the exact weights, rounded once; B + c
+// against c - zero costs the sums two or three of their 24 bits (six in fp16). fp16 has a packed
+// subtraction, and from 33 rows, where P and S cost more than it, P = sum x (c - zero) and sum x w = scale P.
 //
 // Layout, made once (w4_pack_kernel): 16 features x 128 inputs are 1 KiB, lane l of a wave holding 16
 // bytes: word j the codes of feature l % 16, inputs 32 j + 8 (l / 16) + 0 .. 7, which is the operand of one
@@ -830,6 +831,7 @@ W4Plan w4_plan(int64_t m, int64_t n, int64_t k, int64_t group, int32_t dtype) {
   double best = 0.0;  // us, of more than 64 rows
   if (m > 64)
     best = 2.5 + static_cast<double>(rounds(tiles(nt, p.j) * gy)) * (0.5 + 1.85 * static_cast<double>(k) / 1024);
+  if (gy > 65535) best = 1e30;  // (a grid's second axis ends there)
   const int64_t blocks = dtype == SB_DTYPE_BF16 ? sum_blocks(k, group) : 0;
   const int64_t steps = kt + blocks, grid = tiles(m, kBM) * tiles(n, kBN);
   for (int64_t s = 1; m > 64 && s <= 32 && (s == 1 || 2 * s <= steps); ++s) {
@@ -906,7 +908,6 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + sums_bytes(plan, num_rows));
   if (!plan.tiled) {
     const int64_t gy = tiles(num_rows, plan.r);
-    if (gy > 65535) return fail(fn, "too many rows");
     const int64_t nt = tiles(out_features, kTileN);
     // Up to 16 rows: 16 waves where a workgroup has 16 features (a CU has one or two of them then) and a
     // tile of inputs for each wave (one row of 18944 -> 3584 9.8 -> 9.1 us, 16 rows 12.9 -> 11.8; of 896 ->

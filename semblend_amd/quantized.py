@@ -131,7 +131,7 @@ def quantized_linear(
     x: [..., in_features] bf16 or fp16, any number of rows; bias: [out_features] of x's type; ``out``:
     [..., out_features] of x's type with a unit last stride and rows at one stride (a new tensor by
     default; returned). Values of x must be finite and below 2^119 in magnitude: a row that holds an
-    infinity or a NaN gives NaN, other rows are not affected. Extension with no reference counterpart.
+    infinity or a NaN gives NaN (or infinities), other rows are not affected. Extension with no reference counterpart.
     """
     if not isinstance(weight, QuantizedLinear):
         raise TypeError("weight must be a QuantizedLinear")

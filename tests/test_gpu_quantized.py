@@ -262,3 +262,16 @@ def test_codes_out_of_range_are_refused(dev):
         QuantizedLinear.quantize(torch.full((4, 64), math.inf, device="cuda"), group=32)
     with pytest.raises(ValueError, match="range"):
         QuantizedLinear.quantize(torch.full((4, 64), 1e30, device="cuda"), group=32, scale_dtype=FP16)
+
+
+def test_more_rows_than_a_grid_of_the_few_rows_kernel(dev):
+    """4.2 million rows of few features and inputs."""
+    m = 65535 * 64 + 200
+    codes, scales, zeros = ref.make(16, 32, 32, BF16, 1)
+    w = QuantizedLinear(codes.cuda(), scales.cuda(), zeros.cuda())
+    x = randn((1024, 32), BF16, 2)
+    y = quantized_linear(x.cuda().repeat(m // 1024 + 1, 1)[:m], w)
+    ref.check(y[:1024].cpu(), *ref.linear(x, codes, scales, zeros))
+    last = m // 1024 * 1024
+    assert torch.equal(y[:last].view(-1, 1024, 16), y[:1024].expand(last // 1024, 1024, 16))
+    assert torch.equal(y[last:], y[:m - last])

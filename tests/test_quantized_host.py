@@ -139,4 +139,6 @@ def test_sizes():
     assert size("sb_w4_linear_workspace_size", 4, 32, 128, 64, 2) == 0
     assert size("sb_w4_linear_workspace_size", 4096, 8192, 1024, 64, 2) > 0
     assert size("sb_w4_linear_workspace_size", 4096, 32, 128, 48, 2) == 0
+    # the few-rows kernel's grid ends at 65535 x 64 rows: more take tiles, whose sums lie there
+    assert size("sb_w4_linear_workspace_size", 65535 * 64 + 1, 16, 128, 64, 2) > 0
     assert _linear(m=0, x=None) == _lib.SB_OK
