@@ -151,7 +151,9 @@ __device__ __forceinline__ void w4_dma4(const void* src, uint32_t lds_wave) {
 }
 // Rows of x: `rows` describes up to 2^32 bytes from a workgroup's first row to the end of the last one
 // (a load behind it gives zeros or nothing), `at` is a lane's offset, `add` one for all lanes. One
-// register where addresses take two for every four rows.
+// register where addresses take two for every four rows. The offsets are added here and not by the load:
+// its scalar offset may be left out of the check against the end. (In the assembly, or the sums of all
+// copies would be kept in registers.)
 __device__ __forceinline__ u32x4_t w4_rows_of(const char* first, int64_t bytes) {
   const uint64_t p = reinterpret_cast<uint64_t>(first);
   const u32x4_t r = {static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32) & 0xffffu,
@@ -159,11 +161,12 @@ __device__ __forceinline__ u32x4_t w4_rows_of(const char* first, int64_t bytes) 
   return r;
 }
 __device__ __forceinline__ void w4_dma_row(uint32_t at, u32x4_t rows, uint32_t add, uint32_t lds_wave) {
+  uint32_t sum;
   asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %1, %2, %3 offen lds"
-      :
+      "s_mov_b32 m0, %1\n\t"
+      "v_add_u32 %0, %4, %2\n\t"
+      "buffer_load_dwordx4 %0, %3, 0 offen lds"
+      : "=&v"(sum)
       : "s"(lds_wave), "v"(at), "s"(rows), "s"(add)
       : "memory", "m0");
 }
@@ -839,7 +842,7 @@ W4Plan w4_plan(int64_t m, int64_t n, int64_t k, int64_t group, int32_t dtype) {
     if (slices != s) continue;
     const double load = static_cast<double>(rounds(grid * s));
     double t = 3.0 + (blocks ? 4.0 : 0.0) + static_cast<double>(per) * (load <= 1.0 ? 1.08 : 0.85 * load);
-    if (s > 1) t += 4.0 + static_cast<double>(s * m * n) * 8.0 / 6e6;
+    if (s > 1) t += 4.0 + static_cast<double>(s * m) * static_cast<double>(n) * 8.0 / 6e6;
     if (t >= best) continue;
     best = t;
     p.tiled = true;
