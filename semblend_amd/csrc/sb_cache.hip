@@ -34,6 +34,7 @@ namespace {
 // Rows in flight of a thread; half pairs, two vectors a row: 2 (4602 tokens of 32 / 8 heads x 128: 21.1 us,
 // with 4 21.9).
 constexpr int kRowsInFlight = 4, kHalfRowsInFlight = 2;
+
 struct AppendArgs {
   const char* k;
   const char* v;
@@ -126,7 +127,8 @@ __global__ __launch_bounds__(kRowThreads) void append_kv_kernel(const AppendArgs
   __syncthreads();
   if (rsub >= rpi) return;
 
-  turn_rows<DT, VEC, Q4, HALF, false, HALF ? kHalfRowsInFlight : kRowsInFlight>(rows, n, cs, cs64, a.split, a.head_dim, a.pairs, rsub, rpi, unit);
+  constexpr int kFlight = HALF ? kHalfRowsInFlight : kRowsInFlight;
+  turn_rows<DT, VEC, Q4, HALF, false, kFlight>(rows, n, cs, cs64, a.split, a.head_dim, a.pairs, rsub, rpi, unit);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -242,12 +244,6 @@ struct CacheStrides {
 CacheStrides cache_strides(const int64_t* s, int64_t es) {
   return {s[0] * es, s[1] * es, s[2] * es, s[3] * es};
 }
-
-}  // namespace
-}  // namespace sb
-
-namespace sb {
-namespace {
 
 // Both append entries; `pairs` pairs of a row are turned (0: all of it).
 int append_kv(

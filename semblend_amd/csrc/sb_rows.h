@@ -287,22 +287,20 @@ __device__ __forceinline__ void turn_rows(
             else t64 = reinterpret_cast<const double*>(trig);
             // (a sum of two values of the largest fp32 exponent may pass fp32, but not 7 * 2^126: such a
             // block, not finite above, is taken times 2^-2)
-            const bool bad = b[0].bad || b[NV - 1].bad;
-            const double down = bad ? 0.25 : 1.0;
-            const int up = bad ? 2 : 0;
+            const double down = b[0].bad ? 0.25 : 1.0, down_2 = b[NV - 1].bad ? 0.25 : 1.0;
+            const int up[2] = {b[0].bad ? 2 : 0, b[NV - 1].bad ? 2 : 0};
 #pragma unroll
             for (int i = 0; i < VEC; i += HALF ? 1 : 2) {
               const int j = HALF ? i : i + 1, t = HALF ? 2 * i : i;
-              const double e = Elem<DT>::get(x[u][0].e[i]) * down;
-              const double o = Elem<DT>::get(x[u][NV - 1].e[j]) * down;
-              f[0][i] = round_to_odd(e * t64[t] - o * t64[t + 1]);
-              f[NV - 1][j] = round_to_odd(e * t64[t + 1] + o * t64[t]);
+              const double e = Elem<DT>::get(x[u][0].e[i]), o = Elem<DT>::get(x[u][NV - 1].e[j]);
+              f[0][i] = round_to_odd((e * t64[t] - o * t64[t + 1]) * down);
+              f[NV - 1][j] = round_to_odd((e * t64[t + 1] + o * t64[t]) * down_2);
             }
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
               b[v] = block_scale(f[v]);
               w[v] = b[v].bad ? 0u : pack_codes(f[v], b[v].value);
-              if (!b[v].bad) b[v].byte += up;
+              if (!b[v].bad) b[v].byte += up[v];
             }
           }
         } else {

@@ -219,6 +219,26 @@ def test_append_4bit_small_turns(dev, n):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_append_4bit_of_both_ends_of_the_range(dev, dtype):
+    """Half pairs whose first element passes fp32 (not what a scale can hold) under the factor and whose
+    second one lies at the smallest scale: each block has its own exponent."""
+    rot = RotaryEmbedding(torch.zeros(32), 64, factor=2.0)
+    k = torch.empty((2, 1, 64), dtype=FP32)
+    k[..., :32] = randn((2, 1, 32), FP32, 1).clamp(-1, 1) * 2.0 ** 127
+    k[..., 0] = 1.5 * 2.0 ** 127
+    k[..., 32:] = (torch.arange(32) % 8 - 3.0) * 2.0 ** -127
+    k = k.to(dtype)
+    at = torch.tensor([0, 5], dtype=torch.int32)
+    cache = pc.QuantizedKVCache.allocate(1, 1, 16, 64, "cuda")
+    table = torch.zeros(1, dtype=torch.int32)
+    pc.append_kv_paged(cache, k.cuda(), k.cuda(), table.cuda(), at.cuda(), rotary=rot)
+    c, s = pref.quantize(k.double() * 2.0)
+    assert torch.equal(cache.scales.cpu()[0, 0, :, at.long()].transpose(0, 1).long(), s)
+    assert torch.equal(cache.codes.cpu()[0, 0, :, at.long()].transpose(0, 1),
+                       (c[..., 0::2] | c[..., 1::2] << 4).to(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_interleaved_whole_heads_are_rope_base(dev, dtype):
     """The path's own convention given as an embedding: the same bits as ``rope_base``."""
     d, num, bs = 64, 300, 16
