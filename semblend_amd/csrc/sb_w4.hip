@@ -814,26 +814,41 @@ struct W4Plan {
   int splits, split_steps, sum_blocks;
 };
 
-// Up to 64 rows take the few-rows kernel: R the smallest that holds them, J = 2 where that leaves enough
-// workgroups. More rows take what the model below says is faster, in us for K inputs on 256 CUs. Few rows,
-// R = 64: 2.5 + rounds (0.5 + 1.85 K / 1024), a round a workgroup per CU. Tiles: 3, the sums' launch 4
-// (bf16), a step 1.08 with one workgroup a CU and 0.85 each with more; slices: the merge's launch 4 and
-// their traffic. Measured, few rows against tiles in their best split: 3584 -> 4608, 128 rows 15.1 and
-// 22.7 us, 256 rows 22.9 and 26.1; 18944 -> 3584 (groups of 64), 128 rows 35.6 and 40.8, 192 rows 63.0
-// and 56.4; 3584 -> 37888, 96 rows 72.1 and 52.8; 896 -> 1152, 256 rows 5.3 and 14.3.
+// Up to 64 rows take the few-rows kernel, R the smallest that holds them. A workgroup reads its rows once
+// for all of its features, so that more features read them less often, in fewer and longer workgroups: J is
+// the one with the least rounds (a workgroup per CU) times a round's time, kRound, in those of J = 1.
+// Measured, J = 1 to 4, us: 64 rows of 3584 -> 4608 13.7, 9.0, 11.0, 13.4; 4096 -> 12288 25.8, 19.0, 14.7,
+// 14.6; 3584 -> 37888 59.0, 38.8, 38.8, 36.2; 18944 -> 3584 29.8, 39.0, 45.0, 59.0; 128 rows of 3584 -> 4608
+// 19.1, 15.5, 11.4, 13.6; 32 of 4096 -> 131072 (fp16) 146, 106, 88, 80; 16 of 4096 -> 12288 9.2, 8.4, 7.5,
+// 7.9. (Up to 4 rows J = 1 or 2: what is left is the codes.)
+// More than 64 rows take what the model below says is faster, in us for K inputs on 256 CUs. Few rows, R =
+// 64: 2.5 + rounds 0.5 + rounds 1.47 kRound K / 1024, the last a fifth more from five rounds on. Tiles: 3, the
+// sums' launch 4 (bf16), a step 1.08 with one workgroup a CU and 0.85 each with more; slices: the merge's
+// launch 4 and their traffic. Measured, few rows against tiles in their best split: 3584 -> 4608, 128 rows
+// 11.4 and 22.9 us, 256 rows 20.5 and 26.0, 614 rows 38.3 and 37.2; 18944 -> 3584 (groups of 64), 192 rows
+// 50.7 and 55.2, 320 rows 94.1 and 72.6; 3584 -> 37888, 96 rows 61.9 and 53.8; 896 -> 1152, 256 rows 5.1 and
+// 14.7.
 W4Plan w4_plan(int64_t m, int64_t n, int64_t k, int64_t group, int32_t dtype) {
   W4Plan p = {};
   const int64_t nt = tiles(n, kTileN), kt = tiles(k, kTileK);
   p.r = m <= 4 ? 4 : m <= 16 ? 16 : m <= 32 ? 32 : 64;
   const int64_t gy = tiles(m, p.r);
   const auto rounds = [](int64_t wgs) { return tiles(wgs, 256); };
-  // (a workgroup of 32 features takes about a fifth longer than one of 16)
-  p.j = rounds(tiles(nt, 2) * gy) * 1.2 < static_cast<double>(rounds(nt * gy)) ? 2 : 1;
+  constexpr double kRound[2][4] = {{1.0, 1.25, 1.85, 2.3}, {1.0, 1.25, 1.6, 1.95}};  // up to 16 rows, more
+  const double* round = kRound[p.r > 16];
+  double least = 0.0;
+  for (int j = 1; j <= (p.r == 4 ? 2 : 4); ++j) {
+    const double t = static_cast<double>(rounds(tiles(nt, j) * gy)) * round[j - 1];
+    if (j == 1 || t < least) least = t, p.j = j;
+  }
   p.splits = 1;
   p.split_steps = static_cast<int>(kt);
   double best = 0.0;  // us, of more than 64 rows
-  if (m > 64)
-    best = 2.5 + static_cast<double>(rounds(tiles(nt, p.j) * gy)) * (0.5 + 1.85 * static_cast<double>(k) / 1024);
+  if (m > 64) {
+    const int64_t turns = rounds(tiles(nt, p.j) * gy);
+    best = 2.5 + static_cast<double>(turns) * 0.5 +
+           least * (turns > 4 ? 1.2 : 1.0) * 1.47 * static_cast<double>(k) / 1024;
+  }
   if (gy > 65535) best = 1e30;  // (a grid's second axis ends there)
   const int64_t blocks = dtype == SB_DTYPE_BF16 ? sum_blocks(k, group) : 0;
   const int64_t steps = kt + blocks, grid = tiles(m, kBM) * tiles(n, kBN);
@@ -917,9 +932,10 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
     // 1152 2.9 and 3.0), and codes read past the caches where these cannot keep them until the next call
     // (one row of 4096 -> 131072, 268 MB: 47.9 -> 45.2 us; 16 of 3584 -> 37888, 68 MB, 15.3 and 19.6).
     const bool many = plan.r <= 16 && plan.j == 1 && a.k_tiles > 16;
-    const bool once = plan.r <= 16 && plan.j == 2 &&
+    const bool once = plan.r <= 16 && plan.j > 1 &&
                       sb_w4_codes_size(out_features, in_features) >= (int64_t{192} << 20);
     // Two steps in flight where a CU's LDS holds two such workgroups, else one (other waves run meanwhile).
+    // (64 rows and features: LDS holds seven waves' steps)
 #define SB_W4_L(DT, R, J, GPT, W, ONCE)                                                               \
   do {                                                                                                \
     constexpr int kAhead = 2 * W * RowsStage<R, J, GPT>::kBytes <= 80 * 1024 ? 2 : 1;                 \
@@ -930,19 +946,20 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
   if (dtype == DT && plan.r == R && plan.j == J && gpt == GPT) {                                      \
     if constexpr (R <= 16) {                                                                          \
       if (J == 1 && many) SB_W4_L(DT, R, 1, GPT, 16, false);                                          \
-      else if (J == 2 && once) SB_W4_L(DT, R, 2, GPT, 8, true);                                       \
+      else if (J > 1 && once) SB_W4_L(DT, R, (J > 1 ? J : 2), GPT, 8, true);                          \
       else SB_W4_L(DT, R, J, GPT, 8, false);                                                          \
     } else {                                                                                          \
-      SB_W4_L(DT, R, J, GPT, 8, false);                                                               \
+      SB_W4_L(DT, R, J, GPT, (R == 64 && J == 4 ? 7 : 8), false);                                     \
     }                                                                                                 \
   }
-#define SB_W4_(DT, J)                                          \
-  SB_W4(DT, 4, J, 1) SB_W4(DT, 4, J, 2) SB_W4(DT, 4, J, 4)     \
-  SB_W4(DT, 16, J, 1) SB_W4(DT, 16, J, 2) SB_W4(DT, 16, J, 4)  \
-  SB_W4(DT, 32, J, 1) SB_W4(DT, 32, J, 2) SB_W4(DT, 32, J, 4)  \
-  SB_W4(DT, 64, J, 1) SB_W4(DT, 64, J, 2) SB_W4(DT, 64, J, 4)
-    SB_W4_(SB_DTYPE_BF16, 1) SB_W4_(SB_DTYPE_BF16, 2)
-    SB_W4_(SB_DTYPE_F16, 1) SB_W4_(SB_DTYPE_F16, 2)
+#define SB_W4_(DT, R, J) SB_W4(DT, R, J, 1) SB_W4(DT, R, J, 2) SB_W4(DT, R, J, 4)
+#define SB_W4_R(DT, J) SB_W4_(DT, 16, J) SB_W4_(DT, 32, J) SB_W4_(DT, 64, J)
+#define SB_W4_D(DT)                                                                                  \
+  SB_W4_(DT, 4, 1) SB_W4_(DT, 4, 2) SB_W4_R(DT, 1) SB_W4_R(DT, 2) SB_W4_R(DT, 3) SB_W4_R(DT, 4)
+    SB_W4_D(SB_DTYPE_BF16)
+    SB_W4_D(SB_DTYPE_F16)
+#undef SB_W4_D
+#undef SB_W4_R
 #undef SB_W4_
 #undef SB_W4
 #undef SB_W4_L

@@ -275,3 +275,26 @@ def test_more_rows_than_a_grid_of_the_few_rows_kernel(dev):
     last = m // 1024 * 1024
     assert torch.equal(y[:last].view(-1, 1024, 16), y[:1024].expand(last // 1024, 1024, 16))
     assert torch.equal(y[last:], y[:m - last])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n", [9000, 16300])
+@pytest.mark.parametrize("m", [9, 20, 50, 70])
+def test_features_of_a_workgroup(dev, m, n, group, dtype):
+    """Feature counts at which a workgroup of few rows takes three and four tiles of them, the last
+    workgroup not all of its own."""
+    codes, scales, zeros = ref.make(n, 384, group, dtype, 1)
+    x = randn((m, 384), dtype, 2)
+    w = QuantizedLinear(codes.cuda(), scales.cuda(), zeros.cuda())
+    ref.check(quantized_linear(x.cuda(), w).cpu(), *ref.linear(x, codes, scales, zeros))
+
+
+@pytest.mark.parametrize("m,n,k", [(2, 131072, 4096), (16, 131072, 4096), (16, 9000, 45056)])
+def test_weights_past_the_caches(dev, m, n, k):
+    """Codes of 200 MB and more; some of the features against 64 bits."""
+    codes, scales, zeros = ref.make(n, k, 128, FP16, 1)
+    x = randn((m, k), FP16, 2)
+    y = quantized_linear(x.cuda(), QuantizedLinear(codes.cuda(), scales.cuda(), zeros.cuda())).cpu()
+    at = torch.cat([torch.arange(0, n, 97), torch.arange(n - 70, n)])
+    ref.check(y[:, at], *ref.linear(x, codes[at], scales[at], zeros[at]))
