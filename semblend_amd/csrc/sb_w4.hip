@@ -814,42 +814,45 @@ struct W4Plan {
   int splits, split_steps, sum_blocks;
 };
 
-// Up to 64 rows take the few-rows kernel, R the smallest that holds them. A workgroup reads its rows once
-// for all of its features, so that more features read them less often, in fewer and longer workgroups: J is
-// the one with the least rounds (a workgroup per CU) times a round's time, kRound, in those of J = 1.
-// Measured, J = 1 to 4, us: 64 rows of 3584 -> 4608 13.7, 9.0, 11.0, 13.4; 4096 -> 12288 25.8, 19.0, 14.7,
-// 14.6; 3584 -> 37888 59.0, 38.8, 38.8, 36.2; 18944 -> 3584 29.8, 39.0, 45.0, 59.0; 128 rows of 3584 -> 4608
-// 19.1, 15.5, 11.4, 13.6; 32 of 4096 -> 131072 (fp16) 146, 106, 88, 80; 16 of 4096 -> 12288 9.2, 8.4, 7.5,
-// 7.9. (Up to 4 rows J = 1 or 2: what is left is the codes.)
-// More than 64 rows take what the model below says is faster, in us for K inputs on 256 CUs. Few rows, R =
-// 64: 2.5 + rounds 0.5 + rounds 1.47 kRound K / 1024, the last a fifth more from five rounds on. Tiles: 3, the
-// sums' launch 4 (bf16), a step 1.08 with one workgroup a CU and 0.85 each with more; slices: the merge's
-// launch 4 and their traffic. Measured, few rows against tiles in their best split: 3584 -> 4608, 128 rows
-// 11.4 and 22.9 us, 256 rows 20.5 and 26.0, 614 rows 38.3 and 37.2; 18944 -> 3584 (groups of 64), 192 rows
-// 50.7 and 55.2, 320 rows 94.1 and 72.6; 3584 -> 37888, 96 rows 61.9 and 53.8; 896 -> 1152, 256 rows 5.1 and
-// 14.7.
+// The few-rows kernel: a workgroup reads its rows once for all of its features and its codes once for all
+// of its rows, so that more of either mean fewer reads and fewer, longer workgroups. R (no larger than holds
+// the rows) and J are those of the least time by this model, in us for K inputs on 256 CUs: 2.5 + rounds (0.5
+// + kRound K / 1024), a round a workgroup per CU (32 and 64 rows: its second part a fifth more from five
+// rounds on). Measured, J = 1 to 4: 64 rows, R = 64, of 3584 -> 4608 13.7, 9.0, 11.0, 13.4 us; 4096 -> 12288
+// 25.8, 19.0, 14.7, 14.6; 3584 -> 37888 59.0, 38.8, 38.8, 36.2; 18944 -> 3584 29.8, 39.0, 45.0, 59.0; 32
+// rows, R = 32, of 4096 -> 131072 (fp16) 146, 106, 88, 80; 16 of 4096 -> 12288 9.2, 8.4, 7.5, 7.9. The
+// largest R and the one taken: 64 rows of 3584 -> 4608 8.9 and 7.7 (R = 32, J = 3), of 18944 -> 3584 29.5 and
+// 22.4 (32, 2); 32 rows of 18944 -> 3584 18.1 and 16.5 (16, 2). (Up to 4 rows J = 1 or 2: what is left is
+// the codes.)
+// More than 64 rows take tiles where their model is less: 3, the sums' launch 4 (bf16), a step 1.08 with one
+// workgroup a CU and 0.85 each with more; slices: the merge's launch 4 and their traffic. Measured, few rows
+// against tiles in their best split: 3584 -> 4608, 128 rows 11.4 and 22.9 us, 256 rows 20.5 and 26.0, 614 rows
+// 38.3 and 37.2; 18944 -> 3584 (groups of 64), 192 rows 50.7 and 55.2, 320 rows 94.1 and 72.6; 3584 -> 37888,
+// 96 rows 61.9 and 53.8; 896 -> 1152, 256 rows 5.1 and 14.7.
 W4Plan w4_plan(int64_t m, int64_t n, int64_t k, int64_t group, int32_t dtype) {
   W4Plan p = {};
   const int64_t nt = tiles(n, kTileN), kt = tiles(k, kTileK);
-  p.r = m <= 4 ? 4 : m <= 16 ? 16 : m <= 32 ? 32 : 64;
-  const int64_t gy = tiles(m, p.r);
   const auto rounds = [](int64_t wgs) { return tiles(wgs, 256); };
-  constexpr double kRound[2][4] = {{1.0, 1.25, 1.85, 2.3}, {1.0, 1.25, 1.6, 1.95}};  // up to 16 rows, more
-  const double* round = kRound[p.r > 16];
-  double least = 0.0;
-  for (int j = 1; j <= (p.r == 4 ? 2 : 4); ++j) {
-    const double t = static_cast<double>(rounds(tiles(nt, j) * gy)) * round[j - 1];
-    if (j == 1 || t < least) least = t, p.j = j;
-  }
+  constexpr int kRows[4] = {4, 16, 32, 64};
+  constexpr double kNever = 1e30;
+  constexpr double kRound[4][4] = {{0.6, 0.7, kNever, kNever},
+                                   {0.6, 0.75, 1.1, 1.38},
+                                   {0.83, 1.1, 1.5, 1.75},
+                                   {1.47, 1.84, 2.35, 2.87}};
+  const int first = m <= 4 ? 0 : 1, last = m <= 4 ? 0 : m <= 16 ? 1 : m <= 32 ? 2 : 3;
+  double best = kNever;
+  for (int r = first; r <= last; ++r)
+    for (int j = 1; j <= 4; ++j) {
+      const int64_t gy = tiles(m, kRows[r]), turns = rounds(tiles(nt, j) * gy);
+      const double more = r > 1 && turns > 4 ? 1.2 : 1.0;
+      const double t = 2.5 + static_cast<double>(turns) *
+                                 (0.5 + kRound[r][j - 1] * more * static_cast<double>(k) / 1024);
+      if (gy > 65535 || t >= best) continue;  // (a grid's second axis ends there)
+      best = t;
+      p.r = kRows[r], p.j = j;
+    }
   p.splits = 1;
   p.split_steps = static_cast<int>(kt);
-  double best = 0.0;  // us, of more than 64 rows
-  if (m > 64) {
-    const int64_t turns = rounds(tiles(nt, p.j) * gy);
-    best = 2.5 + static_cast<double>(turns) * 0.5 +
-           least * (turns > 4 ? 1.2 : 1.0) * 1.47 * static_cast<double>(k) / 1024;
-  }
-  if (gy > 65535) best = 1e30;  // (a grid's second axis ends there)
   const int64_t blocks = dtype == SB_DTYPE_BF16 ? sum_blocks(k, group) : 0;
   const int64_t steps = kt + blocks, grid = tiles(m, kBM) * tiles(n, kBN);
   for (int64_t s = 1; m > 64 && s <= 32 && (s == 1 || 2 * s <= steps); ++s) {
@@ -932,7 +935,7 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
     // 1152 2.9 and 3.0), and codes read past the caches where these cannot keep them until the next call
     // (one row of 4096 -> 131072, 268 MB: 47.9 -> 45.2 us; 16 of 3584 -> 37888, 68 MB, 15.3 and 19.6).
     const bool many = plan.r <= 16 && plan.j == 1 && a.k_tiles > 16;
-    const bool once = plan.r <= 16 && plan.j > 1 &&
+    const bool once = plan.r <= 16 && plan.j > 1 && gy == 1 &&
                       sb_w4_codes_size(out_features, in_features) >= (int64_t{192} << 20);
     // Two steps in flight where a CU's LDS holds two such workgroups, else one (other waves run meanwhile).
     // (64 rows and features: LDS holds seven waves' steps)
