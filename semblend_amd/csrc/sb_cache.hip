@@ -65,7 +65,7 @@ template <int DT, int VEC, bool Q4, bool HALF>
 __global__ __launch_bounds__(kRowThreads) void append_kv_kernel(const AppendArgs a) {
   using CS = std::conditional_t<DT == SB_DTYPE_F32, double, float>;
   constexpr bool kBoth = Q4 && DT != SB_DTYPE_F32;         // 64-bit sines and cosines besides
-  __shared__ CS cs[2 * kTableEntries];                    // cosine, sine of each (token, pair)
+  __shared__ __align__(16) CS cs[2 * kTableEntries];       // cosine, sine of each (token, pair)
   __shared__ double cs64[kBoth ? 2 * kTableEntries : 1];
   __shared__ __align__(16) RowRef rows[kRowsMax];
   const int tid = threadIdx.x;
@@ -119,8 +119,9 @@ __global__ __launch_bounds__(kRowThreads) void append_kv_kernel(const AppendArgs
       double s, c;
       sincos_cw(static_cast<double>(p) * static_cast<double>(a.inv_freq[f]), &s, &c);
       c *= a.factor, s *= a.factor;
-      cs[2 * i] = static_cast<CS>(c);
-      cs[2 * i + 1] = static_cast<CS>(s);
+      CS* to = cs + 2 * tok * half + Sines<DT, VEC, HALF>::at(f, half);
+      to[0] = static_cast<CS>(c);
+      to[1] = static_cast<CS>(s);
       if constexpr (kBoth) cs64[2 * i] = c, cs64[2 * i + 1] = s;
     }
   }

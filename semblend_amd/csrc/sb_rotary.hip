@@ -62,7 +62,7 @@ template <int DT, int VEC, bool HALF, int MODE, bool ONCE, bool INLINE>
 __global__ __launch_bounds__(kRowThreads) void rotary_rows_kernel(
     const RotaryArgs a, const std::conditional_t<INLINE, RotaryInline, NoInline> list) {
   using CS = std::conditional_t<DT == SB_DTYPE_F32, double, float>;
-  __shared__ CS cs[2 * kTableEntries];
+  __shared__ __align__(16) CS cs[2 * kTableEntries];
   __shared__ __align__(16) RowRef rows[kRowsMax];
   const int tid = threadIdx.x;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens_per_wg;
@@ -131,8 +131,9 @@ __global__ __launch_bounds__(kRowThreads) void rotary_rows_kernel(
     const int tok = a.pair_div.of(i), f = i - tok * a.pairs;
     double s, c;
     sincos_cw(static_cast<double>(angle(t0 + tok)) * static_cast<double>(a.inv_freq[f]), &s, &c);
-    cs[2 * i] = static_cast<CS>(c * a.factor);
-    cs[2 * i + 1] = static_cast<CS>(s * a.factor);
+    CS* to = cs + 2 * tok * a.pairs + Sines<DT, VEC, HALF>::at(f, a.pairs);
+    to[0] = static_cast<CS>(c * a.factor);
+    to[1] = static_cast<CS>(s * a.factor);
   }
   __syncthreads();
   const int rpi = kRowThreads / a.split.units;

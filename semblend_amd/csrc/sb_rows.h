@@ -190,8 +190,34 @@ struct RowSplit {
   }
 };
 
+// A token's cosines and sines in LDS, 2 * pairs numbers. A thread's pairs are 32 or 64 bytes; they lie in
+// pieces of 16, piece after piece of all threads of a row, so that the threads' reads of a piece are 16 bytes
+// apart and fall on all banks.
+template <int DT, int VEC, bool HALF> struct Sines {
+  using CS = std::conditional_t<DT == SB_DTYPE_F32, double, float>;
+  static constexpr int kPairs = HALF ? VEC : VEC / 2;  // of a thread
+  static constexpr int kPiece = 16 / sizeof(CS);       // numbers
+  static constexpr int kPieces = 2 * kPairs / kPiece;  // (0, 1: as they come)
+  // Place of pair f's cosine (its sine follows), of `pairs`.
+  __device__ __forceinline__ static int at(int f, int pairs) {
+    if constexpr (kPieces <= 1) return 2 * f;
+    const int e = f % kPairs * 2;
+    return (e / kPiece * (pairs / kPairs) + f / kPairs) * kPiece + e % kPiece;
+  }
+  const CS* first;
+  int step;
+  __device__ __forceinline__ Sines(const CS* token, int unit, int pairs)
+      : first(token + (kPieces <= 1 ? 2 * kPairs : kPiece) * unit), step(pairs / kPairs * kPiece) {}
+  // Cosine and sine of the thread's pair i.
+  template <typename T> __device__ __forceinline__ void get(int i, T* c, T* s) const {
+    const CS* p = kPieces <= 1 ? first + 2 * i : first + 2 * i / kPiece * step + 2 * i % kPiece;
+    *c = p[0], *s = p[1];
+  }
+};
+
 // Rows rows[0 .. n) by a workgroup: thread `unit` of a row takes rows rsub + k rpi, FLIGHT of them at
-// a time. cs: cosine and sine of each (token, pair); cs64: the same in 64 bits (4-bit rows).
+// a time. cs: cosine and sine of each (token, pair), in Sines' order; cs64: the same in 64 bits, pair after pair
+// (4-bit rows).
 template <int DT, int VEC, bool Q4, bool HALF, bool ONCE, int FLIGHT>
 __device__ __forceinline__ void turn_rows(
     const RowRef* rows, int n, const std::conditional_t<DT == SB_DTYPE_F32, double, float>* cs,
@@ -206,7 +232,6 @@ __device__ __forceinline__ void turn_rows(
   at[0] = HALF && !paired ? unit + split.half : unit;
   if constexpr (HALF) at[1] = at[0] + (paired ? split.half : split.rest);
   const bool second = HALF && at[NV - 1] * VEC < head_dim;
-  const int trig_at = unit * VEC * NV;
 
   for (int ib = rsub; ib < n; ib += FLIGHT * rpi) {
     RowVec<DT, VEC> x[FLIGHT][NV];
@@ -224,7 +249,7 @@ __device__ __forceinline__ void turn_rows(
       if (ib + u * rpi >= n) break;
       const RowRef ref = rows[ib + u * rpi];
       if (!ref.src) continue;
-      const CS* trig = cs + (ref.info >> 2) + trig_at;
+      const Sines<DT, VEC, HALF> trig(cs + (ref.info >> 2), unit, pairs);
       const bool turn = (ref.info & 1u) && paired;
       float f[NV][VEC];
       if constexpr (HALF) {
@@ -232,7 +257,8 @@ __device__ __forceinline__ void turn_rows(
         for (int i = 0; i < VEC; ++i) {
           const CS e = Elem<DT>::get(x[u][0].e[i]), o = Elem<DT>::get(x[u][NV - 1].e[i]);
           if (turn) {
-            const CS c = trig[2 * i], s = trig[2 * i + 1];
+            CS c, s;
+            trig.get(i, &c, &s);
             f[0][i] = static_cast<float>(e * c - o * s);
             f[NV - 1][i] = static_cast<float>(e * s + o * c);
           } else {
@@ -245,7 +271,8 @@ __device__ __forceinline__ void turn_rows(
         for (int i = 0; i < VEC; i += 2) {
           const CS e = Elem<DT>::get(x[u][0].e[i]), o = Elem<DT>::get(x[u][0].e[i + 1]);
           if (turn) {
-            const CS c = trig[i], s = trig[i + 1];
+            CS c, s;
+            trig.get(i / 2, &c, &s);
             f[0][i] = static_cast<float>(e * c - o * s);
             f[0][i + 1] = static_cast<float>(e * s + o * c);
           } else {
@@ -282,9 +309,7 @@ __device__ __forceinline__ void turn_rows(
             unsure |= w[v] ^ pack_codes(hi, b[v].value);
           }
           if (block_max<VEC>(unsure)) {
-            const double* t64;
-            if constexpr (kBoth) t64 = cs64 + (ref.info >> 2) + trig_at;
-            else t64 = reinterpret_cast<const double*>(trig);
+            const double* t64 = kBoth ? cs64 + (ref.info >> 2) + unit * VEC * NV : nullptr;
             // (a sum of two values of the largest fp32 exponent may pass fp32, but not 7 * 2^126: such a
             // block, not finite above, is taken times 2^-2)
             const double down = b[0].bad ? 0.25 : 1.0, down_2 = b[NV - 1].bad ? 0.25 : 1.0;
@@ -293,8 +318,11 @@ __device__ __forceinline__ void turn_rows(
             for (int i = 0; i < VEC; i += HALF ? 1 : 2) {
               const int j = HALF ? i : i + 1, t = HALF ? 2 * i : i;
               const double e = Elem<DT>::get(x[u][0].e[i]), o = Elem<DT>::get(x[u][NV - 1].e[j]);
-              f[0][i] = round_to_odd((e * t64[t] - o * t64[t + 1]) * down);
-              f[NV - 1][j] = round_to_odd((e * t64[t + 1] + o * t64[t]) * down_2);
+              double c, s;
+              if constexpr (kBoth) c = t64[t], s = t64[t + 1];
+              else trig.get(t / 2, &c, &s);
+              f[0][i] = round_to_odd((e * c - o * s) * down);
+              f[NV - 1][j] = round_to_odd((e * s + o * c) * down_2);
             }
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
