@@ -17,9 +17,10 @@ namespace {
 
 // Tokens of a dense workgroup (8192 tokens of 32 / 8 heads x 128, bf16 / fp32: 1 31.8 / 61.5 us, 2 27.7 /
 // 62.3, 4 27.7 / 66.2, 8 28.5 / 70.4), rows of a scattering one (28 layers x 6963 pairs of 4 heads x 128: 64
-// 141 us, 128 145, 256 149). Rows in flight of a thread, half pairs: 2 (4: 155 us with 64 rows).
+// 141 us, 128 145, 256 149) and of a shifting one (32 layers x 3001 positions of 8 heads x 128: 32 74 us, 64
+// 76, 128 77, 256 79). Rows in flight of a thread, half pairs: 2 (scatter, 4: 155 us with 64 rows).
 constexpr int kDenseTokens = 2;
-constexpr int kScatterRows = 64;
+constexpr int kScatterRows = 64, kShiftRows = 32;
 enum RotaryMode : int { ROTARY_DENSE = 0, ROTARY_SCATTER = 1, ROTARY_SHIFT = 2 };
 
 struct RotaryArgs {
@@ -162,7 +163,8 @@ int launch_rotary(const char* fn, RotaryArgs a, int32_t layout, int32_t dtype, i
   const int64_t units = a.num_tokens * ((a.rows_per_token + kRowsMax - 1) / kRowsMax);
   a.tokens_per_wg = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(fit, units / 1024)));
   const int64_t gx = (a.num_tokens + a.tokens_per_wg - 1) / a.tokens_per_wg;
-  int per = std::max(1, (MODE == ROTARY_SCATTER ? kScatterRows : kRowsMax) / a.tokens_per_wg);
+  constexpr int kRows = MODE == ROTARY_SCATTER ? kScatterRows : MODE == ROTARY_SHIFT ? kShiftRows : kRowsMax;
+  int per = std::max(1, kRows / a.tokens_per_wg);
   if (a.tokens_per_wg == 1) {
     const int steps = (a.rows_per_token + rpi - 1) / rpi;
     const int ny = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, 512 / gx), steps));
