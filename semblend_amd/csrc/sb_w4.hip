@@ -380,33 +380,40 @@ __device__ __forceinline__ void split3(float x, uint16_t* p) {
   p[2] = f32_to_bf16(r - bf16_to_f32(p[1]));
 }
 
-// sums [rows][blocks of 32 groups][4][32]: thread (row, group of `step` inputs). 8 lanes a group and up.
+// sums [rows][blocks of 32 groups][4][32]: thread (kSumRows rows, 8 inputs of a group of STEP).
+constexpr int kSumRows = 4;
 template <int DT, int STEP>
 __global__ __launch_bounds__(256) void w4_sums_kernel(uint16_t* sums, const char* x, int64_t x_row,
                                                       int64_t num_rows, int k, int blocks) {
-  constexpr int kLanes = STEP / 8;  // lanes of a group, 8 values each
+  constexpr int kLanes = STEP / 8;  // lanes of a group
   const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t per = static_cast<int64_t>(blocks) * 32 * kLanes;
-  const int64_t row = idx / per;
-  const int64_t rest = idx - row * per;
+  const int64_t row0 = idx / per * kSumRows;
+  const int64_t rest = idx - idx / per * per;
   const int64_t k0 = rest * 8;
-  float v = 0.f;
-  if (row < num_rows && k0 < k) {
-    const u32x4_t w = *reinterpret_cast<const u32x4_t*>(x + row * x_row + k0 * 2);
+  u32x4_t w[kSumRows];
+#pragma unroll
+  for (int r = 0; r < kSumRows; ++r) {
+    w[r] = u32x4_t{};
+    if (row0 + r < num_rows && k0 < k) w[r] = *reinterpret_cast<const u32x4_t*>(x + (row0 + r) * x_row + k0 * 2);
+  }
+  const int64_t g = rest / kLanes;
+  const int sub = static_cast<int>(rest % kLanes);
+#pragma unroll
+  for (int r = 0; r < kSumRows; ++r) {
+    float v = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      v += W4<DT>::value(static_cast<uint16_t>(w[i])) + W4<DT>::value(static_cast<uint16_t>(w[i] >> 16));
-  }
+      v += W4<DT>::value(static_cast<uint16_t>(w[r][i])) + W4<DT>::value(static_cast<uint16_t>(w[r][i] >> 16));
 #pragma unroll
-  for (int o = 1; o < kLanes; o <<= 1) v += __shfl_xor(v, o, 64);
-  if (row >= num_rows) return;
-  const int64_t g = rest / kLanes;
-  uint16_t p[3];
-  split3(v, p);
-  uint16_t* out = sums + (row * blocks + g / 32) * 128 + g % 32;
-  // (lanes of the group share the stores: parts, and zeros behind them)
-  const int sub = static_cast<int>(rest % kLanes);
-  if (sub < 4) out[sub * 32] = sub == 0 ? p[0] : sub == 1 ? p[1] : sub == 2 ? p[2] : 0;
+    for (int o = 1; o < kLanes; o <<= 1) v += __shfl_xor(v, o, 64);
+    uint16_t p[3];
+    split3(v, p);
+    // (lanes of the group share the stores: parts, and zeros behind them)
+    if (row0 + r < num_rows && sub < 4)
+      sums[((row0 + r) * blocks + g / 32) * 128 + g % 32 + sub * 32] =
+          sub == 0 ? p[0] : sub == 1 ? p[1] : sub == 2 ? p[2] : 0;
+  }
 }
 
 constexpr int kXcds = 8;
@@ -972,7 +979,7 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
   const int64_t grid = grid_tiles * plan.splits;
   if (grid > 0x7fffffff) return fail(fn, "grid too large");
   a.tiles = static_cast<uint32_t>(grid_tiles);
-  const int64_t work = num_rows * a.sum_blocks * 32 * (table_step(group) / 8);
+  const int64_t work = tiles(num_rows, kSumRows) * a.sum_blocks * 32 * (table_step(group) / 8);
   if (tiles(work, 256) > 0x7fffffff) return fail(fn, "grid too large");
 #define SB_W4(DT, GPT)                                                                                \
   if (dtype == DT && gpt == GPT) {                                                                    \
