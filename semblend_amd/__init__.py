@@ -9,8 +9,10 @@ Drop-in modules (same call surface as SemBlend's ``semblend_core`` modules):
 * :mod:`semblend_amd.pipeline`         — ``PositionMapping``.
 
 Extensions: :mod:`semblend_amd.batch` (several requests over one paged pool),
-:mod:`semblend_amd.multi_donor` (composite scatter from several donors in one pass) and
-:mod:`semblend_amd.paged_cache` (a serving batch's appends and attention, 4-bit pages).
+:mod:`semblend_amd.multi_donor` (composite scatter from several donors in one pass),
+:mod:`semblend_amd.paged_cache` (a serving batch's appends and attention, 4-bit pages),
+:mod:`semblend_amd.rotary` (a model's own rotary positions: half pairs, part of the head, scaled
+frequencies) and :mod:`semblend_amd.quantized` (products with 4-bit weights).
 
 The compute runs in hand-written HIP kernels (``libsemblend_hip.so``, C ABI in
 ``include/semblend_hip.h``) on torch's current stream. ``semblend_amd.compat.install()``

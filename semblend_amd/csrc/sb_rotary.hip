@@ -9,7 +9,11 @@
 //
 // What bounds it: bytes. A workgroup takes a few tokens and some of their rows (heads, or layers x
 // K/V x heads): the sines of a (token, pair), about 45 fp64 instructions, are evaluated once in LDS
-// and serve all of these, and one thread per row works out its addresses (sb_rows.h).
+// and serve all of these, and one thread per row works out its addresses (sb_rows.h). Kernel times: 8192
+// tokens of 32 / 8 heads x 128 in bf16 26.5 us (168 MB, 6.3 TB/s; a large copy reaches 6.6), in fp32 60.5
+// (336 MB, 5.5); 28 layers x 6963 pairs of 4 heads scattered 137 us (799 MB, 5.8 TB/s: rows of 256 bytes, two
+// dependent reads before them); 32 layers x 3001 positions of 8 heads shifted in place 74 us (393 MB, 5.3
+// TB/s); 32 tokens 3.9 us, a launch and its chain.
 #include "sb_rows.h"
 
 namespace sb {
