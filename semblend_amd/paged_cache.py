@@ -285,19 +285,22 @@ def append_kv_paged(
         rot = _index(rotations, dev)
         if rot.shape[0] != num:
             raise ValueError("rotations must have one entry per token")
-    entry, more = "sb_append_kv_paged", ()
-    if rotary is not None:
-        inv = rotary._table(dev, d)
-        entry = "sb_append_kv_rotary_paged"
-        more = (inv.shape[0], rotary._code, 1.0 if rot is not None else rotary._factor)
-    else:
+    qp, qop = (None, None) if q is None else (q.data_ptr(), query_out.data_ptr())
+    if rotary is None:
         inv = inv_freq_table(rope_base, d, dev) if rope_base is not None else None
-    _lib.launch(
-        dev, entry,
-        base, sbase, k.data_ptr(), v.data_ptr(), _lib.ptr(q),
-        None if q is None else query_out.data_ptr(), bt.data_ptr(), bt.stride(0), pos.data_ptr(),
-        _lib.ptr(rot), _lib.ptr(starts), _lib.ptr(inv), num, requests, heads, hq, d, bs, shape[0],
-        width, kst, vst, qst, ost, st, sst, *more, dt, code)
+        _lib.launch(
+            dev, "sb_append_kv_paged",
+            base, sbase, k.data_ptr(), v.data_ptr(), qp, qop, bt.data_ptr(), bt.stride(0),
+            pos.data_ptr(), _lib.ptr(rot), _lib.ptr(starts), _lib.ptr(inv), num, requests, heads, hq, d,
+            bs, shape[0], width, kst, vst, qst, ost, st, sst, dt, code)
+    else:
+        inv = rotary._table(dev, d)
+        _lib.launch(
+            dev, "sb_append_kv_rotary_paged",
+            base, sbase, k.data_ptr(), v.data_ptr(), qp, qop, bt.data_ptr(), bt.stride(0),
+            pos.data_ptr(), _lib.ptr(rot), _lib.ptr(starts), inv.data_ptr(), num, requests, heads, hq, d,
+            bs, shape[0], width, kst, vst, qst, ost, st, sst, inv.shape[0], rotary._code,
+            1.0 if rot is not None else rotary._factor, dt, code)
     if new and query.requires_grad:
         return _recorded("append_kv_paged", query_out, query)
     return query_out
