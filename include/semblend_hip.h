@@ -689,9 +689,9 @@ int sb_paged_attention(void* out, const void* q, const void* kv_cache, const voi
  * pairs of whole heads by plain frequencies)
  *
  * Shared by the entries, and by sb_append_kv_rotary_paged: the first 2 * pairs elements of a row
- * are turned and the others kept; layout SB_ROTARY_INTERLEAVED, or SB_ROTARY_HALF with an even number of pairs;
- * inv_freq: device fp32 [pairs], at most 1. Angles, sines and cosines in 64 bits, one rounding to
- * dtype. head_dim even, at most 512.
+ * are turned and the others kept; layout SB_ROTARY_INTERLEAVED, or SB_ROTARY_HALF with an even number
+ * of pairs; inv_freq: device fp32 [pairs], 0 to 1. Angles, sines and cosines in 64 bits, one rounding
+ * to dtype. head_dim even, at most 512. Addresses of layers are 16-byte aligned.
  * ---------------------------------------------------------------------------------------- */
 
 /* query_out[t, h] = query[t, h] turned by positions[t] (any int32), and key likewise (NULL: none):
@@ -760,9 +760,9 @@ int sb_w4_dequantize(void* out, const void* packed, const void* table, int64_t o
                      int32_t dtype, void* stream);
 
 /* y [num_rows, out_features] = x [num_rows, in_features] w^T + bias (NULL: none), rows by strides
- * in elements, x 16-byte aligned in base and stride, all in dtype (bf16 or fp16): exact weights,
- * fp32 sums, one rounding. workspace: 16-byte aligned, sb_w4_linear_workspace_size bytes (may be
- * NULL where that is 0). */
+ * in elements (those of y must not overlap), x 16-byte aligned in base and stride, all in dtype (bf16
+ * or fp16): exact weights, fp32 sums, one rounding. workspace: 16-byte aligned,
+ * sb_w4_linear_workspace_size bytes (may be NULL where that is 0). */
 int64_t sb_w4_linear_workspace_size(int64_t num_rows, int64_t out_features, int64_t in_features,
                                     int64_t group, int32_t dtype);
 int sb_w4_linear(void* y, const void* x, const void* packed, const void* table, const void* bias,

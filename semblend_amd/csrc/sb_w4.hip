@@ -914,6 +914,8 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
   if (x_stride < 0 || x_stride > kInputsMax) return fail(fn, "row stride past its limit");
   if (reinterpret_cast<uintptr_t>(x) % 16 || x_stride * 2 % 16)
     return fail(fn, "rows of x must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(packed) % 16 || reinterpret_cast<uintptr_t>(table) % 16)
+    return fail(fn, "packed codes and table must be 16-byte aligned");
   W4Args a = {};
   a.y = static_cast<char*>(y);
   a.x = static_cast<const char*>(x);
@@ -933,6 +935,7 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
   const int64_t need = sb_w4_linear_workspace_size(num_rows, out_features, in_features, group, dtype);
   if (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < need))
     return fail(fn, "workspace too small or not 16-byte aligned");
+  if (num_rows > 1 && y_stride < out_features) return fail(fn, "rows of y must not overlap");
   a.wide_out = reinterpret_cast<uintptr_t>(y) % 16 == 0 && a.y_row % 16 == 0;
   a.sums = static_cast<const char*>(workspace);
   a.sum_blocks = plan.sum_blocks;

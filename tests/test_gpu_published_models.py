@@ -223,6 +223,37 @@ def test_decode_steps_captured(dev, quant):
         pos += 1
 
 
+def test_projection_captured(dev):
+    """The projection in parts captured with positions and hidden states that change from replay to
+    replay, rows outside the hidden states among them."""
+    hq, hkv, d, hidden, bs, seq, rows = 4, 2, 64, 256, 16, 90, 37
+    _, qw = _weight((hq + 2 * hkv) * d, hidden, 64, BF16, 1)
+    rot = RotaryEmbedding.from_config(d, 1e4)
+    table, nb = _table(seq + 40, bs, 2)
+    bt = table.cuda()
+    x = torch.zeros((seq, hidden), dtype=BF16, device="cuda")
+    pos = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    a, b = (torch.zeros((nb, 2, hkv, bs, d), dtype=BF16, device="cuda") for _ in range(2))
+    for kw in (dict(rotary=rot), dict(rope_base=1e4), {}):
+        step = lambda c: tk.qkv_projection_paged(x, qw, pos, c, bt, hq, hkv, d, **kw)
+        pos.copy_(torch.arange(rows))
+        step(a.clone())
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step(a)
+        for i in range(4):
+            x.copy_(randn((seq, hidden), BF16, 10 + i))
+            pos.copy_(torch.randperm(seq + 30, generator=gen(20 + i))[:rows])
+            want = step(b)
+            got.fill_(3.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert_bit_exact(got.cpu(), want.cpu())
+            assert_bit_exact(a.cpu(), b.cpu())
+            assert (got.cpu()[pos.cpu() >= seq] == 0).all()
+
+
 def _packed(x):
     c, s = pref.quantize(x)
     return (c[..., 0::2] | c[..., 1::2] << 4).to(torch.uint8), s

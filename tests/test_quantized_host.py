@@ -120,6 +120,8 @@ def _unpack(**over):
     (_linear, dict(k=(1 << 22) + 64), b"limit"), (_linear, dict(xs=(1 << 22) + 8), b"limit"),
     (_linear, dict(m=4096, n=8192, k=1024, xs=1024), b"workspace"),
     (_linear, dict(m=4096, n=8192, k=1024, xs=1024, ws=FAKE, wsb=100), b"workspace"),
+    (_linear, dict(w=FAKE + 8), b"aligned"), (_linear, dict(t=FAKE + 4), b"aligned"),
+    (_linear, dict(ys=0), b"overlap"), (_linear, dict(ys=31), b"overlap"),
     (_pack, dict(c=None), b"null"), (_pack, dict(g=16), b"multiple of 32"), (_pack, dict(k=0), b"positive"),
     (_pack, dict(w=FAKE + 8), b"aligned"), (_unpack, dict(dt=3), b"invalid dtype"),
     (_unpack, dict(sdt=3), b"scales"), (_unpack, dict(o=None), b"null"),

@@ -211,7 +211,8 @@ Q4 = dict(cdt=3, scales=FAKE, ss=_i64(1, 1, 1, 1, 1))
     (_apply, dict(d=63), b"even"), (_apply, dict(d=514), b"512"), (_apply, dict(pairs=0), b"pair"),
     (_apply, dict(pairs=31), b"even number"), (_apply, dict(layout=2), b"layout"),
     (_apply, dict(factor=0.0), b"factor"), (_apply, dict(factor=math.nan), b"factor"),
-    (_apply, dict(qs=_i64(256, 64, 2)), b"contiguous"), (_apply, dict(n=1 << 31), b"limit"),
+    (_apply, dict(qs=_i64(256, 64, 2)), b"contiguous"),
+    (_apply, dict(qos=_i64(0, 64, 1)), b"overlap"), (_apply, dict(qos=_i64(256, 0, 1)), b"overlap"), (_apply, dict(n=1 << 31), b"limit"),
     (_append, dict(inv=None), b"null"), (_append, dict(pairs=65), b"head_dim / 2"),
     (_append, dict(layout=-1), b"layout"), (_append, dict(Q4, pairs=16), b"whole blocks"),
     (_append, dict(Q4, pairs=48), b"whole blocks"), (_append, dict(Q4, pairs=8, layout=0), b"whole blocks"),
