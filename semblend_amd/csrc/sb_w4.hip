@@ -6,7 +6,8 @@
 // S = sum x from the matrix cores, sum x w = scale (P - (B + zero) S). Nothing is rounded on the way but
 // the fp32 sums, so that the result is that of the 16-bit inputs and the exact weights, rounded once; B + c
 // against c - zero costs the sums two or three of their 24 bits (six in fp16). fp16 has a packed
-// subtraction, and from 33 rows, where P and S cost more than it, P = sum x (c - zero) and sum x w = scale P.
+// subtraction: with 64 rows a workgroup and in tiles, where S costs more than it, P = sum x (c - zero) and
+// sum x w = scale P.
 //
 // Layout, made once (w4_pack_kernel): 16 features x 128 inputs are 1 KiB, lane l of a wave holding 16
 // bytes: word j the codes of feature l % 16, inputs 32 j + 8 (l / 16) + 0 .. 7, which is the operand of one
