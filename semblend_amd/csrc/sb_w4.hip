@@ -15,6 +15,7 @@
 // and zeros share words (scale's bits, 16 + zero as the upper half of an fp32) per feature and group of
 // 32, 64 or 128 inputs, 16 features in a row.
 #include "sb_common.h"
+#include "sb_w4_plan.h"
 
 #include <algorithm>
 
@@ -26,8 +27,6 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kTileN = 16;    // features of a tile
-constexpr int kTileK = 128;   // inputs of a tile
 constexpr int64_t kInputsMax = int64_t{1} << 22;  // inputs, and row stride: 128 rows stay within 2^31 bytes
 
 // A constant that the compiler does not know as one, in a scalar or a vector register: (w & mask) | base
@@ -425,7 +424,6 @@ __global__ __launch_bounds__(256) void w4_sums_kernel(uint16_t* sums, const char
 
 constexpr int kXcds = 8;
 constexpr int kBand = 8;       // row tiles of a band of the tile order
-constexpr int kBM = 128, kBN = 128;
 
 // Tile of workgroup b: workgroups go round-robin to the XCDs, each of which gets a contiguous range of
 // an order that walks bands of kBand row tiles, feature tile by feature tile, so that the workgroups of
@@ -740,11 +738,6 @@ __global__ __launch_bounds__(256) void w4_unpack_kernel(char* out, const uint32_
   }
 }
 
-int64_t tiles(int64_t x, int64_t by) { return (x + by - 1) / by; }
-
-// Inputs that share a table word: the group, or the largest of 32, 64 and 128 that divides it.
-int64_t table_step(int64_t group) { return group % 128 == 0 ? 128 : group % 64 == 0 ? 64 : 32; }
-
 const char* shape_fault(int64_t n, int64_t k, int64_t group) {
   if (n <= 0 || k <= 0 || group <= 0) return "sizes must be positive";
   if (n > 0x7fffffe0 || k > kInputsMax) return "size past its limit";
@@ -818,75 +811,6 @@ extern "C" int sb_w4_dequantize(void* out, const void* packed, const void* table
 namespace sb {
 namespace {
 
-int64_t sum_blocks(int64_t k, int64_t group) { return tiles(tiles(k, kTileK) * (kTileK / table_step(group)), 32); }
-
-// How a call runs: few rows (workgroups of R rows and 16 J features), or 128 x 128 tiles with the steps
-// (tiles of inputs, and of sums) in `splits` slices.
-struct W4Plan {
-  bool tiled;
-  int r, j;
-  int splits, split_steps, sum_blocks;
-};
-
-// The few-rows kernel: a workgroup reads its rows once for all of its features and its codes once for all
-// of its rows, so that more of either mean fewer reads and fewer, longer workgroups. R (no larger than holds
-// the rows) and J are those of the least time by this model, in us for K inputs on 256 CUs: 2.5 + rounds (0.5
-// + kRound K / 1024), a round a workgroup per CU (32 and 64 rows: its second part a fifth more from five
-// rounds on). Measured, J = 1 to 4: 64 rows, R = 64, of 3584 -> 4608 13.7, 9.0, 11.0, 13.4 us; 4096 -> 12288
-// 25.8, 19.0, 14.7, 14.6; 3584 -> 37888 59.0, 38.8, 38.8, 36.2; 18944 -> 3584 29.8, 39.0, 45.0, 59.0; 32
-// rows, R = 32, of 4096 -> 131072 (fp16) 146, 106, 88, 80; 16 of 4096 -> 12288 9.2, 8.4, 7.5, 7.9. The
-// largest R and the one taken: 64 rows of 3584 -> 4608 8.9 and 7.7 (R = 32, J = 3), of 18944 -> 3584 29.5 and
-// 22.4 (32, 2); 32 rows of 18944 -> 3584 18.1 and 16.5 (16, 2). (Up to 4 rows J = 1 or 2: what is left is
-// the codes.)
-// More than 64 rows take tiles where their model is less: 3, the sums' launch 4 (bf16), a step 1.08 with one
-// workgroup a CU and 0.85 each with more; slices: the merge's launch 4 and their traffic. Measured, few rows
-// against tiles in their best split: 3584 -> 4608, 128 rows 11.4 and 22.9 us, 256 rows 20.5 and 26.0, 614 rows
-// 38.3 and 37.2; 18944 -> 3584 (groups of 64), 192 rows 50.7 and 55.2, 320 rows 94.1 and 72.6; 3584 -> 37888,
-// 96 rows 61.9 and 53.8; 896 -> 1152, 256 rows 5.1 and 14.7. (Of 60 sizes drawn at random, up to 630 rows, 30000
-// features and 16384 inputs, the form taken is within 6% of the fastest one, but for six of under 10 us that
-// are 8 to 22% behind. Tiles of 32 and 64 rows that four waves share were no faster: 64 rows of 3584 ->
-// 37888 42 us.)
-W4Plan w4_plan(int64_t m, int64_t n, int64_t k, int64_t group, int32_t dtype) {
-  W4Plan p = {};
-  const int64_t nt = tiles(n, kTileN), kt = tiles(k, kTileK);
-  const auto rounds = [](int64_t wgs) { return tiles(wgs, 256); };
-  constexpr int kRows[4] = {4, 16, 32, 64};
-  constexpr double kNever = 1e30;
-  constexpr double kRound[4][4] = {{0.6, 0.7, kNever, kNever},
-                                   {0.6, 0.75, 1.1, 1.38},
-                                   {0.83, 1.1, 1.5, 1.75},
-                                   {1.47, 1.84, 2.35, 2.87}};
-  const int first = m <= 4 ? 0 : 1, last = m <= 4 ? 0 : m <= 16 ? 1 : m <= 32 ? 2 : 3;
-  double best = kNever;
-  for (int r = first; r <= last; ++r)
-    for (int j = 1; j <= 4; ++j) {
-      const int64_t gy = tiles(m, kRows[r]), turns = rounds(tiles(nt, j) * gy);
-      const double more = r > 1 && turns > 4 ? 1.2 : 1.0;
-      const double t = 2.5 + static_cast<double>(turns) *
-                                 (0.5 + kRound[r][j - 1] * more * static_cast<double>(k) / 1024);
-      if (gy > 65535 || t >= best) continue;  // (a grid's second axis ends there)
-      best = t;
-      p.r = kRows[r], p.j = j;
-    }
-  p.splits = 1;
-  p.split_steps = static_cast<int>(kt);
-  const int64_t blocks = dtype == SB_DTYPE_BF16 ? sum_blocks(k, group) : 0;
-  const int64_t steps = kt + blocks, grid = tiles(m, kBM) * tiles(n, kBN);
-  for (int64_t s = 1; m > 64 && s <= 32 && (s == 1 || 2 * s <= steps); ++s) {
-    const int64_t per = tiles(steps, s), slices = tiles(steps, per);
-    if (slices != s) continue;
-    const double load = static_cast<double>(rounds(grid * s));
-    double t = 3.0 + (blocks ? 4.0 : 0.0) + static_cast<double>(per) * (load <= 1.0 ? 1.08 : 0.85 * load);
-    if (s > 1) t += 4.0 + static_cast<double>(s * m) * static_cast<double>(n) * 8.0 / 6e6;
-    if (t >= best) continue;
-    best = t;
-    p.tiled = true;
-    p.splits = static_cast<int>(s);
-    p.split_steps = static_cast<int>(per);
-    p.sum_blocks = static_cast<int>(blocks);
-  }
-  return p;
-}
 int64_t sums_bytes(const W4Plan& p, int64_t m) { return m * p.sum_blocks * 256; }
 
 }  // namespace
@@ -896,7 +820,7 @@ extern "C" int64_t sb_w4_linear_workspace_size(int64_t num_rows, int64_t out_fea
                                                int64_t group, int32_t dtype) {
   using namespace sb;
   if (num_rows <= 0 || shape_fault(out_features, in_features, group)) return 0;
-  const W4Plan p = w4_plan(num_rows, out_features, in_features, group, dtype);
+  const W4Plan p = w4_plan(num_rows, out_features, in_features, group, dtype == SB_DTYPE_BF16);
   return sums_bytes(p, num_rows) + (p.splits > 1 ? p.splits * num_rows * out_features * 4 : 0);
 }
 
@@ -935,7 +859,7 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
   a.scales_f16 = scale_dtype == SB_DTYPE_F16;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int gpt = static_cast<int>(kTileK / table_step(group));
-  const W4Plan plan = w4_plan(num_rows, out_features, in_features, group, dtype);
+  const W4Plan plan = w4_plan(num_rows, out_features, in_features, group, dtype == SB_DTYPE_BF16);
   const int64_t need = sb_w4_linear_workspace_size(num_rows, out_features, in_features, group, dtype);
   if (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < need))
     return fail(fn, "workspace too small or not 16-byte aligned");
@@ -950,15 +874,7 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
   if (!plan.tiled) {
     const int64_t gy = tiles(num_rows, plan.r);
     const int64_t nt = tiles(out_features, kTileN);
-    // Up to 16 rows: 16 waves where a workgroup has 16 features (a CU has one or two of them then) and a
-    // tile of inputs for each wave (one row of 18944 -> 3584 9.8 -> 9.1 us, 16 rows 12.9 -> 11.8; of 896 ->
-    // 1152 2.9 and 3.0), and codes read past the caches where these cannot keep them until the next call
-    // (one row of 4096 -> 131072, 268 MB: 47.9 -> 45.2 us; 16 of 3584 -> 37888, 68 MB, 15.3 and 19.6).
-    const bool many = plan.r <= 16 && plan.j == 1 && a.k_tiles > 16;
-    const bool once = plan.r <= 16 && plan.j > 1 && gy == 1 &&
-                      sb_w4_codes_size(out_features, in_features) >= (int64_t{192} << 20);
     // Two steps in flight where a CU's LDS holds two such workgroups, else one (other waves run meanwhile).
-    // (64 rows and features: LDS holds seven waves' steps)
 #define SB_W4_L(DT, R, J, GPT, W, ONCE)                                                               \
   do {                                                                                                \
     constexpr int kAhead = 2 * W * RowsStage<R, J, GPT>::kBytes <= 80 * 1024 ? 2 : 1;                 \
@@ -968,8 +884,8 @@ extern "C" int sb_w4_linear(void* y, const void* x, const void* packed, const vo
 #define SB_W4(DT, R, J, GPT)                                                                          \
   if (dtype == DT && plan.r == R && plan.j == J && gpt == GPT) {                                      \
     if constexpr (R <= 16) {                                                                          \
-      if (J == 1 && many) SB_W4_L(DT, R, 1, GPT, 16, false);                                          \
-      else if (J > 1 && once) SB_W4_L(DT, R, (J > 1 ? J : 2), GPT, 8, true);                          \
+      if (J == 1 && plan.waves == 16) SB_W4_L(DT, R, 1, GPT, 16, false);                              \
+      else if (J > 1 && plan.once) SB_W4_L(DT, R, (J > 1 ? J : 2), GPT, 8, true);                     \
       else SB_W4_L(DT, R, J, GPT, 8, false);                                                          \
     } else {                                                                                          \
       SB_W4_L(DT, R, J, GPT, (R == 64 && J == 4 ? 7 : 8), false);                                     \
