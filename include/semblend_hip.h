@@ -761,7 +761,8 @@ int sb_w4_dequantize(void* out, const void* packed, const void* table, int64_t o
 
 /* y [num_rows, out_features] = x [num_rows, in_features] w^T + bias (NULL: none), rows by strides
  * in elements (those of y must not overlap), x 16-byte aligned in base and stride, all in dtype (bf16
- * or fp16): exact weights, fp32 sums, one rounding. workspace: 16-byte aligned,
+ * or fp16): exact weights, fp32 sums, one rounding. |x| below 2^116, scales below 2^122 and an output's
+ * sum of |x| |scale| below 2^120 keep the sums within fp32. workspace: 16-byte aligned,
  * sb_w4_linear_workspace_size bytes (may be NULL where that is 0). */
 int64_t sb_w4_linear_workspace_size(int64_t num_rows, int64_t out_features, int64_t in_features,
                                     int64_t group, int32_t dtype);

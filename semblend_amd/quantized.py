@@ -130,8 +130,10 @@ def quantized_linear(
 
     x: [..., in_features] bf16 or fp16, any number of rows; bias: [out_features] of x's type; ``out``:
     [..., out_features] of x's type with a unit last stride and rows at one stride (a new tensor by
-    default; returned). Values of x must be finite and below 2^119 in magnitude: a row that holds an
-    infinity or a NaN gives NaN (or infinities), other rows are not affected. ``out`` must not overlap x.
+    default; returned). Range: x finite and below 2^116 in magnitude, scales below 2^122, and an output's
+    sum of |x| |scale| below 2^120 (those of fp16 inputs and scales always are): the fp32 sums of a group of
+    inputs are up to 31 times as large. A row that holds an infinity or a NaN gives NaN (or infinities), other rows
+    are not affected. ``out`` must not overlap x.
     Groups of 128 in bf16: one row of 3584 -> 4608 6.5 us, 8 of 3584 -> 37888 14, 2458 of 3584 -> 4608
     91; one of 4096 -> 131072 in fp16 44. Extension with no reference counterpart.
     """
