@@ -178,7 +178,8 @@ class RotaryEmbedding:
             if dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a rotary embedding's first call on a device cannot be captured "
                                    "into a graph: make one call before")
-            table = self._tables[dev] = self._inv_freq.to(dev)  # (waits: any stream may use it)
+            # (waits: any stream may use it; of two threads' first calls one's copy is kept, for both)
+            table = self._tables.setdefault(dev, self._inv_freq.to(dev))
         return table
 
 
