@@ -696,7 +696,8 @@ int sb_paged_attention(void* out, const void* q, const void* kv_cache, const voi
 
 /* query_out[t, h] = query[t, h] turned by positions[t] (any int32), and key likewise (NULL: none):
  * [num_tokens, heads, head_dim] by strides (token, head, dim) in elements. cosine and sine are
- * multiplied by factor. An output may be its input; it must not overlap it otherwise. */
+ * multiplied by factor. An output may be its input; it must not overlap it otherwise, and its rows must not
+ * overlap each other (checked). */
 int sb_apply_rotary(void* query_out, const void* query, void* key_out, const void* key,
                     const int32_t* positions, const float* inv_freq, int64_t num_tokens,
                     int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,

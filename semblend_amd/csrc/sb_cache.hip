@@ -289,6 +289,8 @@ int append_kv(
   if (k_strides[2] != 1 || v_strides[2] != 1 || kv_strides[4] != 1 ||
       (q4 && scale_strides[4] != 1) || (has_q && (q_strides[2] != 1 || qo_strides[2] != 1)))
     return fail(fn, "the last dimension must be contiguous");
+  if (has_q && rows_overlap(num_tokens, num_q_heads, head_dim, qo_strides[0], qo_strides[1]))
+    return fail(fn, "rows of query_out must not overlap");
   const int64_t es = elem_size(dtype);
   AppendArgs a = {};
   a.k = static_cast<const char*>(key);

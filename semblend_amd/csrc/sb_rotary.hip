@@ -279,10 +279,8 @@ extern "C" int sb_apply_rotary(void* query_out, const void* query, void* key_out
   if (const char* why = rotary_fault(head_dim, pairs, layout, factor)) return fail(fn, why);
   if (q_strides[2] != 1 || qo_strides[2] != 1 || (has_k && (k_strides[2] != 1 || ko_strides[2] != 1)))
     return fail(fn, "the last dimension must be contiguous");
-  const auto overlap = [&](const int64_t* st, int64_t heads) {
-    return (num_tokens > 1 && st[0] == 0) || (heads > 1 && st[1] == 0);
-  };
-  if (overlap(qo_strides, num_q_heads) || (has_k && overlap(ko_strides, num_kv_heads)))
+  if (rows_overlap(num_tokens, num_q_heads, head_dim, qo_strides[0], qo_strides[1]) ||
+      (has_k && rows_overlap(num_tokens, num_kv_heads, head_dim, ko_strides[0], ko_strides[1])))
     return fail(fn, "rows of an output must not overlap");
   const int64_t es = elem_size(dtype);
   RotaryArgs a = {};

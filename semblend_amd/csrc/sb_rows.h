@@ -8,6 +8,7 @@
 #pragma once
 
 #include "sb_common.h"
+#include "sb_overlap.h"
 
 #include <algorithm>
 #include <type_traits>

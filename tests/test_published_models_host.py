@@ -2,10 +2,16 @@
 
 from __future__ import annotations
 
+import ctypes
+import shutil
+import subprocess
 import threading
+from pathlib import Path
 
+import pytest
 import torch
 
+from semblend_amd import _lib
 from semblend_amd.rotary import RotaryEmbedding
 
 
@@ -34,3 +40,41 @@ def test_first_calls_of_two_threads_share_one_table():
         t.join(20)
     assert got[0] is not None and got[0] is got[1]
     assert rot._table(cpu, 64) is got[0]
+
+
+HERE = Path(__file__).resolve().parent
+FAKE = 4096  # an address that is never read: the checks come first
+
+
+def _i64(*v):
+    return (ctypes.c_int64 * len(v))(*v)
+
+
+def test_rows_overlap_is_that_of_all_pairs(tmp_path):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("g++ not available")
+    exe = tmp_path / "overlap_check"
+    subprocess.run([gxx, "-O2", "-std=c++17", "-o", str(exe), str(HERE / "overlap_check.cpp")], check=True,
+                   capture_output=True, text=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and " 0 wrong" in r.stdout, r.stdout
+
+
+@pytest.mark.parametrize("strides", [(64, 64), (64, 128), (200, 32), (0, 64), (256, 0), (-64, 64), (128, 96)])
+@pytest.mark.parametrize("out", ["query", "key", "append"])
+def test_outputs_whose_rows_overlap_are_refused(out, strides):
+    """Three tokens of four heads of 64."""
+    plain, bad = _i64(256, 64, 1), _i64(*strides, 1)
+    if out == "append":
+        cache = _i64(8192, 4096, 1024, 64, 1)
+        rc = _lib.lib().sb_append_kv_rotary_paged(
+            FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, 4, FAKE, None, None, FAKE, 3, 1, 4, 4, 64, 16, 8, 4, plain,
+            plain, plain, bad, cache, None, 32, 1, 1.0, 2, 2, None)
+    else:
+        key = out == "key"
+        rc = _lib.lib().sb_apply_rotary(
+            FAKE, FAKE, FAKE if key else None, FAKE if key else None, FAKE, FAKE, 3, 4, 4 if key else 0, 64, plain,
+            plain if key else bad, plain if key else None, bad if key else None, 32, 1, 1.0, 2, None)
+    assert rc == _lib.SB_ERR_INVALID_ARGUMENT
+    assert b"overlap" in _lib.lib().sb_last_error_string()
