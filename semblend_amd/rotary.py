@@ -118,14 +118,29 @@ class RotaryEmbedding:
         self._tables: dict = {}
 
     @classmethod
-    def from_config(cls, head_dim: int, rope_base: float = 10000.0, rotary_dim: int | None = None,
-                    layout: str = "half", scaling: dict | None = None) -> "RotaryEmbedding":
+    def from_config(cls, head_dim: int, rope_base: float | None = None,
+                    rotary_dim: int | None = None, layout: str = "half",
+                    scaling: dict | None = None) -> "RotaryEmbedding":
         """From a model's configuration: ``rotary_dim`` elements of a head are turned (all by default)
-        by 1 / rope_base^(2i / rotary_dim), changed by ``scaling``, a dictionary as configurations
-        hold it ("rope_type" or "type" and its numbers): "default", "linear", "llama3" (by
-        wavelength) and "yarn". Others are refused: give their frequencies to the constructor. (A
+        by 1 / rope_base^(2i / rotary_dim) (10000 by default), changed by ``scaling``, a dictionary as
+        configurations hold it ("rope_type" or "type" and its numbers): "default", "linear", "llama3"
+        (by wavelength) and "yarn". Others are refused: give their frequencies to the constructor. (A
         scaling that changes with the length of the context turns cached K of other lengths by
-        other frequencies, which no shift corrects.)"""
+        other frequencies, which no shift corrects.) Where the dictionary holds "rope_theta" or
+        "partial_rotary_factor", these are the rope_base and the share of the head that is turned; an
+        argument that says otherwise is refused."""
+        theta, part = ((scaling or {}).get(k) for k in ("rope_theta", "partial_rotary_factor"))
+        if theta is not None:
+            if rope_base is not None and float(rope_base) != float(theta):
+                raise ValueError(f"rope_base is {rope_base}, scaling holds a rope_theta of {theta}")
+            rope_base = float(theta)
+        if part is not None:
+            turned = int(head_dim * float(part))
+            if rotary_dim is not None and int(rotary_dim) != turned:
+                raise ValueError(f"rotary_dim is {rotary_dim}, scaling holds a partial_rotary_factor "
+                                 f"of {part}")
+            rotary_dim = turned
+        rope_base = 10000.0 if rope_base is None else rope_base
         n = head_dim if rotary_dim is None else int(rotary_dim)
         if n < 2 or n % 2 or n > head_dim:
             raise ValueError("rotary_dim must be even, between 2 and head_dim")

@@ -78,3 +78,28 @@ def test_outputs_whose_rows_overlap_are_refused(out, strides):
             plain if key else bad, plain if key else None, bad if key else None, 32, 1, 1.0, 2, None)
     assert rc == _lib.SB_ERR_INVALID_ARGUMENT
     assert b"overlap" in _lib.lib().sb_last_error_string()
+
+
+@pytest.mark.parametrize("scaling", [
+    {"rope_type": "default"}, {"type": "linear", "factor": 4.0},
+    {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+     "original_max_position_embeddings": 8192},
+    {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768}])
+def test_base_and_part_of_the_dictionary(scaling):
+    """A dictionary that holds the base and the turned share of the head gives what the arguments give."""
+    want = RotaryEmbedding.from_config(128, 5e5, rotary_dim=64, scaling=scaling)
+    both = {**scaling, "rope_theta": 500000, "partial_rotary_factor": 0.5}
+    for got in (RotaryEmbedding.from_config(128, scaling=both),
+                RotaryEmbedding.from_config(128, 5e5, 64, scaling=both),
+                RotaryEmbedding.from_config(128, rotary_dim=64, scaling={**scaling, "rope_theta": 5e5}),
+                RotaryEmbedding.from_config(128, 5e5, scaling={**scaling, "partial_rotary_factor": 0.5})):
+        assert torch.equal(got.inv_freq, want.inv_freq)
+        assert (got.rotary_dim, got.factor) == (64, want.factor)
+    for bad in (dict(rope_base=1e4), dict(rotary_dim=128), dict(rotary_dim=32)):
+        with pytest.raises(ValueError, match="holds"):
+            RotaryEmbedding.from_config(128, scaling=both, **bad)
+    for part in (0.0, 1.5, 0.01):
+        with pytest.raises(ValueError, match="rotary_dim"):
+            RotaryEmbedding.from_config(128, scaling={**scaling, "partial_rotary_factor": part})
+    plain = RotaryEmbedding.from_config(128)
+    assert torch.equal(plain.inv_freq, RotaryEmbedding.from_config(128, 1e4).inv_freq)
