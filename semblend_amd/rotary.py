@@ -35,7 +35,9 @@ def _base_frequencies(rope_base: float, rotary_dim: int) -> torch.Tensor:
 
 
 def _number(scaling: dict, key: str, default=None) -> float:
-    value = scaling.get(key, default)
+    value = scaling.get(key)
+    if value is None:  # (configurations write null for what is not set)
+        value = default
     if value is None:
         raise ValueError(f"scaling needs {key!r}")
     return float(value)
@@ -72,7 +74,8 @@ def _by_rotations(f: torch.Tensor, rope_base: float, scaling: dict) -> tuple[tor
         return dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(rope_base))
 
     low, high = pair_of(fast), pair_of(slow)
-    if scaling.get("truncate", True):
+    truncate = scaling.get("truncate")
+    if truncate is None or truncate:
         low, high = math.floor(low), math.ceil(high)
     low, high = max(low, 0), min(high, dim - 1)
     if low == high:
@@ -149,7 +152,8 @@ class RotaryEmbedding:
         f, factor = _base_frequencies(rope_base, n), 1.0
         kind = "default"
         if scaling:
-            kind = scaling.get("rope_type", scaling.get("type"))
+            kind = scaling.get("rope_type")
+            kind = scaling.get("type") if kind is None else kind
         if kind == "linear":
             by = _number(scaling, "factor")
             if not by >= 1:

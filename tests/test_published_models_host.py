@@ -103,3 +103,18 @@ def test_base_and_part_of_the_dictionary(scaling):
             RotaryEmbedding.from_config(128, scaling={**scaling, "partial_rotary_factor": part})
     plain = RotaryEmbedding.from_config(128)
     assert torch.equal(plain.inv_freq, RotaryEmbedding.from_config(128, 1e4).inv_freq)
+
+
+def test_null_is_what_is_not_set():
+    yarn = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768}
+    unset = dict.fromkeys(("beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate",
+                           "rope_theta", "partial_rotary_factor", "type"))
+    want = RotaryEmbedding.from_config(128, 1e6, scaling=yarn)
+    got = RotaryEmbedding.from_config(128, 1e6, scaling={**unset, **yarn})
+    assert torch.equal(got.inv_freq, want.inv_freq) and got.factor == want.factor
+    older = {"rope_type": None, "type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768}
+    assert torch.equal(RotaryEmbedding.from_config(128, 1e6, scaling=older).inv_freq, want.inv_freq)
+    whole = RotaryEmbedding.from_config(128, 1e6, scaling={**yarn, "truncate": False})
+    assert not torch.equal(whole.inv_freq, want.inv_freq)
+    with pytest.raises(ValueError, match="factor"):
+        RotaryEmbedding.from_config(128, 1e6, scaling={**yarn, "factor": None})
