@@ -755,7 +755,8 @@ int sb_w4_pack(void* packed, void* table, const uint8_t* codes, const void* scal
                const uint8_t* zeros, int64_t out_features, int64_t in_features, int64_t group,
                int64_t codes_stride, int64_t scales_stride, int64_t zeros_stride, void* stream);
 
-/* out [out_features, in_features] (row stride out_stride) = the weights, rounded once to dtype. */
+/* out [out_features, in_features] (rows by out_stride, not overlapping) = the weights, rounded once to
+ * dtype. */
 int sb_w4_dequantize(void* out, const void* packed, const void* table, int64_t out_features,
                      int64_t in_features, int64_t group, int64_t out_stride, int32_t scale_dtype,
                      int32_t dtype, void* stream);

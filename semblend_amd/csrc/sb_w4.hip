@@ -791,6 +791,9 @@ extern "C" int sb_w4_dequantize(void* out, const void* packed, const void* table
   if (const char* why = shape_fault(out_features, in_features, group)) return fail(fn, why);
   if (elem_size(dtype) == 0) return fail(fn, "invalid dtype");
   if (scale_dtype != SB_DTYPE_F16 && scale_dtype != SB_DTYPE_BF16) return fail(fn, "invalid dtype of scales");
+  if (reinterpret_cast<uintptr_t>(packed) % 16 || reinterpret_cast<uintptr_t>(table) % 16)
+    return fail(fn, "packed codes and table must be 16-byte aligned");
+  if (out_features > 1 && out_stride < in_features) return fail(fn, "rows of out must not overlap");
   const int64_t gx = tiles(out_features * (in_features / 8), 256);
   if (gx > 0x7fffffff) return fail(fn, "grid too large");
   const hipStream_t st = static_cast<hipStream_t>(stream);

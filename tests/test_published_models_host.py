@@ -118,3 +118,13 @@ def test_null_is_what_is_not_set():
     assert not torch.equal(whole.inv_freq, want.inv_freq)
     with pytest.raises(ValueError, match="factor"):
         RotaryEmbedding.from_config(128, 1e6, scaling={**yarn, "factor": None})
+
+
+@pytest.mark.parametrize("over,words", [(dict(stride=127), b"overlap"), (dict(stride=0), b"overlap"),
+                                        (dict(packed=FAKE + 8), b"aligned"), (dict(table=FAKE + 4), b"aligned")])
+def test_dequantize_refusals(over, words):
+    a = dict(packed=FAKE, table=FAKE, stride=128)
+    a.update(over)
+    rc = _lib.lib().sb_w4_dequantize(FAKE, a["packed"], a["table"], 32, 128, 64, a["stride"], 2, 2, None)
+    assert rc == _lib.SB_ERR_INVALID_ARGUMENT
+    assert words in _lib.lib().sb_last_error_string()
