@@ -44,7 +44,8 @@ def _number(scaling: dict, key: str, default=None) -> float:
 
 
 def _by_wavelength(f: torch.Tensor, scaling: dict) -> torch.Tensor:
-    """Frequencies of long waves divided by the factor, of short ones kept, blended between."""
+    """Frequencies of long waves divided by the factor, of short ones kept, blended between: the
+    scaling that the Llama 3.1 models were published with (2024), "llama3" in configurations."""
     factor = _number(scaling, "factor")
     lo, hi = _number(scaling, "low_freq_factor"), _number(scaling, "high_freq_factor")
     length = _number(scaling, "original_max_position_embeddings")
@@ -61,7 +62,9 @@ def _by_rotations(f: torch.Tensor, rope_base: float, scaling: dict) -> tuple[tor
     """(frequencies, factor of cosine and sine) of the YaRN method (B. Peng et al., "YaRN: Efficient
     Context Window Extension of Large Language Models", 2023): pairs that turn less than beta_slow
     times over the trained length are divided by the factor, those of more than beta_fast kept, a
-    linear ramp over the pairs between."""
+    linear ramp over the pairs between. Two keys are not the paper's but later configurations', with
+    the meaning that the transformers library documents: "truncate" (by default the ramp's ends are
+    whole pairs) and "mscale" with "mscale_all_dim" (the factor is a quotient of two)."""
     factor = _number(scaling, "factor")
     length = _number(scaling, "original_max_position_embeddings")
     fast, slow = _number(scaling, "beta_fast", 32.0), _number(scaling, "beta_slow", 1.0)
