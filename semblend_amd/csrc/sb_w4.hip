@@ -193,10 +193,11 @@ __device__ __forceinline__ uint32_t w4_lds_addr(const void* p) {
 // tile of inputs.
 //
 // What bounds it: the codes' bytes where these are many (one row of 4096 -> 131072 in fp16, 277 MB in 43 us,
-// 6.4 TB/s; 8 rows of 3584 -> 37888, 71 MB in 14.5, 4.9 TB/s), else the rows, which every workgroup copies
-// again (64 rows of 3584 -> 4608: 7.7 us, 96 x 2 workgroups of 32 rows, 45 MB of rows and 17 of codes), and a
-// launch with one chain of copies (one row of 3584 -> 4608 4.5 us). Halves of a tile as steps of their own,
-// so that one is copied under the other (64 rows, 128 bytes of eight rows a copy): 8.9 -> 11.0 us.
+// 6.4 TB/s; 8 rows of 3584 -> 37888, 72 MB in no cache in 18.1, 4.0 TB/s, in 14.5 where the last cache holds a
+// part), else the rows, which every workgroup copies again (64 rows of 3584 -> 4608: 7.7 us, 96 x 2 workgroups
+// of 32 rows, 45 MB of rows and 17 of codes), and a launch with one chain of copies (one row of 3584 -> 4608
+// 4.5 us). Halves of a tile as steps of their own, so that one is copied under the other (64 rows, 128 bytes of
+// eight rows a copy): 8.9 -> 11.0 us.
 template <int R, int J, int GPT> struct RowsStage {
   static constexpr int kMi = R < 16 ? 1 : R / 16;
   static constexpr int kTableCopies = (J * GPT + 3) / 4;

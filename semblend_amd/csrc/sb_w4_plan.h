@@ -91,10 +91,15 @@ inline W4Plan w4_plan(int64_t m, int64_t n, int64_t k, int64_t group, bool bf16)
   }
   // Up to 16 rows: 16 waves where a workgroup has 16 features (a CU has one or two of them then) and a
   // tile of inputs for each wave (one row of 18944 -> 3584 9.8 -> 9.1 us, 16 rows 12.9 -> 11.8; of 896 ->
-  // 1152 2.9 and 3.0), and codes read past the caches where these cannot keep them until the next call
-  // (one row of 4096 -> 131072, 268 MB: 47.9 -> 45.2 us; 16 of 3584 -> 37888, 68 MB, 15.3 and 19.6).
-  // (64 rows and features: LDS holds seven waves' steps)
+  // 1152 2.9 and 3.0). (64 rows and features: LDS holds seven waves' steps)
   p.waves = p.r <= 16 && p.j == 1 && kt > 16 ? 16 : p.r == 64 && p.j == 4 ? 7 : 8;
+  // Codes read past the caches (nontemporal) where the 256 MB last one cannot hold them until the next call
+  // with these weights, whatever runs between: from 192 MB on. Measured, plain and nontemporal reads: weights
+  // that are in no cache (a ring of 1.5 GB of them), one row of 4096 -> 131072, 285 MB, 45.6 and 44.1 us, 16
+  // rows 56.5 and 52.6; 16 rows of 3584 -> 37888, 72 MB, 20.3 and 19.0, one of 4096 -> 28672, 62 MB, 13.2 and
+  // 12.7. Weights called again while the cache holds them (three of these in turn): 14.4 and 19.1, 12.6 and
+  // 12.4. Below 192 MB a call cannot know which it is; plain reads lose up to 8% of the one and save a
+  // quarter of the other.
   p.once = p.r <= 16 && p.j > 1 && tiles(m, p.r) == 1 && nt * kt * 1024 >= (int64_t{192} << 20);
   return p;
 }

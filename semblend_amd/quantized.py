@@ -134,8 +134,8 @@ def quantized_linear(
     sum of |x| |scale| below 2^120 (those of fp16 inputs and scales always are): the fp32 sums of a group of
     inputs are up to 31 times as large. A row that holds an infinity or a NaN gives NaN (or infinities), other rows
     are not affected. ``out`` must not overlap x.
-    Groups of 128 in bf16: one row of 3584 -> 4608 6.5 us, 8 of 3584 -> 37888 14, 2458 of 3584 -> 4608
-    91; one of 4096 -> 131072 in fp16 44. Extension with no reference counterpart.
+    Groups of 128 in bf16: one row of 3584 -> 4608 6.6 us, 8 of 3584 -> 37888 14 (18 where the weights
+    are in no cache), 2458 of 3584 -> 4608 91; one of 4096 -> 131072 in fp16 44. Extension with no reference counterpart.
     """
     if not isinstance(weight, QuantizedLinear):
         raise TypeError("weight must be a QuantizedLinear")
