@@ -607,8 +607,8 @@ int sb_partial_attention_paged_varlen(void* out, const void* q, const void* kv_c
  * token, head, dim in elements) to the slots of their positions. With inv_freq (device fp32
  * [head_dim / 2], 1 / base^(2i/head_dim) <= 1), K is rotated in interleaved pairs by rotations[t]
  * (or, NULL, positions[t]) * inv_freq[i], the product and its sine and cosine in 64 bits; and query
- * (NULL: none; [num_tokens, num_q_heads, head_dim]) likewise into query_out. One rounding to the
- * cache's type. 4-bit blocks: 2^e is the smallest power with max |x| <= 7 * 2^e (e >= -127),
+ * (NULL: none; [num_tokens, num_q_heads, head_dim]) likewise into query_out, whose rows must not
+ * overlap. One rounding to the cache's type. 4-bit blocks: 2^e is the smallest power with max |x| <= 7 * 2^e (e >= -127),
  * x / 2^e rounds to the nearest 4-bit value, ties to even; a block with an infinity or a NaN is
  * stored as NaN. Two tokens of one slot race. head_dim even, at most 512. */
 int sb_append_kv_paged(void* kv_cache, void* kv_scales, const void* key, const void* value,

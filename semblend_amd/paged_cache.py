@@ -222,8 +222,9 @@ def append_kv_paged(
     positions: [T], each token's position in its request; row_starts: see the module.
     With ``rope_base`` (at least 1), K is rotated by its position with the interleaved RoPE of
     this path before its one rounding, and so is ``query`` [T, num_q_heads, head_dim], which goes
-    to ``query_out`` (a new tensor by default; returned). The angle is position * inv_freq with
-    the path's fp32 frequencies, the product and its sine and cosine in 64 bits.
+    to ``query_out`` (a new tensor by default; returned; rows that share elements are refused). The
+    angle is position * inv_freq with the path's fp32 frequencies, the product and its sine and
+    cosine in 64 bits.
     ``rotations``: [T], the positions to rotate by instead (a donor's K, rotated already at d and
     appended at t: t - d).
     ``rotary``: a :class:`semblend_amd.rotary.RotaryEmbedding` instead of ``rope_base``: half pairs,

@@ -218,7 +218,8 @@ def apply_rotary(
     query: [T, num_q_heads, head_dim]; key: [T, num_kv_heads, head_dim] of the same type (bf16, fp16
     or fp32), any strides (views of a fused projection's output, for instance); positions: [T]
     int32, any sign. Results go to ``query_out`` / ``key_out`` (new tensors by default), which may be
-    the inputs themselves and must not overlap them otherwise. Returns query_out, or (query_out,
+    the inputs themselves and must not overlap them otherwise; rows of an output that share elements
+    are refused. Returns query_out, or (query_out,
     key_out) with a key. No backward pass: as in :mod:`semblend_amd.paged_cache`, a new result of an
     input that requires a gradient raises when its gradient is asked for.
     8192 tokens of 32 / 8 heads x 128 in bf16: 168 MB in 27 us; 32 tokens of 28 / 4 heads
